@@ -152,3 +152,34 @@ def distance_code(distance):
         return DISTANCES[distance]
     except KeyError:
         raise ValueError("Unrecognized distance type") from None
+
+
+FLOAT_TYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+
+
+def float_type(dtype, what):
+    try:
+        return FLOAT_TYPES[dtype]
+    except KeyError:
+        raise TypeError("%s must be torch.float32, torch.bfloat16 or torch.float16, got %s" % (what, dtype)) from None
+
+
+def refuse_grad(*tensors):
+    """The operators for serving have no backward pass: an operand that asks for
+    a gradient is refused, not cut out of the graph in silence."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t.requires_grad:
+                raise RuntimeError("this operator has no backward pass; call it under torch.no_grad() or "
+                                   "with detached operands")
+
+
+def call(fn, device, *args):
+    """Calls a library entry point on the current stream of `device`, with that
+    device current, and raises for a status other than 0."""
+    stream = torch.cuda.current_stream(device).cuda_stream
+    if torch.cuda.current_device() == device.index:
+        _lib.check(fn(*args, stream))
+    else:
+        with torch.cuda.device(device):
+            _lib.check(fn(*args, stream))

@@ -18,6 +18,7 @@ ABI_VERSION = 1
 
 OP_BMM, OP_MBMM, OP_MIN_BMM, OP_TOPK_BMM, OP_TOPK_1D, OP_MIN_BMM_L2 = range(6)
 DIST_INNER, DIST_L2, DIST_L1 = range(3)
+F32, BF16, F16, MX4 = range(4)
 ERR_INVALID_ARG, ERR_UNSUPPORTED, ERR_WORKSPACE = -1, -2, -3
 
 # every symbol include/cmk.h declares
@@ -30,6 +31,9 @@ EXPORTS = (
     "cmk_min_bmm_f32_static",
     "cmk_topk_bmm_f32",
     "cmk_topk_1d_f32",
+    "cmk_mx4_quantize",
+    "cmk_mx4_dequantize",
+    "cmk_mx4_bmm",
     "cmk_workspace_bytes",
     "cmk_last_error",
     "cmk_abi_version",
@@ -99,8 +103,12 @@ def load():
     lib.cmk_min_bmm_f32_static.argtypes = [p, p, p, p, dp, i, i, p]
     lib.cmk_topk_bmm_f32.argtypes = [p, p, p, p, dp, i, i, i, p, sz, p]
     lib.cmk_topk_1d_f32.argtypes = [p, ll, p, p, i, p, sz, p]
+    lib.cmk_mx4_quantize.argtypes = [p, i, p, p, i, i, i, ll, ll, ll, p]
+    lib.cmk_mx4_dequantize.argtypes = [p, p, p, i, i, i, i, i, p]
+    lib.cmk_mx4_bmm.argtypes = [p, p, p, p, p, i, i, i, i, i, p]
     for name in ("cmk_bmm_f32", "cmk_bmm_ws_f32", "cmk_mbmm_f32", "cmk_derive_masks_u8", "cmk_min_bmm_f32", "cmk_min_bmm_f32_static",
-                 "cmk_topk_bmm_f32", "cmk_topk_1d_f32"):
+                 "cmk_topk_bmm_f32", "cmk_topk_1d_f32", "cmk_mx4_quantize", "cmk_mx4_dequantize",
+                 "cmk_mx4_bmm"):
         getattr(lib, name).restype = i
     lib.cmk_workspace_bytes.argtypes = [i, i, i, i, i, i]
     lib.cmk_workspace_bytes.restype = sz

@@ -1,0 +1,177 @@
+"""Matrices in 4-bit microscaled floating point: quantisation, its inverse and
+the batched product on the matrix pipe's scaled instructions.  No counterpart in
+the reference, whose products are fp32; the class stands beside BMMCUDA."""
+import torch
+
+from . import _common, _lib
+
+BLOCK = 32        # elements along k that share a scale
+SLAB = 128        # elements of k that lie together in storage
+
+
+class MX4Tensor:
+    """One [r, c] or a batch of [l, r, c] matrices in 4 bits, made by
+    ``quantize_mx4`` or ``MX4Tensor.from_blocks``.
+
+    Blocks of 32 elements along one of the last two axes (the contraction axis
+    of a product, `k_axis`, -1 or -2) share a power-of-two scale.  With the other
+    axis called rows:
+        codes  uint8 [l, ceil(k/128), rows, 64]: two elements a byte, the even
+               index in the low half; bit 3 is the sign, the rest indexes
+               0, .5, 1, 1.5, 2, 3, 4, 6
+        scales uint8 [l, ceil(k/128), rows, 4]: byte s stands for 2^(s-127), 255
+               for NaN
+    Elements beyond k are zero codes.  ``transpose`` swaps the matrix axes and
+    shares the storage."""
+
+    def __init__(self, codes, scales, k, k_axis=-1, two_dimensional=False):
+        slabs = -(-k // SLAB)
+        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+            raise TypeError("codes and scales must be torch.uint8")
+        assert k_axis in (-1, -2)
+        assert codes.dim() == 4 and codes.shape[1] == slabs and codes.shape[3] == SLAB // 2
+        assert tuple(scales.shape) == tuple(codes.shape[:3]) + (SLAB // BLOCK,)
+        assert codes.device == scales.device
+        assert codes.is_contiguous() and scales.is_contiguous()
+        assert not two_dimensional or codes.shape[0] == 1
+        self.codes, self.scales, self.k, self.k_axis = codes, scales, k, k_axis
+        self.two_dimensional = two_dimensional
+
+    @property
+    def rows(self):
+        return self.codes.shape[2]
+
+    @property
+    def shape(self):
+        matrix = (self.rows, self.k) if self.k_axis == -1 else (self.k, self.rows)
+        return torch.Size(matrix if self.two_dimensional else (self.codes.shape[0],) + matrix)
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    def dim(self):
+        return 2 if self.two_dimensional else 3
+
+    def transpose(self, dim0=-2, dim1=-1):
+        n = self.dim()
+        assert {dim0 % n, dim1 % n} == {n - 2, n - 1}, "only the two matrix axes can be swapped"
+        return MX4Tensor(self.codes, self.scales, self.k, -3 - self.k_axis, self.two_dimensional)
+
+    def to(self, device):
+        return MX4Tensor(self.codes.to(device), self.scales.to(device), self.k, self.k_axis, self.two_dimensional)
+
+    def dequantize(self, dtype=torch.float32):
+        """The values as a dense tensor of `shape`.  In float32 and bfloat16 they
+        are exact; in float16 they are rounded where its range ends."""
+        code = _common.float_type(dtype, "dtype")
+        assert self.device.type == "cuda"
+        out = torch.empty(self.shape, dtype=dtype, device=self.device)
+        if out.numel():
+            _common.call(_lib.load().cmk_mx4_dequantize, self.device,
+                         self.codes.data_ptr(), self.scales.data_ptr(), out.data_ptr(), code,
+                         self.codes.shape[0], self.rows, self.k, 1 if self.k_axis == -2 else 0)
+        return out
+
+    @classmethod
+    def from_blocks(cls, codes, scales, k, k_axis=-1):
+        """From row-major blocks, as checkpoints hold them: codes uint8
+        [(l,) rows, ceil(k/32)*16], scales uint8 [(l,) rows, ceil(k/32)].  Codes
+        beyond k have to be zero and are cleared here."""
+        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+            raise TypeError("codes and scales must be torch.uint8")
+        assert codes.dim() == scales.dim() and codes.dim() in (2, 3)
+        two_dimensional = codes.dim() == 2
+        if two_dimensional:
+            codes, scales = codes[None], scales[None]
+        blocks = -(-k // BLOCK)
+        l, rows, _ = codes.shape
+        assert tuple(codes.shape) == (l, rows, blocks * BLOCK // 2)
+        assert tuple(scales.shape) == (l, rows, blocks)
+        slabs = -(-k // SLAB)
+        c = torch.zeros(l, rows, slabs * SLAB // 2, dtype=torch.uint8, device=codes.device)
+        c[:, :, :k // 2] = codes[:, :, :k // 2]
+        if k % 2:
+            c[:, :, k // 2] = codes[:, :, k // 2] & 15
+        s = torch.zeros(l, rows, slabs * SLAB // BLOCK, dtype=torch.uint8, device=codes.device)
+        s[:, :, :blocks] = scales
+        c = c.view(l, rows, slabs, SLAB // 2).transpose(1, 2).contiguous()
+        s = s.view(l, rows, slabs, SLAB // BLOCK).transpose(1, 2).contiguous()
+        return cls(c, s, k, k_axis, two_dimensional)
+
+    def blocks(self):
+        """(codes, scales) in the row-major form that ``from_blocks`` takes."""
+        l, slabs, rows, _ = self.codes.shape
+        n = -(-self.k // BLOCK)
+        c = self.codes.transpose(1, 2).reshape(l, rows, slabs * SLAB // 2)[:, :, :n * BLOCK // 2].contiguous()
+        s = self.scales.transpose(1, 2).reshape(l, rows, slabs * SLAB // BLOCK)[:, :, :n].contiguous()
+        return (c[0], s[0]) if self.two_dimensional else (c, s)
+
+
+def quantize_mx4(T, dim=-1):
+    """The 4-bit form of a device tensor [r, c] or [l, r, c] of float32, bfloat16
+    or float16 with any strides; `dim`, the axis along which 32 elements share a
+    scale, is one of the last two: -1 for the left operand of a product, -2 for
+    the right one."""
+    dtype = _common.float_type(T.dtype, "the tensor")
+    n = T.dim()
+    if n not in (2, 3):
+        raise ValueError("the tensor needs to be 2d or 3d")
+    k_axis = dim if dim < 0 else dim - n
+    assert k_axis in (-1, -2), "dim must be one of the two matrix axes"
+    assert T.device.type == "cuda"
+    _common.refuse_grad(T)
+    x = T[None] if n == 2 else T
+    l = x.shape[0]
+    rows, k = (x.shape[1], x.shape[2]) if k_axis == -1 else (x.shape[2], x.shape[1])
+    sl, sr, sk = x.stride(0), x.stride(-3 - k_axis), x.stride(k_axis)
+    slabs = -(-k // SLAB)
+    codes = torch.empty((l, slabs, rows, SLAB // 2), dtype=torch.uint8, device=T.device)
+    scales = torch.empty((l, slabs, rows, SLAB // BLOCK), dtype=torch.uint8, device=T.device)
+    if codes.numel():
+        _common.call(_lib.load().cmk_mx4_quantize, T.device, x.data_ptr(), dtype, codes.data_ptr(),
+                     scales.data_ptr(), l, rows, k, sl, sr, sk)
+    return MX4Tensor(codes, scales, k, k_axis, n == 2)
+
+
+class MX4BMMCUDA:
+    """Batched product of operands in 4 bits: ``MX4BMMCUDA(out_dtype)(A, B)`` is
+    C = A @ B with A [l, m, k] or [m, k], B [l, k, n] or [k, n] and C in
+    `out_dtype` (float32, bfloat16 or float16).
+
+    An operand is an MX4Tensor whose blocks run along k (A: ``dim=-1``, B:
+    ``dim=-2``) or a float tensor, which is quantised in the call.  Sums are held
+    in fp32 and rounded once.  There is no backward pass."""
+
+    def __init__(self, out_dtype=torch.float32):
+        self._out = _common.float_type(out_dtype, "out_dtype")
+        self.out_dtype = out_dtype
+        self._lib = _lib.load()
+
+    def __call__(self, A, B):
+        assert A.dim() == B.dim()
+        n = A.dim()
+        if n not in (2, 3):
+            raise ValueError("A and B need to be 2d or 3d")
+        for T, axis, name in ((A, -1, "A"), (B, -2, "B")):
+            if isinstance(T, MX4Tensor):
+                assert T.k_axis == axis, "the blocks of %s must run along k" % name
+            else:
+                _common.float_type(T.dtype, name)
+                _common.refuse_grad(T)
+        sa, sb = A.shape, B.shape
+        assert sa[-1] == sb[-2]
+        assert n == 2 or sa[0] == sb[0]
+        assert A.device.type == B.device.type == "cuda"
+        assert A.device == B.device
+        l = 1 if n == 2 else sa[0]
+        m, k, c = sa[-2], sa[-1], sb[-1]
+        C = torch.empty((m, c) if n == 2 else (l, m, c), dtype=self.out_dtype, device=A.device)
+        if C.numel():
+            if not isinstance(A, MX4Tensor):
+                A = quantize_mx4(A, -1)
+            if not isinstance(B, MX4Tensor):
+                B = quantize_mx4(B, -2)
+            _common.call(self._lib.cmk_mx4_bmm, C.device, A.codes.data_ptr(), A.scales.data_ptr(),
+                         B.codes.data_ptr(), B.scales.data_ptr(), C.data_ptr(), self._out, l, m, c, k)
+        return C

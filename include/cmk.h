@@ -197,6 +197,46 @@ int cmk_topk_1d_f32(const float* arr, long long n,
                     float* values, long long* indices, int k,
                     void* workspace, size_t workspace_bytes, void* stream);
 
+/* Element types of the entry points below. */
+#define CMK_F32  0
+#define CMK_BF16 1
+#define CMK_F16  2
+#define CMK_MX4  3   /* codes and scales as cmk_mx4_quantize writes them */
+
+/*
+ * 4-bit microscaled form of L matrices of R rows and K elements a row:
+ * 32 consecutive elements along K share a scale 2^(s-127), s = max(e - 2, 0)
+ * with e the fp32 exponent field of their largest magnitude (255, standing for
+ * NaN, if one of them is not finite); an element is the nearest of 0, .5, 1,
+ * 1.5, 2, 3, 4, 6 times the scale with its sign (ties to the even code, beyond
+ * 6 to 6).  Element (l, r, k) of x is x[l*stride_l + r*stride_r + k*stride_k]
+ * (strides in elements, any of them).  Written are
+ *   codes  [L][ceil(K/128)][R][64], two elements a byte, the even one low,
+ *   scales [L][ceil(K/128)][R][4],
+ * every byte of them: elements beyond K are zero codes.  codes must be 16-byte
+ * aligned, scales 4-byte aligned.  No counterpart in the reference.
+ */
+int cmk_mx4_quantize(const void* x, int dtype, uint8_t* codes, uint8_t* scales,
+                     int L, int R, int K, long long stride_l, long long stride_r,
+                     long long stride_k, void* stream);
+
+/*
+ * The values that codes and scales stand for, rounded to `dtype`, dense
+ * [L][R][K], or [L][K][R] with rows_innermost != 0.
+ */
+int cmk_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, void* out,
+                       int dtype, int L, int R, int K, int rows_innermost,
+                       void* stream);
+
+/*
+ * C[l][m][n] = sum_k A[l][m][k] * B[l][k][n] of two matrices in the 4-bit form,
+ * A of M rows, B of N rows (its columns), accumulated in fp32 on the matrix
+ * pipe and rounded once to `dtype`; C is dense and written completely.
+ */
+int cmk_mx4_bmm(const uint8_t* a_codes, const uint8_t* a_scales,
+                const uint8_t* b_codes, const uint8_t* b_scales, void* C,
+                int dtype, int L, int M, int N, int K, void* stream);
+
 /* Bytes of device workspace an operation needs (0 = none).  For
  * CMK_OP_TOPK_1D pass the array length in M (L = 1).  The work is cut for the
  * GPU that is current when this is called (its compute-unit count): call it

@@ -1,0 +1,143 @@
+"""4-bit microscaled matrices without a GPU: the storage form, its import and
+export, and every refusal (each fires before any launch)."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+import _mx4
+from custom_matmul_kernels_amd import MX4BMMCUDA, MX4Tensor, _lib, quantize_mx4
+
+
+def blocks(l, rows, k, seed=0):
+    gen = torch.Generator().manual_seed(seed)
+    codes, scales = _mx4.encode(torch.randn(l, rows, k, generator=gen))
+    return torch.from_numpy(_mx4.packed(codes)), torch.from_numpy(scales)
+
+
+def test_oracle_rounds_ties_to_even_and_saturates():
+    q = np.array([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 5.5, 6.0, 7.9, 0.2501, -0.75, -2.5, 0.0, 4.0])
+    want = np.array([0, 1, 1, 2, 2, 4, 4, 6, 6, 6, 0.5, -1, -2, 0, 4])
+    x = np.concatenate([q, np.zeros(32 - len(q))])           # largest 7.9: scale 1
+    codes, scales = _mx4.encode(x)
+    assert scales[0] == 127
+    assert np.array_equal(_mx4.decode(codes, scales)[:len(q)], want)
+
+
+@pytest.mark.parametrize("k", [1, 31, 32, 33, 96, 128, 129, 200, 256])
+@pytest.mark.parametrize("rows", [1, 3, 17])
+def test_blocks_survive_the_storage_form(rows, k):
+    codes, scales = blocks(2, rows, k)
+    t = MX4Tensor.from_blocks(codes, scales, k)
+    assert t.shape == (2, rows, k) and t.rows == rows
+    assert tuple(t.codes.shape) == (2, -(-k // 128), rows, 64)
+    back = t.blocks()
+    assert torch.equal(back[0], codes) and torch.equal(back[1], scales)
+    # element (l, r, i) sits at slab i // 128, byte (i % 128) // 2, low half first
+    for i in {0, k // 2, k - 1}:
+        byte = t.codes[1, i // 128, rows - 1, i % 128 // 2].item()
+        assert byte >> (4 * (i % 2)) & 15 == codes[1, rows - 1, i // 2].item() >> (4 * (i % 2)) & 15
+        assert t.scales[1, i // 128, rows - 1, i % 128 // 32] == scales[1, rows - 1, i // 32]
+
+
+def test_codes_beyond_k_are_cleared_on_import():
+    codes = torch.full((1, 2, 32), 0x55, dtype=torch.uint8)
+    scales = torch.full((1, 2, 2), 127, dtype=torch.uint8)
+    t = MX4Tensor.from_blocks(codes, scales, 35)
+    assert (t.codes[0, 0, :, :17] == 0x55).all() and (t.codes[0, 0, :, 17] == 5).all()
+    assert (t.codes[0, 0, :, 18:] == 0).all() and (t.scales[0, 0, :, 2:] == 0).all()
+
+
+def test_transpose_and_two_dimensions():
+    codes, scales = blocks(1, 5, 40)
+    t = MX4Tensor.from_blocks(codes[0], scales[0], 40)
+    assert t.shape == (5, 40) and t.dim() == 2
+    u = t.transpose(0, 1)
+    assert u.shape == (40, 5) and u.k_axis == -2 and u.codes is t.codes
+    assert u.transpose().shape == (5, 40)
+    with pytest.raises(AssertionError):
+        MX4Tensor.from_blocks(codes, scales, 40).transpose(0, 1)
+
+
+def test_wrong_storage_is_refused():
+    codes, scales = blocks(1, 5, 40)
+    t = MX4Tensor.from_blocks(codes, scales, 40)
+    with pytest.raises(TypeError):
+        MX4Tensor(t.codes.int(), t.scales, 40)
+    with pytest.raises(TypeError):
+        MX4Tensor.from_blocks(codes.int(), scales, 40)
+    for bad in (lambda: MX4Tensor(t.codes, t.scales, 129), lambda: MX4Tensor(t.codes, t.scales[:, :, :4], 40),
+                lambda: MX4Tensor(t.codes, t.scales, 40, k_axis=0),
+                lambda: MX4Tensor(t.codes.transpose(1, 2), t.scales, 40),
+                lambda: MX4Tensor.from_blocks(codes, scales, 70),
+                lambda: MX4Tensor.from_blocks(codes, scales[:, :, :1], 40)):
+        with pytest.raises(AssertionError):
+            bad()
+
+
+def test_refusals_of_the_python_entry_points():
+    codes, scales = blocks(2, 5, 40)
+    A = MX4Tensor.from_blocks(codes, scales, 40)                       # [2, 5, 40]
+    B = A.transpose()                                                  # [2, 40, 5]
+    product = MX4BMMCUDA()
+    with pytest.raises(TypeError):
+        MX4BMMCUDA(out_dtype=torch.float64)
+    with pytest.raises(TypeError):
+        quantize_mx4(torch.zeros(2, 3, dtype=torch.float64))
+    with pytest.raises(ValueError):
+        quantize_mx4(torch.zeros(3))
+    with pytest.raises(ValueError):
+        quantize_mx4(torch.zeros(3, 3, 3, 3))
+    for dim in (0, -3, 3):
+        with pytest.raises(AssertionError):
+            quantize_mx4(torch.zeros(2, 3, 4), dim=dim)
+    with pytest.raises(AssertionError):
+        quantize_mx4(torch.zeros(2, 3, 4))                             # not on a device
+    with pytest.raises(AssertionError):
+        A.dequantize()
+    with pytest.raises(TypeError):
+        A.dequantize(torch.int32)
+    with pytest.raises(AssertionError):
+        product(A, B)                                                  # not on a device
+    with pytest.raises(AssertionError):
+        product(A, A)                                                  # blocks of B do not run along k
+    with pytest.raises(AssertionError):
+        product(B, B)
+    with pytest.raises(AssertionError):
+        product(torch.zeros(2, 5, 41), B)                              # contraction mismatch
+    with pytest.raises(AssertionError):
+        product(torch.zeros(3, 5, 40), B)                              # batch mismatch
+    with pytest.raises(AssertionError):
+        product(torch.zeros(5, 40), B)                                 # 2d against 3d
+    with pytest.raises(TypeError):
+        product(torch.zeros(2, 5, 40, dtype=torch.float64), B)
+    with pytest.raises(RuntimeError, match="backward"):
+        product(torch.zeros(2, 5, 40, requires_grad=True), B)
+    with pytest.raises(AssertionError):                                # passes the gradient check without grad
+        with torch.no_grad():
+            product(torch.zeros(2, 5, 40, requires_grad=True), B)
+
+
+def test_refusals_of_the_c_entry_points():
+    lib = _lib.load()
+    ok, odd = ctypes.c_void_p(0x1000), ctypes.c_void_p(0x1002)          # never dereferenced
+    bad = _lib.ERR_INVALID_ARG
+    assert lib.cmk_mx4_quantize(ok, 3, ok, ok, 1, 1, 1, 1, 1, 1, None) == bad
+    assert lib.cmk_mx4_quantize(ok, 0, ok, ok, 1, -1, 1, 1, 1, 1, None) == bad
+    assert lib.cmk_mx4_quantize(None, 0, ok, ok, 1, 1, 1, 1, 1, 1, None) == bad
+    assert lib.cmk_mx4_quantize(ok, 0, odd, ok, 1, 1, 1, 1, 1, 1, None) == bad
+    assert b"alignment" in lib.cmk_last_error()
+    assert lib.cmk_mx4_quantize(ok, 0, ok, odd, 1, 1, 1, 1, 1, 1, None) == bad
+    assert lib.cmk_mx4_dequantize(ok, ok, ok, -1, 1, 1, 1, 0, None) == bad
+    assert lib.cmk_mx4_dequantize(ok, ok, None, 0, 1, 1, 1, 0, None) == bad
+    assert lib.cmk_mx4_dequantize(odd, ok, ok, 0, 1, 1, 1, 0, None) == bad
+    assert lib.cmk_mx4_bmm(ok, ok, ok, ok, ok, 7, 1, 1, 1, 1, None) == bad
+    assert lib.cmk_mx4_bmm(ok, ok, ok, ok, ok, 0, 1, 1, -1, 1, None) == bad
+    assert lib.cmk_mx4_bmm(ok, ok, ok, ok, None, 0, 1, 1, 1, 1, None) == bad
+    assert lib.cmk_mx4_bmm(ok, ok, None, ok, ok, 0, 1, 1, 1, 1, None) == bad
+    assert lib.cmk_mx4_bmm(ok, ok, odd, ok, ok, 0, 1, 1, 1, 1, None) == bad
+    # nothing to do is no error
+    assert lib.cmk_mx4_quantize(None, 0, None, None, 1, 0, 5, 1, 1, 1, None) == 0
+    assert lib.cmk_mx4_dequantize(None, None, None, 0, 0, 5, 5, 0, None) == 0
+    assert lib.cmk_mx4_bmm(None, None, None, None, None, 0, 1, 0, 5, 5, None) == 0

@@ -1,0 +1,228 @@
+"""4-bit microscaled matrices on the GPU against the definition in 64 bits.
+
+Quantisation has one right answer: codes and scales are compared bit by bit.
+Products: the values are exact, so an output is off by the fp32 accumulation, at
+most k * 2^-23 * sum |a b| for any order of the sums and rounding or truncating
+adders, plus half a step of the output type."""
+import numpy as np
+import pytest
+import torch
+
+import _mx4
+from custom_matmul_kernels_amd import MX4BMMCUDA, MX4Tensor, quantize_mx4
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def normal(shape, seed, dtype=torch.float32):
+    gen = torch.Generator().manual_seed(seed)
+    x = torch.randn(shape, generator=gen)
+    x[..., ::37] *= 20
+    return x.to(dtype)
+
+
+def check_blocks(x, q):
+    """x: host tensor [l, rows, k]; q: MX4Tensor on the device."""
+    print("blocks", tuple(x.shape), x.dtype, flush=True)
+    codes, scales = _mx4.encode(x.double().numpy())
+    got_c, got_s = q.blocks()
+    if q.two_dimensional:
+        got_c, got_s = got_c[None], got_s[None]
+    assert np.array_equal(got_s.cpu().numpy(), scales)
+    assert np.array_equal(got_c.cpu().numpy(), _mx4.packed(codes))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("l,rows,k", [(1, 1, 1), (1, 1, 32), (2, 3, 31), (1, 17, 33), (3, 16, 128), (2, 65, 129),
+                                      (1, 100, 1000), (2, 130, 520), (1, 7, 4097)])
+def test_quantize_rows(device, dtype, l, rows, k):
+    x = normal((l, rows, k), 1000 * rows + k, dtype)
+    q = quantize_mx4(x.to(device))
+    assert q.shape == (l, rows, k)
+    check_blocks(x, q)
+    # the padding up to a whole slab holds zero codes and zero scales
+    tail = q.codes[:, -1].cpu()
+    used = (k - 1) % 128 + 1
+    assert (tail[:, :, (used + 1) // 2:] == 0).all()
+    assert (q.scales[:, -1].cpu()[:, :, -(-used // 32):] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("l,rows,k", [(1, 1, 1), (2, 3, 31), (1, 65, 33), (3, 64, 128), (2, 130, 257), (1, 1000, 100)])
+def test_quantize_columns(device, dtype, l, rows, k):
+    """Blocks down the columns of a [k, rows] matrix."""
+    x = normal((l, k, rows), 77 * rows + k, dtype)
+    q = quantize_mx4(x.to(device), dim=1)
+    assert q.shape == (l, k, rows) and q.k_axis == -2
+    check_blocks(x.transpose(1, 2), q)
+
+
+def test_quantize_strided_views(device):
+    base = normal((4, 70, 300), 5).to(device)
+    for view in (base[:, 3:50, 7:290], base[::2, ::3], base[:, :, ::2], base[:1].expand(3, 70, 300),
+                 base.transpose(0, 1), base[:, :, 1:2], base[:, 5:6, :]):
+        for dim in (-1, -2):
+            q = quantize_mx4(view, dim=dim)
+            x = view.cpu() if dim == -1 else view.cpu().transpose(1, 2)
+            check_blocks(x, q)
+    q = quantize_mx4(base[1], dim=0)
+    assert q.shape == (70, 300)
+    check_blocks(base[1].cpu().t()[None], q)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_quantize_special_values(device, dtype):
+    """Ties, saturation, zero blocks, the ends of the exponent range, NaN and infinities."""
+    fi = torch.finfo(dtype)
+    rows = []
+    ties = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 5.5, 7.0, 7.9, 0.2, 6.0, -0.25, -0.75, -5.0, -7.9])
+    for scale in (1.0, 2.0 ** -8, 2.0 ** 5):
+        rows.append(torch.cat([ties, -ties]) * scale)
+    rows.append(torch.zeros(32))
+    rows.append(torch.full((32,), -0.0))
+    rows.append(torch.full((32,), fi.max))
+    rows.append(torch.full((32,), fi.tiny))
+    rows.append(torch.arange(32) * fi.smallest_normal / 7)
+    rows.append(torch.arange(32) * float(np.finfo(np.float32).smallest_subnormal) * 3.0)
+    rows.append(torch.arange(32) * 2.0 ** -130)
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        r = torch.ones(32)
+        r[11] = bad
+        rows.append(r)
+    x = torch.stack(rows).to(dtype)
+    q = quantize_mx4(x.to(device))
+    check_blocks(x[None], q)
+    # the same columns-wise
+    q = quantize_mx4(x.t().contiguous().to(device), dim=0)
+    check_blocks(x[None], q)
+    v = q.dequantize().cpu().t()
+    want = _mx4.rounded(x)
+    assert torch.equal(torch.isnan(v), torch.isnan(want))
+    assert torch.isnan(v).all(1).sum() == 3
+    fine = ~torch.isnan(want)
+    assert torch.equal(v.double()[fine], want[fine])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("k_axis", [-1, -2])
+def test_dequantize(device, dtype, k_axis):
+    for l, rows, k in ((1, 1, 1), (2, 33, 70), (3, 65, 129), (1, 200, 512), (2, 5, 1001)):
+        x = normal((l, rows, k), k)
+        want = _mx4.rounded(x)
+        q = quantize_mx4(x.to(device))
+        if k_axis == -2:
+            q, want = q.transpose(), want.transpose(1, 2)
+        got = q.dequantize(dtype)
+        assert got.shape == q.shape and got.is_contiguous()
+        assert torch.equal(got.cpu(), want.to(dtype))
+
+
+def check_product(got, a, b, dtype):
+    """a [l, m, k], b [l, k, n] in float64, the 4-bit values."""
+    assert got.dtype == dtype
+    want, size = a @ b, a.abs() @ b.abs()
+    k = a.shape[2]
+    bound = size * (k * 2.0 ** -23) + want.abs() * (torch.finfo(dtype).eps / 2) * (1 + k * 2.0 ** -23) \
+        + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    off = (got.cpu().double() - want).abs()
+    assert got.shape == want.shape
+    assert (off <= bound).all(), "off by %g of the bound" % (off / bound).max()
+
+
+SHAPES = [(1, 1, 1, 1), (1, 1, 17, 32), (2, 5, 3, 100), (1, 16, 64, 128), (3, 33, 65, 129), (1, 128, 128, 256),
+          (2, 130, 200, 300), (1, 257, 129, 1000), (1, 1, 500, 4096), (1, 64, 1000, 640), (1, 40, 31, 5000),
+          (1, 300, 513, 130), (5, 20, 20, 20), (1, 513, 700, 2050)]
+
+
+@pytest.mark.parametrize("l,m,n,k", SHAPES)
+@pytest.mark.parametrize("dtype", TYPES)
+def test_product(device, dtype, l, m, n, k):
+    print("product", (l, m, n, k), dtype, flush=True)
+    x, w = normal((l, m, k), m + k, dtype), normal((l, k, n), n + k)
+    A, B = quantize_mx4(x.to(device)), quantize_mx4(w.to(device), dim=-2)
+    a, b = _mx4.rounded(x), _mx4.rounded(w.transpose(1, 2)).transpose(1, 2)
+    got = MX4BMMCUDA(out_dtype=dtype)(A, B)
+    check_product(got, a, b, dtype)
+    # quantised in the call: the same bits
+    for left, right in ((x.to(device), B), (A, w.to(device)), (x.to(device), w.to(device))):
+        assert torch.equal(MX4BMMCUDA(out_dtype=dtype)(left, right), got)
+
+
+def test_product_two_dimensions_and_views(device):
+    x, w = normal((70, 300), 1).to(device), normal((300, 90), 2).to(device)
+    product = MX4BMMCUDA()
+    got = product(x, quantize_mx4(w, dim=0))
+    assert got.shape == (70, 90)
+    check_product(got[None], _mx4.rounded(x)[None], _mx4.rounded(w.t()).t()[None], torch.float32)
+    # any strides of a float operand
+    base = normal((3, 40, 520), 3).to(device)
+    for left in (base[:, ::2, 5:305], base[:, :20, ::2][:, :, :150], base[:1, :9, :300].expand(3, 9, 300),
+                 base[:, :, :33].transpose(1, 2)[:, :, :40]):
+        k = left.shape[2]
+        right = normal((3, 50, k), k).to(device)
+        got = product(left, right.transpose(1, 2))
+        check_product(got, _mx4.rounded(left), _mx4.rounded(right).transpose(1, 2), torch.float32)
+
+
+def test_product_with_an_empty_axis(device):
+    product = MX4BMMCUDA()
+    assert product(torch.zeros(2, 0, 40, device=device), torch.zeros(2, 40, 3, device=device)).shape == (2, 0, 3)
+    assert product(torch.zeros(0, 4, 40, device=device), torch.zeros(0, 40, 3, device=device)).shape == (0, 4, 3)
+    assert product(torch.zeros(2, 4, 40, device=device), torch.zeros(2, 40, 0, device=device)).shape == (2, 4, 0)
+    got = product(torch.zeros(2, 4, 0, device=device), torch.zeros(2, 0, 3, device=device))
+    assert got.shape == (2, 4, 3) and (got == 0).all()
+    assert quantize_mx4(torch.zeros(2, 0, 40, device=device)).dequantize().shape == (2, 0, 40)
+
+
+@pytest.mark.parametrize("m", [3, 40, 200])
+def test_nan_stays_in_its_row(device, m):
+    x, w = normal((1, m, 200), 1), normal((1, 200, 70), 2)
+    x[0, m // 2, 150] = float("nan")
+    w[0, 20, 33] = float("inf")
+    got = MX4BMMCUDA()(x.to(device), quantize_mx4(w.to(device), dim=-2)).cpu()
+    bad = torch.zeros(1, m, 70, dtype=torch.bool)
+    bad[0, m // 2] = True
+    bad[0, :, 33] = True
+    assert torch.equal(torch.isnan(got), bad)
+
+
+def test_large_and_small_scales(device):
+    """Block scales far apart: the sums keep fp32's range."""
+    x, w = normal((1, 20, 256), 1), normal((1, 256, 40), 2)
+    x[..., :32] *= 2.0 ** 40
+    x[..., 32:64] *= 2.0 ** -60
+    w[:, 32:64] *= 2.0 ** 50
+    got = MX4BMMCUDA()(x.to(device), w.to(device))
+    check_product(got, _mx4.rounded(x), _mx4.rounded(w.transpose(1, 2)).transpose(1, 2), torch.float32)
+
+
+def test_on_another_stream(device):
+    x, w = normal((1, 5, 1000), 1).to(device), normal((1, 1000, 300), 2).to(device)
+    want = MX4BMMCUDA()(x, w)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        got = [MX4BMMCUDA()(x, w) for _ in range(3)]
+    side.synchronize()
+    for g in got:
+        assert torch.equal(g, want)
+
+
+@pytest.mark.parametrize("m", [1, 16, 200])
+def test_replays_in_a_graph(device, m):
+    x, w = normal((1, m, 600), 1).to(device), normal((1, 600, 300), 2).to(device)
+    B = quantize_mx4(w, dim=-2)
+    product = MX4BMMCUDA(out_dtype=torch.bfloat16)
+    product(x, B)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = product(x, B)
+    for step in range(3):
+        x.copy_(normal((1, m, 600), 10 + step))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = out.clone()
+        assert torch.equal(got, product(x, B)), "replay %d differs" % step
