@@ -9,7 +9,8 @@ from .mbmm import MBMMCUDA
 from .minbmm import MinBMMCUDA
 from .topkbmm import TopkBMMCUDA, BitonicSort
 from .masks import derive_masks
+from .moe import MoECUDA
 from .mx4 import MX4BMMCUDA, MX4Tensor, quantize_mx4
 
 __all__ = ["BMMCUDA", "MBMMCUDA", "MinBMMCUDA", "TopkBMMCUDA", "BitonicSort",
-           "derive_masks", "MX4BMMCUDA", "MX4Tensor", "quantize_mx4", "build", "load", "LIB_PATH", "CmkError"]
+           "derive_masks", "MX4BMMCUDA", "MoECUDA", "MX4Tensor", "quantize_mx4", "build", "load", "LIB_PATH", "CmkError"]

@@ -19,6 +19,7 @@ ABI_VERSION = 1
 OP_BMM, OP_MBMM, OP_MIN_BMM, OP_TOPK_BMM, OP_TOPK_1D, OP_MIN_BMM_L2 = range(6)
 DIST_INNER, DIST_L2, DIST_L1 = range(3)
 F32, BF16, F16, MX4 = range(4)
+ACT_SILU, ACT_GELU = range(2)
 ERR_INVALID_ARG, ERR_UNSUPPORTED, ERR_WORKSPACE = -1, -2, -3
 
 # every symbol include/cmk.h declares
@@ -34,6 +35,8 @@ EXPORTS = (
     "cmk_mx4_quantize",
     "cmk_mx4_dequantize",
     "cmk_mx4_bmm",
+    "cmk_moe",
+    "cmk_moe_workspace_bytes",
     "cmk_workspace_bytes",
     "cmk_last_error",
     "cmk_abi_version",
@@ -55,6 +58,15 @@ class GemmDesc(ctypes.Structure):
         ("strideA", ctypes.c_longlong),
         ("strideB", ctypes.c_longlong),
     ]
+
+
+class MoeDesc(ctypes.Structure):
+    """Mirror of ``cmk_moe_desc`` in include/cmk.h."""
+
+    _fields_ = [(name, ctypes.c_int) for name in
+                ("T", "H", "I", "E", "k", "x_dtype", "router_dtype", "w_dtype", "activation", "renormalize")] + \
+               [(name, ctypes.c_longlong) for name in
+                ("ld_x", "ld_router", "ld_gate_up", "stride_gate_up", "ld_down", "stride_down")]
 
 
 class CmkError(RuntimeError):
@@ -106,9 +118,13 @@ def load():
     lib.cmk_mx4_quantize.argtypes = [p, i, p, p, i, i, i, ll, ll, ll, p]
     lib.cmk_mx4_dequantize.argtypes = [p, p, p, i, i, i, i, i, p]
     lib.cmk_mx4_bmm.argtypes = [p, p, p, p, p, i, i, i, i, i, p]
+    mp = ctypes.POINTER(MoeDesc)
+    lib.cmk_moe.argtypes = [p, p, p, p, p, p, p, p, p, mp, p, sz, p]
+    lib.cmk_moe_workspace_bytes.argtypes = [mp]
+    lib.cmk_moe_workspace_bytes.restype = sz
     for name in ("cmk_bmm_f32", "cmk_bmm_ws_f32", "cmk_mbmm_f32", "cmk_derive_masks_u8", "cmk_min_bmm_f32", "cmk_min_bmm_f32_static",
                  "cmk_topk_bmm_f32", "cmk_topk_1d_f32", "cmk_mx4_quantize", "cmk_mx4_dequantize",
-                 "cmk_mx4_bmm"):
+                 "cmk_mx4_bmm", "cmk_moe"):
         getattr(lib, name).restype = i
     lib.cmk_workspace_bytes.argtypes = [i, i, i, i, i, i]
     lib.cmk_workspace_bytes.restype = sz

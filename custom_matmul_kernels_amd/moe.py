@@ -1,0 +1,94 @@
+"""A mixture-of-experts layer for a few tokens: router, choice, the chosen
+experts' products and their weighted sum.  No counterpart in the reference; the
+router is a top-k of a product and the experts are a routed batched product."""
+import torch
+
+from . import _common, _lib
+from .mx4 import MX4Tensor
+
+ACTIVATIONS = {"silu": _lib.ACT_SILU, "gelu": _lib.ACT_GELU}
+CHUNK = 256        # tokens per library call
+
+
+class MoECUDA:
+    """``MoECUDA(k, activation, renormalize)(x, router, gate_up, down)`` returns
+    (y, weights, experts).
+
+    Per token the `k` experts of the largest x @ router.T (summed in 64 bits; the
+    lowest index of equal ones, NaN above all) are weighted by the softmax of
+    these over the chosen (`renormalize`) or over all experts, and
+        y = sum_j weights_j * ((act(x @ gate.T) * (x @ up.T)) @ down_e.T)
+    with gate and up the first and last i rows of gate_up[e].
+
+    x: bfloat16 or float16 [t, h];  router: x's type or float32 [e, h]
+    gate_up [e, 2i, h], down [e, h, i]: x's type with the last axis contiguous, or
+    MX4Tensors of these shapes with blocks along the last axis
+    returns y [t, h] in x's type, weights float32 [t, k], experts int64 [t, k]
+
+    Made for a few tokens, where reading the chosen experts' weights is all there
+    is; more than 256 run in portions of 256.  There is no backward pass."""
+
+    def __init__(self, k=2, activation="silu", renormalize=True):
+        if activation not in ACTIVATIONS:
+            raise ValueError("Unrecognized activation")
+        assert type(renormalize) == bool
+        assert k >= 1
+        self.k, self.activation, self.renormalize = k, activation, renormalize
+        self._lib = _lib.load()
+
+    @staticmethod
+    def _experts(W, x, name):
+        """(pointer, scales' pointer, row stride, expert stride) of [e, r, c] weights."""
+        if isinstance(W, MX4Tensor):
+            assert W.k_axis == -1, "the blocks of %s must run along its last axis" % name
+            return W.codes.data_ptr(), W.scales.data_ptr(), 0, 0
+        if W.dtype != x.dtype:
+            raise TypeError("%s must be an MX4Tensor or of x's type, got %s" % (name, W.dtype))
+        _common.refuse_grad(W)
+        s0, s1, s2 = W.stride()
+        e, r, c = W.shape
+        if (s2 != 1 and c > 1) or (s1 < c and r > 1) or (s0 < 0 and e > 1):
+            raise ValueError("the last axis of %s must be contiguous" % name)
+        return W.data_ptr(), None, s1 if r > 1 else c, s0 if e > 1 else 0
+
+    def __call__(self, x, router, gate_up, down):
+        if x.dtype not in (torch.bfloat16, torch.float16):
+            raise TypeError("x must be torch.bfloat16 or torch.float16, got %s" % x.dtype)
+        if router.dtype not in (torch.float32, x.dtype):
+            raise TypeError("router must be torch.float32 or of x's type, got %s" % router.dtype)
+        if x.dim() != 2 or router.dim() != 2 or gate_up.dim() != 3 or down.dim() != 3:
+            raise ValueError("x and router need to be 2d, gate_up and down 3d")
+        t, h = x.shape
+        e, two_i, _ = gate_up.shape
+        i = two_i // 2
+        assert tuple(router.shape) == (e, h)
+        assert two_i == 2 * i and i > 0 and h > 0
+        assert tuple(gate_up.shape) == (e, 2 * i, h) and tuple(down.shape) == (e, h, i)
+        assert 0 < self.k <= e
+        _common.refuse_grad(x, router)
+        gp, gs, ldg, sg = self._experts(gate_up, x, "gate_up")
+        dp, ds, ldd, sd = self._experts(down, x, "down")
+        assert isinstance(gate_up, MX4Tensor) == isinstance(down, MX4Tensor)
+        dev = x.device
+        assert dev.type == "cuda"
+        assert router.device == gate_up.device == down.device == dev
+        if h > 1 and x.stride(1) != 1 or t > 1 and x.stride(0) < h:
+            x = x.contiguous()
+        if h > 1 and router.stride(1) != 1 or e > 1 and router.stride(0) < h:
+            router = router.contiguous()
+        y = torch.empty((t, h), dtype=x.dtype, device=dev)
+        weights = torch.empty((t, self.k), dtype=torch.float32, device=dev)
+        experts = torch.empty((t, self.k), dtype=torch.int64, device=dev)
+        for t0 in range(0, t, CHUNK):
+            n = min(CHUNK, t - t0)
+            part = x[t0:t0 + n]
+            d = _lib.MoeDesc(n, h, i, e, self.k, _common.FLOAT_TYPES[x.dtype], _common.FLOAT_TYPES[router.dtype],
+                             _lib.MX4 if gs is not None else _common.FLOAT_TYPES[x.dtype],
+                             ACTIVATIONS[self.activation], int(self.renormalize),
+                             max(part.stride(0), h), max(router.stride(0), h), ldg, sg, ldd, sd)
+            nbytes = self._lib.cmk_moe_workspace_bytes(d)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            _common.call(self._lib.cmk_moe, dev, part.data_ptr(), router.data_ptr(), gp, gs, dp, ds,
+                         y[t0:].data_ptr(), weights[t0:].data_ptr(), experts[t0:].data_ptr(), d,
+                         ws.data_ptr(), nbytes)
+        return y, weights, experts

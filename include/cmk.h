@@ -237,6 +237,52 @@ int cmk_mx4_bmm(const uint8_t* a_codes, const uint8_t* a_scales,
                 const uint8_t* b_codes, const uint8_t* b_scales, void* C,
                 int dtype, int L, int M, int N, int K, void* stream);
 
+/* activations of the experts */
+#define CMK_ACT_SILU 0   /* g / (1 + exp(-g))            */
+#define CMK_ACT_GELU 1   /* g (1 + erf(g / sqrt 2)) / 2  */
+
+/* A mixture-of-experts layer: T tokens of H features, E experts of I inner
+ * features, k of them per token. */
+typedef struct cmk_moe_desc {
+  int T, H, I, E, k;
+  int x_dtype;             /* CMK_BF16 or CMK_F16; y has the same              */
+  int router_dtype;        /* CMK_F32 or x_dtype                               */
+  int w_dtype;             /* CMK_MX4 or x_dtype                               */
+  int activation;          /* CMK_ACT_*                                        */
+  int renormalize;         /* weights: softmax over the chosen / over all      */
+  long long ld_x, ld_router;               /* row strides, elements            */
+  long long ld_gate_up, stride_gate_up;    /* row and expert strides, elements; */
+  long long ld_down, stride_down;          /* not read for CMK_MX4             */
+} cmk_moe_desc;
+
+/*
+ * A whole mixture-of-experts layer for a few tokens (T <= 256, E <= 1024,
+ * k <= 32):
+ *   g[t][e] = sum_h x[t][h] router[e][h], summed in fp64;
+ *   experts[t][0..k-1] = the experts of the k largest g[t], descending, the
+ *     lowest index of equal ones first, NaN above all; weights[t][j] = softmax
+ *     of their g over the k chosen (renormalize != 0) or over all E;
+ *   y[t] = sum_j weights[t][j] * down[e] (act(gate x[t]) * (up x[t])), gate and
+ *     up the first and last I rows of gate_up[e], e = experts[t][j].
+ * x [T][H], router [E][H], gate_up [E][2I][H] and down [E][H][I] have the last
+ * axis contiguous; for CMK_MX4 gate_up and down are the codes, with their
+ * scales, that cmk_mx4_quantize writes of matrices of 2I rows x H and H rows x I.
+ * y is dense [T][H], weights fp32 and experts int64 are dense [T][k].  Sums are
+ * held in fp32; act(..) * (..) is kept as two bf16 (16 bits of mantissa); y is
+ * rounded once.  Only the chosen experts' weights are read.
+ *
+ * `workspace`: cmk_moe_workspace_bytes(d) bytes, 256-byte aligned, not shared
+ * with a call that may run at the same time; 0 is returned for a descriptor that
+ * the call refuses.  No counterpart in the reference.
+ */
+int cmk_moe(const void* x, const void* router,
+            const void* gate_up, const uint8_t* gate_up_scales,
+            const void* down, const uint8_t* down_scales,
+            void* y, float* weights, long long* experts,
+            const cmk_moe_desc* d, void* workspace, size_t workspace_bytes,
+            void* stream);
+size_t cmk_moe_workspace_bytes(const cmk_moe_desc* d);
+
 /* Bytes of device workspace an operation needs (0 = none).  For
  * CMK_OP_TOPK_1D pass the array length in M (L = 1).  The work is cut for the
  * GPU that is current when this is called (its compute-unit count): call it

@@ -1,0 +1,247 @@
+"""Mixture-of-experts layer on the GPU against the formulas in 64 bits.
+
+The choice has one right answer.  Outputs: fp32 sums of H and I products are off
+by at most n * 2^-23 * sum |.| (any order, rounding or truncating adders), the
+activation by a few steps, the kept inner values by 2^-16 (two bf16; in front of
+fp16 weights, which are split too, the smallest of the four partial products is
+left out: 2^-16 more), y by half a step of its type.  The bound is carried through the
+formula in 64 bits, element by element."""
+import math
+
+import pytest
+import torch
+
+import _mx4
+from custom_matmul_kernels_amd import MoECUDA, quantize_mx4
+
+pytestmark = pytest.mark.gpu
+
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+U = 2.0 ** -23
+
+
+def make(t, h, i, e, dtype, seed, router_dtype=None):
+    gen = torch.Generator().manual_seed(seed)
+    x = torch.randn(t, h, generator=gen)
+    x[:, ::29] *= 8
+    return (x.to(dtype), (torch.randn(e, h, generator=gen) * h ** -0.5).to(router_dtype or dtype),
+            (torch.randn(e, 2 * i, h, generator=gen) * h ** -0.5).to(dtype),
+            (torch.randn(e, h, i, generator=gen) * i ** -0.5).to(dtype))
+
+
+def act64(g, name):
+    return g / (1 + torch.exp(-g)) if name == "silu" else g * 0.5 * (1 + torch.erf(g / math.sqrt(2)))
+
+
+def reference(x, router, gate_up, down, k, activation, renormalize):
+    """y, its error bound before the last rounding, weights, experts; all in float64."""
+    x, router, gate_up, down = (v.double() for v in (x, router, gate_up, down))
+    t, h = x.shape
+    i = down.shape[2]
+    score = torch.stack([(x[j] * router).sum(1) for j in range(t)])
+    experts = torch.sort(score, dim=1, descending=True, stable=True).indices[:, :k]
+    picked = score.gather(1, experts)
+    weights = torch.softmax(picked, 1) if renormalize else torch.softmax(score, 1).gather(1, experts)
+    spread = (picked - picked[:, :1]).abs()
+    d_weights = weights * (spread + 16 + score.shape[1]) * U
+    y, dy = torch.zeros(t, h, dtype=torch.float64), torch.zeros(t, h, dtype=torch.float64)
+    for e in experts.unique().tolist():
+        rows, j = (experts == e).nonzero(as_tuple=True)
+        G, V, D = gate_up[e, :i], gate_up[e, i:], down[e]
+        xr = x[rows]
+        g, v = xr @ G.t(), xr @ V.t()
+        # an fp16 x in front of 4-bit weights is two products an element
+        dg, dv = 2 * h * U * (xr.abs() @ G.abs().t()), 2 * h * U * (xr.abs() @ V.abs().t())
+        a = act64(g, activation)
+        da = 1.13 * dg + 8 * U * (a.abs() + g.abs())
+        m = a * v
+        dm = da * v.abs() + a.abs() * dv + da * dv + m.abs() * 2.0 ** -16
+        z = m @ D.t()
+        dz = dm @ D.abs().t() + (3 * i * U + 2.0 ** -16) * ((m.abs() + dm) @ D.abs().t())
+        w, dw = weights[rows, j][:, None], d_weights[rows, j][:, None]
+        y[rows] += w * z
+        dy[rows] += (w + dw) * dz + dw * z.abs() + k * U * w * z.abs()
+    return y, dy, weights, d_weights, experts
+
+
+def check(layer, x, router, gate_up, down, device, four_bit):
+    print("moe", tuple(x.shape), tuple(gate_up.shape), layer.k, x.dtype, "mx4" if four_bit else "plain", flush=True)
+    if four_bit:
+        gd, dd = quantize_mx4(gate_up.to(device)), quantize_mx4(down.to(device))
+        gate_up, down = _mx4.rounded(gate_up), _mx4.rounded(down)
+    else:
+        gd, dd = gate_up.to(device), down.to(device)
+    got = layer(x.to(device), router.to(device), gd, dd)
+    y, dy, weights, d_weights, experts = reference(x, router, gate_up, down, layer.k, layer.activation, layer.renormalize)
+    assert got[0].dtype == x.dtype and got[1].dtype == F32 and got[2].dtype == torch.int64
+    assert torch.equal(got[2].cpu(), experts)
+    assert ((got[1].cpu().double() - weights).abs() <= d_weights + 1e-37).all()
+    fi = torch.finfo(x.dtype)
+    bound = dy + (y.abs() + dy) * fi.eps / 2 + fi.smallest_normal * fi.eps
+    off = (got[0].cpu().double() - y).abs()
+    assert (off <= bound).all(), "off by %g of the bound" % (off / bound).max()
+    return got
+
+
+SHAPES = [(1, 64, 32, 4, 2), (1, 1, 1, 1, 1), (1, 100, 33, 10, 3), (2, 256, 130, 6, 6), (7, 1000, 333, 10, 3),
+          (16, 256, 128, 8, 2), (17, 130, 257, 70, 5), (70, 96, 48, 3, 3), (200, 72, 40, 2, 1), (40, 64, 64, 130, 8),
+          (5, 2048, 64, 33, 32), (3, 40, 1030, 9, 4)]
+
+
+@pytest.mark.parametrize("t,h,i,e,k", SHAPES)
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("four_bit", [False, True])
+def test_layer(device, t, h, i, e, k, dtype, four_bit):
+    check(MoECUDA(k=k), *make(t, h, i, e, dtype, t + h + i), device, four_bit)
+
+
+@pytest.mark.parametrize("activation", ["silu", "gelu"])
+@pytest.mark.parametrize("renormalize", [True, False])
+@pytest.mark.parametrize("router_dtype", [None, F32])
+def test_options(device, activation, renormalize, router_dtype):
+    for dtype, four_bit in ((BF16, False), (F16, True), (F16, False), (BF16, True)):
+        check(MoECUDA(k=3, activation=activation, renormalize=renormalize),
+              *make(9, 160, 70, 12, dtype, 3, router_dtype), device, four_bit)
+
+
+def test_more_tokens_than_one_call_takes(device):
+    check(MoECUDA(k=2), *make(300, 64, 32, 5, BF16, 1), device, False)
+    y, weights, experts = MoECUDA(k=2)(*(v.to(device) for v in make(0, 64, 32, 5, BF16, 1)))
+    assert y.shape == (0, 64) and weights.shape == (0, 2) and experts.shape == (0, 2)
+
+
+def test_equal_logits_go_to_the_lowest_index(device):
+    x, router, gate_up, down = make(6, 96, 40, 12, BF16, 5)
+    router[7] = router[2]
+    router[11] = router[2]
+    router[4] = router[9]
+    check(MoECUDA(k=7), x, router, gate_up, down, device, False)
+    router[:] = 0
+    got = check(MoECUDA(k=5), x, router, gate_up, down, device, True)
+    assert (got[2].cpu() == torch.arange(5)).all() and (got[1] == 0.2).all()
+
+
+def test_close_logits_are_ordered_exactly(device):
+    """Logits that differ by less than an fp32 sum could tell."""
+    x, router, gate_up, down = make(4, 512, 32, 16, BF16, 6)
+    router[:] = router[:1]
+    for e in range(16):
+        router[e, e * 31] += 2.0 ** -10 * ((e * 7) % 16 - 8)
+    check(MoECUDA(k=8), x, router, gate_up, down, device, False)
+
+
+@pytest.mark.parametrize("four_bit", [False, True])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_nan_and_infinity_stay_where_they_belong(device, four_bit, dtype):
+    x, router, gate_up, down = make(20, 200, 70, 9, dtype, 7)
+    layer = MoECUDA(k=3)
+    want = check(layer, x, router, gate_up, down, device, four_bit)
+    def run(x, gate_up, down):
+        if four_bit:
+            gate_up, down = quantize_mx4(gate_up.to(device)), quantize_mx4(down.to(device))
+        return layer(x.to(device), router.to(device), *(v if four_bit else v.to(device) for v in (gate_up, down)))
+    # a token with a NaN: its own row only; its choice is the first experts
+    x2 = x.clone()
+    x2[4, 17] = float("nan")
+    y, w, e = run(x2, gate_up, down)
+    assert torch.isnan(y[4]).all() and torch.isnan(w[4]).all() and e[4].tolist() == [0, 1, 2]
+    keep = torch.arange(20) != 4
+    assert torch.equal(y[keep], want[0][keep]) and torch.equal(e[keep], want[2][keep])
+    # an expert with a NaN: the rows that chose it only
+    bad = int(want[2][0, 0])
+    g2, d2 = gate_up.clone(), down.clone()
+    g2[bad, 5, 3] = float("nan")
+    d2[bad, 9, 2] = float("inf")
+    y, w, e = run(x, g2, d2)
+    hit = (want[2] == bad).any(1)
+    assert hit.any() and not hit.all()
+    assert torch.equal(y[~hit], want[0][~hit]) and torch.equal(e, want[2])
+    assert torch.isnan(y[hit]).all()
+
+
+def test_inner_values_beyond_fp16(device):
+    """act(g) * u of 1e6 and more: the layer's output still fits."""
+    x, router, gate_up, down = make(5, 64, 40, 4, F16, 8)
+    gate_up = (gate_up.float() * 500).half()
+    down = (down.float() * 2.0 ** -12).half()
+    check(MoECUDA(k=2), x, router, gate_up, down, device, False)
+    check(MoECUDA(k=2), x, router, gate_up, down, device, True)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_strided_operands(device, dtype):
+    x, router, gate_up, down = make(11, 130, 45, 6, dtype, 9)
+    layer = MoECUDA(k=2)
+    want = check(layer, x, router, gate_up, down, device, False)
+    def spread(v):     # rows and matrices apart from each other, at odd addresses
+        shape = list(v.shape)
+        shape[-1] += 5
+        shape[0] += 1
+        big = torch.full(shape, float("nan"), dtype=v.dtype, device=device)
+        view = big[1:, ..., 3:3 + v.shape[-1]]
+        view.copy_(v)
+        return view
+    got = layer(spread(x), spread(router), spread(gate_up), spread(down))
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    got = layer(x.t().contiguous().t().to(device), router.t().contiguous().t().to(device), gate_up.to(device), down.to(device))
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    # all experts the same matrix, not copied
+    one = check(layer, x, router, gate_up[:1].expand(6, 90, 130), down[:1].expand(6, 130, 45), device, False)
+    got = layer(x.to(device), router.to(device), gate_up[:1].to(device).expand(6, 90, 130), down[:1].to(device).expand(6, 130, 45))
+    assert torch.equal(got[0], one[0])
+
+
+@pytest.mark.parametrize("t", [1, 30])
+@pytest.mark.parametrize("four_bit", [False, True])
+def test_streams_and_graphs(device, t, four_bit):
+    x, router, gate_up, down = (v.to(device) for v in make(t, 192, 64, 16, BF16, 10))
+    if four_bit:
+        gate_up, down = quantize_mx4(gate_up), quantize_mx4(down)
+    layer = MoECUDA(k=4)
+    want = layer(x, router, gate_up, down)
+    torch.cuda.synchronize()
+    # two streams at once
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for _ in range(3):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(layer(x, router, gate_up, down))
+    torch.cuda.synchronize()
+    for g in got:
+        assert all(torch.equal(a, b) for a, b in zip(g, want))
+    # two graphs, replayed in turn with eager calls between
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = layer(x, router, gate_up, down)
+        graphs.append((graph, out))
+    gen = torch.Generator().manual_seed(0)
+    for step in range(4):
+        x.copy_(torch.randn(t, 192, generator=gen))
+        graph, out = graphs[step % 2]
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [v.clone() for v in out]
+        for a, b in zip(got, layer(x, router, gate_up, down)):
+            assert torch.equal(a, b), "replay %d differs" % step
+
+
+def test_a_run_of_the_operators_together(device):
+    """A decoding step as they would be used: a projection in 4 bits, the layer with
+    4-bit experts on its result, and a 4-bit projection back."""
+    from custom_matmul_kernels_amd import MX4BMMCUDA
+    gen = torch.Generator().manual_seed(11)
+    x = torch.randn(6, 96, generator=gen).to(BF16)
+    w_in, w_out = torch.randn(96, 160, generator=gen) / 10, torch.randn(160, 50, generator=gen) / 13
+    _, router, gate_up, down = make(6, 160, 64, 8, BF16, 12)
+    inner = MX4BMMCUDA(out_dtype=BF16)(x.to(device), quantize_mx4(w_in.to(device), dim=-2))
+    want = _mx4.rounded(x) @ _mx4.rounded(w_in.t()).t()
+    assert torch.equal(inner.cpu(), want.to(BF16)) or (inner.cpu().double() - want).abs().max() <= want.abs().max() * 2.0 ** -8
+    y, _, _ = check(MoECUDA(k=2), inner.cpu(), router, gate_up, down, device, True)
+    out = MX4BMMCUDA()(y, quantize_mx4(w_out.to(device), dim=-2))
+    a, b = _mx4.rounded(y), _mx4.rounded(w_out.t()).t()
+    assert ((out.cpu().double() - a @ b).abs() <= 160 * U * (a.abs() @ b.abs())).all()
