@@ -182,66 +182,206 @@ struct Mx4GemmArgs {
   int tiles_m, tiles_n;
 };
 
-// One work-group of four waves computes a 128 x 128 tile; a wave 64 x 64 of it.
-// The matrix instruction's first operand are the columns n of C, so that a lane
-// ends up with runs of four consecutive n of one row m.
-template <class T>
-__global__ __launch_bounds__(256) void mx4_gemm_kernel(Mx4GemmArgs a) {
-  constexpr int TM = 128, TN = 128;
-  __shared__ __attribute__((aligned(16))) uint8_t sa[TM * kSlabBytes], sb[TN * kSlabBytes];
-  __shared__ unsigned ssa[TM], ssb[TN];
+// A work-group of four waves computes a TM x TN tile of C, a wave a quarter of it
+// in blocks of 32 x 32 (v_mfma_scale_f32_32x32x64_f8f6f4: 64 elements of k, each
+// lane holding one whole 32-element block of one row, so that the lane's scale is
+// one byte).  The matrix instruction's first operand are the columns n of C: a
+// lane ends up with runs of four consecutive n of one row m.
+//
+// Slabs of both operands (codes and scales) travel by direct global-to-LDS loads
+// into a ring of kStages buffers, two slabs ahead of the products.  Half a slab's
+// fragments are in registers at a time; those of the next half are read while the
+// matrix pipe works on them.  The one barrier of a slab sits between its halves:
+// it follows the wait for the next slab, whose first half is read behind it, and
+// frees the buffer of the slab before.  Within a row the four 16-byte blocks are
+// stored at position block ^ ((row >> 2) & 3), so that the 16 rows that the LDS
+// serves at a time spread over all banks; the swizzle is produced by choosing
+// which block each lane of a load asks for.
+constexpr int kStages = 4;
+
+template <int TM, int TN>
+struct Mx4Tile {
+  static constexpr int BM = TM / 64, BN = TN / 64;  // 32 x 32 blocks of a wave
+  static constexpr int kCodesA = TM * kSlabBytes, kCodesB = TN * kSlabBytes;
+  static constexpr int kStageBytes = kCodesA + kCodesB + (TM + TN) * kSlabScales;
+  static constexpr int kLoads = TM / 64 + TN / 64 + 2;  // vector-memory instructions of a wave per slab
+};
+
+typedef const __attribute__((address_space(1))) void* gptr;
+typedef __attribute__((address_space(3))) void* lptr;
+
+// Waits until at most `left` of the wave's vector-memory instructions are under way.
+template <int left>
+__device__ __forceinline__ void wait_loads() {
+  static_assert(left < 64, "the counter has six bits");
+  __builtin_amdgcn_s_waitcnt(0x0f70 | (left & 15) | (left >> 4 << 14));
+}
+
+template <int v>
+struct Int {
+  static constexpr int value = v;
+};
+
+// The barrier of the work-group's waves; memory operations stay on their side of it.
+__device__ __forceinline__ void meet() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+template <class T, int TM, int TN>
+__global__ __launch_bounds__(256, 1) void mx4_gemm_kernel(Mx4GemmArgs a) {
+  using Tile = Mx4Tile<TM, TN>;
+  constexpr int BM = Tile::BM, BN = Tile::BN;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[kStages * Tile::kStageBytes];
   const int per_batch = a.tiles_m * a.tiles_n;
   const int l = blockIdx.x / per_batch;
   const int t = blockIdx.x - l * per_batch;
   const int m0 = t / a.tiles_n * TM, n0 = t % a.tiles_n * TN;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = (wave >> 1) * (TM / 2), wn = (wave & 1) * (TN / 2);
   const int r = lane & 31, h = lane >> 5;
-  f32x16 acc[2][2] = {};
-  for (int s = 0; s < a.slabs; ++s) {
-    const long long arow = ((long long)l * a.slabs + s) * a.M, brow = ((long long)l * a.slabs + s) * a.N;
-    __syncthreads();
+
+  // what this lane asks for: 16 rows x 64 bytes per instruction, rows beyond the
+  // matrix replaced by its last one
+  int oa[TM / 64], ob[TN / 64];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int c = threadIdx.x + 256 * i, row = c >> 2, part = c & 3;
-      const long long ra = arow + min(m0 + row, a.M - 1), rb = brow + min(n0 + row, a.N - 1);
-      *(u32x4v*)(sa + c * 16) = *(const u32x4v*)(a.a_codes + ra * kSlabBytes + part * 16);
-      *(u32x4v*)(sb + c * 16) = *(const u32x4v*)(a.b_codes + rb * kSlabBytes + part * 16);
-    }
-    if (threadIdx.x < 128) ssa[threadIdx.x] = *(const unsigned*)(a.a_scales + (arow + min(m0 + (int)threadIdx.x, a.M - 1)) * kSlabScales);
-    else ssb[threadIdx.x - 128] = *(const unsigned*)(a.b_scales + (brow + min(n0 + (int)threadIdx.x - 128, a.N - 1)) * kSlabScales);
-    __syncthreads();
-#pragma unroll
-    for (int g = 0; g < 2; ++g) {
-      i32x8 fm[2] = {}, fn[2] = {};
-      int cm[2], cn[2];
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        const u32x4v vm = *(const u32x4v*)(sa + (wm + b * 32 + r) * kSlabBytes + (2 * h + g) * 16);
-        const u32x4v vn = *(const u32x4v*)(sb + (wn + b * 32 + r) * kSlabBytes + (2 * h + g) * 16);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) { fm[b][i] = vm[i]; fn[b][i] = vn[i]; }
-        cm[b] = ssa[wm + b * 32 + r] >> (16 * h + 8 * g);
-        cn[b] = ssb[wn + b * 32 + r] >> (16 * h + 8 * g);
-      }
-#pragma unroll
-      for (int bn = 0; bn < 2; ++bn)
-#pragma unroll
-        for (int bm = 0; bm < 2; ++bm)
-          acc[bn][bm] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fn[bn], fm[bm], acc[bn][bm], 4, 4, 0, cn[bn], 0, cm[bm]);
-    }
+  for (int i = 0; i < TM / 64; ++i) {
+    const int row = (wave * (TM / 64) + i) * 16 + (lane >> 2);
+    oa[i] = min(row, a.M - 1 - m0) * kSlabBytes + ((lane & 3) ^ ((row >> 2) & 3)) * 16;
   }
-  T* c = (T*)a.c + (long long)l * a.M * a.N;
 #pragma unroll
-  for (int bm = 0; bm < 2; ++bm) {
+  for (int i = 0; i < TN / 64; ++i) {
+    const int row = (wave * (TN / 64) + i) * 16 + (lane >> 2);
+    ob[i] = min(row, a.N - 1 - n0) * kSlabBytes + ((lane & 3) ^ ((row >> 2) & 3)) * 16;
+  }
+  const int osa = min(wave * (TM / 4) + (lane & (TM / 4 - 1)), a.M - 1 - m0) * kSlabScales;
+  const int osb = min(wave * (TN / 4) + (lane & (TN / 4 - 1)), a.N - 1 - n0) * kSlabScales;
+  auto fetch = [&](int s) {
+    uint8_t* stage = lds + (s & (kStages - 1)) * Tile::kStageBytes;
+    const long long ra = ((long long)l * a.slabs + s) * a.M + m0, rb = ((long long)l * a.slabs + s) * a.N + n0;
+    const uint8_t* pa = a.a_codes + ra * kSlabBytes;
+    const uint8_t* pb = a.b_codes + rb * kSlabBytes;
+#pragma unroll
+    for (int i = 0; i < TM / 64; ++i)
+      __builtin_amdgcn_global_load_lds((gptr)(pa + oa[i]), (lptr)(stage + (wave * (TM / 64) + i) * 1024), 16, 0, 0);
+#pragma unroll
+    for (int i = 0; i < TN / 64; ++i)
+      __builtin_amdgcn_global_load_lds((gptr)(pb + ob[i]), (lptr)(stage + Tile::kCodesA + (wave * (TN / 64) + i) * 1024), 16, 0, 0);
+    uint8_t* scales = stage + Tile::kCodesA + Tile::kCodesB;
+    if (lane < TM / 4)
+      __builtin_amdgcn_global_load_lds((gptr)(a.a_scales + ra * kSlabScales + osa), (lptr)(scales + wave * TM), 4, 0, 0);
+    if (lane < TN / 4)
+      __builtin_amdgcn_global_load_lds((gptr)(a.b_scales + rb * kSlabScales + osb), (lptr)(scales + TM * kSlabScales + wave * TN), 4, 0, 0);
+  };
+
+  struct Half {
+    u32x4v m[BM], n[BN];
+  };
+  int cm[BM], cn[BN];  // scales of the slab: a lane's two blocks in the low bytes
+  const int swizzle = (r >> 2) & 3;
+  auto read = [&](int s, int g, Half& f) {
+    const uint8_t* stage = lds + (s & (kStages - 1)) * Tile::kStageBytes;
+    const uint8_t* pm = stage + (wm + r) * kSlabBytes + ((2 * h + g) ^ swizzle) * 16;
+    const uint8_t* pn = stage + Tile::kCodesA + (wn + r) * kSlabBytes + ((2 * h + g) ^ swizzle) * 16;
+#pragma unroll
+    for (int b = 0; b < BM; ++b) f.m[b] = *(const u32x4v*)(pm + b * 32 * kSlabBytes);
+#pragma unroll
+    for (int b = 0; b < BN; ++b) f.n[b] = *(const u32x4v*)(pn + b * 32 * kSlabBytes);
+  };
+  auto read_scales = [&](int s, int (&dm)[BM], int (&dn)[BN]) {
+    const uint8_t* scales = lds + (s & (kStages - 1)) * Tile::kStageBytes + Tile::kCodesA + Tile::kCodesB;
+#pragma unroll
+    for (int b = 0; b < BM; ++b) dm[b] = *(const unsigned short*)(scales + (wm + b * 32 + r) * kSlabScales + 2 * h);
+#pragma unroll
+    for (int b = 0; b < BN; ++b) dn[b] = *(const unsigned short*)(scales + (TM + wn + b * 32 + r) * kSlabScales + 2 * h);
+  };
+  f32x16 acc[BN][BM] = {};
+  auto wide = [](u32x4v v) { return i32x8{(int)v[0], (int)v[1], (int)v[2], (int)v[3], 0, 0, 0, 0}; };
+
+  // One slab.  Left: loads that may stay under way when the next slab is awaited,
+  // -1 if there is no next slab; Fetch: whether a slab is requested.
+  Half f0, f1;
+  auto slab = [&](int s, auto left, auto fetching) {
+    constexpr int Left = decltype(left)::value;
+    constexpr bool Fetch = decltype(fetching)::value;
+    read(s, 1, f1);
+#pragma unroll
+    for (int bn = 0; bn < BN; ++bn)
+#pragma unroll
+      for (int bm = 0; bm < BM; ++bm)
+        acc[bn][bm] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(f0.n[bn]), wide(f0.m[bm]), acc[bn][bm], 4, 4, 0, cn[bn], 0, cm[bm]);
+    // a read, then as many products as keep the matrix pipe busy until the next
+#pragma unroll
+    for (int i = 0; i < BM + BN; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, BM * BN / (BM + BN), 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    int dm[BM] = {}, dn[BN] = {};
+    if constexpr (Left >= 0) {
+      wait_loads<Left>();
+      meet();
+      if constexpr (Fetch) fetch(s + kStages - 1);
+      read(s + 1, 0, f0);
+      read_scales(s + 1, dm, dn);
+    }
+#pragma unroll
+    for (int bn = 0; bn < BN; ++bn)
+#pragma unroll
+      for (int bm = 0; bm < BM; ++bm)
+        acc[bn][bm] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(f1.n[bn]), wide(f1.m[bm]), acc[bn][bm], 4, 4, 1, cn[bn], 1, cm[bm]);
+#pragma unroll
+    for (int i = 0; i < BM + BN; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, BM * BN / (BM + BN), 0);
+      __builtin_amdgcn_sched_group_barrier(0x020, 2, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int b = 0; b < BM; ++b) cm[b] = dm[b];
+#pragma unroll
+    for (int b = 0; b < BN; ++b) cn[b] = dn[b];
+  };
+  const int slabs = a.slabs;
+  if (slabs > 0) {
+    fetch(0);
+    if (slabs > 1) fetch(1);
+    if (slabs > 2) { fetch(2); wait_loads<2 * Tile::kLoads>(); }
+    else if (slabs > 1) wait_loads<Tile::kLoads>();
+    else wait_loads<0>();
+    meet();
+    read(0, 0, f0);
+    read_scales(0, cm, cn);
+    int s = 0;
+    for (; s + 3 < slabs; ++s) slab(s, Int<Tile::kLoads>{}, Int<1>{});
+    if (s + 2 < slabs) { slab(s, Int<Tile::kLoads>{}, Int<0>{}); ++s; }
+    if (s + 1 < slabs) { slab(s, Int<0>{}, Int<0>{}); ++s; }
+    slab(s, Int<-1>{}, Int<0>{});
+  }
+
+  T* c = (T*)a.c + (long long)l * a.M * a.N;
+  const bool vec = (a.N & 3) == 0;
+#pragma unroll
+  for (int bm = 0; bm < BM; ++bm) {
     const int m = m0 + wm + bm * 32 + r;
     if (m >= a.M) continue;
 #pragma unroll
-    for (int bn = 0; bn < 2; ++bn)
+    for (int bn = 0; bn < BN; ++bn)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int n = n0 + wn + bn * 32 + 8 * (i >> 2) + 4 * h + (i & 3);
-        if (n < a.N) c[(long long)m * a.N + n] = from_f32<T>(acc[bn][bm][i]);
+      for (int i = 0; i < 4; ++i) {
+        const int n = n0 + wn + bn * 32 + 8 * i + 4 * h;
+        T* p = c + (long long)m * a.N + n;
+        T o[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[j] = from_f32<T>(acc[bn][bm][4 * i + j]);
+        if (n + 4 <= a.N && vec) {
+          __builtin_memcpy(p, o, sizeof(o));
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (n + j < a.N) p[j] = o[j];
+        }
       }
   }
 }
@@ -325,11 +465,16 @@ extern "C" int cmk_mx4_bmm(const uint8_t* a_codes, const uint8_t* a_scales, cons
   if (((reinterpret_cast<uintptr_t>(a_codes) | reinterpret_cast<uintptr_t>(b_codes)) & 15) ||
       ((reinterpret_cast<uintptr_t>(a_scales) | reinterpret_cast<uintptr_t>(b_scales)) & 3))
     return fail(CMK_ERR_INVALID_ARG, "cmk_mx4_bmm: codes need 16-byte alignment, scales 4-byte alignment");
-  Mx4GemmArgs a{a_codes, a_scales, b_codes, b_scales, C, L, M, N, (int)mx4_slabs(K), ceil_div(M, 128), ceil_div(N, 128)};
+  const bool large = (long long)L * ceil_div(M, 256) * ceil_div(N, 256) >= compute_units();
+  const int tile = large ? 256 : 128;
+  Mx4GemmArgs a{a_codes, a_scales, b_codes, b_scales, C, L, M, N, (int)mx4_slabs(K), ceil_div(M, tile), ceil_div(N, tile)};
   const long long grid = (long long)L * a.tiles_m * a.tiles_n;
   if (int e = check_grid(grid)) return e;
   hipStream_t st = (hipStream_t)stream;
   const dim3 g((unsigned)grid), b(256);
-  by_dtype(dtype, [&](auto t) { hipLaunchKernelGGL(mx4_gemm_kernel<decltype(t)>, g, b, 0, st, a); });
+  by_dtype(dtype, [&](auto t) {
+    if (large) hipLaunchKernelGGL((mx4_gemm_kernel<decltype(t), 256, 256>), g, b, 0, st, a);
+    else hipLaunchKernelGGL((mx4_gemm_kernel<decltype(t), 128, 128>), g, b, 0, st, a);
+  });
   return hip_status(hipGetLastError(), "cmk_mx4_bmm launch");
 }
