@@ -185,8 +185,7 @@ struct Mx4GemmArgs {
 // A work-group of four waves computes a TM x TN tile of C, a wave a quarter of it
 // in blocks of 32 x 32 (v_mfma_scale_f32_32x32x64_f8f6f4: 64 elements of k, each
 // lane holding one whole 32-element block of one row, so that the lane's scale is
-// one byte).  The matrix instruction's first operand are the columns n of C: a
-// lane ends up with runs of four consecutive n of one row m.
+// one byte).
 //
 // Slabs of both operands (codes and scales) travel by direct global-to-LDS loads
 // into a ring of kStages buffers, two slabs ahead of the products.  Half a slab's
@@ -229,22 +228,37 @@ __device__ __forceinline__ void meet() {
   asm volatile("" ::: "memory");
 }
 
+// Work-groups go round the eight XCDs in turn, each with an L2 of its own: an XCD
+// gets a contiguous run of the tiles of all batches, in strips of eight tile rows,
+// so that what runs on it at a time shares few panels of both operands.
+__device__ __forceinline__ void place_tile(const Mx4GemmArgs& a, int& l, int& tile_m, int& tile_n) {
+  const int total = gridDim.x, xcd = blockIdx.x & 7, turn = blockIdx.x >> 3;
+  const int each = total >> 3, extra = total & 7;
+  const int id = xcd * each + min(xcd, extra) + turn;
+  const int per_batch = a.tiles_m * a.tiles_n;
+  l = id / per_batch;
+  const int t = id - l * per_batch;
+  const int strip = t / (8 * a.tiles_n), in = t - strip * 8 * a.tiles_n;
+  const int height = min(8, a.tiles_m - strip * 8);
+  tile_m = strip * 8 + in % height;
+  tile_n = in / height;
+}
+
 template <class T, int TM, int TN>
 __global__ __launch_bounds__(256, 1) void mx4_gemm_kernel(Mx4GemmArgs a) {
   using Tile = Mx4Tile<TM, TN>;
   constexpr int BM = Tile::BM, BN = Tile::BN;
   __shared__ __attribute__((aligned(16))) uint8_t lds[kStages * Tile::kStageBytes];
-  const int per_batch = a.tiles_m * a.tiles_n;
-  const int l = blockIdx.x / per_batch;
-  const int t = blockIdx.x - l * per_batch;
-  const int m0 = t / a.tiles_n * TM, n0 = t % a.tiles_n * TN;
+  int l, tile_m, tile_n;
+  place_tile(a, l, tile_m, tile_n);
+  const int m0 = tile_m * TM, n0 = tile_n * TN;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = (wave >> 1) * (TM / 2), wn = (wave & 1) * (TN / 2);
   const int r = lane & 31, h = lane >> 5;
 
   // what this lane asks for: 16 rows x 64 bytes per instruction, rows beyond the
   // matrix replaced by its last one
-  int oa[TM / 64], ob[TN / 64];
+  unsigned oa[TM / 64], ob[TN / 64];
 #pragma unroll
   for (int i = 0; i < TM / 64; ++i) {
     const int row = (wave * (TM / 64) + i) * 16 + (lane >> 2);
@@ -255,62 +269,96 @@ __global__ __launch_bounds__(256, 1) void mx4_gemm_kernel(Mx4GemmArgs a) {
     const int row = (wave * (TN / 64) + i) * 16 + (lane >> 2);
     ob[i] = min(row, a.N - 1 - n0) * kSlabBytes + ((lane & 3) ^ ((row >> 2) & 3)) * 16;
   }
-  const int osa = min(wave * (TM / 4) + (lane & (TM / 4 - 1)), a.M - 1 - m0) * kSlabScales;
-  const int osb = min(wave * (TN / 4) + (lane & (TN / 4 - 1)), a.N - 1 - n0) * kSlabScales;
-  auto fetch = [&](int s) {
-    uint8_t* stage = lds + (s & (kStages - 1)) * Tile::kStageBytes;
-    const long long ra = ((long long)l * a.slabs + s) * a.M + m0, rb = ((long long)l * a.slabs + s) * a.N + n0;
-    const uint8_t* pa = a.a_codes + ra * kSlabBytes;
-    const uint8_t* pb = a.b_codes + rb * kSlabBytes;
+  unsigned osa = min(wave * (TM / 4) + (lane & (TM / 4 - 1)), a.M - 1 - m0) * kSlabScales;
+  unsigned osb = min(wave * (TN / 4) + (lane & (TN / 4 - 1)), a.N - 1 - n0) * kSlabScales;
+  // The next slab to be requested.  Beyond the last one the requests repeat it, so
+  // that every slab of the loop issues and awaits the same number of loads.
+  const uint8_t* pa = a.a_codes + ((long long)l * a.slabs * a.M + m0) * kSlabBytes;
+  const uint8_t* pb = a.b_codes + ((long long)l * a.slabs * a.N + n0) * kSlabBytes;
+  const uint8_t* psa = a.a_scales + ((long long)l * a.slabs * a.M + m0) * kSlabScales;
+  const uint8_t* psb = a.b_scales + ((long long)l * a.slabs * a.N + n0) * kSlabScales;
+  const long long step_a = (long long)a.M * kSlabBytes, step_b = (long long)a.N * kSlabBytes;
+  int requested = 0;
+  // scalar base + 32-bit lane offset, no vector addition
+  auto load16 = [&](const uint8_t* base, unsigned& off, uint8_t* to) {
+    asm volatile("" : "+s"(base));
+    asm volatile("" : "+v"(off));
+    __builtin_amdgcn_global_load_lds((gptr)(base + off), (lptr)to, 16, 0, 0);
+  };
+  auto load4 = [&](const uint8_t* base, unsigned& off, uint8_t* to) {
+    asm volatile("" : "+s"(base));
+    asm volatile("" : "+v"(off));
+    __builtin_amdgcn_global_load_lds((gptr)(base + off), (lptr)to, 4, 0, 0);
+  };
+  auto fetch = [&](int stage) {
+    uint8_t* at = lds + stage * Tile::kStageBytes;
 #pragma unroll
-    for (int i = 0; i < TM / 64; ++i)
-      __builtin_amdgcn_global_load_lds((gptr)(pa + oa[i]), (lptr)(stage + (wave * (TM / 64) + i) * 1024), 16, 0, 0);
+    for (int i = 0; i < TM / 64; ++i) load16(pa, oa[i], at + (wave * (TM / 64) + i) * 1024);
 #pragma unroll
-    for (int i = 0; i < TN / 64; ++i)
-      __builtin_amdgcn_global_load_lds((gptr)(pb + ob[i]), (lptr)(stage + Tile::kCodesA + (wave * (TN / 64) + i) * 1024), 16, 0, 0);
-    uint8_t* scales = stage + Tile::kCodesA + Tile::kCodesB;
-    if (lane < TM / 4)
-      __builtin_amdgcn_global_load_lds((gptr)(a.a_scales + ra * kSlabScales + osa), (lptr)(scales + wave * TM), 4, 0, 0);
-    if (lane < TN / 4)
-      __builtin_amdgcn_global_load_lds((gptr)(a.b_scales + rb * kSlabScales + osb), (lptr)(scales + TM * kSlabScales + wave * TN), 4, 0, 0);
+    for (int i = 0; i < TN / 64; ++i) load16(pb, ob[i], at + Tile::kCodesA + (wave * (TN / 64) + i) * 1024);
+    uint8_t* scales = at + Tile::kCodesA + Tile::kCodesB;
+    if (TM == 256 || lane < TM / 4) load4(psa, osa, scales + wave * TM);
+    if (TN == 256 || lane < TN / 4) load4(psb, osb, scales + TM * kSlabScales + wave * TN);
+    const long long more = ++requested < a.slabs ? 1 : 0;
+    pa += more * step_a; pb += more * step_b;
+    psa += more * (step_a / (kSlabBytes / kSlabScales)); psb += more * (step_b / (kSlabBytes / kSlabScales));
   };
 
+  // Where this lane reads: one register per half of a slab, operand and pair of
+  // stages, the rest of an address is the instruction's offset (vector
+  // instructions in the loop cost matrix-pipe time).
+  const unsigned lds0 = (unsigned)(uintptr_t)(lptr)lds;
+  unsigned at_m[2][2], at_n[2][2], at_cm[2], at_cn[2];
+#pragma unroll
+  for (int pair = 0; pair < 2; ++pair) {
+    const unsigned base = lds0 + pair * 2 * Tile::kStageBytes;
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      const unsigned part = ((2 * h + g) ^ ((r >> 2) & 3)) * 16;
+      at_m[pair][g] = base + (wm + r) * kSlabBytes + part;
+      at_n[pair][g] = base + Tile::kCodesA + (wn + r) * kSlabBytes + part;
+      asm("" : "+v"(at_m[pair][g]), "+v"(at_n[pair][g]));
+    }
+    at_cm[pair] = base + Tile::kCodesA + Tile::kCodesB + (wm + r) * kSlabScales + 2 * h;
+    at_cn[pair] = base + Tile::kCodesA + Tile::kCodesB + (TM + wn + r) * kSlabScales + 2 * h;
+    asm("" : "+v"(at_cm[pair]), "+v"(at_cn[pair]));
+  }
   struct Half {
     u32x4v m[BM], n[BN];
   };
-  int cm[BM], cn[BN];  // scales of the slab: a lane's two blocks in the low bytes
-  const int swizzle = (r >> 2) & 3;
-  auto read = [&](int s, int g, Half& f) {
-    const uint8_t* stage = lds + (s & (kStages - 1)) * Tile::kStageBytes;
-    const uint8_t* pm = stage + (wm + r) * kSlabBytes + ((2 * h + g) ^ swizzle) * 16;
-    const uint8_t* pn = stage + Tile::kCodesA + (wn + r) * kSlabBytes + ((2 * h + g) ^ swizzle) * 16;
-#pragma unroll
-    for (int b = 0; b < BM; ++b) f.m[b] = *(const u32x4v*)(pm + b * 32 * kSlabBytes);
-#pragma unroll
-    for (int b = 0; b < BN; ++b) f.n[b] = *(const u32x4v*)(pn + b * 32 * kSlabBytes);
+  struct Scales {
+    int m[BM], n[BN];  // a lane's two blocks of the slab in the low bytes
   };
-  auto read_scales = [&](int s, int (&dm)[BM], int (&dn)[BN]) {
-    const uint8_t* scales = lds + (s & (kStages - 1)) * Tile::kStageBytes + Tile::kCodesA + Tile::kCodesB;
+  typedef const __attribute__((address_space(3))) u32x4v* l16;
+  typedef const __attribute__((address_space(3))) unsigned short* l2;
+  auto read = [&](int stage, int g, Half& f) {
+    const unsigned off = (stage & 1) * Tile::kStageBytes;
 #pragma unroll
-    for (int b = 0; b < BM; ++b) dm[b] = *(const unsigned short*)(scales + (wm + b * 32 + r) * kSlabScales + 2 * h);
+    for (int b = 0; b < BM; ++b) f.m[b] = *(l16)(lptr)(uintptr_t)(at_m[stage >> 1][g] + off + b * 32 * kSlabBytes);
 #pragma unroll
-    for (int b = 0; b < BN; ++b) dn[b] = *(const unsigned short*)(scales + (TM + wn + b * 32 + r) * kSlabScales + 2 * h);
+    for (int b = 0; b < BN; ++b) f.n[b] = *(l16)(lptr)(uintptr_t)(at_n[stage >> 1][g] + off + b * 32 * kSlabBytes);
   };
-  f32x16 acc[BN][BM] = {};
+  auto read_scales = [&](int stage, Scales& c) {
+    const unsigned off = (stage & 1) * Tile::kStageBytes;
+#pragma unroll
+    for (int b = 0; b < BM; ++b) c.m[b] = *(l2)(lptr)(uintptr_t)(at_cm[stage >> 1] + off + b * 32 * kSlabScales);
+#pragma unroll
+    for (int b = 0; b < BN; ++b) c.n[b] = *(l2)(lptr)(uintptr_t)(at_cn[stage >> 1] + off + b * 32 * kSlabScales);
+  };
+  f32x16 acc[BM][BN] = {};
   auto wide = [](u32x4v v) { return i32x8{(int)v[0], (int)v[1], (int)v[2], (int)v[3], 0, 0, 0, 0}; };
 
-  // One slab.  Left: loads that may stay under way when the next slab is awaited,
-  // -1 if there is no next slab; Fetch: whether a slab is requested.
+  // One slab of ring position `stage`, c its scales, d the next one's.
   Half f0, f1;
-  auto slab = [&](int s, auto left, auto fetching) {
-    constexpr int Left = decltype(left)::value;
-    constexpr bool Fetch = decltype(fetching)::value;
-    read(s, 1, f1);
+  auto slab = [&](auto stage, Scales& c, Scales& d) {
+    constexpr int Stage = decltype(stage)::value;
+    constexpr int Next = (Stage + 1) % kStages;
+    read(Stage, 1, f1);
 #pragma unroll
-    for (int bn = 0; bn < BN; ++bn)
+    for (int bm = 0; bm < BM; ++bm)
 #pragma unroll
-      for (int bm = 0; bm < BM; ++bm)
-        acc[bn][bm] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(f0.n[bn]), wide(f0.m[bm]), acc[bn][bm], 4, 4, 0, cn[bn], 0, cm[bm]);
+      for (int bn = 0; bn < BN; ++bn)
+        acc[bm][bn] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(f0.m[bm]), wide(f0.n[bn]), acc[bm][bn], 4, 4, 0, c.m[bm], 0, c.n[bn]);
     // a read, then as many products as keep the matrix pipe busy until the next
 #pragma unroll
     for (int i = 0; i < BM + BN; ++i) {
@@ -318,72 +366,67 @@ __global__ __launch_bounds__(256, 1) void mx4_gemm_kernel(Mx4GemmArgs a) {
       __builtin_amdgcn_sched_group_barrier(0x008, BM * BN / (BM + BN), 0);
     }
     __builtin_amdgcn_sched_barrier(0);
-    int dm[BM] = {}, dn[BN] = {};
-    if constexpr (Left >= 0) {
-      wait_loads<Left>();
-      meet();
-      if constexpr (Fetch) fetch(s + kStages - 1);
-      read(s + 1, 0, f0);
-      read_scales(s + 1, dm, dn);
-    }
+    wait_loads<Tile::kLoads>();
+    meet();
+    read_scales(Next, d);
+    read(Next, 0, f0);
+    fetch((Stage + kStages - 1) % kStages);
 #pragma unroll
-    for (int bn = 0; bn < BN; ++bn)
+    for (int bm = 0; bm < BM; ++bm)
 #pragma unroll
-      for (int bm = 0; bm < BM; ++bm)
-        acc[bn][bm] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(f1.n[bn]), wide(f1.m[bm]), acc[bn][bm], 4, 4, 1, cn[bn], 1, cm[bm]);
+      for (int bn = 0; bn < BN; ++bn)
+        acc[bm][bn] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(f1.m[bm]), wide(f1.n[bn]), acc[bm][bn], 4, 4, 1, c.m[bm], 1, c.n[bn]);
+    // what the next slab starts with first, the requests behind it
 #pragma unroll
     for (int i = 0; i < BM + BN; ++i) {
-      __builtin_amdgcn_sched_group_barrier(0x008, BM * BN / (BM + BN), 0);
-      __builtin_amdgcn_sched_group_barrier(0x020, 2, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, BM * BN / 2 / (BM + BN), 0);
       __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
     }
+#pragma unroll
+    for (int i = 0; i < Tile::kLoads; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    }
     __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int b = 0; b < BM; ++b) cm[b] = dm[b];
-#pragma unroll
-    for (int b = 0; b < BN; ++b) cn[b] = dn[b];
   };
-  const int slabs = a.slabs;
-  if (slabs > 0) {
+  if (a.slabs > 0) {
+    Scales c0, c1;
     fetch(0);
-    if (slabs > 1) fetch(1);
-    if (slabs > 2) { fetch(2); wait_loads<2 * Tile::kLoads>(); }
-    else if (slabs > 1) wait_loads<Tile::kLoads>();
-    else wait_loads<0>();
+    fetch(1);
+    fetch(2);
+    wait_loads<2 * Tile::kLoads>();
     meet();
+    read_scales(0, c0);
     read(0, 0, f0);
-    read_scales(0, cm, cn);
-    int s = 0;
-    for (; s + 3 < slabs; ++s) slab(s, Int<Tile::kLoads>{}, Int<1>{});
-    if (s + 2 < slabs) { slab(s, Int<Tile::kLoads>{}, Int<0>{}); ++s; }
-    if (s + 1 < slabs) { slab(s, Int<0>{}, Int<0>{}); ++s; }
-    slab(s, Int<-1>{}, Int<0>{});
+    int left = a.slabs;
+    for (; left >= 4; left -= 4) {
+      slab(Int<0>{}, c0, c1);
+      slab(Int<1>{}, c1, c0);
+      slab(Int<2>{}, c0, c1);
+      slab(Int<3>{}, c1, c0);
+    }
+    if (left > 0) slab(Int<0>{}, c0, c1);
+    if (left > 1) slab(Int<1>{}, c1, c0);
+    if (left > 2) slab(Int<2>{}, c0, c1);
+    wait_loads<0>();  // no load may land after the work-group has ended
   }
 
+  // lane: column n = lane & 31, rows 8 * (i / 4) + 4 * h + i % 4: a store covers two
+  // runs of 32 columns
   T* c = (T*)a.c + (long long)l * a.M * a.N;
-  const bool vec = (a.N & 3) == 0;
 #pragma unroll
-  for (int bm = 0; bm < BM; ++bm) {
-    const int m = m0 + wm + bm * 32 + r;
-    if (m >= a.M) continue;
+  for (int bm = 0; bm < BM; ++bm)
 #pragma unroll
-    for (int bn = 0; bn < BN; ++bn)
+    for (int i = 0; i < 16; ++i) {
+      const int m = m0 + wm + bm * 32 + 8 * (i >> 2) + 4 * h + (i & 3);
+      if (m >= a.M) continue;
+      T* row = c + (long long)m * a.N;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int n = n0 + wn + bn * 32 + 8 * i + 4 * h;
-        T* p = c + (long long)m * a.N + n;
-        T o[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) o[j] = from_f32<T>(acc[bn][bm][4 * i + j]);
-        if (n + 4 <= a.N && vec) {
-          __builtin_memcpy(p, o, sizeof(o));
-        } else {
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (n + j < a.N) p[j] = o[j];
-        }
+      for (int bn = 0; bn < BN; ++bn) {
+        const int n = n0 + wn + bn * 32 + r;
+        if (n < a.N) row[n] = from_f32<T>(acc[bm][bn][i]);
       }
-  }
+    }
 }
 
 static int check_mx4(const char* who, int L, int R, int K) {
