@@ -35,6 +35,7 @@ EXPORTS = (
     "cmk_mx4_quantize",
     "cmk_mx4_dequantize",
     "cmk_mx4_bmm",
+    "cmk_mx4_bmm_rows",
     "cmk_moe",
     "cmk_moe_workspace_bytes",
     "cmk_workspace_bytes",
@@ -118,13 +119,14 @@ def load():
     lib.cmk_mx4_quantize.argtypes = [p, i, p, p, i, i, i, ll, ll, ll, p]
     lib.cmk_mx4_dequantize.argtypes = [p, p, p, i, i, i, i, i, p]
     lib.cmk_mx4_bmm.argtypes = [p, p, p, p, p, i, i, i, i, i, p]
+    lib.cmk_mx4_bmm_rows.argtypes = [p, i, ll, ll, p, p, p, i, i, i, i, i, p]
     mp = ctypes.POINTER(MoeDesc)
     lib.cmk_moe.argtypes = [p, p, p, p, p, p, p, p, p, mp, p, sz, p]
     lib.cmk_moe_workspace_bytes.argtypes = [mp]
     lib.cmk_moe_workspace_bytes.restype = sz
     for name in ("cmk_bmm_f32", "cmk_bmm_ws_f32", "cmk_mbmm_f32", "cmk_derive_masks_u8", "cmk_min_bmm_f32", "cmk_min_bmm_f32_static",
                  "cmk_topk_bmm_f32", "cmk_topk_1d_f32", "cmk_mx4_quantize", "cmk_mx4_dequantize",
-                 "cmk_mx4_bmm", "cmk_moe"):
+                 "cmk_mx4_bmm", "cmk_mx4_bmm_rows", "cmk_moe"):
         getattr(lib, name).restype = i
     lib.cmk_workspace_bytes.argtypes = [i, i, i, i, i, i]
     lib.cmk_workspace_bytes.restype = sz

@@ -16,7 +16,6 @@ constexpr int kMoeExperts = 1024;
 constexpr int kMoeChoices = 32;
 
 typedef double f64x4 __attribute__((ext_vector_type(4)));
-typedef unsigned short u16;
 
 // Pieces of the workspace, each 256-byte aligned.
 struct MoePlan {
@@ -83,9 +82,9 @@ __global__ __launch_bounds__(512) void moe_logits_kernel(MoeArgs a) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         if constexpr (PLANES == 1) {
-          hi[i] = __builtin_bit_cast(u16, ox.v[i]);
+          hi[i] = ox.bits(i);
         } else {
-          const float f = (float)ox.v[i];
+          const float f = ox.get(i);
           const __bf16 b = (__bf16)f;
           hi[i] = __builtin_bit_cast(u16, b);
           // an infinity or a NaN stays in the first plane alone
@@ -97,7 +96,7 @@ __global__ __launch_bounds__(512) void moe_logits_kernel(MoeArgs a) {
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)(float)ow.v[i], (double)(float)ox.v[i], acc, 0, 0, 0);
+      acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)ow.get(i), (double)ox.get(i), acc, 0, 0, 0);
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) part[wave][lane][i] = acc[i];

@@ -69,7 +69,7 @@ __global__ __launch_bounds__(256) void mx4_quantize_columns_kernel(QuantArgs a) 
     Octet<T> o[4];
 #pragma unroll
     for (int i = 0; i < 32; ++i)
-      o[i >> 3].v[i & 7] = k0 + i < a.K ? x[(k0 + i) * a.sk] : (T)0.0f;
+      o[i >> 3].set(i & 7, k0 + i < a.K ? x[(k0 + i) * a.sk] : (T)0.0f);
     const unsigned top = max(max(o[0].top(), o[1].top()), max(o[2].top(), o[3].top()));
     const unsigned s = scale_byte(top);
     const float f = scale_float(s);
@@ -429,6 +429,145 @@ __global__ __launch_bounds__(256, 1) void mx4_gemm_kernel(Mx4GemmArgs a) {
     }
 }
 
+// ------------------------------------------------------- product with few rows
+
+struct Mx4RowsArgs {
+  const void* x;  // the left operand: codes, or elements with k contiguous
+  const uint8_t *x_scales, *b_codes, *b_scales;
+  void* c;
+  int M, N, K, slabs;
+  long long sl, sm;  // strides of x in elements
+};
+
+// A lane's share of one slab of 16 rows: 32 elements of row lane & 15, those of
+// block lane >> 4, as the 16x16x128 instruction takes them.
+struct Mx4Fragment {
+  u32x4v codes;
+  int scale;
+};
+
+__device__ __forceinline__ void load_fragment(Mx4Fragment& f, const uint8_t* codes, const uint8_t* scales, long long at, int q) {
+  f.codes = *(const u32x4v*)(codes + at * kSlabBytes + q * 16);
+  f.scale = scales[at * kSlabScales + q];
+}
+
+// Quantises 32 elements in one lane.
+template <class T>
+__device__ __forceinline__ void quantize_fragment(Mx4Fragment& f, const Octet<T> (&o)[4]) {
+  const unsigned s = scale_byte(max(max(o[0].top(), o[1].top()), max(o[2].top(), o[3].top())));
+  const float scale = scale_float(s);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f.codes[i] = s == 255u ? 0u : o[i].codes(scale);
+  f.scale = (int)s;
+}
+
+// A work-group takes 16 * RG columns of C and all its rows (up to 16 * MB); its
+// waves split the slabs and their sums meet in LDS, in the order of the waves.
+// There is nothing to gain but the stream of the right operand: its fragments
+// (1 KB of contiguous codes per instruction) go straight to registers, U slabs at
+// a time.  TX: the left operand's elements, quantised on the way, or uint8_t for
+// codes.
+template <class TX, class T, int W, int RG, int MB, int U>
+__global__ __launch_bounds__(64 * W) void mx4_rows_kernel(Mx4RowsArgs a) {
+  constexpr bool kCodes = sizeof(TX) == 1;
+  __shared__ float part[W][RG][MB][64][4];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r = lane & 15, q = lane >> 4;
+  const int l = blockIdx.y, n0 = blockIdx.x * 16 * RG;
+  const long long batch_b = (long long)l * a.slabs * a.N;
+  int row[RG];
+#pragma unroll
+  for (int g = 0; g < RG; ++g) row[g] = min(n0 + g * 16 + r, a.N - 1);
+  f32x4 acc[RG][MB] = {};
+  auto wide = [](u32x4v v) { return i32x8{(int)v[0], (int)v[1], (int)v[2], (int)v[3], 0, 0, 0, 0}; };
+  for (int s0 = wave; s0 < a.slabs; s0 += W * U) {
+    Mx4Fragment fb[U][RG], fx[U][MB];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int s = s0 + u * W;
+      if (s >= a.slabs) break;
+#pragma unroll
+      for (int g = 0; g < RG; ++g) load_fragment(fb[u][g], a.b_codes, a.b_scales, batch_b + (long long)s * a.N + row[g], q);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int s = s0 + u * W;
+      if (s >= a.slabs) break;
+#pragma unroll
+      for (int b = 0; b < MB; ++b) {
+        if constexpr (kCodes) {
+          const int m = min(b * 16 + r, a.M - 1);
+          load_fragment(fx[u][b], (const uint8_t*)a.x, a.x_scales, ((long long)l * a.slabs + s) * a.M + m, q);
+        } else {
+          const int m = b * 16 + r, k = s * kSlab + q * 32;
+          const TX* x = (const TX*)a.x + l * a.sl + m * a.sm + k;
+          Octet<TX> o[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[i] = load_octet(x + i * 8, m < a.M ? a.K - k - i * 8 : 0);
+          quantize_fragment(fx[u][b], o);
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (s0 + u * W >= a.slabs) break;
+#pragma unroll
+      for (int g = 0; g < RG; ++g)
+#pragma unroll
+        for (int b = 0; b < MB; ++b)
+          acc[g][b] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wide(fb[u][g].codes), wide(fx[u][b].codes), acc[g][b], 4, 4, 0,
+                                                                      fb[u][g].scale, 0, fx[u][b].scale);
+    }
+  }
+#pragma unroll
+  for (int g = 0; g < RG; ++g)
+#pragma unroll
+    for (int b = 0; b < MB; ++b)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) part[wave][g][b][lane][i] = acc[g][b][i];
+  __syncthreads();
+  T* c = (T*)a.c + (long long)l * a.M * a.N;
+  for (int v = threadIdx.x; v < RG * MB * 256; v += 64 * W) {
+    // neighbouring threads take neighbouring columns of one row
+    const int n = v % (16 * RG), m = v / (16 * RG);
+    const int g = n >> 4, i = n & 3, from = ((n & 15) >> 2) * 16 + (m & 15), b = m >> 4;
+    if (m < a.M && n0 + n < a.N) {
+      float sum = 0;
+#pragma unroll
+      for (int w = 0; w < W; ++w) sum += part[w][g][b][from][i];
+      c[(long long)m * a.N + n0 + n] = from_f32<T>(sum);
+    }
+  }
+}
+
+// Rows up to this many are served by mx4_rows_kernel.
+constexpr int kMx4Rows = 64;
+// and up to this many with the left operand quantised on the way
+constexpr int kMx4RowsFloat = 16;
+
+// TX: uint8_t or the element type of the left operand.
+template <class TX, class T>
+static void launch_rows(const Mx4RowsArgs& a, int L, hipStream_t st) {
+  const long long groups = (long long)ceil_div(a.N, 16) * L;
+  // Four row groups a wave share one fragment of the left operand; one each where
+  // that would leave compute units without work.
+  const bool many = groups >= 4LL * compute_units();
+  auto grid = [&](int rg) { return dim3(ceil_div(a.N, 16 * rg), L); };
+  if (a.M <= 16) {
+    if (many) hipLaunchKernelGGL((mx4_rows_kernel<TX, T, 8, 4, 1, 2>), grid(4), dim3(512), 0, st, a);
+    else if (a.slabs > 32) hipLaunchKernelGGL((mx4_rows_kernel<TX, T, 16, 1, 1, 4>), grid(1), dim3(1024), 0, st, a);
+    else hipLaunchKernelGGL((mx4_rows_kernel<TX, T, 8, 1, 1, 4>), grid(1), dim3(512), 0, st, a);
+  } else if constexpr (sizeof(TX) == 1) {
+    if (a.M <= 32) {
+      if (many) hipLaunchKernelGGL((mx4_rows_kernel<TX, T, 8, 4, 2, 2>), grid(4), dim3(512), 0, st, a);
+      else hipLaunchKernelGGL((mx4_rows_kernel<TX, T, 8, 1, 2, 4>), grid(1), dim3(512), 0, st, a);
+    } else {
+      if (many) hipLaunchKernelGGL((mx4_rows_kernel<TX, T, 8, 2, 4, 2>), grid(2), dim3(512), 0, st, a);
+      else hipLaunchKernelGGL((mx4_rows_kernel<TX, T, 8, 1, 4, 2>), grid(1), dim3(512), 0, st, a);
+    }
+  }
+}
+
 static int check_mx4(const char* who, int L, int R, int K) {
   if (L < 0 || R < 0 || K < 0) return fail(CMK_ERR_INVALID_ARG, "%s: negative extent (L=%d R=%d K=%d)", who, L, R, K);
   return CMK_OK;
@@ -508,6 +647,11 @@ extern "C" int cmk_mx4_bmm(const uint8_t* a_codes, const uint8_t* a_scales, cons
   if (((reinterpret_cast<uintptr_t>(a_codes) | reinterpret_cast<uintptr_t>(b_codes)) & 15) ||
       ((reinterpret_cast<uintptr_t>(a_scales) | reinterpret_cast<uintptr_t>(b_scales)) & 3))
     return fail(CMK_ERR_INVALID_ARG, "cmk_mx4_bmm: codes need 16-byte alignment, scales 4-byte alignment");
+  if (M <= kMx4Rows && L <= 65535) {
+    const Mx4RowsArgs r{a_codes, a_scales, b_codes, b_scales, C, M, N, K, (int)mx4_slabs(K), 0, 0};
+    by_dtype(dtype, [&](auto t) { launch_rows<uint8_t, decltype(t)>(r, L, (hipStream_t)stream); });
+    return hip_status(hipGetLastError(), "cmk_mx4_bmm launch");
+  }
   const bool large = (long long)L * ceil_div(M, 256) * ceil_div(N, 256) >= compute_units();
   const int tile = large ? 256 : 128;
   Mx4GemmArgs a{a_codes, a_scales, b_codes, b_scales, C, L, M, N, (int)mx4_slabs(K), ceil_div(M, tile), ceil_div(N, tile)};
@@ -520,4 +664,23 @@ extern "C" int cmk_mx4_bmm(const uint8_t* a_codes, const uint8_t* a_scales, cons
     else hipLaunchKernelGGL((mx4_gemm_kernel<decltype(t), 128, 128>), g, b, 0, st, a);
   });
   return hip_status(hipGetLastError(), "cmk_mx4_bmm launch");
+}
+
+extern "C" int cmk_mx4_bmm_rows(const void* x, int x_dtype, long long stride_l, long long stride_m, const uint8_t* b_codes,
+                                const uint8_t* b_scales, void* C, int dtype, int L, int M, int N, int K, void* stream) {
+  if (L < 0 || M < 0 || N < 0 || K < 0)
+    return fail(CMK_ERR_INVALID_ARG, "cmk_mx4_bmm_rows: negative extent (L=%d M=%d N=%d K=%d)", L, M, N, K);
+  if (int e = check_dtype("cmk_mx4_bmm_rows", dtype)) return e;
+  if (int e = check_dtype("cmk_mx4_bmm_rows", x_dtype)) return e;
+  if (M > kMx4RowsFloat || L > 65535)
+    return fail(CMK_ERR_UNSUPPORTED, "cmk_mx4_bmm_rows: at most %d rows and 65535 batches (M=%d L=%d)", kMx4RowsFloat, M, L);
+  if (L == 0 || M == 0 || N == 0) return CMK_OK;
+  if (!C || (K > 0 && (!x || !b_codes || !b_scales))) return fail(CMK_ERR_INVALID_ARG, "cmk_mx4_bmm_rows: null pointer");
+  if ((reinterpret_cast<uintptr_t>(b_codes) & 15) || (reinterpret_cast<uintptr_t>(b_scales) & 3))
+    return fail(CMK_ERR_INVALID_ARG, "cmk_mx4_bmm_rows: codes need 16-byte alignment, scales 4-byte alignment");
+  const Mx4RowsArgs a{x, nullptr, b_codes, b_scales, C, M, N, K, (int)mx4_slabs(K), stride_l, stride_m};
+  by_dtype(x_dtype, [&](auto tx) {
+    by_dtype(dtype, [&](auto t) { launch_rows<decltype(tx), decltype(t)>(a, L, (hipStream_t)stream); });
+  });
+  return hip_status(hipGetLastError(), "cmk_mx4_bmm_rows launch");
 }

@@ -37,6 +37,9 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 static inline long long mx4_slabs(int K) { return ((long long)K + kSlab - 1) / kSlab; }
 
+typedef unsigned short u16;
+typedef u16 u16x2 __attribute__((ext_vector_type(2)));
+
 // Eight consecutive elements of one type; addresses need the element's alignment
 // only (the hardware takes unaligned 16-byte loads).
 template <class T>
@@ -45,6 +48,8 @@ struct Octet;
 template <>
 struct Octet<float> {
   float v[8];
+  __device__ __forceinline__ void set(int i, float x) { v[i] = x; }
+  __device__ __forceinline__ float get(int i) const { return v[i]; }
   __device__ __forceinline__ unsigned top() const {  // largest |x| as fp32 bits
     unsigned m = 0;
 #pragma unroll
@@ -60,42 +65,50 @@ struct Octet<float> {
   }
 };
 
-template <>
-struct Octet<__bf16> {
-  __bf16 v[8];
-  __device__ __forceinline__ unsigned top() const {
-    unsigned m = 0;
+// 16-bit elements, two to a register: the largest magnitude takes one mask and one
+// packed 16-bit maximum per pair.
+struct Octet16 {
+  unsigned v[4];
+  __device__ __forceinline__ unsigned top16() const {
+    u16x2 m = __builtin_bit_cast(u16x2, v[0] & 0x7fff7fffu);
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      m = max(m, (unsigned)__builtin_bit_cast(unsigned short, v[i]) & 0x7fffu);
-    return m << 16;
+    for (int i = 1; i < 4; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, v[i] & 0x7fff7fffu));
+    return max((unsigned)m[0], (unsigned)m[1]);
   }
-  __device__ __forceinline__ unsigned codes(float scale) const {
-    unsigned w = 0;
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, bf16x2{v[0], v[1]}, scale, 0);
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, bf16x2{v[2], v[3]}, scale, 1);
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, bf16x2{v[4], v[5]}, scale, 2);
-    return __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, bf16x2{v[6], v[7]}, scale, 3);
+  __device__ __forceinline__ u16 bits(int i) const { return (u16)(v[i >> 1] >> (16 * (i & 1))); }
+  __device__ __forceinline__ void set_bits(int i, u16 b) {
+    v[i >> 1] = i & 1 ? (v[i >> 1] & 0xffffu) | (unsigned)b << 16 : (v[i >> 1] & 0xffff0000u) | b;
   }
 };
 
 template <>
-struct Octet<_Float16> {
-  _Float16 v[8];
+struct Octet<__bf16> : Octet16 {
+  __device__ __forceinline__ void set(int i, __bf16 x) { set_bits(i, __builtin_bit_cast(u16, x)); }
+  __device__ __forceinline__ float get(int i) const { return __uint_as_float((unsigned)bits(i) << 16); }
+  __device__ __forceinline__ unsigned top() const { return top16() << 16; }
+  __device__ __forceinline__ unsigned codes(float scale) const {
+    unsigned w = 0;
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, __builtin_bit_cast(bf16x2, v[0]), scale, 0);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, __builtin_bit_cast(bf16x2, v[1]), scale, 1);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, __builtin_bit_cast(bf16x2, v[2]), scale, 2);
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, __builtin_bit_cast(bf16x2, v[3]), scale, 3);
+  }
+};
+
+template <>
+struct Octet<_Float16> : Octet16 {
+  __device__ __forceinline__ void set(int i, _Float16 x) { set_bits(i, __builtin_bit_cast(u16, x)); }
+  __device__ __forceinline__ float get(int i) const { return (float)__builtin_bit_cast(_Float16, bits(i)); }
+  // as fp32: infinities and NaN keep the top exponent
   __device__ __forceinline__ unsigned top() const {
-    unsigned m = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      m = max(m, (unsigned)__builtin_bit_cast(unsigned short, v[i]) & 0x7fffu);
-    // as fp32: infinities and NaN keep the top exponent
-    return __float_as_uint((float)__builtin_bit_cast(_Float16, (unsigned short)m));
+    return __float_as_uint((float)__builtin_bit_cast(_Float16, (u16)top16()));
   }
   __device__ __forceinline__ unsigned codes(float scale) const {
     unsigned w = 0;
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(w, f16x2{v[0], v[1]}, scale, 0);
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(w, f16x2{v[2], v[3]}, scale, 1);
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(w, f16x2{v[4], v[5]}, scale, 2);
-    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(w, f16x2{v[6], v[7]}, scale, 3);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(w, __builtin_bit_cast(f16x2, v[0]), scale, 0);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(w, __builtin_bit_cast(f16x2, v[1]), scale, 1);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(w, __builtin_bit_cast(f16x2, v[2]), scale, 2);
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(w, __builtin_bit_cast(f16x2, v[3]), scale, 3);
   }
 };
 
@@ -108,7 +121,12 @@ __device__ __forceinline__ Octet<T> load_octet(const T* p, int left) {
     __builtin_memcpy(o.v, p, sizeof(o.v));
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) o.v[i] = i < left ? p[i] : (T)0.0f;
+    for (int i = 0; i < (int)(sizeof(o.v) / 4); ++i) o.v[i] = 0;
+    if (left > 0) {
+#pragma unroll
+      for (int i = 0; i < 7; ++i)
+        if (i < left) o.set(i, p[i]);
+    }
   }
   return o;
 }

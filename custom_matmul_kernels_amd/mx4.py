@@ -7,6 +7,7 @@ from . import _common, _lib
 
 BLOCK = 32        # elements along k that share a scale
 SLAB = 128        # elements of k that lie together in storage
+ROWS_IN_CALL = 16 # rows of a float left operand that the product itself quantises
 
 
 class MX4Tensor:
@@ -168,10 +169,15 @@ class MX4BMMCUDA:
         m, k, c = sa[-2], sa[-1], sb[-1]
         C = torch.empty((m, c) if n == 2 else (l, m, c), dtype=self.out_dtype, device=A.device)
         if C.numel():
-            if not isinstance(A, MX4Tensor):
-                A = quantize_mx4(A, -1)
             if not isinstance(B, MX4Tensor):
                 B = quantize_mx4(B, -2)
+            if not isinstance(A, MX4Tensor):
+                if m <= ROWS_IN_CALL and l <= 65535 and (A.stride(-1) == 1 or k <= 1):
+                    _common.call(self._lib.cmk_mx4_bmm_rows, C.device, A.data_ptr(), _common.FLOAT_TYPES[A.dtype],
+                                 A.stride(0) if n == 3 else 0, A.stride(-2), B.codes.data_ptr(), B.scales.data_ptr(),
+                                 C.data_ptr(), self._out, l, m, c, k)
+                    return C
+                A = quantize_mx4(A, -1)
             _common.call(self._lib.cmk_mx4_bmm, C.device, A.codes.data_ptr(), A.scales.data_ptr(),
                          B.codes.data_ptr(), B.scales.data_ptr(), C.data_ptr(), self._out, l, m, c, k)
         return C

@@ -237,6 +237,16 @@ int cmk_mx4_bmm(const uint8_t* a_codes, const uint8_t* a_scales,
                 const uint8_t* b_codes, const uint8_t* b_scales, void* C,
                 int dtype, int L, int M, int N, int K, void* stream);
 
+/*
+ * The same product for a left operand of at most 16 rows in `x_dtype`, element
+ * (l, m, k) at x[l*stride_l + m*stride_m + k], quantised on the way: the bits of
+ * cmk_mx4_quantize and cmk_mx4_bmm in one launch.
+ */
+int cmk_mx4_bmm_rows(const void* x, int x_dtype, long long stride_l,
+                     long long stride_m, const uint8_t* b_codes,
+                     const uint8_t* b_scales, void* C, int dtype,
+                     int L, int M, int N, int K, void* stream);
+
 /* activations of the experts */
 #define CMK_ACT_SILU 0   /* g / (1 + exp(-g))            */
 #define CMK_ACT_GELU 1   /* g (1 + erf(g / sqrt 2)) / 2  */
