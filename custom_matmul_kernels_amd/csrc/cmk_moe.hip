@@ -7,6 +7,8 @@
 //
 // For a few tokens the time is that of reading the chosen experts' weights once;
 // everything here is laid out around that stream.
+#include <algorithm>
+
 #include "cmk_mx4.hpp"
 
 namespace cmk {
@@ -14,6 +16,7 @@ namespace cmk {
 constexpr int kMoeTokens = 256;    // of one call
 constexpr int kMoeExperts = 1024;
 constexpr int kMoeChoices = 32;
+constexpr int kRouterWaves = 4;
 
 typedef double f64x4 __attribute__((ext_vector_type(4)));
 
@@ -21,6 +24,7 @@ typedef double f64x4 __attribute__((ext_vector_type(4)));
 struct MoePlan {
   size_t logits, chosen, x, h, y, bytes;
   int Hp, Ip;      // H and I rounded up to whole slabs
+  int splits;      // partial sums a logit comes in
   int x_planes;    // 16-bit planes of x
 };
 
@@ -30,8 +34,11 @@ static MoePlan moe_plan(int T, int H, int I, int E, int k, int x_dtype, int w_dt
   p.Hp = (int)(mx4_slabs(H) * kSlab);
   p.Ip = (int)(mx4_slabs(I) * kSlab);
   p.x_planes = x_dtype == CMK_F16 && w_dtype == CMK_MX4 ? 2 : 1;
+  // a wave of the router's kernel sums 128 elements where that takes no more than
+  // 16 work-groups a tile
+  p.splits = std::min(16, (p.Hp / kSlab + kRouterWaves - 1) / kRouterWaves);
   size_t at = 0;
-  p.logits = at; at += up((size_t)T * E * 8);
+  p.logits = at; at += up((size_t)p.splits * T * E * 8);
   p.chosen = at; at += up((size_t)T * k * 4);
   p.x = at; at += up((size_t)p.x_planes * T * p.Hp * 2);
   p.h = at; at += up((size_t)2 * T * k * p.Ip * 2);
@@ -47,7 +54,7 @@ struct MoeArgs {
   float* weights;
   long long* experts;
   long long ld_x, ld_router, ld_gate_up, stride_gate_up, ld_down, stride_down;
-  int T, H, I, E, k, Hp, Ip;
+  int T, H, I, E, k, Hp, Ip, splits;
   int act, renormalize;
   double* logits;
   int* chosen;     // [T*k]
@@ -57,58 +64,77 @@ struct MoeArgs {
 
 // ------------------------------------------------------------------- the router
 
+// The planes of activations in front of 4-bit weights hold the 128 elements of a
+// slab in the order in which the products take them: element q*32 + s*8 + i (block
+// q of the weights, step s) at s*32 + q*8 + i.  Then a step's loads are contiguous
+// for the four lanes of a row.  In front of 16-bit weights the order is natural.
+template <bool four_bit>
+__device__ __forceinline__ int plane_position(int k) {
+  return four_bit ? (k & ~127) | (k & 24) << 2 | (k & 96) >> 2 | (k & 7) : k;
+}
+
 // Logits by fp64 matrix instructions: the products of the operands are exact in
 // fp64 and the sums off by 2^-53 a step, so that the order of the choice does not
 // hang on the order of the sums; equal rows of the router give equal bits.  A
-// work-group takes 16 experts x 16 tokens, its waves split H; the work-groups of
-// the first experts also write x as zero-padded planes for the products: its own
-// bits, or (fp16 in front of 4-bit weights) the two bf16 that sum to it exactly.
-template <class TX, class TR, int PLANES>
-__global__ __launch_bounds__(512) void moe_logits_kernel(MoeArgs a) {
-  __shared__ double part[8][64][4];
+// work-group takes 16 experts x 16 tokens x a range of H, its waves split the
+// range, and the choice adds the ranges up.  The work-groups of the first experts
+// also write x as zero-padded planes for the products: its own bits, or (fp16 in
+// front of 4-bit weights) the two bf16 that sum to it exactly.
+template <class TX, class TR, bool FOUR, int PLANES>
+__global__ __launch_bounds__(64 * kRouterWaves) void moe_logits_kernel(MoeArgs a) {
+  __shared__ double part[kRouterWaves][64][4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int r = lane & 15, q = lane >> 4;
   const int e0 = blockIdx.x * 16, t0 = blockIdx.y * 16;
   const int t = min(t0 + r, a.T - 1), e = min(e0 + r, a.E - 1);
   const TX* x = (const TX*)a.x + t * a.ld_x;
   const TR* w = (const TR*)a.router + e * a.ld_router;
-  f64x4 acc = {0, 0, 0, 0};
-  for (int h0 = wave * 32; h0 < a.Hp; h0 += 8 * 32) {
-    const int h = h0 + q * 8;
-    const Octet<TX> ox = load_octet(x + h, a.H - h);
-    const Octet<TR> ow = load_octet(w + h, a.H - h);
-    if (blockIdx.x == 0 && t0 + r < a.T) {
-      u16 hi[8], lo[8];
+  f64x4 acc[2] = {};
+  for (int slab = blockIdx.z * kRouterWaves + wave; slab < a.Hp / kSlab; slab += a.splits * kRouterWaves) {
+    Octet<TX> ox[4];
+    Octet<TR> ow[4];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if constexpr (PLANES == 1) {
-          hi[i] = ox.bits(i);
-        } else {
-          const float f = ox.get(i);
-          const __bf16 b = (__bf16)f;
-          hi[i] = __builtin_bit_cast(u16, b);
-          // an infinity or a NaN stays in the first plane alone
-          lo[i] = __builtin_bit_cast(u16, (__bf16)(__builtin_isfinite(f) ? f - (float)b : 0.0f));
+    for (int s = 0; s < 4; ++s) {
+      const int h = slab * kSlab + s * 32 + q * 8;
+      ox[s] = load_octet(x + h, a.H - h);
+      ow[s] = load_octet(w + h, a.H - h);
+    }
+    if (blockIdx.x == 0 && t0 + r < a.T) {
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        u16 hi[8], lo[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if constexpr (PLANES == 1) {
+            hi[i] = ox[s].bits(i);
+          } else {
+            const float f = ox[s].get(i);
+            const __bf16 b = (__bf16)f;
+            hi[i] = __builtin_bit_cast(u16, b);
+            // an infinity or a NaN stays in the first plane alone
+            lo[i] = __builtin_bit_cast(u16, (__bf16)(__builtin_isfinite(f) ? f - (float)b : 0.0f));
+          }
         }
+        const long long at = (long long)t * a.Hp + plane_position<FOUR>(slab * kSlab + s * 32 + q * 8);
+        __builtin_memcpy(a.xp + at, hi, 16);
+        if constexpr (PLANES == 2) __builtin_memcpy(a.xp + (long long)a.T * a.Hp + at, lo, 16);
       }
-      __builtin_memcpy(a.xp + (long long)t * a.Hp + h, hi, 16);
-      if constexpr (PLANES == 2) __builtin_memcpy(a.xp + ((long long)a.T + t) * a.Hp + h, lo, 16);
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)ow.get(i), (double)ox.get(i), acc, 0, 0, 0);
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        acc[i & 1] = __builtin_amdgcn_mfma_f64_16x16x4f64((double)ow[s].get(i), (double)ox[s].get(i), acc[i & 1], 0, 0, 0);
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) part[wave][lane][i] = acc[i];
+  for (int i = 0; i < 4; ++i) part[wave][lane][i] = acc[0][i] + acc[1][i];
   __syncthreads();
-  if (threadIdx.x < 256) {
-    const int l = threadIdx.x & 63, i = threadIdx.x >> 6;
-    double s = 0;
+  const int l = threadIdx.x & 63, i = threadIdx.x >> 6;
+  double s = 0;
 #pragma unroll
-    for (int v = 0; v < 8; ++v) s += part[v][l][i];
-    const int ee = e0 + (l >> 4) + 4 * i, tt = t0 + (l & 15);
-    if (ee < a.E && tt < a.T) a.logits[(long long)tt * a.E + ee] = s;
-  }
+  for (int v = 0; v < kRouterWaves; ++v) s += part[v][l][i];
+  const int ee = e0 + (l >> 4) + 4 * i, tt = t0 + (l & 15);
+  if (ee < a.E && tt < a.T) a.logits[((long long)blockIdx.z * a.T + tt) * a.E + ee] = s;
 }
 
 // Larger keys for larger logits, NaN above all; never 0.
@@ -119,69 +145,114 @@ __device__ __forceinline__ unsigned long long order_key(double v) {
   return b >> 63 ? ~b : b | 0x8000000000000000ull;
 }
 
-// A wave per token: k rounds of the largest key that is left, the lowest index of
-// equal ones.
-__global__ __launch_bounds__(64) void moe_select_kernel(MoeArgs a) {
-  __shared__ unsigned long long key[kMoeExperts];
-  __shared__ int pick[kMoeChoices];
-  const int t = blockIdx.x, lane = threadIdx.x;
-  const double* logits = a.logits + (long long)t * a.E;
-  for (int e = lane; e < a.E; e += 64) key[e] = order_key(logits[e]);
-  __syncthreads();
-  for (int j = 0; j < a.k; ++j) {
-    unsigned long long best = 0;
-    int at = 0x7fffffff;
-    for (int e = lane; e < a.E; e += 64)
-      if (key[e] > best) { best = key[e]; at = e; }
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const unsigned long long ob = __shfl_xor(best, d);
-      const int oa = __shfl_xor(at, d);
-      if (ob > best || (ob == best && oa < at)) { best = ob; at = oa; }
-    }
-    if (lane == 0) { pick[j] = at; key[at] = 0; }
-    __syncthreads();
+constexpr int kRankedExperts = 256;
+
+// The choice of token t, by a work-group of 256 threads: pick[j] and weight[j] in
+// LDS, valid after the barrier at its end.  Up to 256 experts each is ranked by
+// counting those in front of it, the counting spread over the threads; beyond, k
+// rounds look for the largest that is left.
+struct MoeChoice {
+  unsigned long long key[kMoeExperts];
+  double logit[kMoeExperts];
+  int rank[kRankedExperts];
+  int pick[kMoeChoices];
+  float raised[kMoeChoices];
+  float sum;
+};
+
+__device__ __forceinline__ void moe_choose(const MoeArgs& a, int t, MoeChoice& c) {
+  const int tid = threadIdx.x;
+  for (int e = tid; e < a.E; e += 256) {
+    double v = 0;
+    for (int s = 0; s < a.splits; ++s) v += a.logits[((long long)s * a.T + t) * a.E + e];
+    c.logit[e] = v;
+    c.key[e] = order_key(v);
+    if (e < kRankedExperts) c.rank[e] = 0;
   }
-  const double top = logits[pick[0]];
-  float sum = 0;
-  if (a.renormalize) {
-    for (int j = 0; j < a.k; ++j) sum += expf((float)(logits[pick[j]] - top));
+  __syncthreads();
+  if (a.E <= kRankedExperts) {
+    // threads per expert: a power of two, so that a wave's threads share what they compare with
+    const int width = a.E <= 64 ? 64 : a.E <= 128 ? 128 : 256;
+    const int e = tid & (width - 1), share = tid / width, shares = 256 / width;
+    if (e < a.E) {
+      const unsigned long long mine = c.key[e];
+      int before = 0;
+      for (int o = share; o < a.E; o += shares) before += c.key[o] > mine || (c.key[o] == mine && o < e);
+      if (before) atomicAdd(&c.rank[e], before);
+    }
+    __syncthreads();
+    if (tid < a.E && c.rank[tid] < a.k) c.pick[c.rank[tid]] = tid;
+    __syncthreads();
   } else {
-    for (int e = lane; e < a.E; e += 64) sum += expf((float)(logits[e] - top));
+    for (int j = 0; j < a.k; ++j) {
+      if (tid < 64) {
+        unsigned long long best = 0;
+        int at = 0x7fffffff;
+        for (int e = tid; e < a.E; e += 64)
+          if (c.key[e] > best) { best = c.key[e]; at = e; }
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+          const unsigned long long ob = __shfl_xor(best, d);
+          const int oa = __shfl_xor(at, d);
+          if (ob > best || (ob == best && oa < at)) { best = ob; at = oa; }
+        }
+        if (tid == 0) { c.pick[j] = at; c.key[at] = 0; }
+      }
+      __syncthreads();
+    }
+  }
+  const double top = c.logit[c.pick[0]];
+  if (tid < a.k) c.raised[tid] = expf((float)(c.logit[c.pick[tid]] - top));
+  if (!a.renormalize && tid < 64) {
+    float sum = 0;
+    for (int e = tid; e < a.E; e += 64) sum += expf((float)(c.logit[e] - top));
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
+    if (tid == 0) c.sum = sum;
   }
-  if (lane < a.k) {
-    const int s = t * a.k + lane;
-    a.chosen[s] = pick[lane];
-    a.experts[s] = pick[lane];
-    a.weights[s] = expf((float)(logits[pick[lane]] - top)) / sum;
+  __syncthreads();
+}
+
+__device__ __forceinline__ float moe_weight(const MoeArgs& a, const MoeChoice& c, int j) {
+  float sum = 0;
+  if (a.renormalize)
+    for (int i = 0; i < a.k; ++i) sum += c.raised[i];
+  else sum = c.sum;
+  return c.raised[j] / sum;
+}
+
+__global__ __launch_bounds__(256) void moe_select_kernel(MoeArgs a) {
+  __shared__ MoeChoice c;
+  moe_choose(a, blockIdx.x, c);
+  if ((int)threadIdx.x < a.k) {
+    const int s = blockIdx.x * a.k + threadIdx.x;
+    a.chosen[s] = c.pick[threadIdx.x];
+    a.experts[s] = c.pick[threadIdx.x];
+    a.weights[s] = moe_weight(a, c, threadIdx.x);
   }
 }
 
 // ------------------------------------------------------------ experts' products
 
-// What a lane reads of 16 rows x one slab of weights: its row (lane & 15) at the
-// 32 elements (lane >> 4) * 32 of the slab, the 64 (16) bytes of which feed four
-// steps of the 16x16x32 matrix instruction, 8 elements each.  The other operand
-// reads its elements the same way: a sum over k does not mind the order.
+// What a lane reads of 16 rows x one slab of weights, row (lane & 15), as it feeds
+// four steps of the 16x16x32 matrix instruction, 8 elements each: of 16-bit
+// weights 16 bytes per step (64 contiguous bytes of a row per instruction), of
+// 4-bit weights one block of 32, whose quarter s belongs to step s.  A sum over k
+// does not mind the order as long as both operands use the same one.
 template <int WF>
 struct WeightSlab {  // 16-bit weights
   u32x4v v[4];
   __device__ __forceinline__ void load(const void* base, const uint8_t*, long long, long long row, long long ld, int slab, int K) {
-    const int q = (threadIdx.x & 63) >> 4;
-    const int k = slab * kSlab + q * 32;
+    const int k = slab * kSlab + ((threadIdx.x & 63) >> 4) * 8;
     const u16* p = (const u16*)base + row * ld + k;
+    if (slab * kSlab + kSlab <= K) {
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      const int left = K - k - s * 8;
-      if (left >= 8) {
-        __builtin_memcpy(&v[s], p + s * 8, 16);
-      } else {
-        u16 e[8];
+      for (int s = 0; s < 4; ++s) __builtin_memcpy(&v[s], p + s * 32, 16);
+    } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) e[i] = i < left ? p[s * 8 + i] : (u16)0;
-        __builtin_memcpy(&v[s], e, 16);
+      for (int s = 0; s < 4; ++s) {
+        const Octet<__bf16> o = load_octet((const __bf16*)p + s * 32, K - k - s * 32);
+        __builtin_memcpy(&v[s], o.v, 16);
       }
     }
   }
@@ -201,13 +272,17 @@ struct WeightSlab<CMK_MX4> {
   }
   __device__ __forceinline__ u32x4v step(int s) const {  // as bf16, exactly
     const float f = scale_float(scale);
-    const unsigned nan = scale == 255u ? 0x7fff7fffu : 0u;
     const unsigned w = v[s];
     u32x4v o;
-    o[0] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 0)) | nan;
-    o[1] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 1)) | nan;
-    o[2] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 2)) | nan;
-    o[3] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 3)) | nan;
+    o[0] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 0));
+    o[1] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 1));
+    o[2] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 2));
+    o[3] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 3));
+    if (__any(scale == 255u)) {  // a block that stands for NaN
+      const unsigned nan = scale == 255u ? 0x7fff7fffu : 0u;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] |= nan;
+    }
     return o;
   }
 };
@@ -236,31 +311,25 @@ __device__ __forceinline__ void split_f16(u32x4v w, u32x4v& hi, u32x4v& lo) {
   lo = __builtin_bit_cast(u32x4v, l);
 }
 
-constexpr int kMoeWaves = 4;
-constexpr int kMoeBlocks = 4;  // column blocks of 16 tokens at a time
-
 // The expert a work-group serves and the slots t*k+j that chose it, in order.
 // Returns their count, 0 if there is nothing to do.
 __device__ __forceinline__ int moe_slots(const MoeArgs& a, int unit, int* list, int& expert) {
   const int n = a.T * a.k;
   __shared__ int count;
-  if (n <= a.E) {  // a unit is a slot: the first one that chose the expert serves it
-    expert = a.chosen[unit];
-    for (int s = 0; s < unit; ++s)
-      if (a.chosen[s] == expert) return 0;
-  } else {
-    expert = unit;
-  }
+  const bool by_slot = n <= a.E;  // a unit is a slot: the first one that chose an expert serves it
+  expert = by_slot ? a.chosen[unit] : unit;
   if (threadIdx.x < 64) {
     int found = 0;
+    bool first = true;
     for (int s0 = 0; s0 < n; s0 += 64) {
       const int s = s0 + (int)threadIdx.x;
       const bool mine = s < n && a.chosen[s] == expert;
       const unsigned long long m = __ballot(mine);
+      if (by_slot && __ballot(mine && s < unit)) { first = false; break; }
       if (mine) list[found + __popcll(m & ((1ull << threadIdx.x) - 1))] = s;
       found += __popcll(m);
     }
-    if (threadIdx.x == 0) count = found;
+    if (threadIdx.x == 0) count = first ? found : 0;
   }
   __syncthreads();
   return count;
@@ -271,133 +340,160 @@ __device__ __forceinline__ float activate(float g, int act) {
   return 0.5f * g * (1.0f + erff(g * 0.70710678118654752f));
 }
 
-// 16 gate rows and the 16 up rows that go with them, against the tokens of one
-// expert; the waves split H and their sums meet in LDS, in order.
-template <int WF, int PLANES>
-__global__ __launch_bounds__(64 * kMoeWaves) void moe_gate_up_kernel(MoeArgs a) {
-  __shared__ int list[kMoeTokens];
-  __shared__ float part[kMoeWaves][2][kMoeBlocks][64][4];
-  int expert;
-  const int count = moe_slots(a, blockIdx.y, list, expert);
-  if (count == 0) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int r = lane & 15, q = lane >> 4;
-  const int i0 = blockIdx.x * 16;
-  const int row = min(i0 + r, a.I - 1);
-  const char* base = (const char*)a.gate_up + (WF == CMK_MX4 ? (long long)expert * (a.Hp / 2) * (2 * a.I) : expert * a.stride_gate_up * 2);
-  const uint8_t* scales = WF == CMK_MX4 ? a.gate_up_scales + (long long)expert * (a.Hp / 32) * (2 * a.I) : nullptr;
-  const int slabs = a.Hp / kSlab;
-  for (int c0 = 0; c0 < count; c0 += 16 * kMoeBlocks) {
-    const int blocks = min(kMoeBlocks, (count - c0 + 15) / 16);
-    f32x4 g[kMoeBlocks] = {}, u[kMoeBlocks] = {};
-    const u16* xs[kMoeBlocks];
+// The products of RG groups of 16 rows of one expert's matrix with up to NB * 16
+// of its slots, over the slabs of one wave; M products (gate and up, or one) share
+// the activations.  U slabs of weights are requested at a time.
+template <int WF, int PLANES, int M, int RG, int NB, int U, bool SPLIT>
+__device__ __forceinline__ void moe_products(f32x4 (&acc)[M][RG][NB], const void* base, const uint8_t* scales, long long rows,
+                                             const long long (&row)[M][RG], long long ld, int K, const u16* const (&act)[NB],
+                                             long long plane, int wave, int waves) {
+  const int slabs = (K + kSlab - 1) / kSlab;
+  for (int s0 = wave; s0 < slabs; s0 += waves * U) {
+    WeightSlab<WF> w[U][M][RG];
 #pragma unroll
-    for (int b = 0; b < kMoeBlocks; ++b) {
-      const int t = list[min(c0 + b * 16 + r, count - 1)] / a.k;
-      xs[b] = a.xp + (long long)t * a.Hp + q * 32;
+    for (int u = 0; u < U; ++u) {
+      if (s0 + u * waves >= slabs) break;
+#pragma unroll
+      for (int m = 0; m < M; ++m)
+#pragma unroll
+        for (int g = 0; g < RG; ++g) w[u][m][g].load(base, scales, rows, row[m][g], ld, s0 + u * waves, K);
     }
-    for (int slab = wave; slab < slabs; slab += kMoeWaves) {
-      WeightSlab<WF> wg, wu;
-      wg.load(base, scales, 2 * a.I, row, a.ld_gate_up, slab, a.H);
-      wu.load(base, scales, 2 * a.I, a.I + row, a.ld_gate_up, slab, a.H);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (s0 + u * waves >= slabs) break;
+      const int at = (s0 + u * waves) * kSlab;
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
-        const u32x4v fg = wg.step(s), fu = wu.step(s);
+        u32x4v x[NB][PLANES];
 #pragma unroll
-        for (int b = 0; b < kMoeBlocks; ++b) {
-          if (b >= blocks) break;
+        for (int b = 0; b < NB; ++b)
 #pragma unroll
-          for (int p = 0; p < PLANES; ++p) {
-            const u32x4v x = *(const u32x4v*)(xs[b] + (long long)p * a.T * a.Hp + slab * kSlab + s * 8);
-            if (WF == CMK_F16) { g[b] = mfma_f16(fg, x, g[b]); u[b] = mfma_f16(fu, x, u[b]); }
-            else { g[b] = mfma_bf16(fg, x, g[b]); u[b] = mfma_bf16(fu, x, u[b]); }
+          for (int p = 0; p < PLANES; ++p) x[b][p] = *(const u32x4v*)(act[b] + p * plane + at + s * 32);
+#pragma unroll
+        for (int m = 0; m < M; ++m)
+#pragma unroll
+          for (int g = 0; g < RG; ++g) {
+            u32x4v f = w[u][m][g].step(s), f2;
+            if constexpr (SPLIT) split_f16(w[u][m][g].step(s), f, f2);
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+#pragma unroll
+              for (int p = 0; p < PLANES; ++p)
+                acc[m][g][b] = WF == CMK_F16 && !SPLIT ? mfma_f16(f, x[b][p], acc[m][g][b]) : mfma_bf16(f, x[b][p], acc[m][g][b]);
+              if constexpr (SPLIT) acc[m][g][b] = mfma_bf16(f2, x[b][0], acc[m][g][b]);
+            }
           }
-        }
       }
     }
-#pragma unroll
-    for (int b = 0; b < kMoeBlocks; ++b)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) { part[wave][0][b][lane][i] = g[b][i]; part[wave][1][b][lane][i] = u[b][i]; }
-    __syncthreads();
-    for (int v = threadIdx.x; v < blocks * 256; v += 64 * kMoeWaves) {
-      // 16 rows of one token next to each other
-      const int row_in = v & 15, col = v >> 4 & 15, b = v >> 8;
-      const int l = (row_in >> 2) * 16 + col, i = row_in & 3;
-      float sg = 0, su = 0;
-#pragma unroll
-      for (int w = 0; w < kMoeWaves; ++w) { sg += part[w][0][b][l][i]; su += part[w][1][b][l][i]; }
-      const int c = c0 + b * 16 + col;
-      if (c < count) {
-        const float h = i0 + row_in < a.I ? activate(sg, a.act) * su : 0.0f;
-        // two bf16: 16 bits of mantissa and fp32's range
-        const __bf16 hi = (__bf16)h;
-        const __bf16 lo = (__bf16)(__builtin_isfinite(h) ? h - (float)hi : 0.0f);
-        const long long at = (long long)list[c] * a.Ip + i0 + row_in;
-        a.hp[at] = __builtin_bit_cast(u16, hi);
-        a.hp[at + (long long)a.T * a.k * a.Ip] = __builtin_bit_cast(u16, lo);
-      }
-    }
-    __syncthreads();
   }
 }
 
-// 16 rows of an expert's down matrix against its slots' activations.
-template <int WF>
-__global__ __launch_bounds__(64 * kMoeWaves) void moe_down_kernel(MoeArgs a) {
+// RG * 16 gate rows and the up rows that go with them, against the tokens of one
+// expert; the W waves split H and their sums meet in LDS, in order.
+template <int WF, int PLANES, int W, int RG, int NB, int U>
+__device__ __forceinline__ void moe_gate_up_tokens(const MoeArgs& a, int expert, const int* list, int c0, int count, float (*part)[2][RG][NB][64][4]) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r = lane & 15, q = lane >> 4;
+  const int i0 = blockIdx.x * 16 * RG;
+  const char* base = (const char*)a.gate_up + (WF == CMK_MX4 ? (long long)expert * (a.Hp / 2) * (2 * a.I) : expert * a.stride_gate_up * 2);
+  const uint8_t* scales = WF == CMK_MX4 ? a.gate_up_scales + (long long)expert * (a.Hp / 32) * (2 * a.I) : nullptr;
+  long long row[2][RG];
+#pragma unroll
+  for (int g = 0; g < RG; ++g) {
+    row[0][g] = min(i0 + g * 16 + r, a.I - 1);
+    row[1][g] = a.I + row[0][g];
+  }
+  f32x4 acc[2][RG][NB] = {};
+  const u16* xs[NB];
+#pragma unroll
+  for (int b = 0; b < NB; ++b) xs[b] = a.xp + (long long)(list[min(c0 + b * 16 + r, count - 1)] / a.k) * a.Hp + q * 8;
+  moe_products<WF, PLANES, 2, RG, NB, U, false>(acc, base, scales, 2 * a.I, row, a.ld_gate_up, a.H, xs, (long long)a.T * a.Hp, wave, W);
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int g = 0; g < RG; ++g)
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) part[wave][m][g][b][lane][i] = acc[m][g][b][i];
+  __syncthreads();
+  for (int v = threadIdx.x; v < NB * RG * 256; v += 64 * W) {
+    // the rows of one token next to each other
+    const int in = v % (16 * RG), c = v / (16 * RG);
+    const int g = in >> 4, l = ((in & 15) >> 2) * 16 + (c & 15), i = in & 3, b = c >> 4;
+    if (c0 + c < count && i0 + in < a.Ip) {
+      float sg = 0, su = 0;
+#pragma unroll
+      for (int w = 0; w < W; ++w) { sg += part[w][0][g][b][l][i]; su += part[w][1][g][b][l][i]; }
+      const float h = i0 + in < a.I ? activate(sg, a.act) * su : 0.0f;
+      // two bf16: 16 bits of mantissa and fp32's range
+      const __bf16 hi = (__bf16)h;
+      const __bf16 lo = (__bf16)(__builtin_isfinite(h) ? h - (float)hi : 0.0f);
+      const long long at = (long long)list[c0 + c] * a.Ip + plane_position<WF == CMK_MX4>(i0 + in);
+      a.hp[at] = __builtin_bit_cast(u16, hi);
+      a.hp[at + (long long)a.T * a.k * a.Ip] = __builtin_bit_cast(u16, lo);
+    }
+  }
+  __syncthreads();
+}
+
+template <int WF, int PLANES, int W, int RG, int U>
+__global__ __launch_bounds__(64 * W) void moe_gate_up_kernel(MoeArgs a) {
   __shared__ int list[kMoeTokens];
-  __shared__ float part[kMoeWaves][kMoeBlocks][64][4];
+  __shared__ float part[W][2][RG][2][64][4];
   int expert;
   const int count = moe_slots(a, blockIdx.y, list, expert);
-  if (count == 0) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  for (int c0 = 0; c0 < count; c0 += 32) {
+    if (count - c0 <= 16) moe_gate_up_tokens<WF, PLANES, W, RG, 1, U>(a, expert, list, c0, count, (float(*)[2][RG][1][64][4])part);
+    else moe_gate_up_tokens<WF, PLANES, W, RG, 2, U>(a, expert, list, c0, count, part);
+  }
+}
+
+// RG * 16 rows of an expert's down matrix against its slots' activations.
+template <int WF, int W, int RG, int NB, int U>
+__device__ __forceinline__ void moe_down_tokens(const MoeArgs& a, int expert, const int* list, int c0, int count, float (*part)[RG][NB][64][4]) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, q = lane >> 4;
-  const int n0 = blockIdx.x * 16;
-  const int row = min(n0 + r, a.H - 1);
+  const int n0 = blockIdx.x * 16 * RG;
   const char* base = (const char*)a.down + (WF == CMK_MX4 ? (long long)expert * (a.Ip / 2) * a.H : expert * a.stride_down * 2);
   const uint8_t* scales = WF == CMK_MX4 ? a.down_scales + (long long)expert * (a.Ip / 32) * a.H : nullptr;
-  const int slabs = a.Ip / kSlab;
-  const long long plane = (long long)a.T * a.k * a.Ip;
-  for (int c0 = 0; c0 < count; c0 += 16 * kMoeBlocks) {
-    const int blocks = min(kMoeBlocks, (count - c0 + 15) / 16);
-    f32x4 y[kMoeBlocks] = {};
-    const u16* hs[kMoeBlocks];
+  long long row[1][RG];
 #pragma unroll
-    for (int b = 0; b < kMoeBlocks; ++b)
-      hs[b] = a.hp + (long long)list[min(c0 + b * 16 + r, count - 1)] * a.Ip + q * 32;
-    for (int slab = wave; slab < slabs; slab += kMoeWaves) {
-      WeightSlab<WF> w;
-      w.load(base, scales, a.H, row, a.ld_down, slab, a.I);
+  for (int g = 0; g < RG; ++g) row[0][g] = min(n0 + g * 16 + r, a.H - 1);
+  f32x4 acc[1][RG][NB] = {};
+  const u16* hs[NB];
 #pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        u32x4v f = w.step(s), f2 = f;
-        if (WF == CMK_F16) split_f16(w.step(s), f, f2);
+  for (int b = 0; b < NB; ++b) hs[b] = a.hp + (long long)list[min(c0 + b * 16 + r, count - 1)] * a.Ip + q * 8;
+  moe_products<WF, 2, 1, RG, NB, U, WF == CMK_F16>(acc, base, scales, a.H, row, a.ld_down, a.I, hs, (long long)a.T * a.k * a.Ip, wave, W);
 #pragma unroll
-        for (int b = 0; b < kMoeBlocks; ++b) {
-          if (b >= blocks) break;
-          const u32x4v hi = *(const u32x4v*)(hs[b] + slab * kSlab + s * 8);
-          const u32x4v lo = *(const u32x4v*)(hs[b] + plane + slab * kSlab + s * 8);
-          y[b] = mfma_bf16(f, hi, y[b]);
-          y[b] = mfma_bf16(f, lo, y[b]);
-          if (WF == CMK_F16) y[b] = mfma_bf16(f2, hi, y[b]);
-        }
-      }
-    }
+  for (int g = 0; g < RG; ++g)
 #pragma unroll
-    for (int b = 0; b < kMoeBlocks; ++b)
+    for (int b = 0; b < NB; ++b)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) part[wave][b][lane][i] = y[b][i];
-    __syncthreads();
-    for (int v = threadIdx.x; v < blocks * 256; v += 64 * kMoeWaves) {
-      const int row_in = v & 15, col = v >> 4 & 15, b = v >> 8;
-      const int l = (row_in >> 2) * 16 + col, i = row_in & 3;
+      for (int i = 0; i < 4; ++i) part[wave][g][b][lane][i] = acc[0][g][b][i];
+  __syncthreads();
+  for (int v = threadIdx.x; v < NB * RG * 256; v += 64 * W) {
+    const int in = v % (16 * RG), c = v / (16 * RG);
+    const int g = in >> 4, l = ((in & 15) >> 2) * 16 + (c & 15), i = in & 3, b = c >> 4;
+    if (c0 + c < count && n0 + in < a.H) {
       float s = 0;
 #pragma unroll
-      for (int w = 0; w < kMoeWaves; ++w) s += part[w][b][l][i];
-      const int c = c0 + b * 16 + col;
-      if (c < count && n0 + row_in < a.H) a.yp[(long long)list[c] * a.H + n0 + row_in] = s;
+      for (int w = 0; w < W; ++w) s += part[w][g][b][l][i];
+      a.yp[(long long)list[c0 + c] * a.H + n0 + in] = s;
     }
-    __syncthreads();
+  }
+  __syncthreads();
+}
+
+template <int WF, int W, int RG, int U>
+__global__ __launch_bounds__(64 * W) void moe_down_kernel(MoeArgs a) {
+  __shared__ int list[kMoeTokens];
+  __shared__ float part[W][RG][2][64][4];
+  int expert;
+  const int count = moe_slots(a, blockIdx.y, list, expert);
+  for (int c0 = 0; c0 < count; c0 += 32) {
+    if (count - c0 <= 16) moe_down_tokens<WF, W, RG, 1, U>(a, expert, list, c0, count, (float(*)[RG][1][64][4])part);
+    else moe_down_tokens<WF, W, RG, 2, U>(a, expert, list, c0, count, part);
   }
 }
 
@@ -462,34 +558,34 @@ extern "C" int cmk_moe(const void* x, const void* router, const void* gate_up, c
   char* ws = (char*)workspace;
   MoeArgs a{x, router, gate_up, down, gate_up_scales, down_scales, y, weights, experts,
             d->ld_x, d->ld_router, d->ld_gate_up, d->stride_gate_up, d->ld_down, d->stride_down,
-            d->T, d->H, d->I, d->E, d->k, p.Hp, p.Ip, d->activation, d->renormalize,
+            d->T, d->H, d->I, d->E, d->k, p.Hp, p.Ip, p.splits, d->activation, d->renormalize,
             (double*)(ws + p.logits), (int*)(ws + p.chosen), (u16*)(ws + p.x), (u16*)(ws + p.h), (float*)(ws + p.y)};
   hipStream_t st = (hipStream_t)stream;
-  const dim3 router_grid(ceil_div(d->E, 16), ceil_div(d->T, 16));
-  const bool r32 = d->router_dtype == CMK_F32;
+  const dim3 router_grid(ceil_div(d->E, 16), ceil_div(d->T, 16), p.splits);
+  const bool r32 = d->router_dtype == CMK_F32, four = d->w_dtype == CMK_MX4;
+  auto logits = [&](auto kernel) { hipLaunchKernelGGL(kernel, router_grid, dim3(64 * kRouterWaves), 0, st, a); };
   if (d->x_dtype == CMK_BF16) {
-    if (r32) hipLaunchKernelGGL((moe_logits_kernel<__bf16, float, 1>), router_grid, dim3(512), 0, st, a);
-    else hipLaunchKernelGGL((moe_logits_kernel<__bf16, __bf16, 1>), router_grid, dim3(512), 0, st, a);
-  } else if (p.x_planes == 1) {
-    if (r32) hipLaunchKernelGGL((moe_logits_kernel<_Float16, float, 1>), router_grid, dim3(512), 0, st, a);
-    else hipLaunchKernelGGL((moe_logits_kernel<_Float16, _Float16, 1>), router_grid, dim3(512), 0, st, a);
+    if (four) r32 ? logits(moe_logits_kernel<__bf16, float, true, 1>) : logits(moe_logits_kernel<__bf16, __bf16, true, 1>);
+    else r32 ? logits(moe_logits_kernel<__bf16, float, false, 1>) : logits(moe_logits_kernel<__bf16, __bf16, false, 1>);
   } else {
-    if (r32) hipLaunchKernelGGL((moe_logits_kernel<_Float16, float, 2>), router_grid, dim3(512), 0, st, a);
-    else hipLaunchKernelGGL((moe_logits_kernel<_Float16, _Float16, 2>), router_grid, dim3(512), 0, st, a);
+    if (four) r32 ? logits(moe_logits_kernel<_Float16, float, true, 2>) : logits(moe_logits_kernel<_Float16, _Float16, true, 2>);
+    else r32 ? logits(moe_logits_kernel<_Float16, float, false, 1>) : logits(moe_logits_kernel<_Float16, _Float16, false, 1>);
   }
-  hipLaunchKernelGGL(moe_select_kernel, dim3(d->T), dim3(64), 0, st, a);
+  hipLaunchKernelGGL(moe_select_kernel, dim3(d->T), dim3(256), 0, st, a);
   const int units = d->T * d->k <= d->E ? d->T * d->k : d->E;
-  const dim3 up_grid(p.Ip / 16, units), down_grid(ceil_div(d->H, 16), units), b(64 * kMoeWaves);
+  auto experts_kernel = [&](auto kernel, int rows, int rg, int w) {
+    hipLaunchKernelGGL(kernel, dim3(ceil_div(rows, 16 * rg), units), dim3(64 * w), 0, st, a);
+  };
   if (d->w_dtype == CMK_MX4) {
-    if (p.x_planes == 1) hipLaunchKernelGGL((moe_gate_up_kernel<CMK_MX4, 1>), up_grid, b, 0, st, a);
-    else hipLaunchKernelGGL((moe_gate_up_kernel<CMK_MX4, 2>), up_grid, b, 0, st, a);
-    hipLaunchKernelGGL(moe_down_kernel<CMK_MX4>, down_grid, b, 0, st, a);
+    if (p.x_planes == 1) experts_kernel(moe_gate_up_kernel<CMK_MX4, 1, 4, 2, 2>, p.Ip, 2, 4);
+    else experts_kernel(moe_gate_up_kernel<CMK_MX4, 2, 4, 2, 2>, p.Ip, 2, 4);
+    experts_kernel(moe_down_kernel<CMK_MX4, 4, 4, 2>, d->H, 4, 4);
   } else if (d->w_dtype == CMK_BF16) {
-    hipLaunchKernelGGL((moe_gate_up_kernel<CMK_BF16, 1>), up_grid, b, 0, st, a);
-    hipLaunchKernelGGL(moe_down_kernel<CMK_BF16>, down_grid, b, 0, st, a);
+    experts_kernel(moe_gate_up_kernel<CMK_BF16, 1, 4, 1, 2>, p.Ip, 1, 4);
+    experts_kernel(moe_down_kernel<CMK_BF16, 4, 1, 2>, d->H, 1, 4);
   } else {
-    hipLaunchKernelGGL((moe_gate_up_kernel<CMK_F16, 1>), up_grid, b, 0, st, a);
-    hipLaunchKernelGGL(moe_down_kernel<CMK_F16>, down_grid, b, 0, st, a);
+    experts_kernel(moe_gate_up_kernel<CMK_F16, 1, 4, 1, 2>, p.Ip, 1, 4);
+    experts_kernel(moe_down_kernel<CMK_F16, 4, 1, 2>, d->H, 1, 4);
   }
   const dim3 out_grid(ceil_div(d->H, 256), d->T);
   if (d->x_dtype == CMK_BF16) hipLaunchKernelGGL(moe_combine_kernel<__bf16>, out_grid, dim3(256), 0, st, a);
