@@ -311,28 +311,30 @@ __device__ __forceinline__ void split_f16(u32x4v w, u32x4v& hi, u32x4v& lo) {
   lo = __builtin_bit_cast(u32x4v, l);
 }
 
-// The expert a work-group serves and the slots t*k+j that chose it, in order.
-// Returns their count, 0 if there is nothing to do.
+// The expert a work-group serves and the slots t*k+j that chose it.  Returns their
+// count, 0 if there is nothing to do.  The order of the list may differ from run to
+// run and does not matter: a slot's column is computed by itself.
+template <int W>
 __device__ __forceinline__ int moe_slots(const MoeArgs& a, int unit, int* list, int& expert) {
   const int n = a.T * a.k;
-  __shared__ int count;
+  __shared__ int count, taken;
+  if (threadIdx.x == 0) count = taken = 0;
   const bool by_slot = n <= a.E;  // a unit is a slot: the first one that chose an expert serves it
   expert = by_slot ? a.chosen[unit] : unit;
-  if (threadIdx.x < 64) {
-    int found = 0;
-    bool first = true;
-    for (int s0 = 0; s0 < n; s0 += 64) {
-      const int s = s0 + (int)threadIdx.x;
-      const bool mine = s < n && a.chosen[s] == expert;
-      const unsigned long long m = __ballot(mine);
-      if (by_slot && __ballot(mine && s < unit)) { first = false; break; }
-      if (mine) list[found + __popcll(m & ((1ull << threadIdx.x) - 1))] = s;
-      found += __popcll(m);
-    }
-    if (threadIdx.x == 0) count = first ? found : 0;
+  __syncthreads();
+  for (int s0 = threadIdx.x; s0 < n; s0 += 4 * 64 * W) {
+    int c[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c[i] = s0 + i * 64 * W < n ? a.chosen[s0 + i * 64 * W] : -1;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (c[i] == expert) {
+        list[atomicAdd(&count, 1)] = s0 + i * 64 * W;
+        if (by_slot && s0 + i * 64 * W < unit) taken = 1;
+      }
   }
   __syncthreads();
-  return count;
+  return taken ? 0 : count;
 }
 
 __device__ __forceinline__ float activate(float g, int act) {
@@ -342,33 +344,38 @@ __device__ __forceinline__ float activate(float g, int act) {
 
 // The products of RG groups of 16 rows of one expert's matrix with up to NB * 16
 // of its slots, over the slabs of one wave; M products (gate and up, or one) share
-// the activations.  U slabs of weights are requested at a time.
+// the activations.  A ring of U slabs of weights and activations is under way:
+// vector-memory loads are awaited in the order of their issue, so that activations
+// requested behind later weights would wait for those.
 template <int WF, int PLANES, int M, int RG, int NB, int U, bool SPLIT>
 __device__ __forceinline__ void moe_products(f32x4 (&acc)[M][RG][NB], const void* base, const uint8_t* scales, long long rows,
                                              const long long (&row)[M][RG], long long ld, int K, const u16* const (&act)[NB],
                                              long long plane, int wave, int waves) {
   const int slabs = (K + kSlab - 1) / kSlab;
+  WeightSlab<WF> w[U][M][RG];
+  u32x4v x[U][4][NB][PLANES];
+  auto request = [&](int u, int slab) {
+#pragma unroll
+    for (int m = 0; m < M; ++m)
+#pragma unroll
+      for (int g = 0; g < RG; ++g) w[u][m][g].load(base, scales, rows, row[m][g], ld, slab, K);
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int p = 0; p < PLANES; ++p) x[u][s][b][p] = *(const u32x4v*)(act[b] + p * plane + slab * kSlab + s * 32);
+  };
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (wave + u * waves < slabs) request(u, wave + u * waves);
   for (int s0 = wave; s0 < slabs; s0 += waves * U) {
-    WeightSlab<WF> w[U][M][RG];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (s0 + u * waves >= slabs) break;
+      const int slab = s0 + u * waves;
+      if (slab >= slabs) break;
 #pragma unroll
-      for (int m = 0; m < M; ++m)
-#pragma unroll
-        for (int g = 0; g < RG; ++g) w[u][m][g].load(base, scales, rows, row[m][g], ld, s0 + u * waves, K);
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (s0 + u * waves >= slabs) break;
-      const int at = (s0 + u * waves) * kSlab;
-#pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        u32x4v x[NB][PLANES];
-#pragma unroll
-        for (int b = 0; b < NB; ++b)
-#pragma unroll
-          for (int p = 0; p < PLANES; ++p) x[b][p] = *(const u32x4v*)(act[b] + p * plane + at + s * 32);
+      for (int s = 0; s < 4; ++s)
 #pragma unroll
         for (int m = 0; m < M; ++m)
 #pragma unroll
@@ -379,22 +386,57 @@ __device__ __forceinline__ void moe_products(f32x4 (&acc)[M][RG][NB], const void
             for (int b = 0; b < NB; ++b) {
 #pragma unroll
               for (int p = 0; p < PLANES; ++p)
-                acc[m][g][b] = WF == CMK_F16 && !SPLIT ? mfma_f16(f, x[b][p], acc[m][g][b]) : mfma_bf16(f, x[b][p], acc[m][g][b]);
-              if constexpr (SPLIT) acc[m][g][b] = mfma_bf16(f2, x[b][0], acc[m][g][b]);
+                acc[m][g][b] = WF == CMK_F16 && !SPLIT ? mfma_f16(f, x[u][s][b][p], acc[m][g][b]) : mfma_bf16(f, x[u][s][b][p], acc[m][g][b]);
+              if constexpr (SPLIT) acc[m][g][b] = mfma_bf16(f2, x[u][s][b][0], acc[m][g][b]);
             }
           }
-      }
+      if (slab + U * waves < slabs) request(u, slab + U * waves);
     }
   }
 }
 
-// RG * 16 gate rows and the up rows that go with them, against the tokens of one
-// expert; the W waves split H and their sums meet in LDS, in order.
-template <int WF, int PLANES, int W, int RG, int NB, int U>
-__device__ __forceinline__ void moe_gate_up_tokens(const MoeArgs& a, int expert, const int* list, int c0, int count, float (*part)[2][RG][NB][64][4]) {
+// Stores four values to consecutive addresses, of which `left` exist.
+template <class T>
+__device__ __forceinline__ void store4(T* p, const T (&v)[4], int left, bool aligned) {
+  if (left >= 4 && aligned) {
+    __builtin_memcpy(p, v, sizeof(v));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < left) p[i] = v[i];
+  }
+}
+
+// Sums of the KS waves that share rows, in the order of the waves; wave 0 of them
+// gets the result.  Every wave of the work-group takes part.
+template <int KS, int N>
+__device__ __forceinline__ void join_waves(f32x4 (&acc)[N], f32x4 (*part)[N][64], int share) {
+  if constexpr (KS > 1) {
+    const int lane = threadIdx.x & 63;
+    if (share > 0)
+#pragma unroll
+      for (int n = 0; n < N; ++n) part[share - 1][n][lane] = acc[n];
+    __syncthreads();
+    if (share == 0)
+#pragma unroll
+      for (int w = 0; w < KS - 1; ++w)
+#pragma unroll
+        for (int n = 0; n < N; ++n) acc[n] += part[w][n][lane];
+    __syncthreads();
+  }
+}
+
+constexpr int kMoeWaves = 4;
+
+// RG * 16 gate rows and the up rows that go with them, against NB * 16 tokens of
+// one expert.  KS waves split H between them; the other waves of the work-group
+// take the next rows.
+template <int WF, int PLANES, int KS, int RG, int NB, int U>
+__device__ __forceinline__ void moe_gate_up_tokens(const MoeArgs& a, int expert, const int* list, int c0, int count, void* part) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int share = wave % KS;
   const int r = lane & 15, q = lane >> 4;
-  const int i0 = blockIdx.x * 16 * RG;
+  const int i0 = (blockIdx.x * (kMoeWaves / KS) + wave / KS) * 16 * RG;
   const char* base = (const char*)a.gate_up + (WF == CMK_MX4 ? (long long)expert * (a.Hp / 2) * (2 * a.I) : expert * a.stride_gate_up * 2);
   const uint8_t* scales = WF == CMK_MX4 ? a.gate_up_scales + (long long)expert * (a.Hp / 32) * (2 * a.I) : nullptr;
   long long row[2][RG];
@@ -407,54 +449,54 @@ __device__ __forceinline__ void moe_gate_up_tokens(const MoeArgs& a, int expert,
   const u16* xs[NB];
 #pragma unroll
   for (int b = 0; b < NB; ++b) xs[b] = a.xp + (long long)(list[min(c0 + b * 16 + r, count - 1)] / a.k) * a.Hp + q * 8;
-  moe_products<WF, PLANES, 2, RG, NB, U, false>(acc, base, scales, 2 * a.I, row, a.ld_gate_up, a.H, xs, (long long)a.T * a.Hp, wave, W);
+  if (i0 < a.I)
+    moe_products<WF, PLANES, 2, RG, NB, U, false>(acc, base, scales, 2 * a.I, row, a.ld_gate_up, a.H, xs, (long long)a.T * a.Hp, share, KS);
+  join_waves<KS, 2 * RG * NB>((f32x4(&)[2 * RG * NB])acc, (f32x4(*)[2 * RG * NB][64])part, share);
+  if (share > 0) return;
 #pragma unroll
-  for (int m = 0; m < 2; ++m)
+  for (int b = 0; b < NB; ++b) {
+    const int c = c0 + b * 16 + r;
+    if (c >= count) continue;
+    u16* h = a.hp + (long long)list[c] * a.Ip;
 #pragma unroll
-    for (int g = 0; g < RG; ++g)
+    for (int g = 0; g < RG; ++g) {
+      const int i1 = i0 + g * 16 + q * 4;  // four consecutive inner features of one token
+      if (i1 >= a.Ip) continue;
+      u16 hi[4], lo[4];
 #pragma unroll
-      for (int b = 0; b < NB; ++b)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) part[wave][m][g][b][lane][i] = acc[m][g][b][i];
-  __syncthreads();
-  for (int v = threadIdx.x; v < NB * RG * 256; v += 64 * W) {
-    // the rows of one token next to each other
-    const int in = v % (16 * RG), c = v / (16 * RG);
-    const int g = in >> 4, l = ((in & 15) >> 2) * 16 + (c & 15), i = in & 3, b = c >> 4;
-    if (c0 + c < count && i0 + in < a.Ip) {
-      float sg = 0, su = 0;
-#pragma unroll
-      for (int w = 0; w < W; ++w) { sg += part[w][0][g][b][l][i]; su += part[w][1][g][b][l][i]; }
-      const float h = i0 + in < a.I ? activate(sg, a.act) * su : 0.0f;
-      // two bf16: 16 bits of mantissa and fp32's range
-      const __bf16 hi = (__bf16)h;
-      const __bf16 lo = (__bf16)(__builtin_isfinite(h) ? h - (float)hi : 0.0f);
-      const long long at = (long long)list[c0 + c] * a.Ip + plane_position<WF == CMK_MX4>(i0 + in);
-      a.hp[at] = __builtin_bit_cast(u16, hi);
-      a.hp[at + (long long)a.T * a.k * a.Ip] = __builtin_bit_cast(u16, lo);
+      for (int i = 0; i < 4; ++i) {
+        const float v = i1 + i < a.I ? activate(acc[0][g][b][i], a.act) * acc[1][g][b][i] : 0.0f;
+        // two bf16: 16 bits of mantissa and fp32's range
+        const __bf16 top = (__bf16)v;
+        hi[i] = __builtin_bit_cast(u16, top);
+        lo[i] = __builtin_bit_cast(u16, (__bf16)(__builtin_isfinite(v) ? v - (float)top : 0.0f));
+      }
+      u16* at = h + plane_position<WF == CMK_MX4>(i1);
+      __builtin_memcpy(at, hi, 8);
+      __builtin_memcpy(at + (long long)a.T * a.k * a.Ip, lo, 8);
     }
   }
-  __syncthreads();
 }
 
-template <int WF, int PLANES, int W, int RG, int U>
-__global__ __launch_bounds__(64 * W) void moe_gate_up_kernel(MoeArgs a) {
+template <int WF, int PLANES, int KS, int RG, int U>
+__global__ __launch_bounds__(64 * kMoeWaves) void moe_gate_up_kernel(MoeArgs a) {
   __shared__ int list[kMoeTokens];
-  __shared__ float part[W][2][RG][2][64][4];
+  __shared__ f32x4 part[KS > 1 ? (KS - 1) * 2 * RG * 2 * 64 : 1];
   int expert;
-  const int count = moe_slots(a, blockIdx.y, list, expert);
+  const int count = moe_slots<kMoeWaves>(a, blockIdx.y, list, expert);
   for (int c0 = 0; c0 < count; c0 += 32) {
-    if (count - c0 <= 16) moe_gate_up_tokens<WF, PLANES, W, RG, 1, U>(a, expert, list, c0, count, (float(*)[2][RG][1][64][4])part);
-    else moe_gate_up_tokens<WF, PLANES, W, RG, 2, U>(a, expert, list, c0, count, part);
+    if (count - c0 <= 16) moe_gate_up_tokens<WF, PLANES, KS, RG, 1, U>(a, expert, list, c0, count, part);
+    else moe_gate_up_tokens<WF, PLANES, KS, RG, 2, 1>(a, expert, list, c0, count, part);
   }
 }
 
 // RG * 16 rows of an expert's down matrix against its slots' activations.
-template <int WF, int W, int RG, int NB, int U>
-__device__ __forceinline__ void moe_down_tokens(const MoeArgs& a, int expert, const int* list, int c0, int count, float (*part)[RG][NB][64][4]) {
+template <int WF, int KS, int RG, int NB, int U>
+__device__ __forceinline__ void moe_down_tokens(const MoeArgs& a, int expert, const int* list, int c0, int count, void* part) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int share = wave % KS;
   const int r = lane & 15, q = lane >> 4;
-  const int n0 = blockIdx.x * 16 * RG;
+  const int n0 = (blockIdx.x * (kMoeWaves / KS) + wave / KS) * 16 * RG;
   const char* base = (const char*)a.down + (WF == CMK_MX4 ? (long long)expert * (a.Ip / 2) * a.H : expert * a.stride_down * 2);
   const uint8_t* scales = WF == CMK_MX4 ? a.down_scales + (long long)expert * (a.Ip / 32) * a.H : nullptr;
   long long row[1][RG];
@@ -464,36 +506,33 @@ __device__ __forceinline__ void moe_down_tokens(const MoeArgs& a, int expert, co
   const u16* hs[NB];
 #pragma unroll
   for (int b = 0; b < NB; ++b) hs[b] = a.hp + (long long)list[min(c0 + b * 16 + r, count - 1)] * a.Ip + q * 8;
-  moe_products<WF, 2, 1, RG, NB, U, WF == CMK_F16>(acc, base, scales, a.H, row, a.ld_down, a.I, hs, (long long)a.T * a.k * a.Ip, wave, W);
+  if (n0 < a.H)
+    moe_products<WF, 2, 1, RG, NB, U, WF == CMK_F16>(acc, base, scales, a.H, row, a.ld_down, a.I, hs, (long long)a.T * a.k * a.Ip, share, KS);
+  join_waves<KS, RG * NB>((f32x4(&)[RG * NB])acc, (f32x4(*)[RG * NB][64])part, share);
+  if (share > 0) return;
 #pragma unroll
-  for (int g = 0; g < RG; ++g)
+  for (int b = 0; b < NB; ++b) {
+    const int c = c0 + b * 16 + r;
+    if (c >= count) continue;
+    float* y = a.yp + (long long)list[c] * a.H;
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) part[wave][g][b][lane][i] = acc[0][g][b][i];
-  __syncthreads();
-  for (int v = threadIdx.x; v < NB * RG * 256; v += 64 * W) {
-    const int in = v % (16 * RG), c = v / (16 * RG);
-    const int g = in >> 4, l = ((in & 15) >> 2) * 16 + (c & 15), i = in & 3, b = c >> 4;
-    if (c0 + c < count && n0 + in < a.H) {
-      float s = 0;
-#pragma unroll
-      for (int w = 0; w < W; ++w) s += part[w][g][b][l][i];
-      a.yp[(long long)list[c0 + c] * a.H + n0 + in] = s;
+    for (int g = 0; g < RG; ++g) {
+      const int n = n0 + g * 16 + q * 4;
+      const float v[4] = {acc[0][g][b][0], acc[0][g][b][1], acc[0][g][b][2], acc[0][g][b][3]};
+      store4(y + n, v, a.H - n, (a.H & 3) == 0);
     }
   }
-  __syncthreads();
 }
 
-template <int WF, int W, int RG, int U>
-__global__ __launch_bounds__(64 * W) void moe_down_kernel(MoeArgs a) {
+template <int WF, int KS, int RG, int U>
+__global__ __launch_bounds__(64 * kMoeWaves) void moe_down_kernel(MoeArgs a) {
   __shared__ int list[kMoeTokens];
-  __shared__ float part[W][RG][2][64][4];
+  __shared__ f32x4 part[KS > 1 ? (KS - 1) * RG * 2 * 64 : 1];
   int expert;
-  const int count = moe_slots(a, blockIdx.y, list, expert);
+  const int count = moe_slots<kMoeWaves>(a, blockIdx.y, list, expert);
   for (int c0 = 0; c0 < count; c0 += 32) {
-    if (count - c0 <= 16) moe_down_tokens<WF, W, RG, 1, U>(a, expert, list, c0, count, (float(*)[RG][1][64][4])part);
-    else moe_down_tokens<WF, W, RG, 2, U>(a, expert, list, c0, count, part);
+    if (count - c0 <= 16) moe_down_tokens<WF, KS, RG, 1, U>(a, expert, list, c0, count, part);
+    else moe_down_tokens<WF, KS, RG, 2, 1>(a, expert, list, c0, count, part);
   }
 }
 
@@ -573,19 +612,31 @@ extern "C" int cmk_moe(const void* x, const void* router, const void* gate_up, c
   }
   hipLaunchKernelGGL(moe_select_kernel, dim3(d->T), dim3(256), 0, st, a);
   const int units = d->T * d->k <= d->E ? d->T * d->k : d->E;
-  auto experts_kernel = [&](auto kernel, int rows, int rg, int w) {
-    hipLaunchKernelGGL(kernel, dim3(ceil_div(rows, 16 * rg), units), dim3(64 * w), 0, st, a);
+  // rows a work-group: 16 * rg for each of the kMoeWaves / ks groups of waves
+  auto experts_kernel = [&](auto kernel, int rows, int rg, int ks) {
+    hipLaunchKernelGGL(kernel, dim3(ceil_div(rows, 16 * rg * kMoeWaves / ks), units), dim3(64 * kMoeWaves), 0, st, a);
   };
+  const bool many = units >= 32;
   if (d->w_dtype == CMK_MX4) {
-    if (p.x_planes == 1) experts_kernel(moe_gate_up_kernel<CMK_MX4, 1, 4, 2, 2>, p.Ip, 2, 4);
-    else experts_kernel(moe_gate_up_kernel<CMK_MX4, 2, 4, 2, 2>, p.Ip, 2, 4);
-    experts_kernel(moe_down_kernel<CMK_MX4, 4, 4, 2>, d->H, 4, 4);
+    if (p.x_planes == 1) {
+      if (many) experts_kernel(moe_gate_up_kernel<CMK_MX4, 1, 1, 1, 2>, p.Ip, 1, 1);
+      else experts_kernel(moe_gate_up_kernel<CMK_MX4, 1, 4, 1, 2>, p.Ip, 1, 4);
+    } else {
+      if (many) experts_kernel(moe_gate_up_kernel<CMK_MX4, 2, 1, 1, 2>, p.Ip, 1, 1);
+      else experts_kernel(moe_gate_up_kernel<CMK_MX4, 2, 4, 1, 2>, p.Ip, 1, 4);
+    }
+    if (many) experts_kernel(moe_down_kernel<CMK_MX4, 1, 2, 2>, d->H, 2, 1);
+    else experts_kernel(moe_down_kernel<CMK_MX4, 4, 2, 2>, d->H, 2, 4);
   } else if (d->w_dtype == CMK_BF16) {
-    experts_kernel(moe_gate_up_kernel<CMK_BF16, 1, 4, 1, 2>, p.Ip, 1, 4);
-    experts_kernel(moe_down_kernel<CMK_BF16, 4, 1, 2>, d->H, 1, 4);
+    if (many) experts_kernel(moe_gate_up_kernel<CMK_BF16, 1, 1, 1, 2>, p.Ip, 1, 1);
+    else experts_kernel(moe_gate_up_kernel<CMK_BF16, 1, 4, 1, 2>, p.Ip, 1, 4);
+    if (many) experts_kernel(moe_down_kernel<CMK_BF16, 1, 1, 2>, d->H, 1, 1);
+    else experts_kernel(moe_down_kernel<CMK_BF16, 4, 1, 2>, d->H, 1, 4);
   } else {
-    experts_kernel(moe_gate_up_kernel<CMK_F16, 1, 4, 1, 2>, p.Ip, 1, 4);
-    experts_kernel(moe_down_kernel<CMK_F16, 4, 1, 2>, d->H, 1, 4);
+    if (many) experts_kernel(moe_gate_up_kernel<CMK_F16, 1, 1, 1, 2>, p.Ip, 1, 1);
+    else experts_kernel(moe_gate_up_kernel<CMK_F16, 1, 4, 1, 2>, p.Ip, 1, 4);
+    if (many) experts_kernel(moe_down_kernel<CMK_F16, 1, 1, 2>, d->H, 1, 1);
+    else experts_kernel(moe_down_kernel<CMK_F16, 4, 1, 2>, d->H, 1, 4);
   }
   const dim3 out_grid(ceil_div(d->H, 256), d->T);
   if (d->x_dtype == CMK_BF16) hipLaunchKernelGGL(moe_combine_kernel<__bf16>, out_grid, dim3(256), 0, st, a);
