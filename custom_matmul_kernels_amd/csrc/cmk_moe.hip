@@ -17,6 +17,7 @@ constexpr int kMoeTokens = 256;    // of one call
 constexpr int kMoeExperts = 1024;
 constexpr int kMoeChoices = 32;
 constexpr int kRouterWaves = 4;
+constexpr int kMoeWaves = 4;  // of the experts' kernels
 
 typedef double f64x4 __attribute__((ext_vector_type(4)));
 
@@ -342,56 +343,85 @@ __device__ __forceinline__ float activate(float g, int act) {
   return 0.5f * g * (1.0f + erff(g * 0.70710678118654752f));
 }
 
-// The products of RG groups of 16 rows of one expert's matrix with up to NB * 16
-// of its slots, over the slabs of one wave; M products (gate and up, or one) share
-// the activations.  A ring of U slabs of weights and activations is under way:
-// vector-memory loads are awaited in the order of their issue, so that activations
-// requested behind later weights would wait for those.
-template <int WF, int PLANES, int M, int RG, int NB, int U, bool SPLIT>
+// Activations of one pass in LDS: rows of 16-bit elements, plane by plane, a row
+// 16 bytes longer than what it holds so that the 16 rows of a fragment spread over
+// the banks.  Where the rows do not fit whole, the pass goes through k in pieces.
+constexpr int kActBytes = 36 * 1024;
+
+// The products of RG groups of 16 rows of one expert's matrix with the `count`
+// activation rows (at most NB * 16) that `source` gives, over the slabs of one wave
+// of the KS that split them; M products (gate and up, or one) share the activations.
+//
+// A ring of U slabs of weights is under way in registers.  The activations come
+// through LDS: vector-memory loads are awaited in the order of their issue, so that
+// activations loaded between the weights would wait for weights of later slabs (and
+// they are read by four waves).
+template <int WF, int PLANES, int M, int RG, int NB, int U, int KS, bool SPLIT, class Source>
 __device__ __forceinline__ void moe_products(f32x4 (&acc)[M][RG][NB], const void* base, const uint8_t* scales, long long rows,
-                                             const long long (&row)[M][RG], long long ld, int K, const u16* const (&act)[NB],
-                                             long long plane, int wave, int waves) {
+                                             const long long (&row)[M][RG], long long ld, int K, int count, Source source,
+                                             long long plane, int share, bool idle, char* lds) {
+  const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
   const int slabs = (K + kSlab - 1) / kSlab;
-  WeightSlab<WF> w[U][M][RG];
-  u32x4v x[U][4][NB][PLANES];
-  auto request = [&](int u, int slab) {
+  const int fit = (kActBytes / (PLANES * count) - 16) / (2 * kSlab);  // slabs of all rows that LDS holds
+  const int piece = slabs <= fit ? slabs : fit;
+  const int pitch = piece * 2 * kSlab + 16;
+  const char* mine[NB];
 #pragma unroll
-    for (int m = 0; m < M; ++m)
+  for (int b = 0; b < NB; ++b) mine[b] = lds + min(b * 16 + r, count - 1) * pitch + q * 16;
+  const int plane_bytes = count * pitch;
+  for (int first = 0; first < slabs; first += piece) {
+    const int end = min(slabs, first + piece);
+    WeightSlab<WF> w[U][M][RG];
+    auto request = [&](int u, int slab) {
 #pragma unroll
-      for (int g = 0; g < RG; ++g) w[u][m][g].load(base, scales, rows, row[m][g], ld, slab, K);
+      for (int m = 0; m < M; ++m)
 #pragma unroll
-    for (int s = 0; s < 4; ++s)
+        for (int g = 0; g < RG; ++g) w[u][m][g].load(base, scales, rows, row[m][g], ld, slab, K);
+    };
+    if (!idle)
 #pragma unroll
-      for (int b = 0; b < NB; ++b)
+      for (int u = 0; u < U; ++u)
+        if (first + share + u * KS < end) request(u, first + share + u * KS);
+    if (first > 0) __syncthreads();
+    const int units = (end - first) * 16;  // 16-byte units of a row
+    for (int v = threadIdx.x; v < PLANES * count * units; v += 64 * kMoeWaves) {
+      const int line = v / units, at = v - line * units;
+      const int c = line % count, p = line / count;
+      *(u32x4v*)(lds + p * plane_bytes + c * pitch + at * 16) = *(const u32x4v*)(source(c) + p * plane + first * kSlab + at * 8);
+    }
+    __syncthreads();
+    if (!idle)
+      for (int s0 = first + share; s0 < end; s0 += KS * U) {
 #pragma unroll
-        for (int p = 0; p < PLANES; ++p) x[u][s][b][p] = *(const u32x4v*)(act[b] + p * plane + slab * kSlab + s * 32);
-  };
+        for (int u = 0; u < U; ++u) {
+          const int slab = s0 + u * KS;
+          if (slab >= end) break;
 #pragma unroll
-  for (int u = 0; u < U; ++u)
-    if (wave + u * waves < slabs) request(u, wave + u * waves);
-  for (int s0 = wave; s0 < slabs; s0 += waves * U) {
+          for (int s = 0; s < 4; ++s) {
+            u32x4v x[NB][PLANES];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int slab = s0 + u * waves;
-      if (slab >= slabs) break;
-#pragma unroll
-      for (int s = 0; s < 4; ++s)
-#pragma unroll
-        for (int m = 0; m < M; ++m)
-#pragma unroll
-          for (int g = 0; g < RG; ++g) {
-            u32x4v f = w[u][m][g].step(s), f2;
-            if constexpr (SPLIT) split_f16(w[u][m][g].step(s), f, f2);
-#pragma unroll
-            for (int b = 0; b < NB; ++b) {
+            for (int b = 0; b < NB; ++b)
 #pragma unroll
               for (int p = 0; p < PLANES; ++p)
-                acc[m][g][b] = WF == CMK_F16 && !SPLIT ? mfma_f16(f, x[u][s][b][p], acc[m][g][b]) : mfma_bf16(f, x[u][s][b][p], acc[m][g][b]);
-              if constexpr (SPLIT) acc[m][g][b] = mfma_bf16(f2, x[u][s][b][0], acc[m][g][b]);
-            }
+                x[b][p] = *(const u32x4v*)(mine[b] + p * plane_bytes + (slab - first) * 2 * kSlab + s * 64);
+#pragma unroll
+            for (int m = 0; m < M; ++m)
+#pragma unroll
+              for (int g = 0; g < RG; ++g) {
+                u32x4v f = w[u][m][g].step(s), f2;
+                if constexpr (SPLIT) split_f16(w[u][m][g].step(s), f, f2);
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+#pragma unroll
+                  for (int p = 0; p < PLANES; ++p)
+                    acc[m][g][b] = WF == CMK_F16 && !SPLIT ? mfma_f16(f, x[b][p], acc[m][g][b]) : mfma_bf16(f, x[b][p], acc[m][g][b]);
+                  if constexpr (SPLIT) acc[m][g][b] = mfma_bf16(f2, x[b][0], acc[m][g][b]);
+                }
+              }
           }
-      if (slab + U * waves < slabs) request(u, slab + U * waves);
-    }
+          if (slab + U * KS < end) request(u, slab + U * KS);
+        }
+      }
   }
 }
 
@@ -407,12 +437,16 @@ __device__ __forceinline__ void store4(T* p, const T (&v)[4], int left, bool ali
   }
 }
 
-// Sums of the KS waves that share rows, in the order of the waves; wave 0 of them
-// gets the result.  Every wave of the work-group takes part.
+// Sums of the KS waves that share rows, in the order of the waves; the first of
+// them gets the result.  Every wave of the work-group takes part; the LDS is the
+// activations'.
 template <int KS, int N>
 __device__ __forceinline__ void join_waves(f32x4 (&acc)[N], f32x4 (*part)[N][64], int share) {
+  static_assert((size_t)kMoeWaves / KS * (KS - 1) * N * 64 * 16 <= kActBytes, "the partial sums fit");
+  const int lane = threadIdx.x & 63;
+  __syncthreads();  // the activations have been read
   if constexpr (KS > 1) {
-    const int lane = threadIdx.x & 63;
+    part += (threadIdx.x >> 6) / KS * (KS - 1);
     if (share > 0)
 #pragma unroll
       for (int n = 0; n < N; ++n) part[share - 1][n][lane] = acc[n];
@@ -426,13 +460,11 @@ __device__ __forceinline__ void join_waves(f32x4 (&acc)[N], f32x4 (*part)[N][64]
   }
 }
 
-constexpr int kMoeWaves = 4;
-
 // RG * 16 gate rows and the up rows that go with them, against NB * 16 tokens of
 // one expert.  KS waves split H between them; the other waves of the work-group
 // take the next rows.
 template <int WF, int PLANES, int KS, int RG, int NB, int U>
-__device__ __forceinline__ void moe_gate_up_tokens(const MoeArgs& a, int expert, const int* list, int c0, int count, void* part) {
+__device__ __forceinline__ void moe_gate_up_tokens(const MoeArgs& a, int expert, const int* list, int c0, int count, char* lds) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int share = wave % KS;
   const int r = lane & 15, q = lane >> 4;
@@ -446,12 +478,10 @@ __device__ __forceinline__ void moe_gate_up_tokens(const MoeArgs& a, int expert,
     row[1][g] = a.I + row[0][g];
   }
   f32x4 acc[2][RG][NB] = {};
-  const u16* xs[NB];
-#pragma unroll
-  for (int b = 0; b < NB; ++b) xs[b] = a.xp + (long long)(list[min(c0 + b * 16 + r, count - 1)] / a.k) * a.Hp + q * 8;
-  if (i0 < a.I)
-    moe_products<WF, PLANES, 2, RG, NB, U, false>(acc, base, scales, 2 * a.I, row, a.ld_gate_up, a.H, xs, (long long)a.T * a.Hp, share, KS);
-  join_waves<KS, 2 * RG * NB>((f32x4(&)[2 * RG * NB])acc, (f32x4(*)[2 * RG * NB][64])part, share);
+  auto source = [&](int c) { return a.xp + (long long)(list[c0 + c] / a.k) * a.Hp; };
+  moe_products<WF, PLANES, 2, RG, NB, U, KS, false>(acc, base, scales, 2 * a.I, row, a.ld_gate_up, a.H, min(count - c0, NB * 16),
+                                                    source, (long long)a.T * a.Hp, share, i0 >= a.I, lds);
+  join_waves<KS, 2 * RG * NB>((f32x4(&)[2 * RG * NB])acc, (f32x4(*)[2 * RG * NB][64])lds, share);
   if (share > 0) return;
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
@@ -481,18 +511,18 @@ __device__ __forceinline__ void moe_gate_up_tokens(const MoeArgs& a, int expert,
 template <int WF, int PLANES, int KS, int RG, int U>
 __global__ __launch_bounds__(64 * kMoeWaves) void moe_gate_up_kernel(MoeArgs a) {
   __shared__ int list[kMoeTokens];
-  __shared__ f32x4 part[KS > 1 ? (KS - 1) * 2 * RG * 2 * 64 : 1];
+  __shared__ __attribute__((aligned(16))) char lds[kActBytes];
   int expert;
   const int count = moe_slots<kMoeWaves>(a, blockIdx.y, list, expert);
   for (int c0 = 0; c0 < count; c0 += 32) {
-    if (count - c0 <= 16) moe_gate_up_tokens<WF, PLANES, KS, RG, 1, U>(a, expert, list, c0, count, part);
-    else moe_gate_up_tokens<WF, PLANES, KS, RG, 2, 1>(a, expert, list, c0, count, part);
+    if (count - c0 <= 16) moe_gate_up_tokens<WF, PLANES, KS, RG, 1, U>(a, expert, list, c0, count, lds);
+    else moe_gate_up_tokens<WF, PLANES, KS, RG, 2, U>(a, expert, list, c0, count, lds);
   }
 }
 
 // RG * 16 rows of an expert's down matrix against its slots' activations.
 template <int WF, int KS, int RG, int NB, int U>
-__device__ __forceinline__ void moe_down_tokens(const MoeArgs& a, int expert, const int* list, int c0, int count, void* part) {
+__device__ __forceinline__ void moe_down_tokens(const MoeArgs& a, int expert, const int* list, int c0, int count, char* lds) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int share = wave % KS;
   const int r = lane & 15, q = lane >> 4;
@@ -503,12 +533,10 @@ __device__ __forceinline__ void moe_down_tokens(const MoeArgs& a, int expert, co
 #pragma unroll
   for (int g = 0; g < RG; ++g) row[0][g] = min(n0 + g * 16 + r, a.H - 1);
   f32x4 acc[1][RG][NB] = {};
-  const u16* hs[NB];
-#pragma unroll
-  for (int b = 0; b < NB; ++b) hs[b] = a.hp + (long long)list[min(c0 + b * 16 + r, count - 1)] * a.Ip + q * 8;
-  if (n0 < a.H)
-    moe_products<WF, 2, 1, RG, NB, U, WF == CMK_F16>(acc, base, scales, a.H, row, a.ld_down, a.I, hs, (long long)a.T * a.k * a.Ip, share, KS);
-  join_waves<KS, RG * NB>((f32x4(&)[RG * NB])acc, (f32x4(*)[RG * NB][64])part, share);
+  auto source = [&](int c) { return a.hp + (long long)list[c0 + c] * a.Ip; };
+  moe_products<WF, 2, 1, RG, NB, U, KS, WF == CMK_F16>(acc, base, scales, a.H, row, a.ld_down, a.I, min(count - c0, NB * 16), source,
+                                                       (long long)a.T * a.k * a.Ip, share, n0 >= a.H, lds);
+  join_waves<KS, RG * NB>((f32x4(&)[RG * NB])acc, (f32x4(*)[RG * NB][64])lds, share);
   if (share > 0) return;
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
@@ -527,12 +555,12 @@ __device__ __forceinline__ void moe_down_tokens(const MoeArgs& a, int expert, co
 template <int WF, int KS, int RG, int U>
 __global__ __launch_bounds__(64 * kMoeWaves) void moe_down_kernel(MoeArgs a) {
   __shared__ int list[kMoeTokens];
-  __shared__ f32x4 part[KS > 1 ? (KS - 1) * RG * 2 * 64 : 1];
+  __shared__ __attribute__((aligned(16))) char lds[kActBytes];
   int expert;
   const int count = moe_slots<kMoeWaves>(a, blockIdx.y, list, expert);
   for (int c0 = 0; c0 < count; c0 += 32) {
-    if (count - c0 <= 16) moe_down_tokens<WF, KS, RG, 1, U>(a, expert, list, c0, count, part);
-    else moe_down_tokens<WF, KS, RG, 2, 1>(a, expert, list, c0, count, part);
+    if (count - c0 <= 16) moe_down_tokens<WF, KS, RG, 1, U>(a, expert, list, c0, count, lds);
+    else moe_down_tokens<WF, KS, RG, 2, U>(a, expert, list, c0, count, lds);
   }
 }
 
@@ -619,18 +647,18 @@ extern "C" int cmk_moe(const void* x, const void* router, const void* gate_up, c
   const bool many = units >= 32;
   if (d->w_dtype == CMK_MX4) {
     if (p.x_planes == 1) {
-      if (many) experts_kernel(moe_gate_up_kernel<CMK_MX4, 1, 1, 1, 2>, p.Ip, 1, 1);
+      if (many) experts_kernel(moe_gate_up_kernel<CMK_MX4, 1, 1, 1, 3>, p.Ip, 1, 1);
       else experts_kernel(moe_gate_up_kernel<CMK_MX4, 1, 4, 1, 2>, p.Ip, 1, 4);
     } else {
       if (many) experts_kernel(moe_gate_up_kernel<CMK_MX4, 2, 1, 1, 2>, p.Ip, 1, 1);
       else experts_kernel(moe_gate_up_kernel<CMK_MX4, 2, 4, 1, 2>, p.Ip, 1, 4);
     }
-    if (many) experts_kernel(moe_down_kernel<CMK_MX4, 1, 2, 2>, d->H, 2, 1);
+    if (many) experts_kernel(moe_down_kernel<CMK_MX4, 2, 2, 2>, d->H, 2, 2);
     else experts_kernel(moe_down_kernel<CMK_MX4, 4, 2, 2>, d->H, 2, 4);
   } else if (d->w_dtype == CMK_BF16) {
-    if (many) experts_kernel(moe_gate_up_kernel<CMK_BF16, 1, 1, 1, 2>, p.Ip, 1, 1);
+    if (many) experts_kernel(moe_gate_up_kernel<CMK_BF16, 1, 2, 1, 2>, p.Ip, 1, 2);
     else experts_kernel(moe_gate_up_kernel<CMK_BF16, 1, 4, 1, 2>, p.Ip, 1, 4);
-    if (many) experts_kernel(moe_down_kernel<CMK_BF16, 1, 1, 2>, d->H, 1, 1);
+    if (many) experts_kernel(moe_down_kernel<CMK_BF16, 2, 2, 3>, d->H, 2, 2);
     else experts_kernel(moe_down_kernel<CMK_BF16, 4, 1, 2>, d->H, 1, 4);
   } else {
     if (many) experts_kernel(moe_gate_up_kernel<CMK_F16, 1, 1, 1, 2>, p.Ip, 1, 1);
