@@ -167,19 +167,21 @@ def float_type(dtype, what):
 def refuse_grad(*tensors):
     """The operators for serving have no backward pass: an operand that asks for
     a gradient is refused, not cut out of the graph in silence."""
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t.requires_grad:
-                raise RuntimeError("this operator has no backward pass; call it under torch.no_grad() or "
-                                   "with detached operands")
+    for t in tensors:
+        if t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("this operator has no backward pass; call it under torch.no_grad() or "
+                               "with detached operands")
 
 
 def call(fn, device, *args):
     """Calls a library entry point on the current stream of `device`, with that
-    device current, and raises for a status other than 0."""
-    stream = torch.cuda.current_stream(device).cuda_stream
-    if torch.cuda.current_device() == device.index:
-        _lib.check(fn(*args, stream))
+    device current, and raises for a status other than 0.  (The raw stream handle
+    costs 0.1 us where a Stream object costs 2.)"""
+    index = device.index
+    if torch.cuda.current_device() == index:
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(device):
-            _lib.check(fn(*args, stream))
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status:
+        _lib.check(status)

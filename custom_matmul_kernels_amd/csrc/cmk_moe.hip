@@ -520,6 +520,27 @@ __global__ __launch_bounds__(64 * kMoeWaves) void moe_gate_up_kernel(MoeArgs a) 
   }
 }
 
+// The same for a single token, with the choice made on the way: every work-group
+// makes it for itself (one L2 read of the logits; a kernel of its own took 4 us of
+// 32 at 64 experts x 2048 x 1024), the first one writes it down.
+template <int WF, int PLANES, int KS, int RG, int U>
+__global__ __launch_bounds__(64 * kMoeWaves) void moe_gate_up_single_kernel(MoeArgs a) {
+  static_assert(sizeof(MoeChoice) <= kActBytes && kMoeWaves == 4, "the choice takes 256 threads");
+  __shared__ __attribute__((aligned(16))) char lds[kActBytes];
+  __shared__ int list[1];
+  MoeChoice& c = *(MoeChoice*)lds;
+  moe_choose(a, 0, c);
+  const int expert = __builtin_amdgcn_readfirstlane(c.pick[blockIdx.y]);
+  if (blockIdx.x == 0 && blockIdx.y == 0 && (int)threadIdx.x < a.k) {
+    a.chosen[threadIdx.x] = c.pick[threadIdx.x];
+    a.experts[threadIdx.x] = c.pick[threadIdx.x];
+    a.weights[threadIdx.x] = moe_weight(a, c, threadIdx.x);
+  }
+  if (threadIdx.x == 0) list[0] = blockIdx.y;
+  __syncthreads();  // list is there and the choice has been read
+  moe_gate_up_tokens<WF, PLANES, KS, RG, 1, U>(a, expert, list, 0, 1, lds);
+}
+
 // RG * 16 rows of an expert's down matrix against its slots' activations.
 template <int WF, int KS, int RG, int NB, int U>
 __device__ __forceinline__ void moe_down_tokens(const MoeArgs& a, int expert, const int* list, int c0, int count, char* lds) {
@@ -571,6 +592,85 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(MoeArgs a) {
   float s = 0;
   for (int j = 0; j < a.k; ++j) s = fmaf(a.weights[t * a.k + j], a.yp[((long long)t * a.k + j) * a.H + n], s);
   ((T*)a.y)[(long long)t * a.H + n] = from_f32<T>(s);
+}
+
+// The down products of a single token and their weighted sum: a work-group takes 16
+// rows and all the chosen experts.  A unit is one slab of one of them; the W waves
+// take units in turn, a ring of U under way each, and their sums meet in LDS in the
+// order of the waves.  The activations are multiplied by the weights as they are
+// staged and split into two bf16 again.
+constexpr int kSingleUnits = 96;  // staged at a time
+
+template <int WF, class T, int W, int U>
+__global__ __launch_bounds__(64 * W) void moe_down_single_kernel(MoeArgs a) {
+  __shared__ __attribute__((aligned(16))) char lds[kSingleUnits * 4 * kSlab];
+  __shared__ f32x4 part[W][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r = lane & 15, q = lane >> 4;
+  const int n0 = blockIdx.x * 16;
+  const int row = min(n0 + r, a.H - 1);
+  const int slabs = a.Ip / kSlab, units = a.k * slabs;
+  const long long plane = (long long)a.k * a.Ip;
+  f32x4 acc = {};
+  for (int first = 0; first < units; first += kSingleUnits) {
+    const int end = min(units, first + kSingleUnits);
+    WeightSlab<WF> w[U];
+    auto request = [&](int u, int unit) {
+      const int j = unit / slabs, expert = a.chosen[j];
+      const char* base = (const char*)a.down + (WF == CMK_MX4 ? (long long)expert * (a.Ip / 2) * a.H : expert * a.stride_down * 2);
+      const uint8_t* scales = WF == CMK_MX4 ? a.down_scales + (long long)expert * (a.Ip / 32) * a.H : nullptr;
+      w[u].load(base, scales, a.H, row, a.ld_down, unit - j * slabs, a.I);
+    };
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (first + wave + u * W < end) request(u, first + wave + u * W);
+    if (first > 0) __syncthreads();
+    for (int v = threadIdx.x; v < (end - first) * (kSlab / 8); v += 64 * W) {
+      const int unit = v / (kSlab / 8), at = v % (kSlab / 8) * 8;
+      const long long from = (long long)(first + unit) * kSlab + at;  // units are consecutive in memory
+      const float weight = a.weights[(first + unit) / slabs];
+      u16 hi[8], lo[8];
+      __builtin_memcpy(hi, a.hp + from, 16);
+      __builtin_memcpy(lo, a.hp + plane + from, 16);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float f = weight * (__uint_as_float((unsigned)hi[i] << 16) + __uint_as_float((unsigned)lo[i] << 16));
+        const __bf16 top = (__bf16)f;
+        hi[i] = __builtin_bit_cast(u16, top);
+        lo[i] = __builtin_bit_cast(u16, (__bf16)(__builtin_isfinite(f) ? f - (float)top : 0.0f));
+      }
+      __builtin_memcpy(lds + unit * 4 * kSlab + at * 2, hi, 16);
+      __builtin_memcpy(lds + unit * 4 * kSlab + 2 * kSlab + at * 2, lo, 16);
+    }
+    __syncthreads();
+    for (int s0 = first + wave; s0 < end; s0 += W * U) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int unit = s0 + u * W;
+        if (unit >= end) break;
+        const char* x = lds + (unit - first) * 4 * kSlab + q * 16;
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          const u32x4v hi = *(const u32x4v*)(x + s * 64), lo = *(const u32x4v*)(x + 2 * kSlab + s * 64);
+          u32x4v f = w[u].step(s), f2;
+          if constexpr (WF == CMK_F16) split_f16(w[u].step(s), f, f2);
+          acc = mfma_bf16(f, hi, acc);
+          acc = mfma_bf16(f, lo, acc);
+          if constexpr (WF == CMK_F16) acc = mfma_bf16(f2, hi, acc);
+        }
+        if (unit + U * W < end) request(u, unit + U * W);
+      }
+    }
+  }
+  part[wave][lane] = acc;
+  __syncthreads();
+  // every column holds the token's sums: row 4 q + i in component i of lane 16 q
+  if (threadIdx.x < 16 && n0 + (int)threadIdx.x < a.H) {
+    float sum = 0;
+#pragma unroll
+    for (int v = 0; v < W; ++v) sum += part[v][threadIdx.x >> 2 << 4][threadIdx.x & 3];
+    ((T*)a.y)[n0 + threadIdx.x] = from_f32<T>(sum);
+  }
 }
 
 static int check_moe(const cmk_moe_desc* d) {
@@ -638,6 +738,23 @@ extern "C" int cmk_moe(const void* x, const void* router, const void* gate_up, c
     if (four) r32 ? logits(moe_logits_kernel<_Float16, float, true, 2>) : logits(moe_logits_kernel<_Float16, _Float16, true, 2>);
     else r32 ? logits(moe_logits_kernel<_Float16, float, false, 1>) : logits(moe_logits_kernel<_Float16, _Float16, false, 1>);
   }
+  if (d->T == 1) {
+    const dim3 up(ceil_div(p.Ip, 16), d->k), dn(ceil_div(d->H, 16)), b(64 * kMoeWaves);
+    if (d->w_dtype == CMK_BF16) {
+      hipLaunchKernelGGL((moe_gate_up_single_kernel<CMK_BF16, 1, 4, 1, 4>), up, b, 0, st, a);
+      hipLaunchKernelGGL((moe_down_single_kernel<CMK_BF16, __bf16, 16, 3>), dn, dim3(1024), 0, st, a);
+    } else if (d->w_dtype == CMK_F16) {
+      hipLaunchKernelGGL((moe_gate_up_single_kernel<CMK_F16, 1, 4, 1, 4>), up, b, 0, st, a);
+      hipLaunchKernelGGL((moe_down_single_kernel<CMK_F16, _Float16, 16, 3>), dn, dim3(1024), 0, st, a);
+    } else if (d->x_dtype == CMK_BF16) {
+      hipLaunchKernelGGL((moe_gate_up_single_kernel<CMK_MX4, 1, 4, 1, 4>), up, b, 0, st, a);
+      hipLaunchKernelGGL((moe_down_single_kernel<CMK_MX4, __bf16, 16, 4>), dn, dim3(1024), 0, st, a);
+    } else {
+      hipLaunchKernelGGL((moe_gate_up_single_kernel<CMK_MX4, 2, 4, 1, 4>), up, b, 0, st, a);
+      hipLaunchKernelGGL((moe_down_single_kernel<CMK_MX4, _Float16, 16, 4>), dn, dim3(1024), 0, st, a);
+    }
+    return hip_status(hipGetLastError(), "cmk_moe launch");
+  }
   hipLaunchKernelGGL(moe_select_kernel, dim3(d->T), dim3(256), 0, st, a);
   const int units = d->T * d->k <= d->E ? d->T * d->k : d->E;
   // rows a work-group: 16 * rg for each of the kMoeWaves / ks groups of waves
@@ -650,20 +767,20 @@ extern "C" int cmk_moe(const void* x, const void* router, const void* gate_up, c
       if (many) experts_kernel(moe_gate_up_kernel<CMK_MX4, 1, 1, 1, 3>, p.Ip, 1, 1);
       else experts_kernel(moe_gate_up_kernel<CMK_MX4, 1, 4, 1, 2>, p.Ip, 1, 4);
     } else {
-      if (many) experts_kernel(moe_gate_up_kernel<CMK_MX4, 2, 1, 1, 2>, p.Ip, 1, 1);
+      if (many) experts_kernel(moe_gate_up_kernel<CMK_MX4, 2, 1, 1, 3>, p.Ip, 1, 1);
       else experts_kernel(moe_gate_up_kernel<CMK_MX4, 2, 4, 1, 2>, p.Ip, 1, 4);
     }
-    if (many) experts_kernel(moe_down_kernel<CMK_MX4, 2, 2, 2>, d->H, 2, 2);
+    if (many) experts_kernel(moe_down_kernel<CMK_MX4, 2, 4, 2>, d->H, 4, 2);
     else experts_kernel(moe_down_kernel<CMK_MX4, 4, 2, 2>, d->H, 2, 4);
   } else if (d->w_dtype == CMK_BF16) {
-    if (many) experts_kernel(moe_gate_up_kernel<CMK_BF16, 1, 2, 1, 2>, p.Ip, 1, 2);
+    if (many) experts_kernel(moe_gate_up_kernel<CMK_BF16, 1, 4, 1, 1>, p.Ip, 1, 4);
     else experts_kernel(moe_gate_up_kernel<CMK_BF16, 1, 4, 1, 2>, p.Ip, 1, 4);
-    if (many) experts_kernel(moe_down_kernel<CMK_BF16, 2, 2, 3>, d->H, 2, 2);
+    if (many) experts_kernel(moe_down_kernel<CMK_BF16, 1, 1, 4>, d->H, 1, 1);
     else experts_kernel(moe_down_kernel<CMK_BF16, 4, 1, 2>, d->H, 1, 4);
   } else {
-    if (many) experts_kernel(moe_gate_up_kernel<CMK_F16, 1, 1, 1, 2>, p.Ip, 1, 1);
+    if (many) experts_kernel(moe_gate_up_kernel<CMK_F16, 1, 4, 1, 1>, p.Ip, 1, 4);
     else experts_kernel(moe_gate_up_kernel<CMK_F16, 1, 4, 1, 2>, p.Ip, 1, 4);
-    if (many) experts_kernel(moe_down_kernel<CMK_F16, 1, 1, 2>, d->H, 1, 1);
+    if (many) experts_kernel(moe_down_kernel<CMK_F16, 1, 1, 4>, d->H, 1, 1);
     else experts_kernel(moe_down_kernel<CMK_F16, 4, 1, 2>, d->H, 1, 4);
   }
   const dim3 out_grid(ceil_div(d->H, 256), d->T);

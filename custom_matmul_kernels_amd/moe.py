@@ -41,7 +41,7 @@ class MoECUDA:
         """(pointer, scales' pointer, row stride, expert stride) of [e, r, c] weights."""
         if isinstance(W, MX4Tensor):
             assert W.k_axis == -1, "the blocks of %s must run along its last axis" % name
-            return W.codes.data_ptr(), W.scales.data_ptr(), 0, 0
+            return W._pointers() + (0, 0)
         if W.dtype != x.dtype:
             raise TypeError("%s must be an MX4Tensor or of x's type, got %s" % (name, W.dtype))
         _common.refuse_grad(W)

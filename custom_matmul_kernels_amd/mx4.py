@@ -34,22 +34,49 @@ class MX4Tensor:
         assert tuple(scales.shape) == tuple(codes.shape[:3]) + (SLAB // BLOCK,)
         assert codes.device == scales.device
         assert codes.is_contiguous() and scales.is_contiguous()
+        assert codes.data_ptr() % 16 == 0 and scales.data_ptr() % 4 == 0
         assert not two_dimensional or codes.shape[0] == 1
-        self.codes, self.scales, self.k, self.k_axis = codes, scales, k, k_axis
+        self._set((codes, scales), codes.shape[0], codes.shape[2], k, k_axis, two_dimensional)
+
+    def _set(self, storage, batch, rows, k, k_axis, two_dimensional):
+        # storage: (codes, scales), or one buffer that holds the codes and behind
+        # them the scales (one allocation less per call of quantize_mx4)
+        self._storage = storage
+        self.batch, self.rows, self.k, self.k_axis = batch, rows, k, k_axis
         self.two_dimensional = two_dimensional
+        self.device = storage[0].device if type(storage) is tuple else storage.device
+        matrix = (rows, k) if k_axis == -1 else (k, rows)
+        self.shape = matrix if two_dimensional else (batch,) + matrix
+
+    @classmethod
+    def _wrap(cls, *args):
+        t = object.__new__(cls)
+        t._set(*args)
+        return t
+
+    def _blocks4(self):
+        return self.batch * -(-self.k // SLAB) * self.rows
+
+    def _pointers(self):
+        if type(self._storage) is tuple:
+            return self._storage[0].data_ptr(), self._storage[1].data_ptr()
+        p = self._storage.data_ptr()
+        return p, p + self._blocks4() * (SLAB // 2)
+
+    def _views(self):
+        if type(self._storage) is not tuple:
+            head, n = (self.batch, -(-self.k // SLAB), self.rows), self._blocks4() * (SLAB // 2)
+            self._storage = (self._storage[:n].view(head + (SLAB // 2,)),
+                             self._storage[n:].view(head + (SLAB // BLOCK,)))
+        return self._storage
 
     @property
-    def rows(self):
-        return self.codes.shape[2]
+    def codes(self):
+        return self._views()[0]
 
     @property
-    def shape(self):
-        matrix = (self.rows, self.k) if self.k_axis == -1 else (self.k, self.rows)
-        return torch.Size(matrix if self.two_dimensional else (self.codes.shape[0],) + matrix)
-
-    @property
-    def device(self):
-        return self.codes.device
+    def scales(self):
+        return self._views()[1]
 
     def dim(self):
         return 2 if self.two_dimensional else 3
@@ -57,7 +84,7 @@ class MX4Tensor:
     def transpose(self, dim0=-2, dim1=-1):
         n = self.dim()
         assert {dim0 % n, dim1 % n} == {n - 2, n - 1}, "only the two matrix axes can be swapped"
-        return MX4Tensor(self.codes, self.scales, self.k, -3 - self.k_axis, self.two_dimensional)
+        return MX4Tensor._wrap(self._storage, self.batch, self.rows, self.k, -3 - self.k_axis, self.two_dimensional)
 
     def to(self, device):
         return MX4Tensor(self.codes.to(device), self.scales.to(device), self.k, self.k_axis, self.two_dimensional)
@@ -69,9 +96,9 @@ class MX4Tensor:
         assert self.device.type == "cuda"
         out = torch.empty(self.shape, dtype=dtype, device=self.device)
         if out.numel():
-            _common.call(_lib.load().cmk_mx4_dequantize, self.device,
-                         self.codes.data_ptr(), self.scales.data_ptr(), out.data_ptr(), code,
-                         self.codes.shape[0], self.rows, self.k, 1 if self.k_axis == -2 else 0)
+            codes, scales = self._pointers()
+            _common.call(_lib.load().cmk_mx4_dequantize, self.device, codes, scales, out.data_ptr(), code,
+                         self.batch, self.rows, self.k, 1 if self.k_axis == -2 else 0)
         return out
 
     @classmethod
@@ -115,24 +142,23 @@ def quantize_mx4(T, dim=-1):
     scale, is one of the last two: -1 for the left operand of a product, -2 for
     the right one."""
     dtype = _common.float_type(T.dtype, "the tensor")
-    n = T.dim()
+    shape, stride, device = T.shape, T.stride(), T.device
+    n = len(shape)
     if n not in (2, 3):
         raise ValueError("the tensor needs to be 2d or 3d")
     k_axis = dim if dim < 0 else dim - n
-    assert k_axis in (-1, -2), "dim must be one of the two matrix axes"
-    assert T.device.type == "cuda"
+    assert k_axis == -1 or k_axis == -2, "dim must be one of the two matrix axes"
+    assert device.type == "cuda"
     _common.refuse_grad(T)
-    x = T[None] if n == 2 else T
-    l = x.shape[0]
-    rows, k = (x.shape[1], x.shape[2]) if k_axis == -1 else (x.shape[2], x.shape[1])
-    sl, sr, sk = x.stride(0), x.stride(-3 - k_axis), x.stride(k_axis)
-    slabs = -(-k // SLAB)
-    codes = torch.empty((l, slabs, rows, SLAB // 2), dtype=torch.uint8, device=T.device)
-    scales = torch.empty((l, slabs, rows, SLAB // BLOCK), dtype=torch.uint8, device=T.device)
-    if codes.numel():
-        _common.call(_lib.load().cmk_mx4_quantize, T.device, x.data_ptr(), dtype, codes.data_ptr(),
-                     scales.data_ptr(), l, rows, k, sl, sr, sk)
-    return MX4Tensor(codes, scales, k, k_axis, n == 2)
+    l = 1 if n == 2 else shape[0]
+    rows, k = shape[-3 - k_axis], shape[k_axis]
+    units = l * -(-k // SLAB) * rows
+    storage = torch.empty(units * (SLAB // 2 + SLAB // BLOCK), dtype=torch.uint8, device=device)
+    if units:
+        p = storage.data_ptr()
+        _common.call(_lib.load().cmk_mx4_quantize, device, T.data_ptr(), dtype, p, p + units * (SLAB // 2), l, rows, k,
+                     0 if n == 2 else stride[0], stride[-3 - k_axis], stride[k_axis])
+    return MX4Tensor._wrap(storage, l, rows, k, k_axis, n == 2)
 
 
 class MX4BMMCUDA:
@@ -150,34 +176,42 @@ class MX4BMMCUDA:
         self._lib = _lib.load()
 
     def __call__(self, A, B):
-        assert A.dim() == B.dim()
-        n = A.dim()
+        four_a, four_b = isinstance(A, MX4Tensor), isinstance(B, MX4Tensor)
+        sa, sb, device = A.shape, B.shape, A.device
+        n = len(sa)
+        assert len(sb) == n
         if n not in (2, 3):
             raise ValueError("A and B need to be 2d or 3d")
-        for T, axis, name in ((A, -1, "A"), (B, -2, "B")):
-            if isinstance(T, MX4Tensor):
-                assert T.k_axis == axis, "the blocks of %s must run along k" % name
-            else:
-                _common.float_type(T.dtype, name)
-                _common.refuse_grad(T)
-        sa, sb = A.shape, B.shape
-        assert sa[-1] == sb[-2]
-        assert n == 2 or sa[0] == sb[0]
-        assert A.device.type == B.device.type == "cuda"
-        assert A.device == B.device
+        if four_a:
+            assert A.k_axis == -1, "the blocks of A must run along k"
+        else:
+            a_type = _common.float_type(A.dtype, "A")
+            _common.refuse_grad(A)
+        if four_b:
+            assert B.k_axis == -2, "the blocks of B must run along k"
+        else:
+            _common.float_type(B.dtype, "B")
+            _common.refuse_grad(B)
+        m, k = sa[-2:]
+        c = sb[-1]
         l = 1 if n == 2 else sa[0]
-        m, k, c = sa[-2], sa[-1], sb[-1]
-        C = torch.empty((m, c) if n == 2 else (l, m, c), dtype=self.out_dtype, device=A.device)
-        if C.numel():
-            if not isinstance(B, MX4Tensor):
+        assert sb[-2] == k
+        assert n == 2 or sb[0] == l
+        assert device.type == "cuda"
+        assert device == B.device
+        C = torch.empty((m, c) if n == 2 else (l, m, c), dtype=self.out_dtype, device=device)
+        if l and m and c:
+            if not four_b:
                 B = quantize_mx4(B, -2)
-            if not isinstance(A, MX4Tensor):
-                if m <= ROWS_IN_CALL and l <= 65535 and (A.stride(-1) == 1 or k <= 1):
-                    _common.call(self._lib.cmk_mx4_bmm_rows, C.device, A.data_ptr(), _common.FLOAT_TYPES[A.dtype],
-                                 A.stride(0) if n == 3 else 0, A.stride(-2), B.codes.data_ptr(), B.scales.data_ptr(),
-                                 C.data_ptr(), self._out, l, m, c, k)
+            b_codes, b_scales = B._pointers()
+            if not four_a:
+                stride = A.stride()
+                if m <= ROWS_IN_CALL and l <= 65535 and (stride[-1] == 1 or k <= 1):
+                    _common.call(self._lib.cmk_mx4_bmm_rows, device, A.data_ptr(), a_type, stride[0] if n == 3 else 0,
+                                 stride[-2], b_codes, b_scales, C.data_ptr(), self._out, l, m, c, k)
                     return C
                 A = quantize_mx4(A, -1)
-            _common.call(self._lib.cmk_mx4_bmm, C.device, A.codes.data_ptr(), A.scales.data_ptr(),
-                         B.codes.data_ptr(), B.scales.data_ptr(), C.data_ptr(), self._out, l, m, c, k)
+            a_codes, a_scales = A._pointers()
+            _common.call(self._lib.cmk_mx4_bmm, device, a_codes, a_scales, b_codes, b_scales, C.data_ptr(), self._out,
+                         l, m, c, k)
         return C
