@@ -148,41 +148,47 @@ __device__ __forceinline__ unsigned long long order_key(double v) {
 
 constexpr int kRankedExperts = 256;
 
-// The choice of token t, by a work-group of 256 threads: pick[j] and weight[j] in
-// LDS, valid after the barrier at its end.  Up to 256 experts each is ranked by
-// counting those in front of it, the counting spread over the threads; beyond, k
-// rounds look for the largest that is left.
+// The choice of a token, by a work-group of 256 threads.
 struct MoeChoice {
   unsigned long long key[kMoeExperts];
   double logit[kMoeExperts];
-  int rank[kRankedExperts];
   int pick[kMoeChoices];
   float raised[kMoeChoices];
   float sum;
 };
 
+// pick[0..k-1] of token t, valid after the barrier at the end.  Up to 256 experts
+// each is ranked by counting those in front of it, by one, two or four neighbouring
+// lanes; beyond, k rounds look for the largest that is left.
 __device__ __forceinline__ void moe_choose(const MoeArgs& a, int t, MoeChoice& c) {
   const int tid = threadIdx.x;
   for (int e = tid; e < a.E; e += 256) {
-    double v = 0;
-    for (int s = 0; s < a.splits; ++s) v += a.logits[((long long)s * a.T + t) * a.E + e];
+    double v = 0, part[4];
+    for (int s0 = 0; s0 < a.splits; s0 += 4) {
+#pragma unroll
+      for (int s = 0; s < 4; ++s) part[s] = s0 + s < a.splits ? a.logits[((long long)(s0 + s) * a.T + t) * a.E + e] : 0.0;
+#pragma unroll
+      for (int s = 0; s < 4; ++s) v += part[s];
+    }
     c.logit[e] = v;
     c.key[e] = order_key(v);
-    if (e < kRankedExperts) c.rank[e] = 0;
   }
   __syncthreads();
   if (a.E <= kRankedExperts) {
-    // threads per expert: a power of two, so that a wave's threads share what they compare with
-    const int width = a.E <= 64 ? 64 : a.E <= 128 ? 128 : 256;
-    const int e = tid & (width - 1), share = tid / width, shares = 256 / width;
+    const int shift = a.E <= 64 ? 2 : a.E <= 128 ? 1 : 0;  // lanes per expert: 1 << shift
+    const int e = tid >> shift, share = tid & ((1 << shift) - 1);
+    int before = 0;
     if (e < a.E) {
       const unsigned long long mine = c.key[e];
-      int before = 0;
-      for (int o = share; o < a.E; o += shares) before += c.key[o] > mine || (c.key[o] == mine && o < e);
-      if (before) atomicAdd(&c.rank[e], before);
+#pragma unroll 8
+      for (int o = share; o < a.E; o += 1 << shift) {
+        const unsigned long long other = c.key[o];
+        before += other > mine || (other == mine && o < e);
+      }
     }
-    __syncthreads();
-    if (tid < a.E && c.rank[tid] < a.k) c.pick[c.rank[tid]] = tid;
+    if (shift > 0) before += __shfl_xor(before, 1);
+    if (shift > 1) before += __shfl_xor(before, 2);
+    if (e < a.E && share == 0 && before < a.k) c.pick[before] = e;
     __syncthreads();
   } else {
     for (int j = 0; j < a.k; ++j) {
@@ -202,6 +208,12 @@ __device__ __forceinline__ void moe_choose(const MoeArgs& a, int t, MoeChoice& c
       __syncthreads();
     }
   }
+}
+
+// What the weights are made of: exp of the chosen logits and, where the softmax is
+// over all, its sum.  After moe_choose; valid after the barrier at the end.
+__device__ __forceinline__ void moe_raise(const MoeArgs& a, MoeChoice& c) {
+  const int tid = threadIdx.x;
   const double top = c.logit[c.pick[0]];
   if (tid < a.k) c.raised[tid] = expf((float)(c.logit[c.pick[tid]] - top));
   if (!a.renormalize && tid < 64) {
@@ -225,6 +237,7 @@ __device__ __forceinline__ float moe_weight(const MoeArgs& a, const MoeChoice& c
 __global__ __launch_bounds__(256) void moe_select_kernel(MoeArgs a) {
   __shared__ MoeChoice c;
   moe_choose(a, blockIdx.x, c);
+  moe_raise(a, c);
   if ((int)threadIdx.x < a.k) {
     const int s = blockIdx.x * a.k + threadIdx.x;
     a.chosen[s] = c.pick[threadIdx.x];
@@ -531,10 +544,13 @@ __global__ __launch_bounds__(64 * kMoeWaves) void moe_gate_up_single_kernel(MoeA
   MoeChoice& c = *(MoeChoice*)lds;
   moe_choose(a, 0, c);
   const int expert = __builtin_amdgcn_readfirstlane(c.pick[blockIdx.y]);
-  if (blockIdx.x == 0 && blockIdx.y == 0 && (int)threadIdx.x < a.k) {
-    a.chosen[threadIdx.x] = c.pick[threadIdx.x];
-    a.experts[threadIdx.x] = c.pick[threadIdx.x];
-    a.weights[threadIdx.x] = moe_weight(a, c, threadIdx.x);
+  if (blockIdx.x == 0 && blockIdx.y == 0) {
+    moe_raise(a, c);
+    if ((int)threadIdx.x < a.k) {
+      a.chosen[threadIdx.x] = c.pick[threadIdx.x];
+      a.experts[threadIdx.x] = c.pick[threadIdx.x];
+      a.weights[threadIdx.x] = moe_weight(a, c, threadIdx.x);
+    }
   }
   if (threadIdx.x == 0) list[0] = blockIdx.y;
   __syncthreads();  // list is there and the choice has been read
@@ -585,13 +601,39 @@ __global__ __launch_bounds__(64 * kMoeWaves) void moe_down_kernel(MoeArgs a) {
   }
 }
 
+// y[t] = sum_j w_j y_j in the order of j; four columns a thread, the loads of eight
+// choices under way at a time.
 template <class T>
 __global__ __launch_bounds__(256) void moe_combine_kernel(MoeArgs a) {
-  const int n = blockIdx.x * 256 + threadIdx.x, t = blockIdx.y;
+  const int n = (blockIdx.x * 256 + threadIdx.x) * 4, t = blockIdx.y;
   if (n >= a.H) return;
-  float s = 0;
-  for (int j = 0; j < a.k; ++j) s = fmaf(a.weights[t * a.k + j], a.yp[((long long)t * a.k + j) * a.H + n], s);
-  ((T*)a.y)[(long long)t * a.H + n] = from_f32<T>(s);
+  const bool aligned = (a.H & 3) == 0;
+  const float* from = a.yp + (long long)t * a.k * a.H + n;
+  f32x4 sum = {};
+  for (int j0 = 0; j0 < a.k; j0 += 8) {
+    f32x4 v[8];
+    float w[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (j0 + j >= a.k) break;
+      const float* p = from + (long long)(j0 + j) * a.H;
+      w[j] = a.weights[t * a.k + j0 + j];
+      if (aligned) {
+        v[j] = *(const f32x4*)p;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[j][i] = n + i < a.H ? p[i] : 0.0f;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (j0 + j >= a.k) break;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum[i] = fmaf(w[j], v[j][i], sum[i]);
+    }
+  }
+  const T o[4] = {from_f32<T>(sum[0]), from_f32<T>(sum[1]), from_f32<T>(sum[2]), from_f32<T>(sum[3])};
+  store4((T*)a.y + (long long)t * a.H + n, o, a.H - n, aligned);
 }
 
 // The down products of a single token and their weighted sum: a work-group takes 16
@@ -742,10 +784,10 @@ extern "C" int cmk_moe(const void* x, const void* router, const void* gate_up, c
     const dim3 up(ceil_div(p.Ip, 16), d->k), dn(ceil_div(d->H, 16)), b(64 * kMoeWaves);
     if (d->w_dtype == CMK_BF16) {
       hipLaunchKernelGGL((moe_gate_up_single_kernel<CMK_BF16, 1, 4, 1, 4>), up, b, 0, st, a);
-      hipLaunchKernelGGL((moe_down_single_kernel<CMK_BF16, __bf16, 16, 3>), dn, dim3(1024), 0, st, a);
+      hipLaunchKernelGGL((moe_down_single_kernel<CMK_BF16, __bf16, 16, 2>), dn, dim3(1024), 0, st, a);
     } else if (d->w_dtype == CMK_F16) {
       hipLaunchKernelGGL((moe_gate_up_single_kernel<CMK_F16, 1, 4, 1, 4>), up, b, 0, st, a);
-      hipLaunchKernelGGL((moe_down_single_kernel<CMK_F16, _Float16, 16, 3>), dn, dim3(1024), 0, st, a);
+      hipLaunchKernelGGL((moe_down_single_kernel<CMK_F16, _Float16, 16, 2>), dn, dim3(1024), 0, st, a);
     } else if (d->x_dtype == CMK_BF16) {
       hipLaunchKernelGGL((moe_gate_up_single_kernel<CMK_MX4, 1, 4, 1, 4>), up, b, 0, st, a);
       hipLaunchKernelGGL((moe_down_single_kernel<CMK_MX4, __bf16, 16, 4>), dn, dim3(1024), 0, st, a);
@@ -783,7 +825,7 @@ extern "C" int cmk_moe(const void* x, const void* router, const void* gate_up, c
     if (many) experts_kernel(moe_down_kernel<CMK_F16, 1, 1, 4>, d->H, 1, 1);
     else experts_kernel(moe_down_kernel<CMK_F16, 4, 1, 2>, d->H, 1, 4);
   }
-  const dim3 out_grid(ceil_div(d->H, 256), d->T);
+  const dim3 out_grid(ceil_div(d->H, 1024), d->T);
   if (d->x_dtype == CMK_BF16) hipLaunchKernelGGL(moe_combine_kernel<__bf16>, out_grid, dim3(256), 0, st, a);
   else hipLaunchKernelGGL(moe_combine_kernel<_Float16>, out_grid, dim3(256), 0, st, a);
   return hip_status(hipGetLastError(), "cmk_moe launch");
