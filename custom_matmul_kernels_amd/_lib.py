@@ -36,6 +36,7 @@ EXPORTS = (
     "cmk_mx4_dequantize",
     "cmk_mx4_bmm",
     "cmk_mx4_bmm_rows",
+    "cmk_mx4_workspace_bytes",
     "cmk_moe",
     "cmk_moe_workspace_bytes",
     "cmk_workspace_bytes",
@@ -118,7 +119,9 @@ def load():
     lib.cmk_topk_1d_f32.argtypes = [p, ll, p, p, i, p, sz, p]
     lib.cmk_mx4_quantize.argtypes = [p, i, p, p, i, i, i, ll, ll, ll, p]
     lib.cmk_mx4_dequantize.argtypes = [p, p, p, i, i, i, i, i, p]
-    lib.cmk_mx4_bmm.argtypes = [p, p, p, p, p, i, i, i, i, i, p]
+    lib.cmk_mx4_bmm.argtypes = [p, p, p, p, p, i, i, i, i, i, p, sz, p]
+    lib.cmk_mx4_workspace_bytes.argtypes = [i, i, i, i]
+    lib.cmk_mx4_workspace_bytes.restype = sz
     lib.cmk_mx4_bmm_rows.argtypes = [p, i, ll, ll, p, p, p, i, i, i, i, i, p]
     mp = ctypes.POINTER(MoeDesc)
     lib.cmk_moe.argtypes = [p, p, p, p, p, p, p, p, p, mp, p, sz, p]

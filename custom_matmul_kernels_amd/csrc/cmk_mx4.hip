@@ -1,4 +1,7 @@
 // 4-bit microscaled matrices: quantisation, its inverse, and the batched product.
+#include <algorithm>
+#include <type_traits>
+
 #include "cmk_mx4.hpp"
 
 namespace cmk {
@@ -36,10 +39,7 @@ __global__ __launch_bounds__(256) void mx4_quantize_rows_kernel(QuantArgs a) {
 #pragma unroll
   for (int p = 0; p < 4; ++p) {
     const long long row = rg * 16 + p * 4 + (lane >> 4);
-    unsigned top = o[p].top();
-    top = max(top, (unsigned)__shfl_xor((int)top, 1));
-    top = max(top, (unsigned)__shfl_xor((int)top, 2));
-    const unsigned s = scale_byte(top);
+    const unsigned s = scale_byte(quad_max(o[p].top()));
     const unsigned w = s == 255u ? 0u : o[p].codes(scale_float(s));
     if (row < a.R) {
       const long long at = ls * a.R + row;
@@ -176,10 +176,12 @@ __global__ __launch_bounds__(256) void mx4_dequantize_columns_kernel(DequantArgs
 
 struct Mx4GemmArgs {
   const uint8_t *a_codes, *a_scales, *b_codes, *b_scales;
-  void* c;  // dense [L][M][N]
+  void* c;  // dense [L][M][N]; of several splits: one such after another
   int L, M, N;
   int slabs;
   int tiles_m, tiles_n;
+  int splits;  // ranges of slabs
+  int wide;    // rows of c start on 16-byte boundaries and hold whole multiples of them
 };
 
 // A work-group of four waves computes a TM x TN tile of C, a wave a quarter of it
@@ -188,7 +190,7 @@ struct Mx4GemmArgs {
 // one byte).
 //
 // Slabs of both operands (codes and scales) travel by direct global-to-LDS loads
-// into a ring of kStages buffers, two slabs ahead of the products.  Half a slab's
+// into a ring of S buffers, S - 2 slabs ahead of the products.  Half a slab's
 // fragments are in registers at a time; those of the next half are read while the
 // matrix pipe works on them.  The one barrier of a slab sits between its halves:
 // it follows the wait for the next slab, whose first half is read behind it, and
@@ -196,14 +198,15 @@ struct Mx4GemmArgs {
 // stored at position block ^ ((row >> 2) & 3), so that the 16 rows that the LDS
 // serves at a time spread over all banks; the swizzle is produced by choosing
 // which block each lane of a load asks for.
-constexpr int kStages = 4;
-
-template <int TM, int TN>
+template <int TM, int TN, int S>
 struct Mx4Tile {
   static constexpr int BM = TM / 64, BN = TN / 64;  // 32 x 32 blocks of a wave
   static constexpr int kCodesA = TM * kSlabBytes, kCodesB = TN * kSlabBytes;
   static constexpr int kStageBytes = kCodesA + kCodesB + (TM + TN) * kSlabScales;
   static constexpr int kLoads = TM / 64 + TN / 64 + 2;  // vector-memory instructions of a wave per slab
+  // stages that one address register reaches with the 16-bit offset of an LDS read
+  static constexpr int kReach = (65535 - (BM > BN ? BM : BN) * 32 * kSlabBytes) / kStageBytes + 1;
+  static constexpr int kBases = (S + kReach - 1) / kReach;
 };
 
 typedef const __attribute__((address_space(1))) void* gptr;
@@ -231,26 +234,30 @@ __device__ __forceinline__ void meet() {
 // Work-groups go round the eight XCDs in turn, each with an L2 of its own: an XCD
 // gets a contiguous run of the tiles of all batches, in strips of eight tile rows,
 // so that what runs on it at a time shares few panels of both operands.
-__device__ __forceinline__ void place_tile(const Mx4GemmArgs& a, int& l, int& tile_m, int& tile_n) {
+__device__ __forceinline__ void place_tile(const Mx4GemmArgs& a, int& split, int& l, int& tile_m, int& tile_n) {
   const int total = gridDim.x, xcd = blockIdx.x & 7, turn = blockIdx.x >> 3;
   const int each = total >> 3, extra = total & 7;
   const int id = xcd * each + min(xcd, extra) + turn;
   const int per_batch = a.tiles_m * a.tiles_n;
-  l = id / per_batch;
-  const int t = id - l * per_batch;
+  split = id / (per_batch * a.L);
+  const int in_split = id - split * per_batch * a.L;
+  l = in_split / per_batch;
+  const int t = in_split - l * per_batch;
   const int strip = t / (8 * a.tiles_n), in = t - strip * 8 * a.tiles_n;
   const int height = min(8, a.tiles_m - strip * 8);
   tile_m = strip * 8 + in % height;
   tile_n = in / height;
 }
 
-template <class T, int TM, int TN>
+template <class T, int TM, int TN, int S>
 __global__ __launch_bounds__(256, 1) void mx4_gemm_kernel(Mx4GemmArgs a) {
-  using Tile = Mx4Tile<TM, TN>;
+  using Tile = Mx4Tile<TM, TN, S>;
   constexpr int BM = Tile::BM, BN = Tile::BN;
-  __shared__ __attribute__((aligned(16))) uint8_t lds[kStages * Tile::kStageBytes];
-  int l, tile_m, tile_n;
-  place_tile(a, l, tile_m, tile_n);
+  static_assert((S & 1) == 0, "the slabs' scales alternate between two sets of registers");
+  __shared__ __attribute__((aligned(16))) uint8_t lds[S * Tile::kStageBytes];
+  int split, l, tile_m, tile_n;
+  place_tile(a, split, l, tile_m, tile_n);
+  const int slab0 = (int)((long long)a.slabs * split / a.splits), slabs = (int)((long long)a.slabs * (split + 1) / a.splits) - slab0;
   const int m0 = tile_m * TM, n0 = tile_n * TN;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = (wave >> 1) * (TM / 2), wn = (wave & 1) * (TN / 2);
@@ -273,10 +280,10 @@ __global__ __launch_bounds__(256, 1) void mx4_gemm_kernel(Mx4GemmArgs a) {
   unsigned osb = min(wave * (TN / 4) + (lane & (TN / 4 - 1)), a.N - 1 - n0) * kSlabScales;
   // The next slab to be requested.  Beyond the last one the requests repeat it, so
   // that every slab of the loop issues and awaits the same number of loads.
-  const uint8_t* pa = a.a_codes + ((long long)l * a.slabs * a.M + m0) * kSlabBytes;
-  const uint8_t* pb = a.b_codes + ((long long)l * a.slabs * a.N + n0) * kSlabBytes;
-  const uint8_t* psa = a.a_scales + ((long long)l * a.slabs * a.M + m0) * kSlabScales;
-  const uint8_t* psb = a.b_scales + ((long long)l * a.slabs * a.N + n0) * kSlabScales;
+  const uint8_t* pa = a.a_codes + (((long long)l * a.slabs + slab0) * a.M + m0) * kSlabBytes;
+  const uint8_t* pb = a.b_codes + (((long long)l * a.slabs + slab0) * a.N + n0) * kSlabBytes;
+  const uint8_t* psa = a.a_scales + (((long long)l * a.slabs + slab0) * a.M + m0) * kSlabScales;
+  const uint8_t* psb = a.b_scales + (((long long)l * a.slabs + slab0) * a.N + n0) * kSlabScales;
   const long long step_a = (long long)a.M * kSlabBytes, step_b = (long long)a.N * kSlabBytes;
   int requested = 0;
   // scalar base + 32-bit lane offset, no vector addition
@@ -299,29 +306,30 @@ __global__ __launch_bounds__(256, 1) void mx4_gemm_kernel(Mx4GemmArgs a) {
     uint8_t* scales = at + Tile::kCodesA + Tile::kCodesB;
     if (TM == 256 || lane < TM / 4) load4(psa, osa, scales + wave * TM);
     if (TN == 256 || lane < TN / 4) load4(psb, osb, scales + TM * kSlabScales + wave * TN);
-    const long long more = ++requested < a.slabs ? 1 : 0;
+    const long long more = ++requested < slabs ? 1 : 0;
     pa += more * step_a; pb += more * step_b;
     psa += more * (step_a / (kSlabBytes / kSlabScales)); psb += more * (step_b / (kSlabBytes / kSlabScales));
   };
 
-  // Where this lane reads: one register per half of a slab, operand and pair of
+  // Where this lane reads: one register per half of a slab, operand and group of
   // stages, the rest of an address is the instruction's offset (vector
   // instructions in the loop cost matrix-pipe time).
+  constexpr int kReach = Tile::kReach;
   const unsigned lds0 = (unsigned)(uintptr_t)(lptr)lds;
-  unsigned at_m[2][2], at_n[2][2], at_cm[2], at_cn[2];
+  unsigned at_m[Tile::kBases][2], at_n[Tile::kBases][2], at_cm[Tile::kBases], at_cn[Tile::kBases];
 #pragma unroll
-  for (int pair = 0; pair < 2; ++pair) {
-    const unsigned base = lds0 + pair * 2 * Tile::kStageBytes;
+  for (int p = 0; p < Tile::kBases; ++p) {
+    const unsigned base = lds0 + p * kReach * Tile::kStageBytes;
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
       const unsigned part = ((2 * h + g) ^ ((r >> 2) & 3)) * 16;
-      at_m[pair][g] = base + (wm + r) * kSlabBytes + part;
-      at_n[pair][g] = base + Tile::kCodesA + (wn + r) * kSlabBytes + part;
-      asm("" : "+v"(at_m[pair][g]), "+v"(at_n[pair][g]));
+      at_m[p][g] = base + (wm + r) * kSlabBytes + part;
+      at_n[p][g] = base + Tile::kCodesA + (wn + r) * kSlabBytes + part;
+      asm("" : "+v"(at_m[p][g]), "+v"(at_n[p][g]));
     }
-    at_cm[pair] = base + Tile::kCodesA + Tile::kCodesB + (wm + r) * kSlabScales + 2 * h;
-    at_cn[pair] = base + Tile::kCodesA + Tile::kCodesB + (TM + wn + r) * kSlabScales + 2 * h;
-    asm("" : "+v"(at_cm[pair]), "+v"(at_cn[pair]));
+    at_cm[p] = base + Tile::kCodesA + Tile::kCodesB + (wm + r) * kSlabScales + 2 * h;
+    at_cn[p] = base + Tile::kCodesA + Tile::kCodesB + (TM + wn + r) * kSlabScales + 2 * h;
+    asm("" : "+v"(at_cm[p]), "+v"(at_cn[p]));
   }
   struct Half {
     u32x4v m[BM], n[BN];
@@ -332,18 +340,18 @@ __global__ __launch_bounds__(256, 1) void mx4_gemm_kernel(Mx4GemmArgs a) {
   typedef const __attribute__((address_space(3))) u32x4v* l16;
   typedef const __attribute__((address_space(3))) unsigned short* l2;
   auto read = [&](int stage, int g, Half& f) {
-    const unsigned off = (stage & 1) * Tile::kStageBytes;
+    const unsigned off = stage % kReach * Tile::kStageBytes;
 #pragma unroll
-    for (int b = 0; b < BM; ++b) f.m[b] = *(l16)(lptr)(uintptr_t)(at_m[stage >> 1][g] + off + b * 32 * kSlabBytes);
+    for (int b = 0; b < BM; ++b) f.m[b] = *(l16)(lptr)(uintptr_t)(at_m[stage / kReach][g] + off + b * 32 * kSlabBytes);
 #pragma unroll
-    for (int b = 0; b < BN; ++b) f.n[b] = *(l16)(lptr)(uintptr_t)(at_n[stage >> 1][g] + off + b * 32 * kSlabBytes);
+    for (int b = 0; b < BN; ++b) f.n[b] = *(l16)(lptr)(uintptr_t)(at_n[stage / kReach][g] + off + b * 32 * kSlabBytes);
   };
   auto read_scales = [&](int stage, Scales& c) {
-    const unsigned off = (stage & 1) * Tile::kStageBytes;
+    const unsigned off = stage % kReach * Tile::kStageBytes;
 #pragma unroll
-    for (int b = 0; b < BM; ++b) c.m[b] = *(l2)(lptr)(uintptr_t)(at_cm[stage >> 1] + off + b * 32 * kSlabScales);
+    for (int b = 0; b < BM; ++b) c.m[b] = *(l2)(lptr)(uintptr_t)(at_cm[stage / kReach] + off + b * 32 * kSlabScales);
 #pragma unroll
-    for (int b = 0; b < BN; ++b) c.n[b] = *(l2)(lptr)(uintptr_t)(at_cn[stage >> 1] + off + b * 32 * kSlabScales);
+    for (int b = 0; b < BN; ++b) c.n[b] = *(l2)(lptr)(uintptr_t)(at_cn[stage / kReach] + off + b * 32 * kSlabScales);
   };
   f32x16 acc[BM][BN] = {};
   auto wide = [](u32x4v v) { return i32x8{(int)v[0], (int)v[1], (int)v[2], (int)v[3], 0, 0, 0, 0}; };
@@ -352,7 +360,7 @@ __global__ __launch_bounds__(256, 1) void mx4_gemm_kernel(Mx4GemmArgs a) {
   Half f0, f1;
   auto slab = [&](auto stage, Scales& c, Scales& d) {
     constexpr int Stage = decltype(stage)::value;
-    constexpr int Next = (Stage + 1) % kStages;
+    constexpr int Next = (Stage + 1) % S;
     read(Stage, 1, f1);
 #pragma unroll
     for (int bm = 0; bm < BM; ++bm)
@@ -360,60 +368,101 @@ __global__ __launch_bounds__(256, 1) void mx4_gemm_kernel(Mx4GemmArgs a) {
       for (int bn = 0; bn < BN; ++bn)
         acc[bm][bn] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(f0.m[bm]), wide(f0.n[bn]), acc[bm][bn], 4, 4, 0, c.m[bm], 0, c.n[bn]);
     // a read, then as many products as keep the matrix pipe busy until the next
+    if constexpr (BM * BN >= 4) {
 #pragma unroll
-    for (int i = 0; i < BM + BN; ++i) {
-      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x008, BM * BN / (BM + BN), 0);
+      for (int i = 0; i < BM + BN; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, BM * BN / (BM + BN), 0);
+      }
     }
     __builtin_amdgcn_sched_barrier(0);
-    wait_loads<Tile::kLoads>();
+    wait_loads<(S - 3) * Tile::kLoads>();
     meet();
     read_scales(Next, d);
     read(Next, 0, f0);
-    fetch((Stage + kStages - 1) % kStages);
+    fetch((Stage + S - 1) % S);
 #pragma unroll
     for (int bm = 0; bm < BM; ++bm)
 #pragma unroll
       for (int bn = 0; bn < BN; ++bn)
         acc[bm][bn] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(f1.m[bm]), wide(f1.n[bn]), acc[bm][bn], 4, 4, 1, c.m[bm], 1, c.n[bn]);
     // what the next slab starts with first, the requests behind it
+    if constexpr (BM * BN >= 4) {
 #pragma unroll
-    for (int i = 0; i < BM + BN; ++i) {
-      __builtin_amdgcn_sched_group_barrier(0x008, BM * BN / 2 / (BM + BN), 0);
-      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-    }
+      for (int i = 0; i < BM + BN; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, std::max(1, BM * BN / 2 / (BM + BN)), 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+      }
 #pragma unroll
-    for (int i = 0; i < Tile::kLoads; ++i) {
-      __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      for (int i = 0; i < Tile::kLoads; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      }
     }
     __builtin_amdgcn_sched_barrier(0);
   };
-  if (a.slabs > 0) {
+  if (slabs > 0) {
     Scales c0, c1;
-    fetch(0);
-    fetch(1);
-    fetch(2);
-    wait_loads<2 * Tile::kLoads>();
+#pragma unroll
+    for (int s = 0; s < S - 1; ++s) fetch(s);
+    wait_loads<(S - 2) * Tile::kLoads>();
     meet();
     read_scales(0, c0);
     read(0, 0, f0);
-    int left = a.slabs;
-    for (; left >= 4; left -= 4) {
+    int left = slabs;
+    for (; left >= S; left -= S) {
       slab(Int<0>{}, c0, c1);
       slab(Int<1>{}, c1, c0);
       slab(Int<2>{}, c0, c1);
       slab(Int<3>{}, c1, c0);
+      if constexpr (S == 8) {
+        slab(Int<4>{}, c0, c1);
+        slab(Int<5>{}, c1, c0);
+        slab(Int<6>{}, c0, c1);
+        slab(Int<7>{}, c1, c0);
+      }
     }
     if (left > 0) slab(Int<0>{}, c0, c1);
     if (left > 1) slab(Int<1>{}, c1, c0);
     if (left > 2) slab(Int<2>{}, c0, c1);
+    if constexpr (S == 8) {
+      if (left > 3) slab(Int<3>{}, c1, c0);
+      if (left > 4) slab(Int<4>{}, c0, c1);
+      if (left > 5) slab(Int<5>{}, c1, c0);
+      if (left > 6) slab(Int<6>{}, c0, c1);
+    }
     wait_loads<0>();  // no load may land after the work-group has ended
   }
 
   // lane: column n = lane & 31, rows 8 * (i / 4) + 4 * h + i % 4: a store covers two
-  // runs of 32 columns
-  T* c = (T*)a.c + (long long)l * a.M * a.N;
+  // runs of 32 columns.  16-bit results would be runs of 64 bytes, two at a time; they
+  // go through the wave's share of LDS and out 16 bytes a lane (stores of pairs of
+  // columns, exchanged between neighbouring lanes, took 380 instead of 275 us at
+  // 8192^3).
+  T* c = (T*)a.c + ((long long)split * a.L + l) * a.M * a.N;
+  if constexpr (sizeof(T) == 2) {
+    if (a.wide) {
+      constexpr int WM = TM / 2, WN = TN / 2, kPitch = WN * 2 + 16, kLanes = WN / 8, kRows = 64 / kLanes;
+      static_assert(4 * WM * kPitch <= S * Tile::kStageBytes, "the tile fits into the ring");
+      meet();  // every wave has read its last slab
+      uint8_t* mine = lds + wave * (WM * kPitch);
+#pragma unroll
+      for (int bm = 0; bm < BM; ++bm)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+#pragma unroll
+          for (int bn = 0; bn < BN; ++bn)
+            *(T*)(mine + (bm * 32 + 8 * (i >> 2) + 4 * h + (i & 3)) * kPitch + (bn * 32 + r) * 2) = from_f32<T>(acc[bm][bn][i]);
+      const int col = lane % kLanes * 8, n = n0 + wn + col;
+#pragma unroll 4
+      for (int i = lane / kLanes; i < WM; i += kRows) {
+        const u32x4v v = *(const u32x4v*)(mine + i * kPitch + col * 2);
+        const int m = m0 + wm + i;
+        if (m < a.M && n < a.N) *(u32x4v*)(c + (long long)m * a.N + n) = v;
+      }
+      return;
+    }
+  }
 #pragma unroll
   for (int bm = 0; bm < BM; ++bm)
 #pragma unroll
@@ -427,6 +476,22 @@ __global__ __launch_bounds__(256, 1) void mx4_gemm_kernel(Mx4GemmArgs a) {
         if (n < a.N) row[n] = from_f32<T>(acc[bm][bn][i]);
       }
     }
+}
+
+// The sum of the splits, in their order.
+template <class T>
+__global__ __launch_bounds__(256) void mx4_join_kernel(const float* part, T* c, long long n, int splits) {
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
+    float sum = 0;
+    for (int s0 = 0; s0 < splits; s0 += 8) {
+      float v[8];
+#pragma unroll
+      for (int s = 0; s < 8; ++s) v[s] = s0 + s < splits ? part[(s0 + s) * n + i] : 0.0f;
+#pragma unroll
+      for (int s = 0; s < 8; ++s) sum += v[s];
+    }
+    c[i] = from_f32<T>(sum);
+  }
 }
 
 // ------------------------------------------------------- product with few rows
@@ -446,92 +511,161 @@ struct Mx4Fragment {
   int scale;
 };
 
-__device__ __forceinline__ void load_fragment(Mx4Fragment& f, const uint8_t* codes, const uint8_t* scales, long long at, int q) {
-  f.codes = *(const u32x4v*)(codes + at * kSlabBytes + q * 16);
-  f.scale = scales[at * kSlabScales + q];
-}
+constexpr int kRowsLds = 72 * 1024;
 
-// Quantises 32 elements in one lane.
-template <class T>
-__device__ __forceinline__ void quantize_fragment(Mx4Fragment& f, const Octet<T> (&o)[4]) {
-  const unsigned s = scale_byte(max(max(o[0].top(), o[1].top()), max(o[2].top(), o[3].top())));
-  const float scale = scale_float(s);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) f.codes[i] = s == 255u ? 0u : o[i].codes(scale);
-  f.scale = (int)s;
-}
-
-// A work-group takes 16 * RG columns of C and all its rows (up to 16 * MB); its
+// A work-group takes 16 * RG columns of C and all its rows (up to 16 * MB); its W
 // waves split the slabs and their sums meet in LDS, in the order of the waves.
 // There is nothing to gain but the stream of the right operand: its fragments
-// (1 KB of contiguous codes per instruction) go straight to registers, U slabs at
-// a time.  TX: the left operand's elements, quantised on the way, or uint8_t for
-// codes.
+// (1 KB of contiguous codes per instruction) go straight to registers, a ring of U
+// slabs under way.  The left operand's codes wait in LDS, as many slabs of all rows
+// at a time as fit, quantised on the way there if TX is an element type; uint8_t
+// stands for codes.
 template <class TX, class T, int W, int RG, int MB, int U>
 __global__ __launch_bounds__(64 * W) void mx4_rows_kernel(Mx4RowsArgs a) {
   constexpr bool kCodes = sizeof(TX) == 1;
-  __shared__ float part[W][RG][MB][64][4];
+  constexpr int kSteps = sizeof(TX) == 4 ? 2 : 4;
+  static_assert(W == 8 && W * RG * MB * 1024 <= kRowsLds, "the partial sums fit");
+  __shared__ __attribute__((aligned(16))) char lds[kRowsLds];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, q = lane >> 4;
   const int l = blockIdx.y, n0 = blockIdx.x * 16 * RG;
-  const long long batch_b = (long long)l * a.slabs * a.N;
-  int row[RG];
+  // a row of `piece` slabs: codes and scales, each 16 (4) bytes longer so that the
+  // rows of a fragment spread over the banks
+  const int fit = (kRowsLds / a.M - 20) / (kSlabBytes + kSlabScales);
+  const int piece = min(a.slabs, fit);
+  const int pitch = piece * kSlabBytes + 16, spitch = piece * kSlabScales + 4;
+  char* const scales = lds + a.M * pitch;
+  const int together = a.M > 4 ? 8 : a.M > 2 ? 4 : a.M > 1 ? 2 : 1;  // rows that the waves stage at a time
+  const uint8_t* bc[RG];
+  const uint8_t* bs[RG];
 #pragma unroll
-  for (int g = 0; g < RG; ++g) row[g] = min(n0 + g * 16 + r, a.N - 1);
+  for (int g = 0; g < RG; ++g) {
+    const long long at = (long long)l * a.slabs * a.N + min(n0 + g * 16 + r, a.N - 1);
+    bc[g] = a.b_codes + at * kSlabBytes + q * 16;
+    bs[g] = a.b_scales + at * kSlabScales + q;
+  }
+  const long long step_codes = (long long)a.N * kSlabBytes, step_scales = (long long)a.N * kSlabScales;
   f32x4 acc[RG][MB] = {};
   auto wide = [](u32x4v v) { return i32x8{(int)v[0], (int)v[1], (int)v[2], (int)v[3], 0, 0, 0, 0}; };
-  for (int s0 = wave; s0 < a.slabs; s0 += W * U) {
-    Mx4Fragment fb[U][RG], fx[U][MB];
+  for (int first = 0; first < a.slabs; first += piece) {
+    const int end = min(a.slabs, first + piece);
+    Mx4Fragment fb[U][RG];
+    auto request = [&](int u, int s) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int s = s0 + u * W;
-      if (s >= a.slabs) break;
+      for (int g = 0; g < RG; ++g) {
+        fb[u][g].codes = __builtin_nontemporal_load((const u32x4v*)(bc[g] + s * step_codes));
+        fb[u][g].scale = bs[g][s * step_scales];
+      }
+    };
+    // A wave takes 16 slabs of one row at a time (a step); with few rows several waves
+    // share one.  Four lanes share a block, so that a load reads 1 KB in one run.
+    // Loads are awaited in the order of their issue: the first steps are requested
+    // ahead of the right operand's ring, so that they are quantised while that is on
+    // its way.
+    const int start = first + wave / together * 16, each = W / together * 16;
+    const int whole = min(end, a.K / kSlab);  // slabs up to here hold 128 elements
+    int m = start < end ? wave & (together - 1) : a.M, s0 = start;  // the next step
+    int step_m[kSteps], step_s[kSteps];                             // those under way
+    Octet<std::conditional_t<kCodes, float, TX>> o[kSteps][kCodes ? 1 : 4];
+    Mx4Fragment f[kSteps];
+    auto load_steps = [&]() {
 #pragma unroll
-      for (int g = 0; g < RG; ++g) load_fragment(fb[u][g], a.b_codes, a.b_scales, batch_b + (long long)s * a.N + row[g], q);
-    }
+      for (int i = 0; i < kSteps; ++i) {
+        step_m[i] = m;
+        step_s[i] = s0;
+        if (m < a.M) {
+          if constexpr (kCodes) {
+            const long long at = ((long long)l * a.slabs + min(s0 + (lane >> 2), end - 1)) * a.M + m;
+            f[i].codes = *(const u32x4v*)((const uint8_t*)a.x + at * kSlabBytes + (lane & 3) * 16);
+            f[i].scale = a.x_scales[at * kSlabScales + (lane & 3)];
+          } else {
+            const TX* x = (const TX*)a.x + l * a.sl + m * a.sm + s0 * kSlab + lane * 8;
+            if (s0 + 16 <= whole) {  // no lane is beyond the end
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int s = s0 + u * W;
-      if (s >= a.slabs) break;
+              for (int e = 0; e < 4; ++e) __builtin_memcpy(o[i][e].v, x + 4 * e * kSlab, sizeof(o[i][e].v));
+            } else {
 #pragma unroll
-      for (int b = 0; b < MB; ++b) {
-        if constexpr (kCodes) {
-          const int m = min(b * 16 + r, a.M - 1);
-          load_fragment(fx[u][b], (const uint8_t*)a.x, a.x_scales, ((long long)l * a.slabs + s) * a.M + m, q);
-        } else {
-          const int m = b * 16 + r, k = s * kSlab + q * 32;
-          const TX* x = (const TX*)a.x + l * a.sl + m * a.sm + k;
-          Octet<TX> o[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) o[i] = load_octet(x + i * 8, m < a.M ? a.K - k - i * 8 : 0);
-          quantize_fragment(fx[u][b], o);
+              for (int e = 0; e < 4; ++e) {
+                const int s = s0 + 4 * e + (lane >> 4);
+                o[i][e] = load_octet(x + 4 * e * kSlab, s < end ? a.K - s * kSlab - (lane & 15) * 8 : 0);
+              }
+            }
+          }
+          s0 += each;
+          if (s0 >= end) { s0 = start; m += together; }
         }
       }
+    };
+    load_steps();
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (first + wave + u * W < end) request(u, first + wave + u * W);
+    if (first > 0) __syncthreads();
+    while (step_m[0] < a.M) {
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) {
+        if (step_m[i] >= a.M) break;
+        char* codes = lds + step_m[i] * pitch;
+        char* bytes = scales + step_m[i] * spitch;
+        if constexpr (kCodes) {
+          const int s = step_s[i] + (lane >> 2);
+          if (s < end) {
+            *(u32x4v*)(codes + (s - first) * kSlabBytes + (lane & 3) * 16) = f[i].codes;
+            bytes[(s - first) * kSlabScales + (lane & 3)] = (char)f[i].scale;
+          }
+        } else {
+          // a step's codes and scales are contiguous: 4 bytes a lane and one of four lanes
+          codes += (step_s[i] - first) * kSlabBytes + lane * 4;
+          bytes += (step_s[i] - first) * kSlabScales + (lane >> 2);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const unsigned scale = scale_byte(quad_max(o[i][e].top()));
+            const unsigned w = scale == 255u ? 0u : o[i][e].codes(scale_float(scale));
+            if (step_s[i] + 16 <= end || step_s[i] + 4 * e + (lane >> 4) < end) {
+              *(unsigned*)(codes + 4 * e * kSlabBytes) = w;
+              if ((lane & 3) == 0) bytes[4 * e * kSlabScales] = (char)scale;
+            }
+          }
+        }
+      }
+      load_steps();
     }
+    __syncthreads();
+    for (int s0 = first + wave; s0 < end; s0 += W * U) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (s0 + u * W >= a.slabs) break;
+      for (int u = 0; u < U; ++u) {
+        const int s = s0 + u * W;
+        if (s >= end) break;
+        Mx4Fragment fx[MB];
 #pragma unroll
-      for (int g = 0; g < RG; ++g)
+        for (int b = 0; b < MB; ++b) {
+          const int m = min(b * 16 + r, a.M - 1);
+          fx[b].codes = *(const u32x4v*)(lds + m * pitch + (s - first) * kSlabBytes + q * 16);
+          fx[b].scale = (unsigned char)scales[m * spitch + (s - first) * kSlabScales + q];
+        }
 #pragma unroll
-        for (int b = 0; b < MB; ++b)
-          acc[g][b] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wide(fb[u][g].codes), wide(fx[u][b].codes), acc[g][b], 4, 4, 0,
-                                                                      fb[u][g].scale, 0, fx[u][b].scale);
+        for (int g = 0; g < RG; ++g)
+#pragma unroll
+          for (int b = 0; b < MB; ++b)
+            acc[g][b] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wide(fb[u][g].codes), wide(fx[b].codes), acc[g][b], 4, 4, 0,
+                                                                        fb[u][g].scale, 0, fx[b].scale);
+        if (s + U * W < end) request(u, s + U * W);
+      }
     }
   }
+  f32x4(*part)[RG][MB][64] = (f32x4(*)[RG][MB][64])lds;
+  __syncthreads();
 #pragma unroll
   for (int g = 0; g < RG; ++g)
 #pragma unroll
-    for (int b = 0; b < MB; ++b)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) part[wave][g][b][lane][i] = acc[g][b][i];
+    for (int b = 0; b < MB; ++b) part[wave][g][b][lane] = acc[g][b];
   __syncthreads();
   T* c = (T*)a.c + (long long)l * a.M * a.N;
-  for (int v = threadIdx.x; v < RG * MB * 256; v += 64 * W) {
+  for (int v = threadIdx.x; v < RG * 16 * min(a.M, MB * 16); v += 64 * W) {
     // neighbouring threads take neighbouring columns of one row
     const int n = v % (16 * RG), m = v / (16 * RG);
     const int g = n >> 4, i = n & 3, from = ((n & 15) >> 2) * 16 + (m & 15), b = m >> 4;
-    if (m < a.M && n0 + n < a.N) {
+    if (n0 + n < a.N) {
       float sum = 0;
 #pragma unroll
       for (int w = 0; w < W; ++w) sum += part[w][g][b][from][i];
@@ -549,23 +683,49 @@ constexpr int kMx4RowsFloat = 16;
 template <class TX, class T>
 static void launch_rows(const Mx4RowsArgs& a, int L, hipStream_t st) {
   const long long groups = (long long)ceil_div(a.N, 16) * L;
-  // Four row groups a wave share one fragment of the left operand; one each where
-  // that would leave compute units without work.
-  const bool many = groups >= 4LL * compute_units();
-  auto grid = [&](int rg) { return dim3(ceil_div(a.N, 16 * rg), L); };
+  const int cus = compute_units();
+  // Row groups of a wave share the left operand's fragments and its quantisation;
+  // fewer where that would leave compute units without work.
+  auto run = [&](auto kernel, int rg) { hipLaunchKernelGGL(kernel, dim3(ceil_div(a.N, 16 * rg), L), dim3(512), 0, st, a); };
   if (a.M <= 16) {
-    if (many) hipLaunchKernelGGL((mx4_rows_kernel<TX, T, 8, 4, 1, 2>), grid(4), dim3(512), 0, st, a);
-    else if (a.slabs > 32) hipLaunchKernelGGL((mx4_rows_kernel<TX, T, 16, 1, 1, 4>), grid(1), dim3(1024), 0, st, a);
-    else hipLaunchKernelGGL((mx4_rows_kernel<TX, T, 8, 1, 1, 4>), grid(1), dim3(512), 0, st, a);
+    if (groups >= 4LL * cus) run(mx4_rows_kernel<TX, T, 8, 4, 1, 4>, 4);
+    else if (groups >= 2LL * cus) run(mx4_rows_kernel<TX, T, 8, 2, 1, 4>, 2);
+    else run(mx4_rows_kernel<TX, T, 8, 1, 1, 4>, 1);
   } else if constexpr (sizeof(TX) == 1) {
     if (a.M <= 32) {
-      if (many) hipLaunchKernelGGL((mx4_rows_kernel<TX, T, 8, 4, 2, 2>), grid(4), dim3(512), 0, st, a);
-      else hipLaunchKernelGGL((mx4_rows_kernel<TX, T, 8, 1, 2, 4>), grid(1), dim3(512), 0, st, a);
+      if (groups >= 2LL * cus) run(mx4_rows_kernel<TX, T, 8, 2, 2, 4>, 2);
+      else run(mx4_rows_kernel<TX, T, 8, 1, 2, 4>, 1);
     } else {
-      if (many) hipLaunchKernelGGL((mx4_rows_kernel<TX, T, 8, 2, 4, 2>), grid(2), dim3(512), 0, st, a);
-      else hipLaunchKernelGGL((mx4_rows_kernel<TX, T, 8, 1, 4, 2>), grid(1), dim3(512), 0, st, a);
+      run(mx4_rows_kernel<TX, T, 8, 1, 4, 4>, 1);
     }
   }
+}
+
+static bool use_rows(int L, int M, int N, int K) {
+  if (M > kMx4Rows || L > 65535) return false;
+  // From 17 rows on the tiles win where there are enough of them (64 rows against
+  // 16384 x 8192: 39 us by rows, 19 by tiles; 4096 x 4096: 8 and 13) or k is long
+  // enough to be cut (1024 x 16384: 23 and 13).
+  return M <= 16 || ((long long)L * ceil_div(N, 64) < compute_units() && mx4_slabs(K) <= 64);
+}
+
+struct Mx4Plan {
+  int tile, splits;
+  size_t bytes;
+};
+
+// The largest tile that gives every compute unit one; with fewer than that of the
+// smallest, k is cut into ranges of at least eight slabs and their sums are joined.
+static Mx4Plan mx4_plan(int L, int M, int N, int K) {
+  const int cus = compute_units(), slabs = (int)mx4_slabs(K);
+  auto tiles = [&](int t) { return (long long)L * ceil_div(M, t) * ceil_div(N, t); };
+  Mx4Plan p{64, 1, 0};
+  if (use_rows(L, M, N, K)) return p;
+  if (tiles(256) >= cus) p.tile = 256;
+  else if (tiles(128) >= cus) p.tile = 128;
+  else p.splits = (int)std::max<long long>(1, std::min<long long>(slabs / 8, 2LL * cus / tiles(64)));
+  if (p.splits > 1) p.bytes = (size_t)p.splits * L * M * N * 4;
+  return p;
 }
 
 static int check_mx4(const char* who, int L, int R, int K) {
@@ -637,7 +797,8 @@ extern "C" int cmk_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, v
 }
 
 extern "C" int cmk_mx4_bmm(const uint8_t* a_codes, const uint8_t* a_scales, const uint8_t* b_codes,
-                           const uint8_t* b_scales, void* C, int dtype, int L, int M, int N, int K, void* stream) {
+                           const uint8_t* b_scales, void* C, int dtype, int L, int M, int N, int K, void* workspace,
+                           size_t workspace_bytes, void* stream) {
   if (L < 0 || M < 0 || N < 0 || K < 0)
     return fail(CMK_ERR_INVALID_ARG, "cmk_mx4_bmm: negative extent (L=%d M=%d N=%d K=%d)", L, M, N, K);
   if (int e = check_dtype("cmk_mx4_bmm", dtype)) return e;
@@ -647,23 +808,43 @@ extern "C" int cmk_mx4_bmm(const uint8_t* a_codes, const uint8_t* a_scales, cons
   if (((reinterpret_cast<uintptr_t>(a_codes) | reinterpret_cast<uintptr_t>(b_codes)) & 15) ||
       ((reinterpret_cast<uintptr_t>(a_scales) | reinterpret_cast<uintptr_t>(b_scales)) & 3))
     return fail(CMK_ERR_INVALID_ARG, "cmk_mx4_bmm: codes need 16-byte alignment, scales 4-byte alignment");
-  if (M <= kMx4Rows && L <= 65535) {
+  if (use_rows(L, M, N, K)) {
     const Mx4RowsArgs r{a_codes, a_scales, b_codes, b_scales, C, M, N, K, (int)mx4_slabs(K), 0, 0};
     by_dtype(dtype, [&](auto t) { launch_rows<uint8_t, decltype(t)>(r, L, (hipStream_t)stream); });
     return hip_status(hipGetLastError(), "cmk_mx4_bmm launch");
   }
-  const bool large = (long long)L * ceil_div(M, 256) * ceil_div(N, 256) >= compute_units();
-  const int tile = large ? 256 : 128;
-  Mx4GemmArgs a{a_codes, a_scales, b_codes, b_scales, C, L, M, N, (int)mx4_slabs(K), ceil_div(M, tile), ceil_div(N, tile)};
-  const long long grid = (long long)L * a.tiles_m * a.tiles_n;
+  const Mx4Plan p = mx4_plan(L, M, N, K);
+  if (p.splits > 1 && (!workspace || workspace_bytes < p.bytes || (reinterpret_cast<uintptr_t>(workspace) & 15)))
+    return fail(CMK_ERR_WORKSPACE, "cmk_mx4_bmm: needs a 16-byte aligned workspace of %zu bytes, got %zu", p.bytes, workspace_bytes);
+  Mx4GemmArgs a{a_codes, a_scales, b_codes, b_scales, C, L, M, N, (int)mx4_slabs(K), ceil_div(M, p.tile), ceil_div(N, p.tile), p.splits,
+                (N & 7) == 0 && (reinterpret_cast<uintptr_t>(C) & 15) == 0};
+  const long long grid = (long long)L * a.tiles_m * a.tiles_n * a.splits;
   if (int e = check_grid(grid)) return e;
   hipStream_t st = (hipStream_t)stream;
   const dim3 g((unsigned)grid), b(256);
-  by_dtype(dtype, [&](auto t) {
-    if (large) hipLaunchKernelGGL((mx4_gemm_kernel<decltype(t), 256, 256>), g, b, 0, st, a);
-    else hipLaunchKernelGGL((mx4_gemm_kernel<decltype(t), 128, 128>), g, b, 0, st, a);
-  });
+  auto gemm = [&](auto t) {
+    using T = decltype(t);
+    if (p.tile == 256) hipLaunchKernelGGL((mx4_gemm_kernel<T, 256, 256, 4>), g, b, 0, st, a);
+    else if (p.tile == 128) hipLaunchKernelGGL((mx4_gemm_kernel<T, 128, 128, 4>), g, b, 0, st, a);
+    else hipLaunchKernelGGL((mx4_gemm_kernel<T, 64, 64, 8>), g, b, 0, st, a);
+  };
+  if (p.splits == 1) {
+    by_dtype(dtype, gemm);
+  } else {
+    a.c = workspace;
+    gemm(0.0f);
+    const long long n = (long long)L * M * N;
+    const dim3 joins((unsigned)std::min<long long>((n + 255) / 256, 16LL * compute_units()));
+    by_dtype(dtype, [&](auto t) {
+      hipLaunchKernelGGL(mx4_join_kernel<decltype(t)>, joins, b, 0, st, (const float*)workspace, (decltype(t)*)C, n, p.splits);
+    });
+  }
   return hip_status(hipGetLastError(), "cmk_mx4_bmm launch");
+}
+
+extern "C" size_t cmk_mx4_workspace_bytes(int L, int M, int N, int K) {
+  if (L <= 0 || M <= 0 || N <= 0 || K <= 0) return 0;
+  return mx4_plan(L, M, N, K).bytes;
 }
 
 extern "C" int cmk_mx4_bmm_rows(const void* x, int x_dtype, long long stride_l, long long stride_m, const uint8_t* b_codes,

@@ -131,6 +131,12 @@ __device__ __forceinline__ Octet<T> load_octet(const T* p, int left) {
   return o;
 }
 
+// The largest value of four neighbouring lanes, in each of them.
+__device__ __forceinline__ unsigned quad_max(unsigned v) {
+  v = max(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0xb1, 0xf, 0xf, true));  // lanes 1 0 3 2
+  return max(v, (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x4e, 0xf, 0xf, true));  // lanes 2 3 0 1
+}
+
 // Scale byte of a block whose largest magnitude has these fp32 bits.
 __device__ __forceinline__ unsigned scale_byte(unsigned top) {
   const unsigned e = top >> 23;

@@ -232,10 +232,15 @@ int cmk_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, void* out,
  * C[l][m][n] = sum_k A[l][m][k] * B[l][k][n] of two matrices in the 4-bit form,
  * A of M rows, B of N rows (its columns), accumulated in fp32 on the matrix
  * pipe and rounded once to `dtype`; C is dense and written completely.
+ * `workspace`: cmk_mx4_workspace_bytes(L, M, N, K) bytes, 16-byte aligned (0 for
+ * most shapes): with few tiles and a long contraction k is cut into ranges whose
+ * sums are joined in ascending order, as in cmk_bmm_ws_f32.
  */
 int cmk_mx4_bmm(const uint8_t* a_codes, const uint8_t* a_scales,
                 const uint8_t* b_codes, const uint8_t* b_scales, void* C,
-                int dtype, int L, int M, int N, int K, void* stream);
+                int dtype, int L, int M, int N, int K,
+                void* workspace, size_t workspace_bytes, void* stream);
+size_t cmk_mx4_workspace_bytes(int L, int M, int N, int K);
 
 /*
  * The same product for a left operand of at most 16 rows in `x_dtype`, element

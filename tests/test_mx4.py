@@ -132,12 +132,24 @@ def test_refusals_of_the_c_entry_points():
     assert lib.cmk_mx4_dequantize(ok, ok, ok, -1, 1, 1, 1, 0, None) == bad
     assert lib.cmk_mx4_dequantize(ok, ok, None, 0, 1, 1, 1, 0, None) == bad
     assert lib.cmk_mx4_dequantize(odd, ok, ok, 0, 1, 1, 1, 0, None) == bad
-    assert lib.cmk_mx4_bmm(ok, ok, ok, ok, ok, 7, 1, 1, 1, 1, None) == bad
-    assert lib.cmk_mx4_bmm(ok, ok, ok, ok, ok, 0, 1, 1, -1, 1, None) == bad
-    assert lib.cmk_mx4_bmm(ok, ok, ok, ok, None, 0, 1, 1, 1, 1, None) == bad
-    assert lib.cmk_mx4_bmm(ok, ok, None, ok, ok, 0, 1, 1, 1, 1, None) == bad
-    assert lib.cmk_mx4_bmm(ok, ok, odd, ok, ok, 0, 1, 1, 1, 1, None) == bad
+    assert lib.cmk_mx4_bmm(ok, ok, ok, ok, ok, 7, 1, 1, 1, 1, None, 0, None) == bad
+    assert lib.cmk_mx4_bmm(ok, ok, ok, ok, ok, 0, 1, 1, -1, 1, None, 0, None) == bad
+    assert lib.cmk_mx4_bmm(ok, ok, ok, ok, None, 0, 1, 1, 1, 1, None, 0, None) == bad
+    assert lib.cmk_mx4_bmm(ok, ok, None, ok, ok, 0, 1, 1, 1, 1, None, 0, None) == bad
+    assert lib.cmk_mx4_bmm(ok, ok, odd, ok, ok, 0, 1, 1, 1, 1, None, 0, None) == bad
+    # few tiles and a long contraction: a workspace, and a refusal without it
+    need = lib.cmk_mx4_workspace_bytes(1, 128, 128, 16384)
+    assert need > 0 and need % (128 * 128 * 4) == 0
+    assert lib.cmk_mx4_workspace_bytes(1, 8192, 8192, 8192) == lib.cmk_mx4_workspace_bytes(1, 1, 64, 65536) == 0
+    assert lib.cmk_mx4_bmm(ok, ok, ok, ok, ok, 0, 1, 128, 128, 16384, None, 0, None) == _lib.ERR_WORKSPACE
+    assert lib.cmk_mx4_bmm(ok, ok, ok, ok, ok, 0, 1, 128, 128, 16384, ok, need - 1, None) == _lib.ERR_WORKSPACE
+    assert lib.cmk_mx4_bmm(ok, ok, ok, ok, ok, 0, 1, 128, 128, 16384, odd, need, None) == _lib.ERR_WORKSPACE
+    assert lib.cmk_mx4_bmm_rows(ok, 0, 1, 1, ok, ok, ok, 0, 1, 17, 8, 8, None) == _lib.ERR_UNSUPPORTED
+    assert lib.cmk_mx4_bmm_rows(ok, 3, 1, 1, ok, ok, ok, 0, 1, 1, 8, 8, None) == bad
+    assert lib.cmk_mx4_bmm_rows(ok, 0, 1, 1, odd, ok, ok, 0, 1, 1, 8, 8, None) == bad
+    assert lib.cmk_mx4_bmm_rows(None, 0, 1, 1, ok, ok, ok, 0, 1, 1, 8, 8, None) == bad
+    assert lib.cmk_mx4_bmm_rows(ok, 0, 1, 1, ok, ok, ok, 0, 1, 1, -8, 8, None) == bad
     # nothing to do is no error
     assert lib.cmk_mx4_quantize(None, 0, None, None, 1, 0, 5, 1, 1, 1, None) == 0
     assert lib.cmk_mx4_dequantize(None, None, None, 0, 0, 5, 5, 0, None) == 0
-    assert lib.cmk_mx4_bmm(None, None, None, None, None, 0, 1, 0, 5, 5, None) == 0
+    assert lib.cmk_mx4_bmm(None, None, None, None, None, 0, 1, 0, 5, 5, None, 0, None) == 0

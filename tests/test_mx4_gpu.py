@@ -133,7 +133,12 @@ def check_product(got, a, b, dtype):
 
 SHAPES = [(1, 1, 1, 1), (1, 1, 17, 32), (2, 5, 3, 100), (1, 16, 64, 128), (3, 33, 65, 129), (1, 128, 128, 256),
           (2, 130, 200, 300), (1, 257, 129, 1000), (1, 1, 500, 4096), (1, 64, 1000, 640), (1, 40, 31, 5000),
-          (1, 300, 513, 130), (5, 20, 20, 20), (1, 513, 700, 2050)]
+          (1, 300, 513, 130), (5, 20, 20, 20), (1, 513, 700, 2050),
+          # each tile, with edges, odd widths and every remainder of the ring of slabs
+          (1, 100, 70, 1100), (1, 100, 70, 1030), (1, 100, 71, 800), (1, 100, 70, 700), (1, 100, 70, 600), (1, 100, 70, 513),
+          (1, 65, 64, 300), (1, 100, 70, 1), (64, 200, 150, 300), (64, 200, 151, 640), (64, 260, 300, 130), (64, 257, 259, 900),
+          # a contraction cut into ranges
+          (1, 130, 96, 5000), (2, 70, 101, 9000), (1, 200, 333, 2300)]
 
 
 @pytest.mark.parametrize("l,m,n,k", SHAPES)
