@@ -185,3 +185,17 @@ def call(fn, device, *args):
             status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     if status:
         _lib.check(status)
+
+
+def call_with_workspace(size, fn, device, size_args, args):
+    """The same for an entry point that takes a workspace: `size` says how large,
+    for the device on which the launch will run."""
+    if torch.cuda.current_device() != device.index:
+        with torch.cuda.device(device):
+            return call_with_workspace(size, fn, device, size_args, args)
+    nbytes = size(*size_args)
+    if nbytes:
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        call(fn, device, *args, workspace.data_ptr(), nbytes)
+    else:
+        call(fn, device, *args, None, 0)

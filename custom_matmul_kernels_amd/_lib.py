@@ -35,7 +35,6 @@ EXPORTS = (
     "cmk_mx4_quantize",
     "cmk_mx4_dequantize",
     "cmk_mx4_bmm",
-    "cmk_mx4_bmm_rows",
     "cmk_mx4_workspace_bytes",
     "cmk_moe",
     "cmk_moe_workspace_bytes",
@@ -59,6 +58,20 @@ class GemmDesc(ctypes.Structure):
         ("ldb", ctypes.c_longlong),
         ("strideA", ctypes.c_longlong),
         ("strideB", ctypes.c_longlong),
+    ]
+
+
+class Mx4Operand(ctypes.Structure):
+    """Mirror of ``cmk_mx4_operand`` in include/cmk.h."""
+
+    _fields_ = [
+        ("data", ctypes.c_void_p),
+        ("scales", ctypes.c_void_p),
+        ("dtype", ctypes.c_int),
+        ("reserved", ctypes.c_int),
+        ("stride_l", ctypes.c_longlong),
+        ("stride_r", ctypes.c_longlong),
+        ("stride_k", ctypes.c_longlong),
     ]
 
 
@@ -119,17 +132,17 @@ def load():
     lib.cmk_topk_1d_f32.argtypes = [p, ll, p, p, i, p, sz, p]
     lib.cmk_mx4_quantize.argtypes = [p, i, p, p, i, i, i, ll, ll, ll, p]
     lib.cmk_mx4_dequantize.argtypes = [p, p, p, i, i, i, i, i, p]
-    lib.cmk_mx4_bmm.argtypes = [p, p, p, p, p, i, i, i, i, i, p, sz, p]
-    lib.cmk_mx4_workspace_bytes.argtypes = [i, i, i, i]
+    op = ctypes.POINTER(Mx4Operand)
+    lib.cmk_mx4_bmm.argtypes = [op, op, p, i, i, i, i, i, p, sz, p]
+    lib.cmk_mx4_workspace_bytes.argtypes = [op, op, i, i, i, i]
     lib.cmk_mx4_workspace_bytes.restype = sz
-    lib.cmk_mx4_bmm_rows.argtypes = [p, i, ll, ll, p, p, p, i, i, i, i, i, p]
     mp = ctypes.POINTER(MoeDesc)
     lib.cmk_moe.argtypes = [p, p, p, p, p, p, p, p, p, mp, p, sz, p]
     lib.cmk_moe_workspace_bytes.argtypes = [mp]
     lib.cmk_moe_workspace_bytes.restype = sz
     for name in ("cmk_bmm_f32", "cmk_bmm_ws_f32", "cmk_mbmm_f32", "cmk_derive_masks_u8", "cmk_min_bmm_f32", "cmk_min_bmm_f32_static",
                  "cmk_topk_bmm_f32", "cmk_topk_1d_f32", "cmk_mx4_quantize", "cmk_mx4_dequantize",
-                 "cmk_mx4_bmm", "cmk_mx4_bmm_rows", "cmk_moe"):
+                 "cmk_mx4_bmm", "cmk_moe"):
         getattr(lib, name).restype = i
     lib.cmk_workspace_bytes.argtypes = [i, i, i, i, i, i]
     lib.cmk_workspace_bytes.restype = sz

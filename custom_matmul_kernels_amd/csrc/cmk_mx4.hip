@@ -17,13 +17,21 @@ struct QuantArgs {
   long long sl, sr, sk;  // element strides of x
 };
 
+// Two matrices of one type for one launch; the second may be empty.
+struct QuantPair {
+  QuantArgs of[2];
+};
+
 // k contiguous.  Four lanes share a block (8 elements each), 16 lanes a row's
 // slab, a wave 16 rows x one slab in four steps: it reads 256 (512) contiguous
 // bytes of a row per step and writes one contiguous KB of codes.
 template <class T>
-__global__ __launch_bounds__(256) void mx4_quantize_rows_kernel(QuantArgs a) {
+__global__ __launch_bounds__(256) void mx4_quantize_rows_kernel(QuantPair both) {
   const int lane = threadIdx.x & 63;
-  const long long unit = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  long long unit = (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const bool second = unit >= both.of[0].groups;
+  const QuantArgs& a = both.of[second ? 1 : 0];
+  if (second) unit -= both.of[0].groups;
   if (unit >= a.groups) return;
   const long long rg = unit % a.row_groups;
   const long long ls = unit / a.row_groups;  // l * slabs + slab
@@ -676,8 +684,6 @@ __global__ __launch_bounds__(64 * W) void mx4_rows_kernel(Mx4RowsArgs a) {
 
 // Rows up to this many are served by mx4_rows_kernel.
 constexpr int kMx4Rows = 64;
-// and up to this many with the left operand quantised on the way
-constexpr int kMx4RowsFloat = 16;
 
 // TX: uint8_t or the element type of the left operand.
 template <class TX, class T>
@@ -747,6 +753,33 @@ static void by_dtype(int dtype, F f) {
   else f((_Float16)0.0f);
 }
 
+// Whether the kernel that reads along k takes the matrix.
+static bool along_k(int K, long long stride_k) { return stride_k == 1 || K == 1; }
+
+static QuantArgs quant_args(const void* x, uint8_t* codes, uint8_t* scales, int L, int R, int K, long long sl, long long sr, long long sk) {
+  QuantArgs a{x, codes, scales, L, R, K, mx4_slabs(K), 0, 0, sl, sr, sk};
+  a.row_groups = along_k(K, sk) ? ((long long)R + 15) / 16 : ((long long)R + 63) / 64;
+  a.groups = a.row_groups * a.slabs * L;
+  return a;
+}
+
+// Quantises one matrix, or two of one type that are both read along k (b then).
+static int launch_quantize(int dtype, const QuantArgs& a, const QuantArgs* b, hipStream_t st) {
+  const long long grid = (a.groups + (b ? b->groups : 0) + 3) / 4;
+  if (grid == 0) return CMK_OK;
+  if (int e = check_grid(grid)) return e;
+  by_dtype(dtype, [&](auto t) {
+    using T = decltype(t);
+    if (along_k(a.K, a.sk)) {
+      const QuantPair both{{a, b ? *b : QuantArgs{}}};
+      hipLaunchKernelGGL(mx4_quantize_rows_kernel<T>, dim3((unsigned)grid), dim3(256), 0, st, both);
+    } else {
+      hipLaunchKernelGGL(mx4_quantize_columns_kernel<T>, dim3((unsigned)grid), dim3(256), 0, st, a);
+    }
+  });
+  return hip_status(hipGetLastError(), "quantisation launch");
+}
+
 }  // namespace cmk
 
 using namespace cmk;
@@ -759,19 +792,7 @@ extern "C" int cmk_mx4_quantize(const void* x, int dtype, uint8_t* codes, uint8_
   if (!x || !codes || !scales) return fail(CMK_ERR_INVALID_ARG, "cmk_mx4_quantize: null pointer");
   if ((reinterpret_cast<uintptr_t>(codes) & 15) || (reinterpret_cast<uintptr_t>(scales) & 3))
     return fail(CMK_ERR_INVALID_ARG, "cmk_mx4_quantize: codes need 16-byte alignment, scales 4-byte alignment");
-  QuantArgs a{x, codes, scales, L, R, K, mx4_slabs(K), 0, 0, stride_l, stride_r, stride_k};
-  const bool rows = stride_k == 1 || K == 1;
-  a.row_groups = rows ? ((long long)R + 15) / 16 : ((long long)R + 63) / 64;
-  a.groups = a.row_groups * a.slabs * L;
-  const long long grid = (a.groups + 3) / 4;
-  if (int e = check_grid(grid)) return e;
-  hipStream_t st = (hipStream_t)stream;
-  by_dtype(dtype, [&](auto t) {
-    using T = decltype(t);
-    if (rows) hipLaunchKernelGGL(mx4_quantize_rows_kernel<T>, dim3((unsigned)grid), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL(mx4_quantize_columns_kernel<T>, dim3((unsigned)grid), dim3(256), 0, st, a);
-  });
-  return hip_status(hipGetLastError(), "cmk_mx4_quantize launch");
+  return launch_quantize(dtype, quant_args(x, codes, scales, L, R, K, stride_l, stride_r, stride_k), nullptr, (hipStream_t)stream);
 }
 
 extern "C" int cmk_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, void* out, int dtype, int L, int R,
@@ -796,31 +817,106 @@ extern "C" int cmk_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, v
   return hip_status(hipGetLastError(), "cmk_mx4_dequantize launch");
 }
 
-extern "C" int cmk_mx4_bmm(const uint8_t* a_codes, const uint8_t* a_scales, const uint8_t* b_codes,
-                           const uint8_t* b_scales, void* C, int dtype, int L, int M, int N, int K, void* workspace,
-                           size_t workspace_bytes, void* stream) {
+// Where the pieces of a product's workspace lie: codes and scales of the operands
+// that are quantised in the call, sums of the ranges of k.
+struct Mx4Work {
+  bool on_the_way;  // the left operand is quantised by the product itself
+  size_t codes[2], scales[2], sums, bytes;
+};
+
+// Up to this many rows of a float left operand the product quantises by itself (16
+// rows against 16384 x 8192: 19.0 us that way, 17.1 in a launch before; 4 rows: 13.8
+// and 15.1).
+constexpr int kMx4RowsFloat = 8;
+
+static Mx4Work mx4_work(int a_dtype, int b_dtype, bool a_along_k, int L, int M, int N, int K) {
+  Mx4Work w{};
+  auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+  size_t at = 0;
+  w.on_the_way = a_dtype != CMK_MX4 && a_along_k && M <= kMx4RowsFloat && use_rows(L, M, N, K);
+  const int rows[2] = {M, N};
+  const bool apart[2] = {a_dtype != CMK_MX4 && !w.on_the_way, b_dtype != CMK_MX4};
+  for (int i = 0; i < 2; ++i)
+    if (apart[i]) {
+      const size_t units = (size_t)L * mx4_slabs(K) * rows[i];
+      w.codes[i] = at; at += up(units * kSlabBytes);
+      w.scales[i] = at; at += up(units * kSlabScales);
+    }
+  w.sums = at; at += up(mx4_plan(L, M, N, K).bytes);
+  w.bytes = at;
+  return w;
+}
+
+static int check_product(const char* who, const cmk_mx4_operand* A, const cmk_mx4_operand* B, int dtype, int L, int M, int N, int K) {
+  if (!A || !B) return fail(CMK_ERR_INVALID_ARG, "%s: null operand", who);
   if (L < 0 || M < 0 || N < 0 || K < 0)
-    return fail(CMK_ERR_INVALID_ARG, "cmk_mx4_bmm: negative extent (L=%d M=%d N=%d K=%d)", L, M, N, K);
-  if (int e = check_dtype("cmk_mx4_bmm", dtype)) return e;
+    return fail(CMK_ERR_INVALID_ARG, "%s: negative extent (L=%d M=%d N=%d K=%d)", who, L, M, N, K);
+  if (int e = check_dtype(who, dtype)) return e;
+  for (const cmk_mx4_operand* o : {A, B})
+    if (o->dtype != CMK_MX4)
+      if (int e = check_dtype(who, o->dtype)) return e;
+  return CMK_OK;
+}
+
+extern "C" size_t cmk_mx4_workspace_bytes(const cmk_mx4_operand* A, const cmk_mx4_operand* B, int L, int M, int N, int K) {
+  if (check_product("cmk_mx4_workspace_bytes", A, B, CMK_F32, L, M, N, K) || L == 0 || M == 0 || N == 0) return 0;
+  return mx4_work(A->dtype, B->dtype, along_k(K, A->stride_k), L, M, N, K).bytes;
+}
+
+extern "C" int cmk_mx4_bmm(const cmk_mx4_operand* A, const cmk_mx4_operand* B, void* C, int dtype, int L, int M, int N, int K,
+                           void* workspace, size_t workspace_bytes, void* stream) {
+  if (int e = check_product("cmk_mx4_bmm", A, B, dtype, L, M, N, K)) return e;
   if (L == 0 || M == 0 || N == 0) return CMK_OK;
-  if (!C || (K > 0 && (!a_codes || !a_scales || !b_codes || !b_scales)))
-    return fail(CMK_ERR_INVALID_ARG, "cmk_mx4_bmm: null pointer");
-  if (((reinterpret_cast<uintptr_t>(a_codes) | reinterpret_cast<uintptr_t>(b_codes)) & 15) ||
-      ((reinterpret_cast<uintptr_t>(a_scales) | reinterpret_cast<uintptr_t>(b_scales)) & 3))
-    return fail(CMK_ERR_INVALID_ARG, "cmk_mx4_bmm: codes need 16-byte alignment, scales 4-byte alignment");
+  if (!C) return fail(CMK_ERR_INVALID_ARG, "cmk_mx4_bmm: null pointer");
+  if (K > 0)
+    for (const cmk_mx4_operand* o : {A, B}) {
+      if (!o->data || (o->dtype == CMK_MX4 && !o->scales)) return fail(CMK_ERR_INVALID_ARG, "cmk_mx4_bmm: null pointer");
+      if (o->dtype == CMK_MX4 && ((reinterpret_cast<uintptr_t>(o->data) & 15) || (reinterpret_cast<uintptr_t>(o->scales) & 3)))
+        return fail(CMK_ERR_INVALID_ARG, "cmk_mx4_bmm: codes need 16-byte alignment, scales 4-byte alignment");
+    }
+  const Mx4Work w = mx4_work(A->dtype, B->dtype, along_k(K, A->stride_k), L, M, N, K);
+  if (w.bytes > 0 && (!workspace || workspace_bytes < w.bytes || (reinterpret_cast<uintptr_t>(workspace) & 255)))
+    return fail(CMK_ERR_WORKSPACE, "cmk_mx4_bmm: needs a 256-byte aligned workspace of %zu bytes, got %zu", w.bytes, workspace_bytes);
+  uint8_t* ws = (uint8_t*)workspace;
+  hipStream_t st = (hipStream_t)stream;
+
+  const uint8_t* codes[2] = {(const uint8_t*)A->data, (const uint8_t*)B->data};
+  const uint8_t* scales[2] = {A->scales, B->scales};
+  QuantArgs q[2];
+  const cmk_mx4_operand* pending[2];
+  int count = 0;
+  for (int i = 0; i < 2; ++i) {
+    const cmk_mx4_operand* o = i == 0 ? A : B;
+    if (o->dtype == CMK_MX4 || (i == 0 && w.on_the_way)) continue;
+    codes[i] = ws + w.codes[i];
+    scales[i] = ws + w.scales[i];
+    q[count] = quant_args(o->data, ws + w.codes[i], ws + w.scales[i], L, i == 0 ? M : N, K, o->stride_l, o->stride_r, o->stride_k);
+    pending[count++] = o;
+  }
+  if (count == 2 && pending[0]->dtype == pending[1]->dtype && along_k(K, pending[0]->stride_k) && along_k(K, pending[1]->stride_k)) {
+    if (int e = launch_quantize(pending[0]->dtype, q[0], &q[1], st)) return e;
+  } else {
+    for (int i = 0; i < count; ++i)
+      if (int e = launch_quantize(pending[i]->dtype, q[i], nullptr, st)) return e;
+  }
+
   if (use_rows(L, M, N, K)) {
-    const Mx4RowsArgs r{a_codes, a_scales, b_codes, b_scales, C, M, N, K, (int)mx4_slabs(K), 0, 0};
-    by_dtype(dtype, [&](auto t) { launch_rows<uint8_t, decltype(t)>(r, L, (hipStream_t)stream); });
+    if (w.on_the_way) {
+      const Mx4RowsArgs r{A->data, nullptr, codes[1], scales[1], C, M, N, K, (int)mx4_slabs(K), A->stride_l, A->stride_r};
+      by_dtype(A->dtype, [&](auto tx) {
+        by_dtype(dtype, [&](auto t) { launch_rows<decltype(tx), decltype(t)>(r, L, st); });
+      });
+    } else {
+      const Mx4RowsArgs r{codes[0], scales[0], codes[1], scales[1], C, M, N, K, (int)mx4_slabs(K), 0, 0};
+      by_dtype(dtype, [&](auto t) { launch_rows<uint8_t, decltype(t)>(r, L, st); });
+    }
     return hip_status(hipGetLastError(), "cmk_mx4_bmm launch");
   }
   const Mx4Plan p = mx4_plan(L, M, N, K);
-  if (p.splits > 1 && (!workspace || workspace_bytes < p.bytes || (reinterpret_cast<uintptr_t>(workspace) & 15)))
-    return fail(CMK_ERR_WORKSPACE, "cmk_mx4_bmm: needs a 16-byte aligned workspace of %zu bytes, got %zu", p.bytes, workspace_bytes);
-  Mx4GemmArgs a{a_codes, a_scales, b_codes, b_scales, C, L, M, N, (int)mx4_slabs(K), ceil_div(M, p.tile), ceil_div(N, p.tile), p.splits,
+  Mx4GemmArgs a{codes[0], scales[0], codes[1], scales[1], C, L, M, N, (int)mx4_slabs(K), ceil_div(M, p.tile), ceil_div(N, p.tile), p.splits,
                 (N & 7) == 0 && (reinterpret_cast<uintptr_t>(C) & 15) == 0};
   const long long grid = (long long)L * a.tiles_m * a.tiles_n * a.splits;
   if (int e = check_grid(grid)) return e;
-  hipStream_t st = (hipStream_t)stream;
   const dim3 g((unsigned)grid), b(256);
   auto gemm = [&](auto t) {
     using T = decltype(t);
@@ -831,37 +927,14 @@ extern "C" int cmk_mx4_bmm(const uint8_t* a_codes, const uint8_t* a_scales, cons
   if (p.splits == 1) {
     by_dtype(dtype, gemm);
   } else {
-    a.c = workspace;
+    float* sums = (float*)(ws + w.sums);
+    a.c = sums;
     gemm(0.0f);
     const long long n = (long long)L * M * N;
     const dim3 joins((unsigned)std::min<long long>((n + 255) / 256, 16LL * compute_units()));
     by_dtype(dtype, [&](auto t) {
-      hipLaunchKernelGGL(mx4_join_kernel<decltype(t)>, joins, b, 0, st, (const float*)workspace, (decltype(t)*)C, n, p.splits);
+      hipLaunchKernelGGL(mx4_join_kernel<decltype(t)>, joins, b, 0, st, sums, (decltype(t)*)C, n, p.splits);
     });
   }
   return hip_status(hipGetLastError(), "cmk_mx4_bmm launch");
-}
-
-extern "C" size_t cmk_mx4_workspace_bytes(int L, int M, int N, int K) {
-  if (L <= 0 || M <= 0 || N <= 0 || K <= 0) return 0;
-  return mx4_plan(L, M, N, K).bytes;
-}
-
-extern "C" int cmk_mx4_bmm_rows(const void* x, int x_dtype, long long stride_l, long long stride_m, const uint8_t* b_codes,
-                                const uint8_t* b_scales, void* C, int dtype, int L, int M, int N, int K, void* stream) {
-  if (L < 0 || M < 0 || N < 0 || K < 0)
-    return fail(CMK_ERR_INVALID_ARG, "cmk_mx4_bmm_rows: negative extent (L=%d M=%d N=%d K=%d)", L, M, N, K);
-  if (int e = check_dtype("cmk_mx4_bmm_rows", dtype)) return e;
-  if (int e = check_dtype("cmk_mx4_bmm_rows", x_dtype)) return e;
-  if (M > kMx4RowsFloat || L > 65535)
-    return fail(CMK_ERR_UNSUPPORTED, "cmk_mx4_bmm_rows: at most %d rows and 65535 batches (M=%d L=%d)", kMx4RowsFloat, M, L);
-  if (L == 0 || M == 0 || N == 0) return CMK_OK;
-  if (!C || (K > 0 && (!x || !b_codes || !b_scales))) return fail(CMK_ERR_INVALID_ARG, "cmk_mx4_bmm_rows: null pointer");
-  if ((reinterpret_cast<uintptr_t>(b_codes) & 15) || (reinterpret_cast<uintptr_t>(b_scales) & 3))
-    return fail(CMK_ERR_INVALID_ARG, "cmk_mx4_bmm_rows: codes need 16-byte alignment, scales 4-byte alignment");
-  const Mx4RowsArgs a{x, nullptr, b_codes, b_scales, C, M, N, K, (int)mx4_slabs(K), stride_l, stride_m};
-  by_dtype(x_dtype, [&](auto tx) {
-    by_dtype(dtype, [&](auto t) { launch_rows<decltype(tx), decltype(t)>(a, L, (hipStream_t)stream); });
-  });
-  return hip_status(hipGetLastError(), "cmk_mx4_bmm_rows launch");
 }

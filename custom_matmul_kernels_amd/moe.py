@@ -79,16 +79,14 @@ class MoECUDA:
         y = torch.empty((t, h), dtype=x.dtype, device=dev)
         weights = torch.empty((t, self.k), dtype=torch.float32, device=dev)
         experts = torch.empty((t, self.k), dtype=torch.int64, device=dev)
+        dtype = _common.FLOAT_TYPES[x.dtype]
+        rest = (h, i, e, self.k, dtype, _common.FLOAT_TYPES[router.dtype], _lib.MX4 if gs is not None else dtype,
+                ACTIVATIONS[self.activation], int(self.renormalize), max(x.stride(0), h), max(router.stride(0), h),
+                ldg, sg, ldd, sd)
         for t0 in range(0, t, CHUNK):
-            n = min(CHUNK, t - t0)
-            part = x[t0:t0 + n]
-            d = _lib.MoeDesc(n, h, i, e, self.k, _common.FLOAT_TYPES[x.dtype], _common.FLOAT_TYPES[router.dtype],
-                             _lib.MX4 if gs is not None else _common.FLOAT_TYPES[x.dtype],
-                             ACTIVATIONS[self.activation], int(self.renormalize),
-                             max(part.stride(0), h), max(router.stride(0), h), ldg, sg, ldd, sd)
-            nbytes = self._lib.cmk_moe_workspace_bytes(d)
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-            _common.call(self._lib.cmk_moe, dev, part.data_ptr(), router.data_ptr(), gp, gs, dp, ds,
-                         y[t0:].data_ptr(), weights[t0:].data_ptr(), experts[t0:].data_ptr(), d,
-                         ws.data_ptr(), nbytes)
+            d = _lib.MoeDesc(min(CHUNK, t - t0), *rest)
+            part = (x, y, weights, experts) if t0 == 0 else (x[t0:], y[t0:], weights[t0:], experts[t0:])
+            xp, yp, wp, ep = (v.data_ptr() for v in part)
+            _common.call_with_workspace(self._lib.cmk_moe_workspace_bytes, self._lib.cmk_moe, dev, (d,),
+                                        (xp, router.data_ptr(), gp, gs, dp, ds, yp, wp, ep, d))
         return y, weights, experts

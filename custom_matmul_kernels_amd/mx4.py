@@ -7,8 +7,6 @@ from . import _common, _lib
 
 BLOCK = 32        # elements along k that share a scale
 SLAB = 128        # elements of k that lie together in storage
-ROWS_IN_CALL = 8  # rows of a float left operand that the product itself quantises (16 rows against
-                  # 16384 x 8192: 19.0 us in the call, 17.1 apart; 4 rows: 13.8 and 15.1)
 
 
 class MX4Tensor:
@@ -176,23 +174,25 @@ class MX4BMMCUDA:
         self.out_dtype = out_dtype
         self._lib = _lib.load()
 
+    @staticmethod
+    def _operand(T, k_axis, name):
+        """The library's description of an operand [l, rows, k] with k at `k_axis`."""
+        if isinstance(T, MX4Tensor):
+            assert T.k_axis == k_axis, "the blocks of %s must run along k" % name
+            return _lib.Mx4Operand(*T._pointers(), _lib.MX4)
+        dtype = _common.float_type(T.dtype, name)
+        _common.refuse_grad(T)
+        stride = T.stride()
+        return _lib.Mx4Operand(T.data_ptr(), None, dtype, 0, stride[0] if len(stride) == 3 else 0,
+                               stride[-3 - k_axis], stride[k_axis])
+
     def __call__(self, A, B):
-        four_a, four_b = isinstance(A, MX4Tensor), isinstance(B, MX4Tensor)
         sa, sb, device = A.shape, B.shape, A.device
         n = len(sa)
         assert len(sb) == n
         if n not in (2, 3):
             raise ValueError("A and B need to be 2d or 3d")
-        if four_a:
-            assert A.k_axis == -1, "the blocks of A must run along k"
-        else:
-            a_type = _common.float_type(A.dtype, "A")
-            _common.refuse_grad(A)
-        if four_b:
-            assert B.k_axis == -2, "the blocks of B must run along k"
-        else:
-            _common.float_type(B.dtype, "B")
-            _common.refuse_grad(B)
+        a, b = self._operand(A, -1, "A"), self._operand(B, -2, "B")
         m, k = sa[-2:]
         c = sb[-1]
         l = 1 if n == 2 else sa[0]
@@ -202,20 +202,6 @@ class MX4BMMCUDA:
         assert device == B.device
         C = torch.empty((m, c) if n == 2 else (l, m, c), dtype=self.out_dtype, device=device)
         if l and m and c:
-            if not four_b:
-                B = quantize_mx4(B, -2)
-            b_codes, b_scales = B._pointers()
-            if not four_a:
-                stride = A.stride()
-                if m <= ROWS_IN_CALL and l <= 65535 and (stride[-1] == 1 or k <= 1):
-                    _common.call(self._lib.cmk_mx4_bmm_rows, device, A.data_ptr(), a_type, stride[0] if n == 3 else 0,
-                                 stride[-2], b_codes, b_scales, C.data_ptr(), self._out, l, m, c, k)
-                    return C
-                A = quantize_mx4(A, -1)
-            a_codes, a_scales = A._pointers()
-            nbytes, ws = self._lib.cmk_mx4_workspace_bytes(l, m, c, k), None
-            if nbytes:
-                ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-            _common.call(self._lib.cmk_mx4_bmm, device, a_codes, a_scales, b_codes, b_scales, C.data_ptr(), self._out,
-                         l, m, c, k, ws.data_ptr() if nbytes else None, nbytes)
+            _common.call_with_workspace(self._lib.cmk_mx4_workspace_bytes, self._lib.cmk_mx4_bmm, device, (a, b, l, m, c, k),
+                                        (a, b, C.data_ptr(), self._out, l, m, c, k))
         return C

@@ -228,29 +228,32 @@ int cmk_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, void* out,
                        int dtype, int L, int R, int K, int rows_innermost,
                        void* stream);
 
-/*
- * C[l][m][n] = sum_k A[l][m][k] * B[l][k][n] of two matrices in the 4-bit form,
- * A of M rows, B of N rows (its columns), accumulated in fp32 on the matrix
- * pipe and rounded once to `dtype`; C is dense and written completely.
- * `workspace`: cmk_mx4_workspace_bytes(L, M, N, K) bytes, 16-byte aligned (0 for
- * most shapes): with few tiles and a long contraction k is cut into ranges whose
- * sums are joined in ascending order, as in cmk_bmm_ws_f32.
- */
-int cmk_mx4_bmm(const uint8_t* a_codes, const uint8_t* a_scales,
-                const uint8_t* b_codes, const uint8_t* b_scales, void* C,
-                int dtype, int L, int M, int N, int K,
-                void* workspace, size_t workspace_bytes, void* stream);
-size_t cmk_mx4_workspace_bytes(int L, int M, int N, int K);
+/* An operand of the 4-bit product: R rows of K elements in each of L batches (the
+ * right operand's rows are the columns of the matrix). */
+typedef struct cmk_mx4_operand {
+  const void* data;        /* codes (16-byte aligned) for CMK_MX4, else elements   */
+  const uint8_t* scales;   /* for CMK_MX4 (4-byte aligned)                         */
+  int dtype;               /* CMK_MX4, CMK_F32, CMK_BF16 or CMK_F16                */
+  int reserved;
+  long long stride_l, stride_r, stride_k;  /* elements; not read for CMK_MX4       */
+} cmk_mx4_operand;
 
 /*
- * The same product for a left operand of at most 16 rows in `x_dtype`, element
- * (l, m, k) at x[l*stride_l + m*stride_m + k], quantised on the way: the bits of
- * cmk_mx4_quantize and cmk_mx4_bmm in one launch.
+ * C[l][m][n] = sum_k A[l][m][k] * B[l][k][n] of two matrices in the 4-bit form, A
+ * of M rows, B of N, accumulated in fp32 on the matrix pipe and rounded once to
+ * `dtype`; C is dense and written completely.  An operand given as floats is
+ * quantised in the call, with the bits of cmk_mx4_quantize: a left one of few rows
+ * by the product itself, others into the workspace.
+ * `workspace`: cmk_mx4_workspace_bytes(...) bytes (may be 0), 256-byte aligned.
+ * Apart from the operands' 4-bit forms it holds, where tiles are few and the
+ * contraction is long, the sums of ranges of k that are joined in ascending order,
+ * as in cmk_bmm_ws_f32.
  */
-int cmk_mx4_bmm_rows(const void* x, int x_dtype, long long stride_l,
-                     long long stride_m, const uint8_t* b_codes,
-                     const uint8_t* b_scales, void* C, int dtype,
-                     int L, int M, int N, int K, void* stream);
+int cmk_mx4_bmm(const cmk_mx4_operand* A, const cmk_mx4_operand* B, void* C,
+                int dtype, int L, int M, int N, int K,
+                void* workspace, size_t workspace_bytes, void* stream);
+size_t cmk_mx4_workspace_bytes(const cmk_mx4_operand* A, const cmk_mx4_operand* B,
+                               int L, int M, int N, int K);
 
 /* activations of the experts */
 #define CMK_ACT_SILU 0   /* g / (1 + exp(-g))            */

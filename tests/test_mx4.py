@@ -132,24 +132,49 @@ def test_refusals_of_the_c_entry_points():
     assert lib.cmk_mx4_dequantize(ok, ok, ok, -1, 1, 1, 1, 0, None) == bad
     assert lib.cmk_mx4_dequantize(ok, ok, None, 0, 1, 1, 1, 0, None) == bad
     assert lib.cmk_mx4_dequantize(odd, ok, ok, 0, 1, 1, 1, 0, None) == bad
-    assert lib.cmk_mx4_bmm(ok, ok, ok, ok, ok, 7, 1, 1, 1, 1, None, 0, None) == bad
-    assert lib.cmk_mx4_bmm(ok, ok, ok, ok, ok, 0, 1, 1, -1, 1, None, 0, None) == bad
-    assert lib.cmk_mx4_bmm(ok, ok, ok, ok, None, 0, 1, 1, 1, 1, None, 0, None) == bad
-    assert lib.cmk_mx4_bmm(ok, ok, None, ok, ok, 0, 1, 1, 1, 1, None, 0, None) == bad
-    assert lib.cmk_mx4_bmm(ok, ok, odd, ok, ok, 0, 1, 1, 1, 1, None, 0, None) == bad
+    def four(data=ok, scales=ok):
+        return _lib.Mx4Operand(data, scales, _lib.MX4)
+
+    def floats(data=ok, dtype=_lib.F32, sk=1):
+        return _lib.Mx4Operand(data, None, dtype, 0, 1, 1, sk)
+
+    def bmm(a, b, c=ok, dtype=0, l=1, m=1, n=1, k=1, ws=None, nbytes=0):
+        return lib.cmk_mx4_bmm(a, b, c, dtype, l, m, n, k, ws, nbytes, None)
+
+    def need(a, b, l, m, n, k):
+        return lib.cmk_mx4_workspace_bytes(a, b, l, m, n, k)
+
+    assert bmm(None, four()) == bad
+    assert bmm(four(), four(), dtype=7) == bad
+    assert bmm(four(), four(), dtype=_lib.MX4) == bad
+    assert bmm(floats(dtype=9), four()) == bad
+    assert bmm(four(), four(), n=-1) == bad
+    assert bmm(four(), four(), c=None) == bad
+    assert bmm(four(), four(data=None)) == bad
+    assert bmm(four(scales=None), four()) == bad
+    assert bmm(four(), four(data=odd)) == bad
+    assert bmm(four(scales=odd), four()) == bad
+    assert bmm(floats(data=None), four()) == bad
     # few tiles and a long contraction: a workspace, and a refusal without it
-    need = lib.cmk_mx4_workspace_bytes(1, 128, 128, 16384)
-    assert need > 0 and need % (128 * 128 * 4) == 0
-    assert lib.cmk_mx4_workspace_bytes(1, 8192, 8192, 8192) == lib.cmk_mx4_workspace_bytes(1, 1, 64, 65536) == 0
-    assert lib.cmk_mx4_bmm(ok, ok, ok, ok, ok, 0, 1, 128, 128, 16384, None, 0, None) == _lib.ERR_WORKSPACE
-    assert lib.cmk_mx4_bmm(ok, ok, ok, ok, ok, 0, 1, 128, 128, 16384, ok, need - 1, None) == _lib.ERR_WORKSPACE
-    assert lib.cmk_mx4_bmm(ok, ok, ok, ok, ok, 0, 1, 128, 128, 16384, odd, need, None) == _lib.ERR_WORKSPACE
-    assert lib.cmk_mx4_bmm_rows(ok, 0, 1, 1, ok, ok, ok, 0, 1, 17, 8, 8, None) == _lib.ERR_UNSUPPORTED
-    assert lib.cmk_mx4_bmm_rows(ok, 3, 1, 1, ok, ok, ok, 0, 1, 1, 8, 8, None) == bad
-    assert lib.cmk_mx4_bmm_rows(ok, 0, 1, 1, odd, ok, ok, 0, 1, 1, 8, 8, None) == bad
-    assert lib.cmk_mx4_bmm_rows(None, 0, 1, 1, ok, ok, ok, 0, 1, 1, 8, 8, None) == bad
-    assert lib.cmk_mx4_bmm_rows(ok, 0, 1, 1, ok, ok, ok, 0, 1, 1, -8, 8, None) == bad
+    size = need(four(), four(), 1, 128, 128, 16384)
+    assert size > 0 and size % (128 * 128 * 4) == 0
+    assert need(four(), four(), 1, 8192, 8192, 8192) == need(four(), four(), 1, 1, 64, 65536) == 0
+    fault = _lib.ERR_WORKSPACE
+    assert bmm(four(), four(), m=128, n=128, k=16384) == fault
+    assert bmm(four(), four(), m=128, n=128, k=16384, ws=ok, nbytes=size - 1) == fault
+    assert bmm(four(), four(), m=128, n=128, k=16384, ws=ctypes.c_void_p(0x1010), nbytes=size) == fault
+    # operands that are quantised in the call need room for their 4-bit form, a left one of few rows does not
+    assert need(floats(), four(), 1, 4, 512, 1000) == 0
+    assert need(floats(sk=7), four(), 1, 4, 512, 1000) >= 8 * 4 * 68
+    assert need(floats(), floats(), 2, 100, 512, 1000) >= 2 * 8 * (100 + 512) * 68
+    assert bmm(four(), floats()) == fault and bmm(floats(), floats()) == fault
+    assert need(None, four(), 1, 1, 1, 1) == need(four(), four(), 1, 0, 1, 1) == need(floats(dtype=9), four(), 1, 1, 1, 1) == 0
     # nothing to do is no error
     assert lib.cmk_mx4_quantize(None, 0, None, None, 1, 0, 5, 1, 1, 1, None) == 0
     assert lib.cmk_mx4_dequantize(None, None, None, 0, 0, 5, 5, 0, None) == 0
-    assert lib.cmk_mx4_bmm(None, None, None, None, None, 0, 1, 0, 5, 5, None, 0, None) == 0
+    assert bmm(four(None, None), four(None, None), c=None, m=0, n=5, k=5) == 0
+
+
+def test_operand_layout_matches_header():
+    assert ctypes.sizeof(_lib.Mx4Operand) == 48
+    assert _lib.Mx4Operand.stride_l.offset == 24
