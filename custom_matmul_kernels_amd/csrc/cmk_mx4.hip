@@ -101,6 +101,50 @@ struct DequantArgs {
   long long slabs, row_groups, groups;
 };
 
+// Large results are stored past the caches: they would not stay there, and what ran
+// before and what runs next keep their lines (dequantisation of 8192 x 8192 to bf16
+// 40 -> 34 us and the quantisation in front of it 38 -> 33; a product with 512 MB of
+// results 116 -> 119 us, the quantisation of the next call's operands 62 -> 24).  Only
+// where rows are whole cache lines: partial lines are merged by the L2 alone.
+constexpr size_t kStreamBytes = 32u << 20;
+
+static int streams(const void* out, long long rows, long long row_bytes) {
+  return (size_t)rows * row_bytes >= kStreamBytes && row_bytes % 128 == 0 && (reinterpret_cast<uintptr_t>(out) & 127) == 0;
+}
+
+template <bool STREAM, class V>
+__device__ __forceinline__ void store_as(V* p, V v) {
+  if constexpr (STREAM) __builtin_nontemporal_store(v, p);
+  else *p = v;
+}
+
+template <bool STREAM, class T>
+__device__ __forceinline__ void store_one(T* p, T v) {
+  if constexpr (sizeof(T) == 4) store_as<STREAM>((unsigned*)p, __builtin_bit_cast(unsigned, v));
+  else store_as<STREAM>((u16*)p, __builtin_bit_cast(u16, v));
+}
+
+// N elements, 16 (8) bytes at a time, at any element's address.
+template <bool STREAM, class T, int N>
+__device__ __forceinline__ void store_run(T* p, const T (&v)[N]) {
+  if constexpr (!STREAM) {
+    __builtin_memcpy(p, v, sizeof(v));
+  } else if constexpr (sizeof(v) % 16 == 0) {
+    typedef u32x4v __attribute__((aligned(2))) any16;
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(v) / 16; ++i) {
+      u32x4v w;
+      __builtin_memcpy(&w, (const char*)v + 16 * i, 16);
+      __builtin_nontemporal_store(w, (any16*)((char*)p + 16 * i));
+    }
+  } else {
+    typedef u32x2 __attribute__((aligned(2))) any8;
+    u32x2 w;
+    __builtin_memcpy(&w, v, 8);
+    __builtin_nontemporal_store(w, (any8*)p);
+  }
+}
+
 // Eight values of a word of codes, in fp32.  The conversion is exact: a code times
 // a power of two.  A scale byte of 255 is NaN.
 __device__ __forceinline__ void decode_octet(unsigned w, unsigned s, float* v) {
@@ -120,7 +164,7 @@ __device__ __forceinline__ void decode_octet(unsigned w, unsigned s, float* v) {
   }
 }
 
-template <class T>
+template <class T, bool STREAM>
 __global__ __launch_bounds__(256) void mx4_dequantize_rows_kernel(DequantArgs a) {
   const int lane = threadIdx.x & 63;
   const long long unit = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -143,7 +187,7 @@ __global__ __launch_bounds__(256) void mx4_dequantize_rows_kernel(DequantArgs a)
     for (int i = 0; i < 8; ++i) o[i] = from_f32<T>(v[i]);
     T* out = (T*)a.out + ((long long)l * a.R + row) * a.K + k0;
     if (k0 + 8 <= a.K) {
-      __builtin_memcpy(out, o, sizeof(o));
+      store_run<STREAM>(out, o);
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
@@ -152,32 +196,54 @@ __global__ __launch_bounds__(256) void mx4_dequantize_rows_kernel(DequantArgs a)
   }
 }
 
-template <class T>
+// Rows innermost: a lane takes one slab of V neighbouring rows, so that it stores V
+// values side by side.
+template <class T, int V, bool STREAM>
 __global__ __launch_bounds__(256) void mx4_dequantize_columns_kernel(DequantArgs a) {
   const long long unit = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (unit >= a.groups) return;
   const long long rg = unit % a.row_groups;
   const long long ls = unit / a.row_groups;
   const int l = (int)(ls / a.slabs), slab = (int)(ls % a.slabs);
-  const long long row = rg * 64 + (threadIdx.x & 63);
+  const long long row = (rg * 64 + (threadIdx.x & 63)) * V;
   if (row >= a.R) return;
-  const long long at = ls * a.R + row;
-  const unsigned scales = *(const unsigned*)(a.scales + at * kSlabScales);
+  const int have = (int)min((long long)V, a.R - row);
+  unsigned scales[V];
+  u32x4v w[V][4];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const long long at = ls * a.R + row + min(v, have - 1);
+    scales[v] = *(const unsigned*)(a.scales + at * kSlabScales);
+#pragma unroll
+    for (int b = 0; b < 4; ++b) w[v][b] = *(const u32x4v*)(a.codes + at * kSlabBytes + b * 16);
+  }
   T* out = (T*)a.out + (long long)l * a.K * a.R + row;
 #pragma unroll
-  for (int b = 0; b < 4; ++b) {
-    const u32x4v w = *(const u32x4v*)(a.codes + at * kSlabBytes + b * 16);
+  for (int b = 0; b < 4; ++b)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      float v[8];
-      decode_octet(w[i], scales >> (8 * b) & 255u, v);
+      float x[V][8];
+#pragma unroll
+      for (int v = 0; v < V; ++v) decode_octet(w[v][b][i], scales[v] >> (8 * b) & 255u, x[v]);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int k = slab * kSlab + b * 32 + i * 8 + j;
-        if (k < a.K) out[(long long)k * a.R] = from_f32<T>(v[j]);
+        if (k >= a.K) continue;
+        T* p = out + (long long)k * a.R;
+        T o[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) o[v] = from_f32<T>(x[v][j]);
+        if constexpr (V == 1) {
+          store_one<STREAM>(p, o[0]);
+        } else if (have == V) {
+          store_run<STREAM>(p, o);
+        } else {
+#pragma unroll
+          for (int v = 0; v < V; ++v)
+            if (v < have) p[v] = o[v];
+        }
       }
     }
-  }
 }
 
 // -------------------------------------------------------------------- product
@@ -189,6 +255,7 @@ struct Mx4GemmArgs {
   int slabs;
   int tiles_m, tiles_n;
   int splits;  // ranges of slabs
+  int stream;  // c is stored past the caches
   int wide;    // rows of c start on 16-byte boundaries and hold whole multiples of them
 };
 
@@ -448,42 +515,46 @@ __global__ __launch_bounds__(256, 1) void mx4_gemm_kernel(Mx4GemmArgs a) {
   // columns, exchanged between neighbouring lanes, took 380 instead of 275 us at
   // 8192^3).
   T* c = (T*)a.c + ((long long)split * a.L + l) * a.M * a.N;
-  if constexpr (sizeof(T) == 2) {
-    if (a.wide) {
-      constexpr int WM = TM / 2, WN = TN / 2, kPitch = WN * 2 + 16, kLanes = WN / 8, kRows = 64 / kLanes;
-      static_assert(4 * WM * kPitch <= S * Tile::kStageBytes, "the tile fits into the ring");
-      meet();  // every wave has read its last slab
-      uint8_t* mine = lds + wave * (WM * kPitch);
+  auto store_tile = [&](auto past) {
+    constexpr bool STREAM = decltype(past)::value;
+    if constexpr (sizeof(T) == 2) {
+      if (a.wide) {
+        constexpr int WM = TM / 2, WN = TN / 2, kPitch = WN * 2 + 16, kLanes = WN / 8, kRows = 64 / kLanes;
+        static_assert(4 * WM * kPitch <= S * Tile::kStageBytes, "the tile fits into the ring");
+        meet();  // every wave has read its last slab
+        uint8_t* mine = lds + wave * (WM * kPitch);
 #pragma unroll
-      for (int bm = 0; bm < BM; ++bm)
+        for (int bm = 0; bm < BM; ++bm)
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
+          for (int i = 0; i < 16; ++i)
 #pragma unroll
-          for (int bn = 0; bn < BN; ++bn)
-            *(T*)(mine + (bm * 32 + 8 * (i >> 2) + 4 * h + (i & 3)) * kPitch + (bn * 32 + r) * 2) = from_f32<T>(acc[bm][bn][i]);
-      const int col = lane % kLanes * 8, n = n0 + wn + col;
-#pragma unroll 4
-      for (int i = lane / kLanes; i < WM; i += kRows) {
-        const u32x4v v = *(const u32x4v*)(mine + i * kPitch + col * 2);
-        const int m = m0 + wm + i;
-        if (m < a.M && n < a.N) *(u32x4v*)(c + (long long)m * a.N + n) = v;
-      }
-      return;
-    }
-  }
-#pragma unroll
-  for (int bm = 0; bm < BM; ++bm)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int m = m0 + wm + bm * 32 + 8 * (i >> 2) + 4 * h + (i & 3);
-      if (m >= a.M) continue;
-      T* row = c + (long long)m * a.N;
-#pragma unroll
-      for (int bn = 0; bn < BN; ++bn) {
-        const int n = n0 + wn + bn * 32 + r;
-        if (n < a.N) row[n] = from_f32<T>(acc[bm][bn][i]);
+            for (int bn = 0; bn < BN; ++bn)
+              *(T*)(mine + (bm * 32 + 8 * (i >> 2) + 4 * h + (i & 3)) * kPitch + (bn * 32 + r) * 2) = from_f32<T>(acc[bm][bn][i]);
+        const int col = lane % kLanes * 8, n = n0 + wn + col;
+        for (int i = lane / kLanes; i < WM; i += kRows) {
+          const u32x4v v = *(const u32x4v*)(mine + i * kPitch + col * 2);
+          const int m = m0 + wm + i;
+          if (m < a.M && n < a.N) store_as<STREAM>((u32x4v*)(c + (long long)m * a.N + n), v);
+        }
+        return;
       }
     }
+#pragma unroll
+    for (int bm = 0; bm < BM; ++bm)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int m = m0 + wm + bm * 32 + 8 * (i >> 2) + 4 * h + (i & 3);
+        if (m >= a.M) continue;
+        T* row = c + (long long)m * a.N;
+#pragma unroll
+        for (int bn = 0; bn < BN; ++bn) {
+          const int n = n0 + wn + bn * 32 + r;
+          if (n < a.N) store_one<STREAM>(row + n, from_f32<T>(acc[bm][bn][i]));
+        }
+      }
+  };
+  if (a.stream) store_tile(Int<1>{});
+  else store_tile(Int<0>{});
 }
 
 // The sum of the splits, in their order.
@@ -803,16 +874,23 @@ extern "C" int cmk_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, v
   if (!out || !codes || !scales) return fail(CMK_ERR_INVALID_ARG, "cmk_mx4_dequantize: null pointer");
   if ((reinterpret_cast<uintptr_t>(codes) & 15) || (reinterpret_cast<uintptr_t>(scales) & 3))
     return fail(CMK_ERR_INVALID_ARG, "cmk_mx4_dequantize: codes need 16-byte alignment, scales 4-byte alignment");
+  const int size = dtype == CMK_F32 ? 4 : 2;
   DequantArgs a{codes, scales, out, L, R, K, mx4_slabs(K), 0, 0};
-  a.row_groups = rows_innermost ? ((long long)R + 63) / 64 : ((long long)R + 15) / 16;
+  // four rows a lane where a wave's 256 rows are there
+  const int v = rows_innermost && R >= 256 ? 4 : 1;
+  const bool past = rows_innermost ? (size_t)L * R * K * size >= kStreamBytes && v == 4 : streams(out, (long long)L * R, (long long)K * size);
+  a.row_groups = rows_innermost ? ((long long)R + 64 * v - 1) / (64 * v) : ((long long)R + 15) / 16;
   a.groups = a.row_groups * a.slabs * L;
   const long long grid = (a.groups + 3) / 4;
   if (int e = check_grid(grid)) return e;
   hipStream_t st = (hipStream_t)stream;
   by_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-    if (rows_innermost) hipLaunchKernelGGL(mx4_dequantize_columns_kernel<T>, dim3((unsigned)grid), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL(mx4_dequantize_rows_kernel<T>, dim3((unsigned)grid), dim3(256), 0, st, a);
+    const dim3 g((unsigned)grid), b(256);
+    auto run = [&](auto kernel) { hipLaunchKernelGGL(kernel, g, b, 0, st, a); };
+    if (!rows_innermost) past ? run(mx4_dequantize_rows_kernel<T, true>) : run(mx4_dequantize_rows_kernel<T, false>);
+    else if (v == 4) past ? run(mx4_dequantize_columns_kernel<T, 4, true>) : run(mx4_dequantize_columns_kernel<T, 4, false>);
+    else run(mx4_dequantize_columns_kernel<T, 1, false>);
   });
   return hip_status(hipGetLastError(), "cmk_mx4_dequantize launch");
 }
@@ -914,6 +992,7 @@ extern "C" int cmk_mx4_bmm(const cmk_mx4_operand* A, const cmk_mx4_operand* B, v
   }
   const Mx4Plan p = mx4_plan(L, M, N, K);
   Mx4GemmArgs a{codes[0], scales[0], codes[1], scales[1], C, L, M, N, (int)mx4_slabs(K), ceil_div(M, p.tile), ceil_div(N, p.tile), p.splits,
+                p.splits == 1 && streams(C, (long long)L * M, (long long)N * (dtype == CMK_F32 ? 4 : 2)),
                 (N & 7) == 0 && (reinterpret_cast<uintptr_t>(C) & 15) == 0};
   const long long grid = (long long)L * a.tiles_m * a.tiles_n * a.splits;
   if (int e = check_grid(grid)) return e;
