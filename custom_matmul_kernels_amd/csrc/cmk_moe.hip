@@ -74,6 +74,46 @@ __device__ __forceinline__ int plane_position(int k) {
   return four_bit ? (k & ~127) | (k & 24) << 2 | (k & 96) >> 2 | (k & 7) : k;
 }
 
+// Adds one slab of 16 experts x 16 tokens to the logits; `write`: this lane also
+// writes its elements of x to the planes.
+template <class TX, class TR, bool FOUR, int PLANES>
+__device__ __forceinline__ void moe_router_slab(const MoeArgs& a, f64x4 (&acc)[2], const TX* x, const TR* w, int t, int slab, int q, bool write) {
+  Octet<TX> ox[4];
+  Octet<TR> ow[4];
+#pragma unroll
+  for (int s = 0; s < 4; ++s) {
+    const int h = slab * kSlab + s * 32 + q * 8;
+    ox[s] = load_octet(x + h, a.H - h);
+    ow[s] = load_octet(w + h, a.H - h);
+  }
+  if (write) {
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      u16 hi[8], lo[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if constexpr (PLANES == 1) {
+          hi[i] = ox[s].bits(i);
+        } else {
+          const float f = ox[s].get(i);
+          const __bf16 b = (__bf16)f;
+          hi[i] = __builtin_bit_cast(u16, b);
+          // an infinity or a NaN stays in the first plane alone
+          lo[i] = __builtin_bit_cast(u16, (__bf16)(__builtin_isfinite(f) ? f - (float)b : 0.0f));
+        }
+      }
+      const long long at = (long long)t * a.Hp + plane_position<FOUR>(slab * kSlab + s * 32 + q * 8);
+      __builtin_memcpy(a.xp + at, hi, 16);
+      if constexpr (PLANES == 2) __builtin_memcpy(a.xp + (long long)a.T * a.Hp + at, lo, 16);
+    }
+  }
+#pragma unroll
+  for (int s = 0; s < 4; ++s)
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      acc[i & 1] = __builtin_amdgcn_mfma_f64_16x16x4f64((double)ow[s].get(i), (double)ox[s].get(i), acc[i & 1], 0, 0, 0);
+}
+
 // Logits by fp64 matrix instructions: the products of the operands are exact in
 // fp64 and the sums off by 2^-53 a step, so that the order of the choice does not
 // hang on the order of the sums; equal rows of the router give equal bits.  A
@@ -91,42 +131,8 @@ __global__ __launch_bounds__(64 * kRouterWaves) void moe_logits_kernel(MoeArgs a
   const TX* x = (const TX*)a.x + t * a.ld_x;
   const TR* w = (const TR*)a.router + e * a.ld_router;
   f64x4 acc[2] = {};
-  for (int slab = blockIdx.z * kRouterWaves + wave; slab < a.Hp / kSlab; slab += a.splits * kRouterWaves) {
-    Octet<TX> ox[4];
-    Octet<TR> ow[4];
-#pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      const int h = slab * kSlab + s * 32 + q * 8;
-      ox[s] = load_octet(x + h, a.H - h);
-      ow[s] = load_octet(w + h, a.H - h);
-    }
-    if (blockIdx.x == 0 && t0 + r < a.T) {
-#pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        u16 hi[8], lo[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if constexpr (PLANES == 1) {
-            hi[i] = ox[s].bits(i);
-          } else {
-            const float f = ox[s].get(i);
-            const __bf16 b = (__bf16)f;
-            hi[i] = __builtin_bit_cast(u16, b);
-            // an infinity or a NaN stays in the first plane alone
-            lo[i] = __builtin_bit_cast(u16, (__bf16)(__builtin_isfinite(f) ? f - (float)b : 0.0f));
-          }
-        }
-        const long long at = (long long)t * a.Hp + plane_position<FOUR>(slab * kSlab + s * 32 + q * 8);
-        __builtin_memcpy(a.xp + at, hi, 16);
-        if constexpr (PLANES == 2) __builtin_memcpy(a.xp + (long long)a.T * a.Hp + at, lo, 16);
-      }
-    }
-#pragma unroll
-    for (int s = 0; s < 4; ++s)
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        acc[i & 1] = __builtin_amdgcn_mfma_f64_16x16x4f64((double)ow[s].get(i), (double)ox[s].get(i), acc[i & 1], 0, 0, 0);
-  }
+  for (int slab = blockIdx.z * kRouterWaves + wave; slab < a.Hp / kSlab; slab += a.splits * kRouterWaves)
+    moe_router_slab<TX, TR, FOUR, PLANES>(a, acc, x, w, t, slab, q, blockIdx.x == 0 && t0 + r < a.T);
 #pragma unroll
   for (int i = 0; i < 4; ++i) part[wave][lane][i] = acc[0][i] + acc[1][i];
   __syncthreads();
@@ -243,6 +249,72 @@ __global__ __launch_bounds__(256) void moe_select_kernel(MoeArgs a) {
     a.chosen[s] = c.pick[threadIdx.x];
     a.experts[s] = c.pick[threadIdx.x];
     a.weights[s] = moe_weight(a, c, threadIdx.x);
+  }
+}
+
+// Router and choice in one launch, for a router of few tiles: a work-group takes 16
+// tokens, a wave one (two) of the units of 16 experts x one slab, then a token.  (7
+// tokens, 10 experts, H = 1000: 4.2 + 3.6 us as two launches.)
+constexpr int kSmallUnits = 32, kSmallExperts = 128;
+
+static bool small_router(int E, int Hp) { return E <= kSmallExperts && (E + 15) / 16 * (Hp / kSlab) <= kSmallUnits; }
+
+template <class TX, class TR, bool FOUR, int PLANES>
+__global__ __launch_bounds__(1024) void moe_router_small_kernel(MoeArgs a) {
+  __shared__ double part[kSmallUnits][64][4];
+  __shared__ double logit[16][kSmallExperts];
+  __shared__ unsigned long long key[16][kSmallExperts];
+  __shared__ int pick[16][kMoeChoices];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r = lane & 15, q = lane >> 4;
+  const int t0 = blockIdx.x * 16, slabs = a.Hp / kSlab, units = (a.E + 15) / 16 * slabs;
+  {
+    const int t = min(t0 + r, a.T - 1);
+    const TX* x = (const TX*)a.x + t * a.ld_x;
+    for (int u = wave; u < units; u += 16) {
+      const int tile = u / slabs;
+      const TR* w = (const TR*)a.router + min(tile * 16 + r, a.E - 1) * a.ld_router;
+      f64x4 acc[2] = {};
+      moe_router_slab<TX, TR, FOUR, PLANES>(a, acc, x, w, t, u - tile * slabs, q, tile == 0 && t0 + r < a.T);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) part[u][lane][i] = acc[0][i] + acc[1][i];
+    }
+  }
+  __syncthreads();
+  for (int v = threadIdx.x; v < a.E * 16; v += 1024) {
+    const int e = v >> 4, t = v & 15, in = e & 15;
+    double sum = 0;
+    for (int s = 0; s < slabs; ++s) sum += part[(e >> 4) * slabs + s][(in & 3) * 16 + t][in >> 2];
+    logit[t][e] = sum;
+    key[t][e] = order_key(sum);
+  }
+  __syncthreads();
+  const int t = t0 + wave;
+  if (t < a.T) {
+    for (int e = lane; e < a.E; e += 64) {
+      const unsigned long long mine = key[wave][e];
+      int before = 0;
+#pragma unroll 8
+      for (int o = 0; o < a.E; ++o) {
+        const unsigned long long other = key[wave][o];
+        before += other > mine || (other == mine && o < e);
+      }
+      if (before < a.k) pick[wave][before] = e;
+    }
+  }
+  __syncthreads();
+  if (t >= a.T) return;
+  const double top = logit[wave][pick[wave][0]];
+  float sum = 0;
+  const int count = a.renormalize ? a.k : a.E;
+  for (int e = lane; e < count; e += 64) sum += expf((float)(logit[wave][a.renormalize ? pick[wave][e] : e] - top));
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
+  if (lane < a.k) {
+    const int s = t * a.k + lane, e = pick[wave][lane];
+    a.chosen[s] = e;
+    a.experts[s] = e;
+    a.weights[s] = expf((float)(logit[wave][e] - top)) / sum;
   }
 }
 
@@ -770,34 +842,38 @@ extern "C" int cmk_moe(const void* x, const void* router, const void* gate_up, c
             d->T, d->H, d->I, d->E, d->k, p.Hp, p.Ip, p.splits, d->activation, d->renormalize,
             (double*)(ws + p.logits), (int*)(ws + p.chosen), (u16*)(ws + p.x), (u16*)(ws + p.h), (float*)(ws + p.y)};
   hipStream_t st = (hipStream_t)stream;
-  const dim3 router_grid(ceil_div(d->E, 16), ceil_div(d->T, 16), p.splits);
   const bool r32 = d->router_dtype == CMK_F32, four = d->w_dtype == CMK_MX4;
-  auto logits = [&](auto kernel) { hipLaunchKernelGGL(kernel, router_grid, dim3(64 * kRouterWaves), 0, st, a); };
-  if (d->x_dtype == CMK_BF16) {
-    if (four) r32 ? logits(moe_logits_kernel<__bf16, float, true, 1>) : logits(moe_logits_kernel<__bf16, __bf16, true, 1>);
-    else r32 ? logits(moe_logits_kernel<__bf16, float, false, 1>) : logits(moe_logits_kernel<__bf16, __bf16, false, 1>);
-  } else {
-    if (four) r32 ? logits(moe_logits_kernel<_Float16, float, true, 2>) : logits(moe_logits_kernel<_Float16, _Float16, true, 2>);
-    else r32 ? logits(moe_logits_kernel<_Float16, float, false, 1>) : logits(moe_logits_kernel<_Float16, _Float16, false, 1>);
-  }
-  if (d->T == 1) {
-    const dim3 up(ceil_div(p.Ip, 16), d->k), dn(ceil_div(d->H, 16)), b(64 * kMoeWaves);
-    if (d->w_dtype == CMK_BF16) {
-      hipLaunchKernelGGL((moe_gate_up_single_kernel<CMK_BF16, 1, 4, 1, 4>), up, b, 0, st, a);
-      hipLaunchKernelGGL((moe_down_single_kernel<CMK_BF16, __bf16, 16, 2>), dn, dim3(1024), 0, st, a);
-    } else if (d->w_dtype == CMK_F16) {
-      hipLaunchKernelGGL((moe_gate_up_single_kernel<CMK_F16, 1, 4, 1, 4>), up, b, 0, st, a);
-      hipLaunchKernelGGL((moe_down_single_kernel<CMK_F16, _Float16, 16, 2>), dn, dim3(1024), 0, st, a);
-    } else if (d->x_dtype == CMK_BF16) {
-      hipLaunchKernelGGL((moe_gate_up_single_kernel<CMK_MX4, 1, 4, 1, 4>), up, b, 0, st, a);
-      hipLaunchKernelGGL((moe_down_single_kernel<CMK_MX4, __bf16, 16, 4>), dn, dim3(1024), 0, st, a);
-    } else {
-      hipLaunchKernelGGL((moe_gate_up_single_kernel<CMK_MX4, 2, 4, 1, 4>), up, b, 0, st, a);
-      hipLaunchKernelGGL((moe_down_single_kernel<CMK_MX4, _Float16, 16, 4>), dn, dim3(1024), 0, st, a);
+  const bool small = d->T > 1 && small_router(d->E, p.Hp);
+  auto run_router = [&](auto split_kernel, auto small_kernel) {
+    if (small) {
+      hipLaunchKernelGGL(small_kernel, dim3(ceil_div(d->T, 16)), dim3(1024), 0, st, a);
+      return;
     }
+    hipLaunchKernelGGL(split_kernel, dim3(ceil_div(d->E, 16), ceil_div(d->T, 16), p.splits), dim3(64 * kRouterWaves), 0, st, a);
+    if (d->T > 1) hipLaunchKernelGGL(moe_select_kernel, dim3(d->T), dim3(256), 0, st, a);
+  };
+#define ROUTER(...) run_router(moe_logits_kernel<__VA_ARGS__>, moe_router_small_kernel<__VA_ARGS__>)
+  if (d->x_dtype == CMK_BF16) {
+    if (four) r32 ? ROUTER(__bf16, float, true, 1) : ROUTER(__bf16, __bf16, true, 1);
+    else r32 ? ROUTER(__bf16, float, false, 1) : ROUTER(__bf16, __bf16, false, 1);
+  } else {
+    if (four) r32 ? ROUTER(_Float16, float, true, 2) : ROUTER(_Float16, _Float16, true, 2);
+    else r32 ? ROUTER(_Float16, float, false, 1) : ROUTER(_Float16, _Float16, false, 1);
+  }
+#undef ROUTER
+  if (d->T == 1) {
+    auto run = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(ceil_div(p.Ip, 16), d->k), dim3(64 * kMoeWaves), 0, st, a); };
+    if (d->w_dtype == CMK_BF16) run(moe_gate_up_single_kernel<CMK_BF16, 1, 4, 1, 4>);
+    else if (d->w_dtype == CMK_F16) run(moe_gate_up_single_kernel<CMK_F16, 1, 4, 1, 4>);
+    else if (d->x_dtype == CMK_BF16) run(moe_gate_up_single_kernel<CMK_MX4, 1, 4, 1, 4>);
+    else run(moe_gate_up_single_kernel<CMK_MX4, 2, 4, 1, 4>);
+    auto down = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(ceil_div(d->H, 16)), dim3(1024), 0, st, a); };
+    if (d->w_dtype == CMK_BF16) down(moe_down_single_kernel<CMK_BF16, __bf16, 16, 2>);
+    else if (d->w_dtype == CMK_F16) down(moe_down_single_kernel<CMK_F16, _Float16, 16, 2>);
+    else if (d->x_dtype == CMK_BF16) down(moe_down_single_kernel<CMK_MX4, __bf16, 16, 4>);
+    else down(moe_down_single_kernel<CMK_MX4, _Float16, 16, 4>);
     return hip_status(hipGetLastError(), "cmk_moe launch");
   }
-  hipLaunchKernelGGL(moe_select_kernel, dim3(d->T), dim3(256), 0, st, a);
   const int units = d->T * d->k <= d->E ? d->T * d->k : d->E;
   // rows a work-group: 16 * rg for each of the kMoeWaves / ks groups of waves
   auto experts_kernel = [&](auto kernel, int rows, int rg, int ks) {
@@ -812,16 +888,20 @@ extern "C" int cmk_moe(const void* x, const void* router, const void* gate_up, c
       if (many) experts_kernel(moe_gate_up_kernel<CMK_MX4, 2, 1, 1, 3>, p.Ip, 1, 1);
       else experts_kernel(moe_gate_up_kernel<CMK_MX4, 2, 4, 1, 2>, p.Ip, 1, 4);
     }
-    if (many) experts_kernel(moe_down_kernel<CMK_MX4, 2, 4, 2>, d->H, 4, 2);
-    else experts_kernel(moe_down_kernel<CMK_MX4, 4, 2, 2>, d->H, 2, 4);
   } else if (d->w_dtype == CMK_BF16) {
     if (many) experts_kernel(moe_gate_up_kernel<CMK_BF16, 1, 4, 1, 1>, p.Ip, 1, 4);
     else experts_kernel(moe_gate_up_kernel<CMK_BF16, 1, 4, 1, 2>, p.Ip, 1, 4);
-    if (many) experts_kernel(moe_down_kernel<CMK_BF16, 1, 1, 4>, d->H, 1, 1);
-    else experts_kernel(moe_down_kernel<CMK_BF16, 4, 1, 2>, d->H, 1, 4);
   } else {
     if (many) experts_kernel(moe_gate_up_kernel<CMK_F16, 1, 4, 1, 1>, p.Ip, 1, 4);
     else experts_kernel(moe_gate_up_kernel<CMK_F16, 1, 4, 1, 2>, p.Ip, 1, 4);
+  }
+  if (d->w_dtype == CMK_MX4) {
+    if (many) experts_kernel(moe_down_kernel<CMK_MX4, 2, 4, 2>, d->H, 4, 2);
+    else experts_kernel(moe_down_kernel<CMK_MX4, 4, 2, 2>, d->H, 2, 4);
+  } else if (d->w_dtype == CMK_BF16) {
+    if (many) experts_kernel(moe_down_kernel<CMK_BF16, 1, 1, 4>, d->H, 1, 1);
+    else experts_kernel(moe_down_kernel<CMK_BF16, 4, 1, 2>, d->H, 1, 4);
+  } else {
     if (many) experts_kernel(moe_down_kernel<CMK_F16, 1, 1, 4>, d->H, 1, 1);
     else experts_kernel(moe_down_kernel<CMK_F16, 4, 1, 2>, d->H, 1, 4);
   }
