@@ -658,7 +658,7 @@ __global__ __launch_bounds__(64 * W) void mx4_rows_kernel(Mx4RowsArgs a) {
             f[i].codes = *(const u32x4v*)((const uint8_t*)a.x + at * kSlabBytes + (lane & 3) * 16);
             f[i].scale = a.x_scales[at * kSlabScales + (lane & 3)];
           } else {
-            const TX* x = (const TX*)a.x + l * a.sl + m * a.sm + s0 * kSlab + lane * 8;
+            const TX* x = (const TX*)a.x + l * a.sl + m * a.sm + (long long)s0 * kSlab + lane * 8;
             if (s0 + 16 <= whole) {  // no lane is beyond the end
 #pragma unroll
               for (int e = 0; e < 4; ++e) __builtin_memcpy(o[i][e].v, x + 4 * e * kSlab, sizeof(o[i][e].v));
@@ -754,7 +754,7 @@ __global__ __launch_bounds__(64 * W) void mx4_rows_kernel(Mx4RowsArgs a) {
 }
 
 // Rows up to this many are served by mx4_rows_kernel.
-constexpr int kMx4Rows = 64;
+constexpr int kMx4Rows = 32;
 
 // TX: uint8_t or the element type of the left operand.
 template <class TX, class T>
@@ -769,20 +769,16 @@ static void launch_rows(const Mx4RowsArgs& a, int L, hipStream_t st) {
     else if (groups >= 2LL * cus) run(mx4_rows_kernel<TX, T, 8, 2, 1, 4>, 2);
     else run(mx4_rows_kernel<TX, T, 8, 1, 1, 4>, 1);
   } else if constexpr (sizeof(TX) == 1) {
-    if (a.M <= 32) {
-      if (groups >= 2LL * cus) run(mx4_rows_kernel<TX, T, 8, 2, 2, 4>, 2);
-      else run(mx4_rows_kernel<TX, T, 8, 1, 2, 4>, 1);
-    } else {
-      run(mx4_rows_kernel<TX, T, 8, 1, 4, 4>, 1);
-    }
+    if (groups >= 2LL * cus) run(mx4_rows_kernel<TX, T, 8, 2, 2, 4>, 2);
+    else run(mx4_rows_kernel<TX, T, 8, 1, 2, 4>, 1);
   }
 }
 
 static bool use_rows(int L, int M, int N, int K) {
   if (M > kMx4Rows || L > 65535) return false;
-  // From 17 rows on the tiles win where there are enough of them (64 rows against
-  // 16384 x 8192: 39 us by rows, 19 by tiles; 4096 x 4096: 8 and 13) or k is long
-  // enough to be cut (1024 x 16384: 23 and 13).
+  // From 17 rows on the tiles win where there are enough of them (32 rows against
+  // 16384 x 8192: 24 us by rows, 14 by tiles; 4096 x 4096: 5.4 and 7.6) or k is long
+  // enough to be cut (1024 x 16384: 16 and 8).
   return M <= 16 || ((long long)L * ceil_div(N, 64) < compute_units() && mx4_slabs(K) <= 64);
 }
 
@@ -791,16 +787,34 @@ struct Mx4Plan {
   size_t bytes;
 };
 
-// The largest tile that gives every compute unit one; with fewer than that of the
-// smallest, k is cut into ranges of at least eight slabs and their sums are joined.
+// Microseconds that `tiles` tiles of `slabs` slabs take, as measured on 256 compute
+// units: a fixed part and one per slab, for a compute unit that holds one or two
+// work-groups (the largest tile fills its LDS).  One tile each, 64 slabs: 61, 28, 13
+// us; two each: 45 (of 128), 21 (of 64).
+static double tile_cost(int tile, long long tiles, int slabs, int cus) {
+  const double one = tile == 256 ? 9 + 0.85 * slabs : tile == 128 ? 4.5 + 0.37 * slabs : 3.5 + 0.145 * slabs;
+  const double two = tile == 256 ? 2 * one : tile == 128 ? 5 + 0.63 * slabs : 3.5 + 0.28 * slabs;
+  const long long rest = tiles % (2LL * cus);
+  return tiles / (2LL * cus) * two + (rest == 0 ? 0 : rest <= cus ? one : two);
+}
+
+// The tile, and for the smallest the number of ranges of k, that cost least.  Ranges
+// pay for a second kernel that reads what they wrote (1024 x 1024 with 64 slabs: 13 us
+// whole, 19 in two ranges; 128 x 1024 with 128 slabs: 40 whole, 13 in eight).
 static Mx4Plan mx4_plan(int L, int M, int N, int K) {
   const int cus = compute_units(), slabs = (int)mx4_slabs(K);
   auto tiles = [&](int t) { return (long long)L * ceil_div(M, t) * ceil_div(N, t); };
   Mx4Plan p{64, 1, 0};
   if (use_rows(L, M, N, K)) return p;
-  if (tiles(256) >= cus) p.tile = 256;
-  else if (tiles(128) >= cus) p.tile = 128;
-  else p.splits = (int)std::max<long long>(1, std::min<long long>(slabs / 8, 2LL * cus / tiles(64)));
+  double best = tile_cost(64, tiles(64), slabs, cus);
+  for (int tile : {128, 256}) {
+    const double cost = tile_cost(tile, tiles(tile), slabs, cus);
+    if (cost < best) { best = cost; p.tile = tile; }
+  }
+  for (int s = 2; s <= 16 && s * 4 <= slabs && s * tiles(64) <= 2LL * cus; ++s) {
+    const double cost = tile_cost(64, s * tiles(64), ceil_div(slabs, s), cus) + 4 + 8e-6 / 4.9 * s * L * M * N;
+    if (cost < best) { best = cost; p.tile = 64; p.splits = s; }
+  }
   if (p.splits > 1) p.bytes = (size_t)p.splits * L * M * N * 4;
   return p;
 }
@@ -929,6 +943,8 @@ static int check_product(const char* who, const cmk_mx4_operand* A, const cmk_mx
   if (!A || !B) return fail(CMK_ERR_INVALID_ARG, "%s: null operand", who);
   if (L < 0 || M < 0 || N < 0 || K < 0)
     return fail(CMK_ERR_INVALID_ARG, "%s: negative extent (L=%d M=%d N=%d K=%d)", who, L, M, N, K);
+  if (M > (1 << 30) || N > (1 << 30))
+    return fail(CMK_ERR_UNSUPPORTED, "%s: M and N are at most %d (M=%d N=%d)", who, 1 << 30, M, N);
   if (int e = check_dtype(who, dtype)) return e;
   for (const cmk_mx4_operand* o : {A, B})
     if (o->dtype != CMK_MX4)

@@ -34,59 +34,63 @@ class MoECUDA:
         assert type(renormalize) == bool
         assert k >= 1
         self.k, self.activation, self.renormalize = k, activation, renormalize
+        self._activation = ACTIVATIONS[activation]
         self._lib = _lib.load()
 
     @staticmethod
-    def _experts(W, x, name):
+    def _experts(W, shape, dtype, name):
         """(pointer, scales' pointer, row stride, expert stride) of [e, r, c] weights."""
         if isinstance(W, MX4Tensor):
+            assert W.shape == shape
             assert W.k_axis == -1, "the blocks of %s must run along its last axis" % name
             return W._pointers() + (0, 0)
-        if W.dtype != x.dtype:
+        if W.dtype != dtype:
             raise TypeError("%s must be an MX4Tensor or of x's type, got %s" % (name, W.dtype))
+        assert W.shape == shape
         _common.refuse_grad(W)
+        e, r, c = shape
         s0, s1, s2 = W.stride()
-        e, r, c = W.shape
-        if (s2 != 1 and c > 1) or (s1 < c and r > 1) or (s0 < 0 and e > 1):
+        if (s2 != 1 and c > 1) or (s1 < c and r > 1):
             raise ValueError("the last axis of %s must be contiguous" % name)
         return W.data_ptr(), None, s1 if r > 1 else c, s0 if e > 1 else 0
 
     def __call__(self, x, router, gate_up, down):
-        if x.dtype not in (torch.bfloat16, torch.float16):
-            raise TypeError("x must be torch.bfloat16 or torch.float16, got %s" % x.dtype)
-        if router.dtype not in (torch.float32, x.dtype):
+        dtype, device = x.dtype, x.device
+        if dtype != torch.bfloat16 and dtype != torch.float16:
+            raise TypeError("x must be torch.bfloat16 or torch.float16, got %s" % dtype)
+        if router.dtype != dtype and router.dtype != torch.float32:
             raise TypeError("router must be torch.float32 or of x's type, got %s" % router.dtype)
         if x.dim() != 2 or router.dim() != 2 or gate_up.dim() != 3 or down.dim() != 3:
             raise ValueError("x and router need to be 2d, gate_up and down 3d")
         t, h = x.shape
         e, two_i, _ = gate_up.shape
         i = two_i // 2
-        assert tuple(router.shape) == (e, h)
+        assert router.shape == (e, h)
         assert two_i == 2 * i and i > 0 and h > 0
-        assert tuple(gate_up.shape) == (e, 2 * i, h) and tuple(down.shape) == (e, h, i)
         assert 0 < self.k <= e
         _common.refuse_grad(x, router)
-        gp, gs, ldg, sg = self._experts(gate_up, x, "gate_up")
-        dp, ds, ldd, sd = self._experts(down, x, "down")
-        assert isinstance(gate_up, MX4Tensor) == isinstance(down, MX4Tensor)
-        dev = x.device
-        assert dev.type == "cuda"
-        assert router.device == gate_up.device == down.device == dev
-        if h > 1 and x.stride(1) != 1 or t > 1 and x.stride(0) < h:
+        gp, gs, ldg, sg = self._experts(gate_up, (e, two_i, h), dtype, "gate_up")
+        dp, ds, ldd, sd = self._experts(down, (e, h, i), dtype, "down")
+        assert (gs is None) == (ds is None), "gate_up and down must be of one kind"
+        assert device.type == "cuda"
+        assert router.device == device and gate_up.device == device and down.device == device
+        sx, sr = x.stride(), router.stride()
+        if h > 1 and sx[1] != 1 or t > 1 and sx[0] < h:
             x = x.contiguous()
-        if h > 1 and router.stride(1) != 1 or e > 1 and router.stride(0) < h:
+            sx = (h, 1)
+        if h > 1 and sr[1] != 1 or e > 1 and sr[0] < h:
             router = router.contiguous()
-        y = torch.empty((t, h), dtype=x.dtype, device=dev)
-        weights = torch.empty((t, self.k), dtype=torch.float32, device=dev)
-        experts = torch.empty((t, self.k), dtype=torch.int64, device=dev)
-        dtype = _common.FLOAT_TYPES[x.dtype]
-        rest = (h, i, e, self.k, dtype, _common.FLOAT_TYPES[router.dtype], _lib.MX4 if gs is not None else dtype,
-                ACTIVATIONS[self.activation], int(self.renormalize), max(x.stride(0), h), max(router.stride(0), h),
-                ldg, sg, ldd, sd)
+            sr = (h, 1)
+        y = torch.empty((t, h), dtype=dtype, device=device)
+        weights = torch.empty((t, self.k), dtype=torch.float32, device=device)
+        experts = torch.empty((t, self.k), dtype=torch.int64, device=device)
+        code = _common.FLOAT_TYPES[dtype]
+        rest = (h, i, e, self.k, code, _common.FLOAT_TYPES[router.dtype], code if gs is None else _lib.MX4,
+                self._activation, int(self.renormalize), max(sx[0], h), max(sr[0], h), ldg, sg, ldd, sd)
         for t0 in range(0, t, CHUNK):
             d = _lib.MoeDesc(min(CHUNK, t - t0), *rest)
             part = (x, y, weights, experts) if t0 == 0 else (x[t0:], y[t0:], weights[t0:], experts[t0:])
-            xp, yp, wp, ep = (v.data_ptr() for v in part)
-            _common.call_with_workspace(self._lib.cmk_moe_workspace_bytes, self._lib.cmk_moe, dev, (d,),
-                                        (xp, router.data_ptr(), gp, gs, dp, ds, yp, wp, ep, d))
+            _common.call_with_workspace(self._lib.cmk_moe_workspace_bytes, self._lib.cmk_moe, device, (d,),
+                                        (part[0].data_ptr(), router.data_ptr(), gp, gs, dp, ds, part[1].data_ptr(),
+                                         part[2].data_ptr(), part[3].data_ptr(), d))
         return y, weights, experts

@@ -150,6 +150,7 @@ def test_refusals_of_the_c_entry_points():
     assert bmm(floats(dtype=9), four()) == bad
     assert bmm(four(), four(), n=-1) == bad
     assert bmm(four(), four(), c=None) == bad
+    assert bmm(four(), four(), m=(1 << 30) + 1) == bmm(four(), four(), n=(1 << 30) + 1) == _lib.ERR_UNSUPPORTED
     assert bmm(four(), four(data=None)) == bad
     assert bmm(four(scales=None), four()) == bad
     assert bmm(four(), four(data=odd)) == bad
