@@ -545,29 +545,42 @@ __device__ __forceinline__ void join_waves(f32x4 (&acc)[N], f32x4 (*part)[N][64]
   }
 }
 
-// RG * 16 gate rows and the up rows that go with them, against NB * 16 tokens of
-// one expert.  KS waves split H between them; the other waves of the work-group
-// take the next rows.
-template <int WF, int PLANES, int KS, int RG, int NB, int U>
-__device__ __forceinline__ void moe_gate_up_tokens(const MoeArgs& a, int expert, const int* list, int c0, int count, char* lds) {
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int share = wave % KS;
-  const int r = lane & 15, q = lane >> 4;
-  const int i0 = (blockIdx.x * (kMoeWaves / KS) + wave / KS) * 16 * RG;
-  const char* base = (const char*)a.gate_up + (WF == CMK_MX4 ? (long long)expert * (a.Hp / 2) * (2 * a.I) : expert * a.stride_gate_up * 2);
-  const uint8_t* scales = WF == CMK_MX4 ? a.gate_up_scales + (long long)expert * (a.Hp / 32) * (2 * a.I) : nullptr;
-  long long row[2][RG];
+// Where an expert's matrices lie, and which rows a lane reads; rows beyond the last
+// are replaced by it.
+template <int WF>
+__device__ __forceinline__ const char* moe_gate_up_base(const MoeArgs& a, int expert) {
+  return (const char*)a.gate_up + (WF == CMK_MX4 ? (long long)expert * (a.Hp / 2) * (2 * a.I) : expert * a.stride_gate_up * 2);
+}
+template <int WF>
+__device__ __forceinline__ const uint8_t* moe_gate_up_scales(const MoeArgs& a, int expert) {
+  return WF == CMK_MX4 ? a.gate_up_scales + (long long)expert * (a.Hp / 32) * (2 * a.I) : nullptr;
+}
+template <int WF>
+__device__ __forceinline__ const char* moe_down_base(const MoeArgs& a, int expert) {
+  return (const char*)a.down + (WF == CMK_MX4 ? (long long)expert * (a.Ip / 2) * a.H : expert * a.stride_down * 2);
+}
+template <int WF>
+__device__ __forceinline__ const uint8_t* moe_down_scales(const MoeArgs& a, int expert) {
+  return WF == CMK_MX4 ? a.down_scales + (long long)expert * (a.Ip / 32) * a.H : nullptr;
+}
+template <int RG>
+__device__ __forceinline__ void moe_gate_up_rows(const MoeArgs& a, int i0, long long (&row)[2][RG]) {
 #pragma unroll
   for (int g = 0; g < RG; ++g) {
-    row[0][g] = min(i0 + g * 16 + r, a.I - 1);
+    row[0][g] = min(i0 + g * 16 + ((int)threadIdx.x & 15), a.I - 1);
     row[1][g] = a.I + row[0][g];
   }
-  f32x4 acc[2][RG][NB] = {};
-  auto source = [&](int c) { return a.xp + (long long)(list[c0 + c] / a.k) * a.Hp; };
-  moe_products<WF, PLANES, 2, RG, NB, U, KS, false>(acc, base, scales, 2 * a.I, row, a.ld_gate_up, a.H, min(count - c0, NB * 16),
-                                                    source, (long long)a.T * a.Hp, share, i0 >= a.I, lds);
-  join_waves<KS, 2 * RG * NB>((f32x4(&)[2 * RG * NB])acc, (f32x4(*)[2 * RG * NB][64])lds, share);
-  if (share > 0) return;
+}
+template <int RG>
+__device__ __forceinline__ void moe_down_rows(const MoeArgs& a, int n0, long long (&row)[1][RG]) {
+#pragma unroll
+  for (int g = 0; g < RG; ++g) row[0][g] = min(n0 + g * 16 + ((int)threadIdx.x & 15), a.H - 1);
+}
+
+// act(gate) * up of a wave's rows to the planes of the inner activations.
+template <int WF, int RG, int NB>
+__device__ __forceinline__ void moe_store_inner(const MoeArgs& a, const f32x4 (&acc)[2][RG][NB], const int* list, int c0, int count, int i0) {
+  const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
     const int c = c0 + b * 16 + r;
@@ -591,6 +604,42 @@ __device__ __forceinline__ void moe_gate_up_tokens(const MoeArgs& a, int expert,
       __builtin_memcpy(at + (long long)a.T * a.k * a.Ip, lo, 8);
     }
   }
+}
+
+// A wave's rows of the slots' outputs.
+template <int RG, int NB>
+__device__ __forceinline__ void moe_store_outer(const MoeArgs& a, const f32x4 (&acc)[1][RG][NB], const int* list, int c0, int count, int n0) {
+  const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    const int c = c0 + b * 16 + r;
+    if (c >= count) continue;
+    float* y = a.yp + (long long)list[c] * a.H;
+#pragma unroll
+    for (int g = 0; g < RG; ++g) {
+      const int n = n0 + g * 16 + q * 4;
+      const float v[4] = {acc[0][g][b][0], acc[0][g][b][1], acc[0][g][b][2], acc[0][g][b][3]};
+      store4(y + n, v, a.H - n, (a.H & 3) == 0);
+    }
+  }
+}
+
+// RG * 16 gate rows and the up rows that go with them, against NB * 16 tokens of
+// one expert.  KS waves split H between them; the other waves of the work-group
+// take the next rows.
+template <int WF, int PLANES, int KS, int RG, int NB, int U>
+__device__ __forceinline__ void moe_gate_up_tokens(const MoeArgs& a, int expert, const int* list, int c0, int count, char* lds) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int share = wave % KS;
+  const int i0 = (blockIdx.x * (kMoeWaves / KS) + wave / KS) * 16 * RG;
+  long long row[2][RG];
+  moe_gate_up_rows<RG>(a, i0, row);
+  f32x4 acc[2][RG][NB] = {};
+  auto source = [&](int c) { return a.xp + (long long)(list[c0 + c] / a.k) * a.Hp; };
+  moe_products<WF, PLANES, 2, RG, NB, U, KS, false>(acc, moe_gate_up_base<WF>(a, expert), moe_gate_up_scales<WF>(a, expert), 2 * a.I, row, a.ld_gate_up, a.H, min(count - c0, NB * 16),
+                                                    source, (long long)a.T * a.Hp, share, i0 >= a.I, lds);
+  join_waves<KS, 2 * RG * NB>((f32x4(&)[2 * RG * NB])acc, (f32x4(*)[2 * RG * NB][64])lds, share);
+  if (share == 0) moe_store_inner<WF, RG, NB>(a, acc, list, c0, count, i0);
 }
 
 template <int WF, int PLANES, int KS, int RG, int U>
@@ -632,33 +681,17 @@ __global__ __launch_bounds__(64 * kMoeWaves) void moe_gate_up_single_kernel(MoeA
 // RG * 16 rows of an expert's down matrix against its slots' activations.
 template <int WF, int KS, int RG, int NB, int U>
 __device__ __forceinline__ void moe_down_tokens(const MoeArgs& a, int expert, const int* list, int c0, int count, char* lds) {
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int share = wave % KS;
-  const int r = lane & 15, q = lane >> 4;
   const int n0 = (blockIdx.x * (kMoeWaves / KS) + wave / KS) * 16 * RG;
-  const char* base = (const char*)a.down + (WF == CMK_MX4 ? (long long)expert * (a.Ip / 2) * a.H : expert * a.stride_down * 2);
-  const uint8_t* scales = WF == CMK_MX4 ? a.down_scales + (long long)expert * (a.Ip / 32) * a.H : nullptr;
   long long row[1][RG];
-#pragma unroll
-  for (int g = 0; g < RG; ++g) row[0][g] = min(n0 + g * 16 + r, a.H - 1);
+  moe_down_rows<RG>(a, n0, row);
   f32x4 acc[1][RG][NB] = {};
   auto source = [&](int c) { return a.hp + (long long)list[c0 + c] * a.Ip; };
-  moe_products<WF, 2, 1, RG, NB, U, KS, WF == CMK_F16>(acc, base, scales, a.H, row, a.ld_down, a.I, min(count - c0, NB * 16), source,
+  moe_products<WF, 2, 1, RG, NB, U, KS, WF == CMK_F16>(acc, moe_down_base<WF>(a, expert), moe_down_scales<WF>(a, expert), a.H, row, a.ld_down, a.I, min(count - c0, NB * 16), source,
                                                        (long long)a.T * a.k * a.Ip, share, n0 >= a.H, lds);
   join_waves<KS, RG * NB>((f32x4(&)[RG * NB])acc, (f32x4(*)[RG * NB][64])lds, share);
-  if (share > 0) return;
-#pragma unroll
-  for (int b = 0; b < NB; ++b) {
-    const int c = c0 + b * 16 + r;
-    if (c >= count) continue;
-    float* y = a.yp + (long long)list[c] * a.H;
-#pragma unroll
-    for (int g = 0; g < RG; ++g) {
-      const int n = n0 + g * 16 + q * 4;
-      const float v[4] = {acc[0][g][b][0], acc[0][g][b][1], acc[0][g][b][2], acc[0][g][b][3]};
-      store4(y + n, v, a.H - n, (a.H & 3) == 0);
-    }
-  }
+  if (share == 0) moe_store_outer<RG, NB>(a, acc, list, c0, count, n0);
 }
 
 template <int WF, int KS, int RG, int U>
@@ -670,6 +703,150 @@ __global__ __launch_bounds__(64 * kMoeWaves) void moe_down_kernel(MoeArgs a) {
   for (int c0 = 0; c0 < count; c0 += 32) {
     if (count - c0 <= 16) moe_down_tokens<WF, KS, RG, 1, U>(a, expert, list, c0, count, lds);
     else moe_down_tokens<WF, KS, RG, 2, U>(a, expert, list, c0, count, lds);
+  }
+}
+
+// Where experts have many tokens each, the activations of a pass do not fit LDS and
+// staging them in pieces leaves the memory idle between them (8 experts of 4096 x
+// 4096, 64 tokens: 255 us in bf16, 151 in 4 bits).  These kernels walk k with a ring
+// of four slabs of activations in LDS, fetched by direct loads, and the weights in the
+// register ring as before; the four waves take rows of their own.  Within a row the 16
+// blocks of 16 bytes of a slab are stored at position block ^ (row & 15), so that the
+// 16 rows of a fragment spread over the banks.
+constexpr int kDenseStages = 4;
+constexpr int kDenseBlocks = 2;  // blocks of 16 slots of a pass (four would leave a compute unit one work-group)
+
+template <int WF, int PLANES, int M, int RG, int NB, int U, bool SPLIT, class Source>
+__device__ __forceinline__ void moe_dense_products(f32x4 (&acc)[M][RG][NB], const void* base, const uint8_t* scales, long long rows,
+                                                   const long long (&row)[M][RG], long long ld, int K, int count, Source source,
+                                                   long long plane, uint8_t* lds) {
+  constexpr int kStage = NB * 16 * PLANES * 2 * kSlab;
+  constexpr int kActs = NB * PLANES;                               // requests of a wave per slab of activations,
+  constexpr int kWeights = M * RG * (WF == CMK_MX4 ? 2 : 4);       // and of weights
+  static_assert(U <= kDenseStages - 1 && 2 * kActs + U * kWeights < 64, "the count of requests under way");
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r = lane & 15, q = lane >> 4;
+  const int slabs = (K + kSlab - 1) / kSlab;
+  // an instruction fetches four rows of one plane; rows beyond the slots repeat the last
+  const char* from[kActs];
+#pragma unroll
+  for (int j = 0; j < kActs; ++j) {
+    const int line = (wave * kActs + j) * 4 + (lane >> 4), in = line % (NB * 16), p = line / (NB * 16);
+    from[j] = (const char*)(source(min(in, count - 1)) + p * plane) + ((lane & 15) ^ (in & 15)) * 16;
+  }
+  auto fetch = [&](int slab) {
+    uint8_t* stage = lds + slab % kDenseStages * kStage;
+#pragma unroll
+    for (int j = 0; j < kActs; ++j)
+      __builtin_amdgcn_global_load_lds((gptr)(from[j] + slab * (2LL * kSlab)), (lptr)(stage + (wave * kActs + j) * 1024), 16, 0, 0);
+  };
+  WeightSlab<WF> w[U][M][RG];
+  auto request = [&](int u, int slab) {
+#pragma unroll
+    for (int m = 0; m < M; ++m)
+#pragma unroll
+      for (int g = 0; g < RG; ++g) w[u][m][g].load(base, scales, rows, row[m][g], ld, slab, K);
+  };
+  for (int s = 0; s < kDenseStages - 1 && s < slabs; ++s) fetch(s);
+  asm volatile("" ::: "memory");
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (u < slabs) request(u, u);
+  for (int s0 = 0; s0 < slabs; s0 += U) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int s = s0 + u;
+      if (s >= slabs) break;
+      // Requests are awaited in the order of their issue.  Behind this slab's
+      // activations those of two more and weights of at least U slabs have been
+      // requested; near the end, where they have not (or the last, shorter slab of
+      // weights takes fewer instructions), everything is awaited.
+      asm volatile("" ::: "memory");
+      if (s + kDenseStages - 1 < slabs) wait_loads<2 * kActs + U * kWeights>();
+      else wait_loads<0>();
+      wait_lds();
+      meet();
+      if (s + kDenseStages - 1 < slabs) fetch(s + kDenseStages - 1);  // into the slab before's place
+      asm volatile("" ::: "memory");
+      const uint8_t* stage = lds + s % kDenseStages * kStage;
+#pragma unroll
+      for (int step = 0; step < 4; ++step) {
+        u32x4v x[NB][PLANES];
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int p = 0; p < PLANES; ++p)
+            x[b][p] = *(const u32x4v*)(stage + ((p * NB + b) * 16 + r) * (2 * kSlab) + ((step * 4 + q) ^ r) * 16);
+#pragma unroll
+        for (int m = 0; m < M; ++m)
+#pragma unroll
+          for (int g = 0; g < RG; ++g) {
+            u32x4v f = w[u][m][g].step(step), f2;
+            if constexpr (SPLIT) split_f16(w[u][m][g].step(step), f, f2);
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+#pragma unroll
+              for (int p = 0; p < PLANES; ++p)
+                acc[m][g][b] = WF == CMK_F16 && !SPLIT ? mfma_f16(f, x[b][p], acc[m][g][b]) : mfma_bf16(f, x[b][p], acc[m][g][b]);
+              if constexpr (SPLIT) acc[m][g][b] = mfma_bf16(f2, x[b][0], acc[m][g][b]);
+            }
+          }
+      }
+      asm volatile("" ::: "memory");
+      if (s + U < slabs) request(u, s + U);
+    }
+  }
+  wait_lds();
+  meet();  // the ring is free for the next pass
+}
+
+template <int WF, int PLANES, int RG, int NB, int U>
+__device__ __forceinline__ void moe_gate_up_dense(const MoeArgs& a, int expert, const int* list, int c0, int count, uint8_t* lds) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int i0 = (blockIdx.x * kMoeWaves + wave) * 16 * RG;
+  long long row[2][RG];
+  f32x4 acc[2][RG][NB] = {};
+  moe_gate_up_rows<RG>(a, i0, row);
+  auto source = [&](int c) { return a.xp + (long long)(list[c0 + c] / a.k) * a.Hp; };
+  moe_dense_products<WF, PLANES, 2, RG, NB, U, false>(acc, moe_gate_up_base<WF>(a, expert), moe_gate_up_scales<WF>(a, expert), 2 * a.I, row,
+                                                      a.ld_gate_up, a.H, min(count - c0, NB * 16), source, (long long)a.T * a.Hp, lds);
+  moe_store_inner<WF, RG, NB>(a, acc, list, c0, count, i0);
+}
+
+template <int WF, int RG, int NB, int U>
+__device__ __forceinline__ void moe_down_dense(const MoeArgs& a, int expert, const int* list, int c0, int count, uint8_t* lds) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n0 = (blockIdx.x * kMoeWaves + wave) * 16 * RG;
+  long long row[1][RG];
+  f32x4 acc[1][RG][NB] = {};
+  moe_down_rows<RG>(a, n0, row);
+  auto source = [&](int c) { return a.hp + (long long)list[c0 + c] * a.Ip; };
+  moe_dense_products<WF, 2, 1, RG, NB, U, WF == CMK_F16>(acc, moe_down_base<WF>(a, expert), moe_down_scales<WF>(a, expert), a.H, row,
+                                                         a.ld_down, a.I, min(count - c0, NB * 16), source, (long long)a.T * a.k * a.Ip, lds);
+  moe_store_outer<RG, NB>(a, acc, list, c0, count, n0);
+}
+
+template <int WF, int PLANES, int RG, int U>
+__global__ __launch_bounds__(64 * kMoeWaves) void moe_gate_up_dense_kernel(MoeArgs a) {
+  __shared__ int list[kMoeTokens];
+  __shared__ __attribute__((aligned(16))) uint8_t lds[kDenseStages * kDenseBlocks * 16 * PLANES * 2 * kSlab];
+  int expert;
+  const int count = moe_slots<kMoeWaves>(a, blockIdx.y, list, expert);
+  for (int c0 = 0; c0 < count; c0 += 16 * kDenseBlocks) {
+    if (count - c0 <= 16) moe_gate_up_dense<WF, PLANES, RG, 1, U>(a, expert, list, c0, count, lds);
+    else moe_gate_up_dense<WF, PLANES, RG, 2, U>(a, expert, list, c0, count, lds);
+  }
+}
+
+template <int WF, int RG, int U>
+__global__ __launch_bounds__(64 * kMoeWaves) void moe_down_dense_kernel(MoeArgs a) {
+  __shared__ int list[kMoeTokens];
+  __shared__ __attribute__((aligned(16))) uint8_t lds[kDenseStages * kDenseBlocks * 16 * 2 * 2 * kSlab];
+  int expert;
+  const int count = moe_slots<kMoeWaves>(a, blockIdx.y, list, expert);
+  for (int c0 = 0; c0 < count; c0 += 16 * kDenseBlocks) {
+    if (count - c0 <= 16) moe_down_dense<WF, RG, 1, U>(a, expert, list, c0, count, lds);
+    else moe_down_dense<WF, RG, 2, U>(a, expert, list, c0, count, lds);
   }
 }
 
@@ -880,7 +1057,24 @@ extern "C" int cmk_moe(const void* x, const void* router, const void* gate_up, c
     hipLaunchKernelGGL(kernel, dim3(ceil_div(rows, 16 * rg * kMoeWaves / ks), units), dim3(64 * kMoeWaves), 0, st, a);
   };
   const bool many = units >= 32;
-  if (d->w_dtype == CMK_MX4) {
+  // six tokens an expert and enough rows for every compute unit
+  const bool dense = d->T * d->k >= 6 * d->E && (long long)d->E * std::min(d->H, d->I) >= 64LL * compute_units();
+  auto dense_kernel = [&](auto kernel, int rows, int rg) {
+    hipLaunchKernelGGL(kernel, dim3(ceil_div(rows, 16 * rg * kMoeWaves), units), dim3(64 * kMoeWaves), 0, st, a);
+  };
+  if (dense) {
+    if (d->w_dtype == CMK_MX4) {
+      if (p.x_planes == 1) dense_kernel(moe_gate_up_dense_kernel<CMK_MX4, 1, 1, 3>, p.Ip, 1);
+      else dense_kernel(moe_gate_up_dense_kernel<CMK_MX4, 2, 1, 3>, p.Ip, 1);
+      dense_kernel(moe_down_dense_kernel<CMK_MX4, 2, 3>, d->H, 2);
+    } else if (d->w_dtype == CMK_BF16) {
+      dense_kernel(moe_gate_up_dense_kernel<CMK_BF16, 1, 1, 2>, p.Ip, 1);
+      dense_kernel(moe_down_dense_kernel<CMK_BF16, 1, 3>, d->H, 1);
+    } else {
+      dense_kernel(moe_gate_up_dense_kernel<CMK_F16, 1, 1, 2>, p.Ip, 1);
+      dense_kernel(moe_down_dense_kernel<CMK_F16, 1, 3>, d->H, 1);
+    }
+  } else if (d->w_dtype == CMK_MX4) {
     if (p.x_planes == 1) {
       if (many) experts_kernel(moe_gate_up_kernel<CMK_MX4, 1, 1, 1, 3>, p.Ip, 1, 1);
       else experts_kernel(moe_gate_up_kernel<CMK_MX4, 1, 4, 1, 2>, p.Ip, 1, 4);
@@ -888,20 +1082,16 @@ extern "C" int cmk_moe(const void* x, const void* router, const void* gate_up, c
       if (many) experts_kernel(moe_gate_up_kernel<CMK_MX4, 2, 1, 1, 3>, p.Ip, 1, 1);
       else experts_kernel(moe_gate_up_kernel<CMK_MX4, 2, 4, 1, 2>, p.Ip, 1, 4);
     }
-  } else if (d->w_dtype == CMK_BF16) {
-    if (many) experts_kernel(moe_gate_up_kernel<CMK_BF16, 1, 4, 1, 1>, p.Ip, 1, 4);
-    else experts_kernel(moe_gate_up_kernel<CMK_BF16, 1, 4, 1, 2>, p.Ip, 1, 4);
-  } else {
-    if (many) experts_kernel(moe_gate_up_kernel<CMK_F16, 1, 4, 1, 1>, p.Ip, 1, 4);
-    else experts_kernel(moe_gate_up_kernel<CMK_F16, 1, 4, 1, 2>, p.Ip, 1, 4);
-  }
-  if (d->w_dtype == CMK_MX4) {
     if (many) experts_kernel(moe_down_kernel<CMK_MX4, 2, 4, 2>, d->H, 4, 2);
     else experts_kernel(moe_down_kernel<CMK_MX4, 4, 2, 2>, d->H, 2, 4);
   } else if (d->w_dtype == CMK_BF16) {
+    if (many) experts_kernel(moe_gate_up_kernel<CMK_BF16, 1, 4, 1, 1>, p.Ip, 1, 4);
+    else experts_kernel(moe_gate_up_kernel<CMK_BF16, 1, 4, 1, 2>, p.Ip, 1, 4);
     if (many) experts_kernel(moe_down_kernel<CMK_BF16, 1, 1, 4>, d->H, 1, 1);
     else experts_kernel(moe_down_kernel<CMK_BF16, 4, 1, 2>, d->H, 1, 4);
   } else {
+    if (many) experts_kernel(moe_gate_up_kernel<CMK_F16, 1, 4, 1, 1>, p.Ip, 1, 4);
+    else experts_kernel(moe_gate_up_kernel<CMK_F16, 1, 4, 1, 2>, p.Ip, 1, 4);
     if (many) experts_kernel(moe_down_kernel<CMK_F16, 1, 1, 4>, d->H, 1, 1);
     else experts_kernel(moe_down_kernel<CMK_F16, 4, 1, 2>, d->H, 1, 4);
   }

@@ -284,28 +284,6 @@ struct Mx4Tile {
   static constexpr int kBases = (S + kReach - 1) / kReach;
 };
 
-typedef const __attribute__((address_space(1))) void* gptr;
-typedef __attribute__((address_space(3))) void* lptr;
-
-// Waits until at most `left` of the wave's vector-memory instructions are under way.
-template <int left>
-__device__ __forceinline__ void wait_loads() {
-  static_assert(left < 64, "the counter has six bits");
-  __builtin_amdgcn_s_waitcnt(0x0f70 | (left & 15) | (left >> 4 << 14));
-}
-
-template <int v>
-struct Int {
-  static constexpr int value = v;
-};
-
-// The barrier of the work-group's waves; memory operations stay on their side of it.
-__device__ __forceinline__ void meet() {
-  asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
-}
-
 // Work-groups go round the eight XCDs in turn, each with an L2 of its own: an XCD
 // gets a contiguous run of the tiles of all batches, in strips of eight tile rows,
 // so that what runs on it at a time shares few panels of both operands.

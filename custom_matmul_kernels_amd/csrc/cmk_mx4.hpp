@@ -150,4 +150,29 @@ __device__ __forceinline__ float scale_float(unsigned s) { return __uint_as_floa
 template <class T>
 __device__ __forceinline__ T from_f32(float x) { return (T)x; }
 
+typedef const __attribute__((address_space(1))) void* gptr;
+typedef __attribute__((address_space(3))) void* lptr;
+
+// Waits until at most `left` of the wave's vector-memory instructions are under way.
+template <int left>
+__device__ __forceinline__ void wait_loads() {
+  static_assert(left < 64, "the counter has six bits");
+  __builtin_amdgcn_s_waitcnt(0x0f70 | (left & 15) | (left >> 4 << 14));
+}
+
+// Waits until the wave's LDS reads have returned.
+__device__ __forceinline__ void wait_lds() { __builtin_amdgcn_s_waitcnt(0xc07f); }
+
+template <int v>
+struct Int {
+  static constexpr int value = v;
+};
+
+// The barrier of the work-group's waves; memory operations stay on their side of it.
+__device__ __forceinline__ void meet() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
 }  // namespace cmk

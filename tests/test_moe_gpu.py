@@ -85,7 +85,9 @@ def check(layer, x, router, gate_up, down, device, four_bit):
 
 SHAPES = [(1, 64, 32, 4, 2), (1, 1, 1, 1, 1), (1, 100, 33, 10, 3), (2, 256, 130, 6, 6), (7, 1000, 333, 10, 3),
           (16, 256, 128, 8, 2), (17, 130, 257, 70, 5), (70, 96, 48, 3, 3), (200, 72, 40, 2, 1), (40, 64, 64, 130, 8),
-          (5, 2048, 64, 33, 32), (3, 40, 1030, 9, 4)]
+          (5, 2048, 64, 33, 32), (3, 40, 1030, 9, 4), (33, 128, 300, 300, 3),
+          # many tokens an expert: up to 16, up to 32, more
+          (100, 512, 512, 32, 2), (130, 700, 530, 32, 2), (200, 640, 520, 32, 8), (100, 1300, 513, 32, 2)]
 
 
 @pytest.mark.parametrize("t,h,i,e,k", SHAPES)
