@@ -253,9 +253,10 @@ __global__ __launch_bounds__(256) void moe_select_kernel(MoeArgs a) {
 }
 
 // Router and choice in one launch, for a router of few tiles: a work-group takes 16
-// tokens, a wave one (two) of the units of 16 experts x one slab, then a token.  (7
-// tokens, 10 experts, H = 1000: 4.2 + 3.6 us as two launches.)
-constexpr int kSmallUnits = 32, kSmallExperts = 128;
+// tokens, a wave one of the units of 16 experts x one slab, then a token.  (7 tokens,
+// 10 experts, H = 1000, 8 units: 6.4 us, as two launches 4.2 + 3.6 and one more call on
+// the host; 32 units: 19 us, 5 + 4 apart.)
+constexpr int kSmallUnits = 8, kSmallExperts = 128;
 
 static bool small_router(int E, int Hp) { return E <= kSmallExperts && (E + 15) / 16 * (Hp / kSlab) <= kSmallUnits; }
 
@@ -1077,23 +1078,23 @@ extern "C" int cmk_moe(const void* x, const void* router, const void* gate_up, c
   } else if (d->w_dtype == CMK_MX4) {
     if (p.x_planes == 1) {
       if (many) experts_kernel(moe_gate_up_kernel<CMK_MX4, 1, 1, 1, 3>, p.Ip, 1, 1);
-      else experts_kernel(moe_gate_up_kernel<CMK_MX4, 1, 4, 1, 2>, p.Ip, 1, 4);
+      else experts_kernel(moe_gate_up_kernel<CMK_MX4, 1, 2, 1, 3>, p.Ip, 1, 2);
     } else {
       if (many) experts_kernel(moe_gate_up_kernel<CMK_MX4, 2, 1, 1, 3>, p.Ip, 1, 1);
-      else experts_kernel(moe_gate_up_kernel<CMK_MX4, 2, 4, 1, 2>, p.Ip, 1, 4);
+      else experts_kernel(moe_gate_up_kernel<CMK_MX4, 2, 2, 1, 3>, p.Ip, 1, 2);
     }
     if (many) experts_kernel(moe_down_kernel<CMK_MX4, 2, 4, 2>, d->H, 4, 2);
-    else experts_kernel(moe_down_kernel<CMK_MX4, 4, 2, 2>, d->H, 2, 4);
+    else experts_kernel(moe_down_kernel<CMK_MX4, 2, 2, 2>, d->H, 2, 2);
   } else if (d->w_dtype == CMK_BF16) {
     if (many) experts_kernel(moe_gate_up_kernel<CMK_BF16, 1, 4, 1, 1>, p.Ip, 1, 4);
     else experts_kernel(moe_gate_up_kernel<CMK_BF16, 1, 4, 1, 2>, p.Ip, 1, 4);
     if (many) experts_kernel(moe_down_kernel<CMK_BF16, 1, 1, 4>, d->H, 1, 1);
-    else experts_kernel(moe_down_kernel<CMK_BF16, 4, 1, 2>, d->H, 1, 4);
+    else experts_kernel(moe_down_kernel<CMK_BF16, 2, 1, 3>, d->H, 1, 2);
   } else {
     if (many) experts_kernel(moe_gate_up_kernel<CMK_F16, 1, 4, 1, 1>, p.Ip, 1, 4);
     else experts_kernel(moe_gate_up_kernel<CMK_F16, 1, 4, 1, 2>, p.Ip, 1, 4);
     if (many) experts_kernel(moe_down_kernel<CMK_F16, 1, 1, 4>, d->H, 1, 1);
-    else experts_kernel(moe_down_kernel<CMK_F16, 4, 1, 2>, d->H, 1, 4);
+    else experts_kernel(moe_down_kernel<CMK_F16, 2, 1, 3>, d->H, 1, 2);
   }
   const dim3 out_grid(ceil_div(d->H, 1024), d->T);
   if (d->x_dtype == CMK_BF16) hipLaunchKernelGGL(moe_combine_kernel<__bf16>, out_grid, dim3(256), 0, st, a);
