@@ -695,8 +695,10 @@ __device__ __forceinline__ void moe_down_tokens(const MoeArgs& a, int expert, co
   if (share == 0) moe_store_outer<RG, NB>(a, acc, list, c0, count, n0);
 }
 
+// (Three work-groups a compute unit: left alone, the 4-bit form takes 216 registers and
+// 33 instead of 28 us at 16 tokens x 4096 x 1280 x 64 experts.)
 template <int WF, int KS, int RG, int U>
-__global__ __launch_bounds__(64 * kMoeWaves) void moe_down_kernel(MoeArgs a) {
+__global__ __launch_bounds__(64 * kMoeWaves, 3) void moe_down_kernel(MoeArgs a) {
   __shared__ int list[kMoeTokens];
   __shared__ __attribute__((aligned(16))) char lds[kActBytes];
   int expert;
