@@ -247,3 +247,44 @@ def test_a_run_of_the_operators_together(device):
     out = MX4BMMCUDA()(y, quantize_mx4(w_out.to(device), dim=-2))
     a, b = _mx4.rounded(y), _mx4.rounded(w_out.t()).t()
     assert ((out.cpu().double() - a @ b).abs() <= 160 * U * (a.abs() @ b.abs())).all()
+
+
+def test_offsets_beyond_32_bits(device):
+    """4.7 GB and 2.3 GB of weights; the choice falls on the last experts."""
+    e, h, i = 70, 4096, 4096
+    gen = torch.Generator(device=device).manual_seed(2)
+    gate_up = torch.empty(e, 2 * i, h, dtype=BF16, device=device).normal_(generator=gen).mul_(h ** -0.5)
+    down = torch.empty(e, h, i, dtype=BF16, device=device).normal_(generator=gen).mul_(i ** -0.5)
+    cpu = torch.Generator().manual_seed(3)
+    x = torch.randn(2, h, generator=cpu).to(BF16)
+    router = torch.randn(e, h, generator=cpu) * 1e-3
+    router[e - 1] = x[0].float()
+    router[e - 2] = x[1].float()
+    layer = MoECUDA(k=1)
+    for t in (1, 2):
+        y, weights, experts = layer(x[:t].to(device), router.to(device), gate_up, down)
+        assert experts.flatten().tolist() == [e - 1, e - 2][:t]
+        keep = [e - 1, e - 2]
+        want, dy, _, _, _ = reference(x[:t], router[keep], gate_up[keep].cpu(), down[keep].cpu(), 1, "silu", True)
+        assert ((y.cpu().double() - want).abs() <= dy + (want.abs() + dy) * 2.0 ** -8).all()
+
+
+def test_results_do_not_change_from_run_to_run(device):
+    args = [v.to(device) for v in make(64, 512, 256, 16, BF16, 13)]
+    layer = MoECUDA(k=8)
+    want = layer(*args)
+    for _ in range(5):
+        assert all(torch.equal(a, b) for a, b in zip(layer(*args), want))
+
+
+def test_more_experts_than_are_ranked(device):
+    """Beyond 256 experts the choice is made in rounds."""
+    check(MoECUDA(k=9), *make(5, 130, 40, 300, BF16, 14), device, False)
+    check(MoECUDA(k=32, renormalize=False), *make(1, 64, 32, 1024, F16, 15), device, True)
+    x, router, gate_up, down = make(3, 64, 32, 700, BF16, 16)
+    router[650] = router[3]
+    router[20] = router[3]
+    x[1, 5] = float("nan")
+    y, w, e = MoECUDA(k=6)(*(v.to(device) for v in (x, router, gate_up, down)))
+    assert e[1].tolist() == [0, 1, 2, 3, 4, 5] and torch.isnan(y[1]).all()
+    check(MoECUDA(k=6), x[::2], router, gate_up, down, device, False)

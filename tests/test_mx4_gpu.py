@@ -231,3 +231,60 @@ def test_replays_in_a_graph(device, m):
         torch.cuda.synchronize()
         got = out.clone()
         assert torch.equal(got, product(x, B)), "replay %d differs" % step
+
+
+def test_offsets_beyond_32_bits(device):
+    """18 GB of elements, 4.8 GB of codes: rows far apart against the definition."""
+    rows, k = 140000, 65536
+    gen = torch.Generator(device=device).manual_seed(1)
+    x = torch.empty(rows, k, dtype=torch.bfloat16, device=device).normal_(generator=gen)
+    q = quantize_mx4(x)
+    for r in (0, 70001, rows - 1):
+        codes, scales = _mx4.encode(x[r].cpu().double().numpy())
+        got = torch.stack((q.codes[0, :, r] & 15, q.codes[0, :, r] >> 4), -1).flatten().cpu().numpy()
+        assert np.array_equal(got, codes)
+        assert np.array_equal(q.scales[0, :, r].flatten().cpu().numpy(), scales)
+    some = torch.tensor([0, 1, 32767, 32768, 70001, 139998, rows - 1])
+    b = _mx4.rounded(x[some.to(device)])
+    for m in (3, 40):                                    # by rows and by tiles
+        a = normal((m, k), m)
+        got = MX4BMMCUDA()(a.to(device), q.transpose())[:, some.to(device)]
+        check_product(got[None], _mx4.rounded(a)[None], b.t()[None], torch.float32)
+    del q
+    back = quantize_mx4(x.t(), dim=0).dequantize(torch.bfloat16)      # [k, rows], blocks down the columns
+    assert torch.equal(back[:, some.to(device)].cpu().double(), b.t())
+
+
+def test_small_results_keep_their_values(device):
+    """Products around and below the smallest normal fp32 number."""
+    x, w = normal((1, 20, 256), 1) * 2.0 ** -60, normal((1, 256, 40), 2) * 2.0 ** -64
+    a, b = _mx4.rounded(x), _mx4.rounded(w.transpose(1, 2)).transpose(1, 2)
+    for m in (20, 3):
+        check_product(MX4BMMCUDA()(x[:, :m].to(device), w.to(device)), a[:, :m], b, torch.float32)
+    x = x * 2.0 ** -6                                    # results of 2^-130 to 2^-126
+    got = MX4BMMCUDA()(x.to(device), w.to(device)).cpu().double()
+    want = _mx4.rounded(x) @ b
+    assert ((got - want).abs() <= torch.finfo(torch.float32).smallest_normal).all()      # flushed or not
+
+
+def test_the_same_tensor_on_both_sides(device):
+    x = normal((2, 150, 300), 4).to(device)
+    a = _mx4.rounded(x)
+    check_product(MX4BMMCUDA()(x, x.transpose(1, 2)), a, a.transpose(1, 2), torch.float32)
+    q = quantize_mx4(x)
+    assert torch.equal(MX4BMMCUDA()(q, q.transpose()), MX4BMMCUDA()(x, x.transpose(1, 2)))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_results_past_the_caches(device, dtype):
+    """Results of 32 MB and more, and just less, take different stores."""
+    for l, m, n in ((1, 4096, 4096), (3, 1000, 4224), (1, 4096, 4095)):
+        x, w = normal((l, m, 130), 1, dtype).to(device), normal((l, 130, n), 2, dtype).to(device)
+        got = MX4BMMCUDA(out_dtype=dtype)(x, w)
+        rows = torch.tensor([0, 1, m // 2, m - 1], device=device)
+        check_product(got[:, rows], _mx4.rounded(x[:, rows]), _mx4.rounded(w.transpose(1, 2)).transpose(1, 2), dtype)
+    for dim in (-1, -2):
+        x = normal((2, 2049, 4160), 3, dtype)
+        got = quantize_mx4(x.to(device), dim=dim).dequantize(dtype).cpu()
+        want = _mx4.rounded(x if dim == -1 else x.transpose(1, 2))
+        assert torch.equal(got, (want if dim == -1 else want.transpose(1, 2)).to(dtype))
