@@ -753,7 +753,7 @@ static void launch_rows(const Mx4RowsArgs& a, int L, hipStream_t st) {
 }
 
 static bool use_rows(int L, int M, int N, int K) {
-  if (M > kMx4Rows || L > 65535) return false;
+  if (M > kMx4Rows || L > 65535 || N >= 1 << 29) return false;  // (what one launch holds)
   // From 17 rows on the tiles win where there are enough of them (32 rows against
   // 16384 x 8192: 24 us by rows, 14 by tiles; 4096 x 4096: 5.4 and 7.6) or k is long
   // enough to be cut (1024 x 16384: 16 and 8).
@@ -808,6 +808,15 @@ static int check_dtype(const char* who, int dtype) {
   return CMK_OK;
 }
 
+// A launch holds less than 2^32 threads; more of them wrap round without an error.
+constexpr int kThreads = 256;
+
+static int check_launch(const char* who, long long groups) {
+  if (groups > 0xffffffffLL / kThreads)
+    return fail(CMK_ERR_UNSUPPORTED, "%s: needs %lld work-groups, more than a launch holds", who, groups);
+  return CMK_OK;
+}
+
 // Calls f with a value of the element type.
 template <class F>
 static void by_dtype(int dtype, F f) {
@@ -830,7 +839,7 @@ static QuantArgs quant_args(const void* x, uint8_t* codes, uint8_t* scales, int 
 static int launch_quantize(int dtype, const QuantArgs& a, const QuantArgs* b, hipStream_t st) {
   const long long grid = (a.groups + (b ? b->groups : 0) + 3) / 4;
   if (grid == 0) return CMK_OK;
-  if (int e = check_grid(grid)) return e;
+  if (int e = check_launch("quantisation", grid)) return e;
   by_dtype(dtype, [&](auto t) {
     using T = decltype(t);
     if (along_k(a.K, a.sk)) {
@@ -874,7 +883,7 @@ extern "C" int cmk_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, v
   a.row_groups = rows_innermost ? ((long long)R + 64 * v - 1) / (64 * v) : ((long long)R + 15) / 16;
   a.groups = a.row_groups * a.slabs * L;
   const long long grid = (a.groups + 3) / 4;
-  if (int e = check_grid(grid)) return e;
+  if (int e = check_launch("cmk_mx4_dequantize", grid)) return e;
   hipStream_t st = (hipStream_t)stream;
   by_dtype(dtype, [&](auto t) {
     using T = decltype(t);
@@ -949,6 +958,10 @@ extern "C" int cmk_mx4_bmm(const cmk_mx4_operand* A, const cmk_mx4_operand* B, v
   const Mx4Work w = mx4_work(A->dtype, B->dtype, along_k(K, A->stride_k), L, M, N, K);
   if (w.bytes > 0 && (!workspace || workspace_bytes < w.bytes || (reinterpret_cast<uintptr_t>(workspace) & 255)))
     return fail(CMK_ERR_WORKSPACE, "cmk_mx4_bmm: needs a 256-byte aligned workspace of %zu bytes, got %zu", w.bytes, workspace_bytes);
+  const Mx4Plan p = mx4_plan(L, M, N, K);
+  const long long grid = (long long)L * ceil_div(M, p.tile) * ceil_div(N, p.tile) * p.splits;
+  if (!use_rows(L, M, N, K))
+    if (int e = check_launch("cmk_mx4_bmm", grid)) return e;
   uint8_t* ws = (uint8_t*)workspace;
   hipStream_t st = (hipStream_t)stream;
 
@@ -984,13 +997,10 @@ extern "C" int cmk_mx4_bmm(const cmk_mx4_operand* A, const cmk_mx4_operand* B, v
     }
     return hip_status(hipGetLastError(), "cmk_mx4_bmm launch");
   }
-  const Mx4Plan p = mx4_plan(L, M, N, K);
   Mx4GemmArgs a{codes[0], scales[0], codes[1], scales[1], C, L, M, N, (int)mx4_slabs(K), ceil_div(M, p.tile), ceil_div(N, p.tile), p.splits,
                 p.splits == 1 && streams(C, (long long)L * M, (long long)N * (dtype == CMK_F32 ? 4 : 2)),
                 (N & 7) == 0 && (reinterpret_cast<uintptr_t>(C) & 15) == 0};
-  const long long grid = (long long)L * a.tiles_m * a.tiles_n * a.splits;
-  if (int e = check_grid(grid)) return e;
-  const dim3 g((unsigned)grid), b(256);
+  const dim3 g((unsigned)grid), b(kThreads);
   auto gemm = [&](auto t) {
     using T = decltype(t);
     if (p.tile == 256) hipLaunchKernelGGL((mx4_gemm_kernel<T, 256, 256, 4>), g, b, 0, st, a);

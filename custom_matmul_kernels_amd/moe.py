@@ -26,7 +26,9 @@ class MoECUDA:
     returns y [t, h] in x's type, weights float32 [t, k], experts int64 [t, k]
 
     Made for a few tokens, where reading the chosen experts' weights is all there
-    is; more than 256 run in portions of 256.  There is no backward pass."""
+    is; more than 256 run in portions of 256.  A y_j whose sum an infinite weight of
+    `down` or an infinite inner product enters may be NaN instead of an infinity.
+    There is no backward pass."""
 
     def __init__(self, k=2, activation="silu", renormalize=True):
         if activation not in ACTIVATIONS:

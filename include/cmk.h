@@ -214,7 +214,9 @@ int cmk_topk_1d_f32(const float* arr, long long n,
  *   codes  [L][ceil(K/128)][R][64], two elements a byte, the even one low,
  *   scales [L][ceil(K/128)][R][4],
  * every byte of them: elements beyond K are zero codes.  codes must be 16-byte
- * aligned, scales 4-byte aligned.  No counterpart in the reference.
+ * aligned, scales 4-byte aligned.  Here and below calls of 2^24 work-groups or more
+ * (2^26 matrices of one row; 2^24 products of one tile) are refused.  No counterpart in
+ * the reference.
  */
 int cmk_mx4_quantize(const void* x, int dtype, uint8_t* codes, uint8_t* scales,
                      int L, int R, int K, long long stride_l, long long stride_r,
@@ -287,7 +289,9 @@ typedef struct cmk_moe_desc {
  * scales, that cmk_mx4_quantize writes of matrices of 2I rows x H and H rows x I.
  * y is dense [T][H], weights fp32 and experts int64 are dense [T][k].  Sums are
  * held in fp32; act(..) * (..) is kept as two bf16 (16 bits of mantissa); y is
- * rounded once.  Only the chosen experts' weights are read.
+ * rounded once.  Only the chosen experts' weights are read.  A sum that an infinite
+ * weight of `down` or an infinite act(..) * (..) enters may come out as NaN where the
+ * formula has an infinity.
  *
  * `workspace`: cmk_moe_workspace_bytes(d) bytes, 256-byte aligned, not shared
  * with a call that may run at the same time; 0 is returned for a descriptor that

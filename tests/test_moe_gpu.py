@@ -288,3 +288,20 @@ def test_more_experts_than_are_ranked(device):
     y, w, e = MoECUDA(k=6)(*(v.to(device) for v in (x, router, gate_up, down)))
     assert e[1].tolist() == [0, 1, 2, 3, 4, 5] and torch.isnan(y[1]).all()
     check(MoECUDA(k=6), x[::2], router, gate_up, down, device, False)
+
+
+@pytest.mark.parametrize("t", [1, 20])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_infinite_down_weight_reaches_its_own_feature_only(device, t, dtype):
+    x, router, gate_up, down = make(t, 200, 70, 9, dtype, 7)
+    x, router, gate_up, down = (v.to(device) for v in (x, router, gate_up, down))
+    layer = MoECUDA(k=3)
+    want = layer(x, router, gate_up, down)
+    bad = int(want[2][0, 0])
+    down[bad, 9, 2] = float("inf")
+    y, w, e = layer(x, router, gate_up, down)
+    hit = (want[2] == bad).any(1)
+    assert torch.equal(e, want[2]) and torch.equal(w, want[1])
+    assert not torch.isfinite(y[hit, 9]).any()
+    y[hit, 9] = want[0][hit, 9]
+    assert torch.equal(y, want[0])

@@ -179,3 +179,18 @@ def test_refusals_of_the_c_entry_points():
 def test_operand_layout_matches_header():
     assert ctypes.sizeof(_lib.Mx4Operand) == 48
     assert _lib.Mx4Operand.stride_l.offset == 24
+
+
+def test_more_than_a_launch_holds_is_refused():
+    """2^24 work-groups of 256 threads are 2^32 threads, which wrap round in a launch."""
+    lib = _lib.load()
+    ok = ctypes.c_void_p(0x1000)          # never dereferenced
+    four = _lib.Mx4Operand(ok, ok, _lib.MX4)
+    large = 1 << 26                       # matrices of one row: a wave each
+    assert lib.cmk_mx4_quantize(ok, 0, ok, ok, large, 1, 1, 1, 1, 1, None) == _lib.ERR_UNSUPPORTED
+    assert b"more than a launch holds" in lib.cmk_last_error()
+    assert lib.cmk_mx4_quantize(ok, 0, ok, ok, large, 1, 4, 1, 1, 2, None) == _lib.ERR_UNSUPPORTED
+    for rows_innermost in (0, 1):
+        assert lib.cmk_mx4_dequantize(ok, ok, ok, 0, large, 1, 1, rows_innermost, None) == _lib.ERR_UNSUPPORTED
+    for m, n in [(1, 1), (64, 64)]:       # a work-group each
+        assert lib.cmk_mx4_bmm(four, four, ok, 0, 1 << 24, m, n, 32, None, 0, None) == _lib.ERR_UNSUPPORTED

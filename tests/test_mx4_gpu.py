@@ -288,3 +288,20 @@ def test_results_past_the_caches(device, dtype):
         got = quantize_mx4(x.to(device), dim=dim).dequantize(dtype).cpu()
         want = _mx4.rounded(x if dim == -1 else x.transpose(1, 2))
         assert torch.equal(got, (want if dim == -1 else want.transpose(1, 2)).to(dtype))
+
+
+def test_as_many_matrices_as_a_launch_holds(device):
+    """One row each; a few more would not fit a launch."""
+    l = (1 << 24) - 1
+    x = torch.ones(l, 1, 4, dtype=torch.bfloat16, device=device)
+    x[-1] = 2.0
+    x[l // 2] = 3.0
+    a = quantize_mx4(x)
+    b = quantize_mx4(x.transpose(1, 2), dim=-2)
+    assert torch.equal(a.codes, b.codes) and torch.equal(a.scales, b.scales)
+    c = MX4BMMCUDA(torch.bfloat16)(a, b)
+    want = torch.full((l, 1, 1), 4.0, dtype=torch.bfloat16, device=device)
+    want[-1], want[l // 2] = 16.0, 36.0
+    assert torch.equal(c, want)
+    with pytest.raises(RuntimeError):
+        MX4BMMCUDA(torch.bfloat16)(x[:1].expand(l + 1, 1, 4), x[:1].expand(l + 1, 1, 4).transpose(1, 2))
