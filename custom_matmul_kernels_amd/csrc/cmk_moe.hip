@@ -448,7 +448,10 @@ __device__ __forceinline__ void moe_products(f32x4 (&acc)[M][RG][NB], const void
                                              long long plane, int share, bool idle, char* lds) {
   const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
   const int slabs = (K + kSlab - 1) / kSlab;
-  const int fit = (kActBytes / (PLANES * count) - 16) / (2 * kSlab);  // slabs of all rows that LDS holds
+  static_assert((kActBytes / (PLANES * NB * 16) - 16) / (2 * kSlab) >= KS, "a slab for each wave");
+  // slabs of all rows that LDS holds; a multiple of KS, so that a slab is summed by the
+  // same wave in a pass of any size
+  const int fit = (kActBytes / (PLANES * count) - 16) / (2 * kSlab) / KS * KS;
   const int piece = slabs <= fit ? slabs : fit;
   const int pitch = piece * 2 * kSlab + 16;
   const char* mine[NB];

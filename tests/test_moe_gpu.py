@@ -305,3 +305,16 @@ def test_infinite_down_weight_reaches_its_own_feature_only(device, t, dtype):
     assert not torch.isfinite(y[hit, 9]).any()
     y[hit, 9] = want[0][hit, 9]
     assert torch.equal(y, want[0])
+
+
+@pytest.mark.parametrize("four_bit", [False, True])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_equal_tokens_get_equal_results(device, four_bit, dtype):
+    """237 slots of one expert: the kernels take them in passes of up to 32, in an order
+    that may change from run to run, and the last pass is a smaller one."""
+    x, router, gate_up, down = make(1, 700, 700, 64, dtype, 15)
+    gate_up, down = gate_up.to(device), down.to(device)
+    if four_bit:
+        gate_up, down = quantize_mx4(gate_up), quantize_mx4(down)
+    y, w, e = MoECUDA(k=1)(x.to(device).expand(237, 700), router.to(device), gate_up, down)
+    assert (e == e[0]).all() and torch.equal(y, y[:1].expand_as(y))
