@@ -344,6 +344,7 @@ struct WeightSlab {  // 16-bit weights
     }
   }
   __device__ __forceinline__ u32x4v step(int s) const { return v[s]; }
+  __device__ __forceinline__ unsigned worst(unsigned w) const { return w; }
 };
 
 template <>
@@ -365,14 +366,25 @@ struct WeightSlab<CMK_MX4> {
     o[1] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 1));
     o[2] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 2));
     o[3] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, f, 3));
-    if (__any(scale == 255u)) {  // a block that stands for NaN
-      const unsigned nan = scale == 255u ? 0x7fff7fffu : 0u;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] |= nan;
-    }
     return o;
   }
+  __device__ __forceinline__ unsigned worst(unsigned w) const { return max(w, scale); }
 };
+
+// A block that stands for NaN (scale 255) makes its row's sums NaN whatever it is
+// multiplied by: the largest scale a lane has seen tells it in one instruction a slab,
+// where writing NaN over the elements took more than the conversion itself (68 of 118
+// vector instructions a slab; gate and up of 64 experts x 4096 x 1280, 16 tokens: 51
+// and now 46 us).
+__device__ __forceinline__ void raise_nan(f32x4& acc, unsigned worst) {
+  if (!__any(worst == 255u)) return;
+  const int lane = threadIdx.x & 63;
+  worst = max(worst, (unsigned)__shfl_xor((int)worst, 16));
+  worst = max(worst, (unsigned)__shfl_xor((int)worst, 32));  // of row lane % 16
+#pragma unroll
+  for (int i = 0; i < 4; ++i)  // a lane holds rows 4 (lane / 16) + i
+    if (__shfl((int)worst, (lane >> 4) * 4 + i) == 255) acc[i] = __builtin_nanf("");
+}
 
 __device__ __forceinline__ f32x4 mfma_bf16(u32x4v a, u32x4v b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -442,7 +454,13 @@ constexpr int kActBytes = 36 * 1024;
 // through LDS: vector-memory loads are awaited in the order of their issue, so that
 // activations loaded between the weights would wait for weights of later slabs (and
 // they are read by four waves).
-template <int WF, int PLANES, int M, int RG, int NB, int U, int KS, bool SPLIT, class Source>
+//
+// PACK (for at most eight rows of two planes): the planes are columns of one fragment,
+// plane p of row c at p * count + c, instead of products of their own; the caller adds
+// them (add_planes).  Half the matrix instructions and LDS reads (the down product of 64
+// experts x 4096 x 1280, 16 tokens, in 4 bits: 34 and 30 us).  Whether that is done hangs
+// on the expert's slots alone, not on a pass's, whose members may differ from run to run.
+template <int WF, int PLANES, int M, int RG, int NB, int U, int KS, bool SPLIT, bool PACK, class Source>
 __device__ __forceinline__ void moe_products(f32x4 (&acc)[M][RG][NB], const void* base, const uint8_t* scales, long long rows,
                                              const long long (&row)[M][RG], long long ld, int K, int count, Source source,
                                              long long plane, int share, bool idle, char* lds) {
@@ -454,10 +472,13 @@ __device__ __forceinline__ void moe_products(f32x4 (&acc)[M][RG][NB], const void
   const int fit = (kActBytes / (PLANES * count) - 16) / (2 * kSlab) / KS * KS;
   const int piece = slabs <= fit ? slabs : fit;
   const int pitch = piece * 2 * kSlab + 16;
+  constexpr int kFragments = PACK ? 1 : PLANES;  // of a block of columns
+  const int columns = PACK ? PLANES * count : count;
   const char* mine[NB];
 #pragma unroll
-  for (int b = 0; b < NB; ++b) mine[b] = lds + min(b * 16 + r, count - 1) * pitch + q * 16;
+  for (int b = 0; b < NB; ++b) mine[b] = lds + min(b * 16 + r, columns - 1) * pitch + q * 16;
   const int plane_bytes = count * pitch;
+  unsigned worst[M][RG] = {};
   for (int first = 0; first < slabs; first += piece) {
     const int end = min(slabs, first + piece);
     WeightSlab<WF> w[U][M][RG];
@@ -487,11 +508,11 @@ __device__ __forceinline__ void moe_products(f32x4 (&acc)[M][RG][NB], const void
           if (slab >= end) break;
 #pragma unroll
           for (int s = 0; s < 4; ++s) {
-            u32x4v x[NB][PLANES];
+            u32x4v x[NB][kFragments];
 #pragma unroll
             for (int b = 0; b < NB; ++b)
 #pragma unroll
-              for (int p = 0; p < PLANES; ++p)
+              for (int p = 0; p < kFragments; ++p)
                 x[b][p] = *(const u32x4v*)(mine[b] + p * plane_bytes + (slab - first) * 2 * kSlab + s * 64);
 #pragma unroll
             for (int m = 0; m < M; ++m)
@@ -502,16 +523,37 @@ __device__ __forceinline__ void moe_products(f32x4 (&acc)[M][RG][NB], const void
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
 #pragma unroll
-                  for (int p = 0; p < PLANES; ++p)
+                  for (int p = 0; p < kFragments; ++p)
                     acc[m][g][b] = WF == CMK_F16 && !SPLIT ? mfma_f16(f, x[b][p], acc[m][g][b]) : mfma_bf16(f, x[b][p], acc[m][g][b]);
                   if constexpr (SPLIT) acc[m][g][b] = mfma_bf16(f2, x[b][0], acc[m][g][b]);
                 }
               }
           }
+#pragma unroll
+          for (int m = 0; m < M; ++m)
+#pragma unroll
+            for (int g = 0; g < RG; ++g) worst[m][g] = w[u][m][g].worst(worst[m][g]);
           if (slab + U * KS < end) request(u, slab + U * KS);
         }
       }
   }
+  if constexpr (WF == CMK_MX4)
+#pragma unroll
+    for (int m = 0; m < M; ++m)
+#pragma unroll
+      for (int g = 0; g < RG; ++g)
+#pragma unroll
+        for (int b = 0; b < NB; ++b) raise_nan(acc[m][g][b], worst[m][g]);
+}
+
+// The sum of the planes that PACK left in columns of their own, in the first `count`.
+template <int N>
+__device__ __forceinline__ void add_planes(f32x4 (&acc)[N], int count) {
+  const int from = (threadIdx.x & 63) + count;
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[n][i] += __shfl(acc[n][i], from & 63);
 }
 
 // Stores four values to consecutive addresses, of which `left` exist.
@@ -631,7 +673,7 @@ __device__ __forceinline__ void moe_store_outer(const MoeArgs& a, const f32x4 (&
 // RG * 16 gate rows and the up rows that go with them, against NB * 16 tokens of
 // one expert.  KS waves split H between them; the other waves of the work-group
 // take the next rows.
-template <int WF, int PLANES, int KS, int RG, int NB, int U>
+template <int WF, int PLANES, int KS, int RG, int NB, int U, bool PACK>
 __device__ __forceinline__ void moe_gate_up_tokens(const MoeArgs& a, int expert, const int* list, int c0, int count, char* lds) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int share = wave % KS;
@@ -640,10 +682,13 @@ __device__ __forceinline__ void moe_gate_up_tokens(const MoeArgs& a, int expert,
   moe_gate_up_rows<RG>(a, i0, row);
   f32x4 acc[2][RG][NB] = {};
   auto source = [&](int c) { return a.xp + (long long)(list[c0 + c] / a.k) * a.Hp; };
-  moe_products<WF, PLANES, 2, RG, NB, U, KS, false>(acc, moe_gate_up_base<WF>(a, expert), moe_gate_up_scales<WF>(a, expert), 2 * a.I, row, a.ld_gate_up, a.H, min(count - c0, NB * 16),
+  moe_products<WF, PLANES, 2, RG, NB, U, KS, false, PACK>(acc, moe_gate_up_base<WF>(a, expert), moe_gate_up_scales<WF>(a, expert), 2 * a.I, row, a.ld_gate_up, a.H, min(count - c0, NB * 16),
                                                     source, (long long)a.T * a.Hp, share, i0 >= a.I, lds);
   join_waves<KS, 2 * RG * NB>((f32x4(&)[2 * RG * NB])acc, (f32x4(*)[2 * RG * NB][64])lds, share);
-  if (share == 0) moe_store_inner<WF, RG, NB>(a, acc, list, c0, count, i0);
+  if (share == 0) {
+    if constexpr (PACK) add_planes((f32x4(&)[2 * RG * NB])acc, count - c0);
+    moe_store_inner<WF, RG, NB>(a, acc, list, c0, count, i0);
+  }
 }
 
 template <int WF, int PLANES, int KS, int RG, int U>
@@ -653,8 +698,9 @@ __global__ __launch_bounds__(64 * kMoeWaves) void moe_gate_up_kernel(MoeArgs a) 
   int expert;
   const int count = moe_slots<kMoeWaves>(a, blockIdx.y, list, expert);
   for (int c0 = 0; c0 < count; c0 += 32) {
-    if (count - c0 <= 16) moe_gate_up_tokens<WF, PLANES, KS, RG, 1, U>(a, expert, list, c0, count, lds);
-    else moe_gate_up_tokens<WF, PLANES, KS, RG, 2, U>(a, expert, list, c0, count, lds);
+    if (PLANES == 2 && count <= 8) moe_gate_up_tokens<WF, PLANES, KS, RG, 1, U, PLANES == 2>(a, expert, list, c0, count, lds);
+    else if (count - c0 <= 16) moe_gate_up_tokens<WF, PLANES, KS, RG, 1, U, false>(a, expert, list, c0, count, lds);
+    else moe_gate_up_tokens<WF, PLANES, KS, RG, 2, U, false>(a, expert, list, c0, count, lds);
   }
 }
 
@@ -679,11 +725,11 @@ __global__ __launch_bounds__(64 * kMoeWaves) void moe_gate_up_single_kernel(MoeA
   }
   if (threadIdx.x == 0) list[0] = blockIdx.y;
   __syncthreads();  // list is there and the choice has been read
-  moe_gate_up_tokens<WF, PLANES, KS, RG, 1, U>(a, expert, list, 0, 1, lds);
+  moe_gate_up_tokens<WF, PLANES, KS, RG, 1, U, PLANES == 2>(a, expert, list, 0, 1, lds);
 }
 
 // RG * 16 rows of an expert's down matrix against its slots' activations.
-template <int WF, int KS, int RG, int NB, int U>
+template <int WF, int KS, int RG, int NB, int U, bool PACK>
 __device__ __forceinline__ void moe_down_tokens(const MoeArgs& a, int expert, const int* list, int c0, int count, char* lds) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int share = wave % KS;
@@ -692,14 +738,18 @@ __device__ __forceinline__ void moe_down_tokens(const MoeArgs& a, int expert, co
   moe_down_rows<RG>(a, n0, row);
   f32x4 acc[1][RG][NB] = {};
   auto source = [&](int c) { return a.hp + (long long)list[c0 + c] * a.Ip; };
-  moe_products<WF, 2, 1, RG, NB, U, KS, WF == CMK_F16>(acc, moe_down_base<WF>(a, expert), moe_down_scales<WF>(a, expert), a.H, row, a.ld_down, a.I, min(count - c0, NB * 16), source,
+  moe_products<WF, 2, 1, RG, NB, U, KS, WF == CMK_F16, PACK>(acc, moe_down_base<WF>(a, expert), moe_down_scales<WF>(a, expert), a.H, row, a.ld_down, a.I, min(count - c0, NB * 16), source,
                                                        (long long)a.T * a.k * a.Ip, share, n0 >= a.H, lds);
   join_waves<KS, RG * NB>((f32x4(&)[RG * NB])acc, (f32x4(*)[RG * NB][64])lds, share);
-  if (share == 0) moe_store_outer<RG, NB>(a, acc, list, c0, count, n0);
+  if (share == 0) {
+    if constexpr (PACK) add_planes((f32x4(&)[RG * NB])acc, count - c0);
+    moe_store_outer<RG, NB>(a, acc, list, c0, count, n0);
+  }
 }
 
-// (Three work-groups a compute unit: left alone, the 4-bit form takes 216 registers and
-// 33 instead of 28 us at 16 tokens x 4096 x 1280 x 64 experts.)
+// (Three work-groups a compute unit.  Four groups of rows a wave read 4 KB of codes at a
+// time, with no slab ahead: 24 us at 16 tokens x 4096 x 1280 x 64 experts in 4 bits; a
+// slab ahead takes 29, with fewer rows 26.)
 template <int WF, int KS, int RG, int U>
 __global__ __launch_bounds__(64 * kMoeWaves, 3) void moe_down_kernel(MoeArgs a) {
   __shared__ int list[kMoeTokens];
@@ -707,8 +757,9 @@ __global__ __launch_bounds__(64 * kMoeWaves, 3) void moe_down_kernel(MoeArgs a) 
   int expert;
   const int count = moe_slots<kMoeWaves>(a, blockIdx.y, list, expert);
   for (int c0 = 0; c0 < count; c0 += 32) {
-    if (count - c0 <= 16) moe_down_tokens<WF, KS, RG, 1, U>(a, expert, list, c0, count, lds);
-    else moe_down_tokens<WF, KS, RG, 2, U>(a, expert, list, c0, count, lds);
+    if (count <= 8) moe_down_tokens<WF, KS, RG, 1, U, true>(a, expert, list, c0, count, lds);
+    else if (count - c0 <= 16) moe_down_tokens<WF, KS, RG, 1, U, false>(a, expert, list, c0, count, lds);
+    else moe_down_tokens<WF, KS, RG, 2, U, false>(a, expert, list, c0, count, lds);
   }
 }
 
@@ -753,6 +804,7 @@ __device__ __forceinline__ void moe_dense_products(f32x4 (&acc)[M][RG][NB], cons
 #pragma unroll
       for (int g = 0; g < RG; ++g) w[u][m][g].load(base, scales, rows, row[m][g], ld, slab, K);
   };
+  unsigned worst[M][RG] = {};
   for (int s = 0; s < kDenseStages - 1 && s < slabs; ++s) fetch(s);
   asm volatile("" ::: "memory");
 #pragma unroll
@@ -798,10 +850,21 @@ __device__ __forceinline__ void moe_dense_products(f32x4 (&acc)[M][RG][NB], cons
             }
           }
       }
+#pragma unroll
+      for (int m = 0; m < M; ++m)
+#pragma unroll
+        for (int g = 0; g < RG; ++g) worst[m][g] = w[u][m][g].worst(worst[m][g]);
       asm volatile("" ::: "memory");
       if (s + U < slabs) request(u, s + U);
     }
   }
+  if constexpr (WF == CMK_MX4)
+#pragma unroll
+    for (int m = 0; m < M; ++m)
+#pragma unroll
+      for (int g = 0; g < RG; ++g)
+#pragma unroll
+        for (int b = 0; b < NB; ++b) raise_nan(acc[m][g][b], worst[m][g]);
   wait_lds();
   meet();  // the ring is free for the next pass
 }
@@ -909,6 +972,7 @@ __global__ __launch_bounds__(64 * W) void moe_down_single_kernel(MoeArgs a) {
   const int slabs = a.Ip / kSlab, units = a.k * slabs;
   const long long plane = (long long)a.k * a.Ip;
   f32x4 acc = {};
+  unsigned worst = 0;
   for (int first = 0; first < units; first += kSingleUnits) {
     const int end = min(units, first + kSingleUnits);
     WeightSlab<WF> w[U];
@@ -945,27 +1009,29 @@ __global__ __launch_bounds__(64 * W) void moe_down_single_kernel(MoeArgs a) {
       for (int u = 0; u < U; ++u) {
         const int unit = s0 + u * W;
         if (unit >= end) break;
-        const char* x = lds + (unit - first) * 4 * kSlab + q * 16;
+        const char* x = lds + (unit - first) * 4 * kSlab + (r >> 3) * 2 * kSlab + q * 16;
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
-          const u32x4v hi = *(const u32x4v*)(x + s * 64), lo = *(const u32x4v*)(x + 2 * kSlab + s * 64);
+          const u32x4v h = *(const u32x4v*)(x + s * 64);
           u32x4v f = w[u].step(s), f2;
           if constexpr (WF == CMK_F16) split_f16(w[u].step(s), f, f2);
-          acc = mfma_bf16(f, hi, acc);
-          acc = mfma_bf16(f, lo, acc);
-          if constexpr (WF == CMK_F16) acc = mfma_bf16(f2, hi, acc);
+          acc = mfma_bf16(f, h, acc);
+          if constexpr (WF == CMK_F16) acc = mfma_bf16(f2, h, acc);
         }
+        worst = w[u].worst(worst);
         if (unit + U * W < end) request(u, unit + U * W);
       }
     }
   }
+  if constexpr (WF == CMK_MX4) raise_nan(acc, worst);
   part[wave][lane] = acc;
   __syncthreads();
-  // every column holds the token's sums: row 4 q + i in component i of lane 16 q
+  // the first eight columns hold the sums of the upper plane, the others those of the
+  // lower one: row 4 q + i in component i of lanes 16 q and 16 q + 8
   if (threadIdx.x < 16 && n0 + (int)threadIdx.x < a.H) {
     float sum = 0;
 #pragma unroll
-    for (int v = 0; v < W; ++v) sum += part[v][threadIdx.x >> 2 << 4][threadIdx.x & 3];
+    for (int v = 0; v < W; ++v) sum += part[v][threadIdx.x >> 2 << 4][threadIdx.x & 3] + part[v][(threadIdx.x >> 2 << 4) + 8][threadIdx.x & 3];
     ((T*)a.y)[n0 + threadIdx.x] = from_f32<T>(sum);
   }
 }
@@ -1082,13 +1148,13 @@ extern "C" int cmk_moe(const void* x, const void* router, const void* gate_up, c
     }
   } else if (d->w_dtype == CMK_MX4) {
     if (p.x_planes == 1) {
-      if (many) experts_kernel(moe_gate_up_kernel<CMK_MX4, 1, 1, 1, 3>, p.Ip, 1, 1);
+      if (many) experts_kernel(moe_gate_up_kernel<CMK_MX4, 1, 1, 1, 4>, p.Ip, 1, 1);
       else experts_kernel(moe_gate_up_kernel<CMK_MX4, 1, 2, 1, 3>, p.Ip, 1, 2);
     } else {
       if (many) experts_kernel(moe_gate_up_kernel<CMK_MX4, 2, 1, 1, 3>, p.Ip, 1, 1);
       else experts_kernel(moe_gate_up_kernel<CMK_MX4, 2, 2, 1, 3>, p.Ip, 1, 2);
     }
-    if (many) experts_kernel(moe_down_kernel<CMK_MX4, 2, 4, 2>, d->H, 4, 2);
+    if (many) experts_kernel(moe_down_kernel<CMK_MX4, 1, 4, 1>, d->H, 4, 1);
     else experts_kernel(moe_down_kernel<CMK_MX4, 2, 2, 2>, d->H, 2, 2);
   } else if (d->w_dtype == CMK_BF16) {
     if (many) experts_kernel(moe_gate_up_kernel<CMK_BF16, 1, 4, 1, 1>, p.Ip, 1, 4);
