@@ -1138,7 +1138,13 @@ extern "C" int cmk_moe(const void* x, const void* router, const void* gate_up, c
     if (d->w_dtype == CMK_MX4) {
       if (p.x_planes == 1) dense_kernel(moe_gate_up_dense_kernel<CMK_MX4, 1, 1, 3>, p.Ip, 1);
       else dense_kernel(moe_gate_up_dense_kernel<CMK_MX4, 2, 1, 3>, p.Ip, 1);
-      dense_kernel(moe_down_dense_kernel<CMK_MX4, 2, 3>, d->H, 2);
+      // as many rows a wave as leave two work-groups a compute unit (one, two, four groups
+      // of rows: 8 experts x 4096 x 4096, 64 tokens 80, 84, 110 us; 16 x 6144 x 2048 125,
+      // 118, 117; 64 x 2048 x 1024, 256 tokens 92, 85, 82)
+      auto busy = [&](int rg) { return d->E * ceil_div(d->H, 16 * rg * kMoeWaves) >= 2 * compute_units(); };
+      if (busy(4)) dense_kernel(moe_down_dense_kernel<CMK_MX4, 4, 1>, d->H, 4);
+      else if (busy(2)) dense_kernel(moe_down_dense_kernel<CMK_MX4, 2, 3>, d->H, 2);
+      else dense_kernel(moe_down_dense_kernel<CMK_MX4, 1, 3>, d->H, 1);
     } else if (d->w_dtype == CMK_BF16) {
       dense_kernel(moe_gate_up_dense_kernel<CMK_BF16, 1, 1, 2>, p.Ip, 1);
       dense_kernel(moe_down_dense_kernel<CMK_BF16, 1, 3>, d->H, 1);

@@ -318,3 +318,9 @@ def test_equal_tokens_get_equal_results(device, four_bit, dtype):
         gate_up, down = quantize_mx4(gate_up), quantize_mx4(down)
     y, w, e = MoECUDA(k=1)(x.to(device).expand(237, 700), router.to(device), gate_up, down)
     assert (e == e[0]).all() and torch.equal(y, y[:1].expand_as(y))
+
+
+@pytest.mark.parametrize("t,h,i,e,k,dtype", [(130, 1000, 260, 64, 4, F16), (100, 2040, 300, 64, 4, BF16), (180, 2044, 260, 64, 8, F16)])
+def test_many_tokens_of_many_experts_in_four_bits(device, t, h, i, e, k, dtype):
+    """Two and four groups of rows a wave, with up to 16, up to 32 and more slots."""
+    check(MoECUDA(k=k), *make(t, h, i, e, dtype, t + h + i), device, True)
