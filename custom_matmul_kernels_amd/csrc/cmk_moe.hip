@@ -19,6 +19,12 @@ constexpr int kMoeChoices = 32;
 constexpr int kRouterWaves = 4;
 constexpr int kMoeWaves = 4;  // of the experts' kernels
 
+// act(gate) * up goes to the down product as the sum of three bf16, which holds all 24
+// bits of fp32 and its range.  Of the bf16 results of 64 tokens x 2048 x 1024 x 128
+// experts 0.03 % then differ from the formula's rounded ones; with two (16 bits) it was
+// 0.26 %, and 301 us instead of 307.
+constexpr int kInnerPlanes = 3;
+
 typedef double f64x4 __attribute__((ext_vector_type(4)));
 
 // Pieces of the workspace, each 256-byte aligned.
@@ -42,7 +48,7 @@ static MoePlan moe_plan(int T, int H, int I, int E, int k, int x_dtype, int w_dt
   p.logits = at; at += up((size_t)p.splits * T * E * 8);
   p.chosen = at; at += up((size_t)T * k * 4);
   p.x = at; at += up((size_t)p.x_planes * T * p.Hp * 2);
-  p.h = at; at += up((size_t)2 * T * k * p.Ip * 2);
+  p.h = at; at += up((size_t)kInnerPlanes * T * k * p.Ip * 2);
   p.y = at; at += up((size_t)T * k * H * 4);
   p.bytes = at;
   return p;
@@ -59,7 +65,7 @@ struct MoeArgs {
   int act, renormalize;
   double* logits;
   int* chosen;     // [T*k]
-  u16 *xp, *hp;    // planes [planes][T][Hp], [2][T*k][Ip]
+  u16 *xp, *hp;    // planes [planes][T][Hp], [kInnerPlanes][T*k][Ip]
   float* yp;       // [T*k][H]
 };
 
@@ -393,18 +399,29 @@ __device__ __forceinline__ f32x4 mfma_f16(u32x4v a, u32x4v b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
+// fp32 as the sum of three bf16, exactly.  An infinity or a NaN stays in the first alone.
+__device__ __forceinline__ void split_f32(float v, u16& a, u16& b, u16& c) {
+  const __bf16 hi = (__bf16)v;
+  const float rest = __builtin_isfinite(v) ? v - (float)hi : 0.0f;
+  const __bf16 mid = (__bf16)rest;
+  a = __builtin_bit_cast(u16, hi);
+  b = __builtin_bit_cast(u16, mid);
+  c = __builtin_bit_cast(u16, (__bf16)(rest - (float)mid));
+}
+
 // Eight fp16 as the sum of two times eight bf16, exactly (11 bits = 8 + 3).  The
-// products with activations need it that may not fit fp16.  An infinite weight
-// comes out as NaN.
+// products with activations need it that may not fit fp16.  The second is 2^-9 of the
+// weight at most, and its product with the third plane of an activation (2^-17 of that)
+// below fp32's last bit: it is left out where the planes are products of their own.  An
+// infinite weight comes out as NaN.
 __device__ __forceinline__ void split_f16(u32x4v w, u32x4v& hi, u32x4v& lo) {
   const f16x8 f = __builtin_bit_cast(f16x8, w);
   bf16x8 h, l;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const float v = (float)f[i];
-    const float top = __uint_as_float(__float_as_uint(v) & 0xffff0000u);
-    h[i] = __builtin_bit_cast(__bf16, (u16)(__float_as_uint(v) >> 16));
-    l[i] = __builtin_bit_cast(__bf16, (u16)(__float_as_uint(v - top) >> 16));
+    h[i] = (__bf16)v;
+    l[i] = (__bf16)(v - (float)h[i]);
   }
   hi = __builtin_bit_cast(u32x4v, h);
   lo = __builtin_bit_cast(u32x4v, l);
@@ -444,7 +461,10 @@ __device__ __forceinline__ float activate(float g, int act) {
 // Activations of one pass in LDS: rows of 16-bit elements, plane by plane, a row
 // 16 bytes longer than what it holds so that the 16 rows of a fragment spread over
 // the banks.  Where the rows do not fit whole, the pass goes through k in pieces.
-constexpr int kActBytes = 36 * 1024;
+constexpr int kActBytes = 36 * 1024;       // gate and up
+// Down: four work-groups a compute unit where a wave takes rows of its own, one group of
+// them (64 tokens x 2048 x 1024 x 128 experts: 306 us, 309 with three); three elsewhere.
+constexpr int inner_bytes(int KS, int RG) { return (KS == 1 && RG == 1 ? 36 : 51) * 1024; }
 
 // The products of RG groups of 16 rows of one expert's matrix with the `count`
 // activation rows (at most NB * 16) that `source` gives, over the slabs of one wave
@@ -455,24 +475,24 @@ constexpr int kActBytes = 36 * 1024;
 // activations loaded between the weights would wait for weights of later slabs (and
 // they are read by four waves).
 //
-// PACK (for at most eight rows of two planes): the planes are columns of one fragment,
-// plane p of row c at p * count + c, instead of products of their own; the caller adds
-// them (add_planes).  Half the matrix instructions and LDS reads (the down product of 64
-// experts x 4096 x 1280, 16 tokens, in 4 bits: 34 and 30 us).  Whether that is done hangs
-// on the expert's slots alone, not on a pass's, whose members may differ from run to run.
-template <int WF, int PLANES, int M, int RG, int NB, int U, int KS, bool SPLIT, bool PACK, class Source>
+// PACK (for few rows, PLANES * count <= NB * 16): the planes are columns of the NB
+// fragments, plane p of row c at p * count + c, instead of products of their own; the
+// caller adds them (add_planes).  A third (half) of the matrix instructions and LDS reads.
+// Whether that is done hangs on the expert's slots alone, not on a pass's, whose members
+// may differ from run to run.
+template <int WF, int PLANES, int M, int RG, int NB, int U, int KS, bool SPLIT, bool PACK, int BYTES, class Source>
 __device__ __forceinline__ void moe_products(f32x4 (&acc)[M][RG][NB], const void* base, const uint8_t* scales, long long rows,
                                              const long long (&row)[M][RG], long long ld, int K, int count, Source source,
                                              long long plane, int share, bool idle, char* lds) {
   const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
   const int slabs = (K + kSlab - 1) / kSlab;
-  static_assert((kActBytes / (PLANES * NB * 16) - 16) / (2 * kSlab) >= KS, "a slab for each wave");
+  constexpr int kFragments = PACK ? 1 : PLANES;  // of a block of columns
+  static_assert((BYTES / (kFragments * NB * 16) - 16) / (2 * kSlab) >= KS, "a slab for each wave");
   // slabs of all rows that LDS holds; a multiple of KS, so that a slab is summed by the
   // same wave in a pass of any size
-  const int fit = (kActBytes / (PLANES * count) - 16) / (2 * kSlab) / KS * KS;
+  const int fit = (BYTES / (PLANES * count) - 16) / (2 * kSlab) / KS * KS;
   const int piece = slabs <= fit ? slabs : fit;
   const int pitch = piece * 2 * kSlab + 16;
-  constexpr int kFragments = PACK ? 1 : PLANES;  // of a block of columns
   const int columns = PACK ? PLANES * count : count;
   const char* mine[NB];
 #pragma unroll
@@ -508,6 +528,8 @@ __device__ __forceinline__ void moe_products(f32x4 (&acc)[M][RG][NB], const void
           if (slab >= end) break;
 #pragma unroll
           for (int s = 0; s < 4; ++s) {
+            // reads of four steps at a time would not fit the registers
+            if constexpr (RG * NB * kFragments > 16) __builtin_amdgcn_sched_barrier(0);
             u32x4v x[NB][kFragments];
 #pragma unroll
             for (int b = 0; b < NB; ++b)
@@ -525,7 +547,9 @@ __device__ __forceinline__ void moe_products(f32x4 (&acc)[M][RG][NB], const void
 #pragma unroll
                   for (int p = 0; p < kFragments; ++p)
                     acc[m][g][b] = WF == CMK_F16 && !SPLIT ? mfma_f16(f, x[b][p], acc[m][g][b]) : mfma_bf16(f, x[b][p], acc[m][g][b]);
-                  if constexpr (SPLIT) acc[m][g][b] = mfma_bf16(f2, x[b][0], acc[m][g][b]);
+                  if constexpr (SPLIT)
+#pragma unroll
+                    for (int p = 0; p < std::max(1, kFragments - 1); ++p) acc[m][g][b] = mfma_bf16(f2, x[b][p], acc[m][g][b]);
                 }
               }
           }
@@ -547,13 +571,27 @@ __device__ __forceinline__ void moe_products(f32x4 (&acc)[M][RG][NB], const void
 }
 
 // The sum of the planes that PACK left in columns of their own, in the first `count`.
-template <int N>
-__device__ __forceinline__ void add_planes(f32x4 (&acc)[N], int count) {
-  const int from = (threadIdx.x & 63) + count;
+template <int PLANES, int N, int NB>
+__device__ __forceinline__ void add_planes(f32x4 (&acc)[N][NB], int count) {
+  static_assert(NB <= 2, "columns of one or two fragments");
+  const int lane = threadIdx.x & 63;
 #pragma unroll
   for (int n = 0; n < N; ++n)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) acc[n][i] += __shfl(acc[n][i], from & 63);
+    for (int i = 0; i < 4; ++i) {
+      float lower = 0;
+#pragma unroll
+      for (int p = PLANES - 1; p > 0; --p) {
+        const int column = (lane & 15) + p * count, from = (lane & 48) | (column & 15);
+        float v = __shfl(acc[n][0][i], from);
+        if constexpr (NB == 2) {
+          const float w = __shfl(acc[n][1][i], from);
+          if (column >= 16) v = w;
+        }
+        lower += v;
+      }
+      acc[n][0][i] += lower;
+    }
 }
 
 // Stores four values to consecutive addresses, of which `left` exist.
@@ -571,9 +609,9 @@ __device__ __forceinline__ void store4(T* p, const T (&v)[4], int left, bool ali
 // Sums of the KS waves that share rows, in the order of the waves; the first of
 // them gets the result.  Every wave of the work-group takes part; the LDS is the
 // activations'.
-template <int KS, int N>
+template <int KS, int N, int BYTES>
 __device__ __forceinline__ void join_waves(f32x4 (&acc)[N], f32x4 (*part)[N][64], int share) {
-  static_assert((size_t)kMoeWaves / KS * (KS - 1) * N * 64 * 16 <= kActBytes, "the partial sums fit");
+  static_assert((size_t)kMoeWaves / KS * (KS - 1) * N * 64 * 16 <= BYTES, "the partial sums fit");
   const int lane = threadIdx.x & 63;
   __syncthreads();  // the activations have been read
   if constexpr (KS > 1) {
@@ -636,18 +674,13 @@ __device__ __forceinline__ void moe_store_inner(const MoeArgs& a, const f32x4 (&
     for (int g = 0; g < RG; ++g) {
       const int i1 = i0 + g * 16 + q * 4;  // four consecutive inner features of one token
       if (i1 >= a.Ip) continue;
-      u16 hi[4], lo[4];
+      u16 part[kInnerPlanes][4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float v = i1 + i < a.I ? activate(acc[0][g][b][i], a.act) * acc[1][g][b][i] : 0.0f;
-        // two bf16: 16 bits of mantissa and fp32's range
-        const __bf16 top = (__bf16)v;
-        hi[i] = __builtin_bit_cast(u16, top);
-        lo[i] = __builtin_bit_cast(u16, (__bf16)(__builtin_isfinite(v) ? v - (float)top : 0.0f));
-      }
+      for (int i = 0; i < 4; ++i)
+        split_f32(i1 + i < a.I ? activate(acc[0][g][b][i], a.act) * acc[1][g][b][i] : 0.0f, part[0][i], part[1][i], part[2][i]);
       u16* at = h + plane_position<WF == CMK_MX4>(i1);
-      __builtin_memcpy(at, hi, 8);
-      __builtin_memcpy(at + (long long)a.T * a.k * a.Ip, lo, 8);
+#pragma unroll
+      for (int p = 0; p < kInnerPlanes; ++p) __builtin_memcpy(at + (long long)p * a.T * a.k * a.Ip, part[p], 8);
     }
   }
 }
@@ -682,11 +715,11 @@ __device__ __forceinline__ void moe_gate_up_tokens(const MoeArgs& a, int expert,
   moe_gate_up_rows<RG>(a, i0, row);
   f32x4 acc[2][RG][NB] = {};
   auto source = [&](int c) { return a.xp + (long long)(list[c0 + c] / a.k) * a.Hp; };
-  moe_products<WF, PLANES, 2, RG, NB, U, KS, false, PACK>(acc, moe_gate_up_base<WF>(a, expert), moe_gate_up_scales<WF>(a, expert), 2 * a.I, row, a.ld_gate_up, a.H, min(count - c0, NB * 16),
+  moe_products<WF, PLANES, 2, RG, NB, U, KS, false, PACK, kActBytes>(acc, moe_gate_up_base<WF>(a, expert), moe_gate_up_scales<WF>(a, expert), 2 * a.I, row, a.ld_gate_up, a.H, min(count - c0, NB * 16),
                                                     source, (long long)a.T * a.Hp, share, i0 >= a.I, lds);
-  join_waves<KS, 2 * RG * NB>((f32x4(&)[2 * RG * NB])acc, (f32x4(*)[2 * RG * NB][64])lds, share);
+  join_waves<KS, 2 * RG * NB, kActBytes>((f32x4(&)[2 * RG * NB])acc, (f32x4(*)[2 * RG * NB][64])lds, share);
   if (share == 0) {
-    if constexpr (PACK) add_planes((f32x4(&)[2 * RG * NB])acc, count - c0);
+    if constexpr (PACK) add_planes<PLANES>((f32x4(&)[2 * RG][NB])acc, count - c0);
     moe_store_inner<WF, RG, NB>(a, acc, list, c0, count, i0);
   }
 }
@@ -738,11 +771,11 @@ __device__ __forceinline__ void moe_down_tokens(const MoeArgs& a, int expert, co
   moe_down_rows<RG>(a, n0, row);
   f32x4 acc[1][RG][NB] = {};
   auto source = [&](int c) { return a.hp + (long long)list[c0 + c] * a.Ip; };
-  moe_products<WF, 2, 1, RG, NB, U, KS, WF == CMK_F16, PACK>(acc, moe_down_base<WF>(a, expert), moe_down_scales<WF>(a, expert), a.H, row, a.ld_down, a.I, min(count - c0, NB * 16), source,
+  moe_products<WF, kInnerPlanes, 1, RG, NB, U, KS, WF == CMK_F16, PACK, inner_bytes(KS, RG)>(acc, moe_down_base<WF>(a, expert), moe_down_scales<WF>(a, expert), a.H, row, a.ld_down, a.I, min(count - c0, NB * 16), source,
                                                        (long long)a.T * a.k * a.Ip, share, n0 >= a.H, lds);
-  join_waves<KS, RG * NB>((f32x4(&)[RG * NB])acc, (f32x4(*)[RG * NB][64])lds, share);
+  join_waves<KS, RG * NB, inner_bytes(KS, RG)>((f32x4(&)[RG * NB])acc, (f32x4(*)[RG * NB][64])lds, share);
   if (share == 0) {
-    if constexpr (PACK) add_planes((f32x4(&)[RG * NB])acc, count - c0);
+    if constexpr (PACK) add_planes<kInnerPlanes>((f32x4(&)[RG][NB])acc, count - c0);
     moe_store_outer<RG, NB>(a, acc, list, c0, count, n0);
   }
 }
@@ -753,11 +786,12 @@ __device__ __forceinline__ void moe_down_tokens(const MoeArgs& a, int expert, co
 template <int WF, int KS, int RG, int U>
 __global__ __launch_bounds__(64 * kMoeWaves, 3) void moe_down_kernel(MoeArgs a) {
   __shared__ int list[kMoeTokens];
-  __shared__ __attribute__((aligned(16))) char lds[kActBytes];
+  __shared__ __attribute__((aligned(16))) char lds[inner_bytes(KS, RG)];
   int expert;
   const int count = moe_slots<kMoeWaves>(a, blockIdx.y, list, expert);
   for (int c0 = 0; c0 < count; c0 += 32) {
-    if (count <= 8) moe_down_tokens<WF, KS, RG, 1, U, true>(a, expert, list, c0, count, lds);
+    if (count * kInnerPlanes <= 16) moe_down_tokens<WF, KS, RG, 1, U, true>(a, expert, list, c0, count, lds);
+    else if (count * kInnerPlanes <= 32) moe_down_tokens<WF, KS, RG, 2, U, true>(a, expert, list, c0, count, lds);
     else if (count - c0 <= 16) moe_down_tokens<WF, KS, RG, 1, U, false>(a, expert, list, c0, count, lds);
     else moe_down_tokens<WF, KS, RG, 2, U, false>(a, expert, list, c0, count, lds);
   }
@@ -766,21 +800,21 @@ __global__ __launch_bounds__(64 * kMoeWaves, 3) void moe_down_kernel(MoeArgs a) 
 // Where experts have many tokens each, the activations of a pass do not fit LDS and
 // staging them in pieces leaves the memory idle between them (8 experts of 4096 x
 // 4096, 64 tokens: 255 us in bf16, 151 in 4 bits).  These kernels walk k with a ring
-// of four slabs of activations in LDS, fetched by direct loads, and the weights in the
+// of S slabs of activations in LDS, fetched by direct loads, and the weights in the
 // register ring as before; the four waves take rows of their own.  Within a row the 16
 // blocks of 16 bytes of a slab are stored at position block ^ (row & 15), so that the
 // 16 rows of a fragment spread over the banks.
-constexpr int kDenseStages = 4;
+constexpr int kGateUpStages = 4, kDownStages = 3;
 constexpr int kDenseBlocks = 2;  // blocks of 16 slots of a pass (four would leave a compute unit one work-group)
 
-template <int WF, int PLANES, int M, int RG, int NB, int U, bool SPLIT, class Source>
+template <int WF, int PLANES, int M, int RG, int NB, int U, int S, bool SPLIT, class Source>
 __device__ __forceinline__ void moe_dense_products(f32x4 (&acc)[M][RG][NB], const void* base, const uint8_t* scales, long long rows,
                                                    const long long (&row)[M][RG], long long ld, int K, int count, Source source,
                                                    long long plane, uint8_t* lds) {
   constexpr int kStage = NB * 16 * PLANES * 2 * kSlab;
   constexpr int kActs = NB * PLANES;                               // requests of a wave per slab of activations,
   constexpr int kWeights = M * RG * (WF == CMK_MX4 ? 2 : 4);       // and of weights
-  static_assert(U <= kDenseStages - 1 && 2 * kActs + U * kWeights < 64, "the count of requests under way");
+  static_assert(U <= S - 1 && (S - 2) * kActs + U * kWeights < 64, "the count of requests under way");
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, q = lane >> 4;
   const int slabs = (K + kSlab - 1) / kSlab;
@@ -792,7 +826,7 @@ __device__ __forceinline__ void moe_dense_products(f32x4 (&acc)[M][RG][NB], cons
     from[j] = (const char*)(source(min(in, count - 1)) + p * plane) + ((lane & 15) ^ (in & 15)) * 16;
   }
   auto fetch = [&](int slab) {
-    uint8_t* stage = lds + slab % kDenseStages * kStage;
+    uint8_t* stage = lds + slab % S * kStage;
 #pragma unroll
     for (int j = 0; j < kActs; ++j)
       __builtin_amdgcn_global_load_lds((gptr)(from[j] + slab * (2LL * kSlab)), (lptr)(stage + (wave * kActs + j) * 1024), 16, 0, 0);
@@ -805,7 +839,7 @@ __device__ __forceinline__ void moe_dense_products(f32x4 (&acc)[M][RG][NB], cons
       for (int g = 0; g < RG; ++g) w[u][m][g].load(base, scales, rows, row[m][g], ld, slab, K);
   };
   unsigned worst[M][RG] = {};
-  for (int s = 0; s < kDenseStages - 1 && s < slabs; ++s) fetch(s);
+  for (int s = 0; s < S - 1 && s < slabs; ++s) fetch(s);
   asm volatile("" ::: "memory");
 #pragma unroll
   for (int u = 0; u < U; ++u)
@@ -816,17 +850,17 @@ __device__ __forceinline__ void moe_dense_products(f32x4 (&acc)[M][RG][NB], cons
       const int s = s0 + u;
       if (s >= slabs) break;
       // Requests are awaited in the order of their issue.  Behind this slab's
-      // activations those of two more and weights of at least U slabs have been
+      // activations those of S - 2 more and weights of at least U slabs have been
       // requested; near the end, where they have not (or the last, shorter slab of
       // weights takes fewer instructions), everything is awaited.
       asm volatile("" ::: "memory");
-      if (s + kDenseStages - 1 < slabs) wait_loads<2 * kActs + U * kWeights>();
+      if (s + S - 1 < slabs) wait_loads<(S - 2) * kActs + U * kWeights>();
       else wait_loads<0>();
       wait_lds();
       meet();
-      if (s + kDenseStages - 1 < slabs) fetch(s + kDenseStages - 1);  // into the slab before's place
+      if (s + S - 1 < slabs) fetch(s + S - 1);  // into the slab before's place
       asm volatile("" ::: "memory");
-      const uint8_t* stage = lds + s % kDenseStages * kStage;
+      const uint8_t* stage = lds + s % S * kStage;
 #pragma unroll
       for (int step = 0; step < 4; ++step) {
         u32x4v x[NB][PLANES];
@@ -846,7 +880,9 @@ __device__ __forceinline__ void moe_dense_products(f32x4 (&acc)[M][RG][NB], cons
 #pragma unroll
               for (int p = 0; p < PLANES; ++p)
                 acc[m][g][b] = WF == CMK_F16 && !SPLIT ? mfma_f16(f, x[b][p], acc[m][g][b]) : mfma_bf16(f, x[b][p], acc[m][g][b]);
-              if constexpr (SPLIT) acc[m][g][b] = mfma_bf16(f2, x[b][0], acc[m][g][b]);
+              if constexpr (SPLIT)
+#pragma unroll
+                for (int p = 0; p < PLANES - 1; ++p) acc[m][g][b] = mfma_bf16(f2, x[b][p], acc[m][g][b]);
             }
           }
       }
@@ -877,7 +913,7 @@ __device__ __forceinline__ void moe_gate_up_dense(const MoeArgs& a, int expert, 
   f32x4 acc[2][RG][NB] = {};
   moe_gate_up_rows<RG>(a, i0, row);
   auto source = [&](int c) { return a.xp + (long long)(list[c0 + c] / a.k) * a.Hp; };
-  moe_dense_products<WF, PLANES, 2, RG, NB, U, false>(acc, moe_gate_up_base<WF>(a, expert), moe_gate_up_scales<WF>(a, expert), 2 * a.I, row,
+  moe_dense_products<WF, PLANES, 2, RG, NB, U, kGateUpStages, false>(acc, moe_gate_up_base<WF>(a, expert), moe_gate_up_scales<WF>(a, expert), 2 * a.I, row,
                                                       a.ld_gate_up, a.H, min(count - c0, NB * 16), source, (long long)a.T * a.Hp, lds);
   moe_store_inner<WF, RG, NB>(a, acc, list, c0, count, i0);
 }
@@ -890,7 +926,7 @@ __device__ __forceinline__ void moe_down_dense(const MoeArgs& a, int expert, con
   f32x4 acc[1][RG][NB] = {};
   moe_down_rows<RG>(a, n0, row);
   auto source = [&](int c) { return a.hp + (long long)list[c0 + c] * a.Ip; };
-  moe_dense_products<WF, 2, 1, RG, NB, U, WF == CMK_F16>(acc, moe_down_base<WF>(a, expert), moe_down_scales<WF>(a, expert), a.H, row,
+  moe_dense_products<WF, kInnerPlanes, 1, RG, NB, U, kDownStages, WF == CMK_F16>(acc, moe_down_base<WF>(a, expert), moe_down_scales<WF>(a, expert), a.H, row,
                                                          a.ld_down, a.I, min(count - c0, NB * 16), source, (long long)a.T * a.k * a.Ip, lds);
   moe_store_outer<RG, NB>(a, acc, list, c0, count, n0);
 }
@@ -898,7 +934,7 @@ __device__ __forceinline__ void moe_down_dense(const MoeArgs& a, int expert, con
 template <int WF, int PLANES, int RG, int U>
 __global__ __launch_bounds__(64 * kMoeWaves) void moe_gate_up_dense_kernel(MoeArgs a) {
   __shared__ int list[kMoeTokens];
-  __shared__ __attribute__((aligned(16))) uint8_t lds[kDenseStages * kDenseBlocks * 16 * PLANES * 2 * kSlab];
+  __shared__ __attribute__((aligned(16))) uint8_t lds[kGateUpStages * kDenseBlocks * 16 * PLANES * 2 * kSlab];
   int expert;
   const int count = moe_slots<kMoeWaves>(a, blockIdx.y, list, expert);
   for (int c0 = 0; c0 < count; c0 += 16 * kDenseBlocks) {
@@ -910,7 +946,7 @@ __global__ __launch_bounds__(64 * kMoeWaves) void moe_gate_up_dense_kernel(MoeAr
 template <int WF, int RG, int U>
 __global__ __launch_bounds__(64 * kMoeWaves) void moe_down_dense_kernel(MoeArgs a) {
   __shared__ int list[kMoeTokens];
-  __shared__ __attribute__((aligned(16))) uint8_t lds[kDenseStages * kDenseBlocks * 16 * 2 * 2 * kSlab];
+  __shared__ __attribute__((aligned(16))) uint8_t lds[kDownStages * kDenseBlocks * 16 * kInnerPlanes * 2 * kSlab];
   int expert;
   const int count = moe_slots<kMoeWaves>(a, blockIdx.y, list, expert);
   for (int c0 = 0; c0 < count; c0 += 16 * kDenseBlocks) {
@@ -958,12 +994,13 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(MoeArgs a) {
 // rows and all the chosen experts.  A unit is one slab of one of them; the W waves
 // take units in turn, a ring of U under way each, and their sums meet in LDS in the
 // order of the waves.  The activations are multiplied by the weights as they are
-// staged and split into two bf16 again.
-constexpr int kSingleUnits = 96;  // staged at a time
+// staged and split again.
+constexpr int kSingleUnits = 80;  // staged at a time: two work-groups a compute unit
 
 template <int WF, class T, int W, int U>
 __global__ __launch_bounds__(64 * W) void moe_down_single_kernel(MoeArgs a) {
-  __shared__ __attribute__((aligned(16))) char lds[kSingleUnits * 4 * kSlab];
+  constexpr int kUnit = kInnerPlanes * 2 * kSlab;
+  __shared__ __attribute__((aligned(16))) char lds[kSingleUnits * kUnit];
   __shared__ f32x4 part[W][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, q = lane >> 4;
@@ -990,18 +1027,18 @@ __global__ __launch_bounds__(64 * W) void moe_down_single_kernel(MoeArgs a) {
       const int unit = v / (kSlab / 8), at = v % (kSlab / 8) * 8;
       const long long from = (long long)(first + unit) * kSlab + at;  // units are consecutive in memory
       const float weight = a.weights[(first + unit) / slabs];
-      u16 hi[8], lo[8];
-      __builtin_memcpy(hi, a.hp + from, 16);
-      __builtin_memcpy(lo, a.hp + plane + from, 16);
+      u16 part[kInnerPlanes][8];
+#pragma unroll
+      for (int p = 0; p < kInnerPlanes; ++p) __builtin_memcpy(part[p], a.hp + p * plane + from, 16);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float f = weight * (__uint_as_float((unsigned)hi[i] << 16) + __uint_as_float((unsigned)lo[i] << 16));
-        const __bf16 top = (__bf16)f;
-        hi[i] = __builtin_bit_cast(u16, top);
-        lo[i] = __builtin_bit_cast(u16, (__bf16)(__builtin_isfinite(f) ? f - (float)top : 0.0f));
+        float f = 0;
+#pragma unroll
+        for (int p = 0; p < kInnerPlanes; ++p) f += __uint_as_float((unsigned)part[p][i] << 16);
+        split_f32(weight * f, part[0][i], part[1][i], part[2][i]);
       }
-      __builtin_memcpy(lds + unit * 4 * kSlab + at * 2, hi, 16);
-      __builtin_memcpy(lds + unit * 4 * kSlab + 2 * kSlab + at * 2, lo, 16);
+#pragma unroll
+      for (int p = 0; p < kInnerPlanes; ++p) __builtin_memcpy(lds + unit * kUnit + p * 2 * kSlab + at * 2, part[p], 16);
     }
     __syncthreads();
     for (int s0 = first + wave; s0 < end; s0 += W * U) {
@@ -1009,7 +1046,7 @@ __global__ __launch_bounds__(64 * W) void moe_down_single_kernel(MoeArgs a) {
       for (int u = 0; u < U; ++u) {
         const int unit = s0 + u * W;
         if (unit >= end) break;
-        const char* x = lds + (unit - first) * 4 * kSlab + (r >> 3) * 2 * kSlab + q * 16;
+        const char* x = lds + (unit - first) * kUnit + min(r >> 2, kInnerPlanes - 1) * 2 * kSlab + q * 16;
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
           const u32x4v h = *(const u32x4v*)(x + s * 64);
@@ -1026,12 +1063,17 @@ __global__ __launch_bounds__(64 * W) void moe_down_single_kernel(MoeArgs a) {
   if constexpr (WF == CMK_MX4) raise_nan(acc, worst);
   part[wave][lane] = acc;
   __syncthreads();
-  // the first eight columns hold the sums of the upper plane, the others those of the
-  // lower one: row 4 q + i in component i of lanes 16 q and 16 q + 8
+  // four columns each hold the sums of a plane, the last four repeat one: row 4 q + i of
+  // plane p in component i of lane 16 q + 4 p
   if (threadIdx.x < 16 && n0 + (int)threadIdx.x < a.H) {
     float sum = 0;
 #pragma unroll
-    for (int v = 0; v < W; ++v) sum += part[v][threadIdx.x >> 2 << 4][threadIdx.x & 3] + part[v][(threadIdx.x >> 2 << 4) + 8][threadIdx.x & 3];
+    for (int v = 0; v < W; ++v) {
+      float one = 0;
+#pragma unroll
+      for (int p = kInnerPlanes - 1; p >= 0; --p) one += part[v][(threadIdx.x >> 2 << 4) + 4 * p][threadIdx.x & 3];
+      sum += one;
+    }
     ((T*)a.y)[n0 + threadIdx.x] = from_f32<T>(sum);
   }
 }
@@ -1134,23 +1176,27 @@ extern "C" int cmk_moe(const void* x, const void* router, const void* gate_up, c
   auto dense_kernel = [&](auto kernel, int rows, int rg) {
     hipLaunchKernelGGL(kernel, dim3(ceil_div(rows, 16 * rg * kMoeWaves), units), dim3(64 * kMoeWaves), 0, st, a);
   };
+  // The down products take as few groups of 16 rows a wave as let all work-groups run at
+  // once, two a compute unit.  One, two and four groups: 4 bits, 8 experts x 4096 x 4096,
+  // 64 tokens 91, 95, 126 us; 8 x 5000 x 5000, 48 tokens 149, 125, 152; 16 x 6144 x 2048,
+  // 128 tokens 130, 120, 116; 64 x 2048 x 1024, 256 tokens 158, 142, 139.  One and two,
+  // 16 bits: 8 x 4096 x 4096, 64 tokens 197 and 199; 64 x 2048 x 1024, 256 tokens 306 and 296.
+  auto all_at_once = [&](int rg) { return d->E * ceil_div(d->H, 16 * rg * kMoeWaves) <= 2 * compute_units(); };
   if (dense) {
     if (d->w_dtype == CMK_MX4) {
       if (p.x_planes == 1) dense_kernel(moe_gate_up_dense_kernel<CMK_MX4, 1, 1, 3>, p.Ip, 1);
       else dense_kernel(moe_gate_up_dense_kernel<CMK_MX4, 2, 1, 3>, p.Ip, 1);
-      // as many rows a wave as leave two work-groups a compute unit (one, two, four groups
-      // of rows: 8 experts x 4096 x 4096, 64 tokens 80, 84, 110 us; 16 x 6144 x 2048 125,
-      // 118, 117; 64 x 2048 x 1024, 256 tokens 92, 85, 82)
-      auto busy = [&](int rg) { return d->E * ceil_div(d->H, 16 * rg * kMoeWaves) >= 2 * compute_units(); };
-      if (busy(4)) dense_kernel(moe_down_dense_kernel<CMK_MX4, 4, 1>, d->H, 4);
-      else if (busy(2)) dense_kernel(moe_down_dense_kernel<CMK_MX4, 2, 3>, d->H, 2);
-      else dense_kernel(moe_down_dense_kernel<CMK_MX4, 1, 3>, d->H, 1);
+      if (all_at_once(1)) dense_kernel(moe_down_dense_kernel<CMK_MX4, 1, 2>, d->H, 1);
+      else if (all_at_once(2)) dense_kernel(moe_down_dense_kernel<CMK_MX4, 2, 2>, d->H, 2);
+      else dense_kernel(moe_down_dense_kernel<CMK_MX4, 4, 1>, d->H, 4);
     } else if (d->w_dtype == CMK_BF16) {
       dense_kernel(moe_gate_up_dense_kernel<CMK_BF16, 1, 1, 2>, p.Ip, 1);
-      dense_kernel(moe_down_dense_kernel<CMK_BF16, 1, 3>, d->H, 1);
+      if (all_at_once(1)) dense_kernel(moe_down_dense_kernel<CMK_BF16, 1, 2>, d->H, 1);
+      else dense_kernel(moe_down_dense_kernel<CMK_BF16, 2, 2>, d->H, 2);
     } else {
       dense_kernel(moe_gate_up_dense_kernel<CMK_F16, 1, 1, 2>, p.Ip, 1);
-      dense_kernel(moe_down_dense_kernel<CMK_F16, 1, 3>, d->H, 1);
+      if (all_at_once(1)) dense_kernel(moe_down_dense_kernel<CMK_F16, 1, 2>, d->H, 1);
+      else dense_kernel(moe_down_dense_kernel<CMK_F16, 2, 2>, d->H, 2);
     }
   } else if (d->w_dtype == CMK_MX4) {
     if (p.x_planes == 1) {
@@ -1161,7 +1207,7 @@ extern "C" int cmk_moe(const void* x, const void* router, const void* gate_up, c
       else experts_kernel(moe_gate_up_kernel<CMK_MX4, 2, 2, 1, 3>, p.Ip, 1, 2);
     }
     if (many) experts_kernel(moe_down_kernel<CMK_MX4, 1, 4, 1>, d->H, 4, 1);
-    else experts_kernel(moe_down_kernel<CMK_MX4, 2, 2, 2>, d->H, 2, 2);
+    else experts_kernel(moe_down_kernel<CMK_MX4, 2, 2, 3>, d->H, 2, 2);
   } else if (d->w_dtype == CMK_BF16) {
     if (many) experts_kernel(moe_gate_up_kernel<CMK_BF16, 1, 4, 1, 1>, p.Ip, 1, 4);
     else experts_kernel(moe_gate_up_kernel<CMK_BF16, 1, 4, 1, 2>, p.Ip, 1, 4);

@@ -288,7 +288,7 @@ typedef struct cmk_moe_desc {
  * axis contiguous; for CMK_MX4 gate_up and down are the codes, with their
  * scales, that cmk_mx4_quantize writes of matrices of 2I rows x H and H rows x I.
  * y is dense [T][H], weights fp32 and experts int64 are dense [T][k].  Sums are
- * held in fp32; act(..) * (..) is kept as two bf16 (16 bits of mantissa); y is
+ * held in fp32; act(..) * (..) is kept in fp32's 24 bits (as three bf16); y is
  * rounded once.  Only the chosen experts' weights are read.  A sum that an infinite
  * weight of `down` or an infinite act(..) * (..) enters may come out as NaN where the
  * formula has an infinity.

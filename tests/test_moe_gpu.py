@@ -324,3 +324,51 @@ def test_equal_tokens_get_equal_results(device, four_bit, dtype):
 def test_many_tokens_of_many_experts_in_four_bits(device, t, h, i, e, k, dtype):
     """Two and four groups of rows a wave, with up to 16, up to 32 and more slots."""
     check(MoECUDA(k=k), *make(t, h, i, e, dtype, t + h + i), device, True)
+
+
+def exact_layer(t, four_bit, e=4, h=512, i=512):
+    """Operands (bf16) whose layer has an exact result, and that result in float64.
+
+    g = 32 for every inner feature: 1 + exp(-32) is 1 in fp32, so silu(g) = 32 there.
+    Up values are 1 + a sum of distinct powers of two down to 2^-23, products of powers of
+    two; every row of `down` is the difference of two inner values.  All of that and the
+    choice (equal logits: the first two experts, half each) is exact in fp32 whatever the
+    order of the sums, as long as inner values have 24 bits."""
+    gen = torch.Generator().manual_seed(t)
+    blocks = torch.arange(0, h, 32)[:14]               # one element a block of 32: exact in 4 bits
+    low = blocks[1:]
+    power = torch.arange(1, 14) + 10                   # 2^-11 to 2^-23
+    x = torch.zeros(t, h)
+    x[:, 0] = 1
+    x[:, low] = torch.randint(0, 2, (t, 13), generator=gen) * 2.0 ** -10
+    x[0, low] = 2.0 ** -10
+    gate_up, down = torch.zeros(e, 2 * i, h), torch.zeros(e, h, i)
+    gate_up[:, :i, 0] = 32
+    gate_up[:, i:, 0] = 1
+    gate_up[:, i:, low] = torch.randint(0, 2, (e, i, 13), generator=gen) * torch.exp2(10.0 - power)
+    minus = (torch.arange(h) * 7 + 3) % i
+    plus = torch.where((torch.arange(h) * 5) % i == minus, (minus + 1) % i, (torch.arange(h) * 5) % i)
+    down[:, torch.arange(h), plus], down[:, torch.arange(h), minus] = 1, -1
+    v = x.double() @ gate_up[:2, i:].double().transpose(1, 2)                       # [2, t, i]
+    y = ((32 * v) @ down[:2].double().transpose(1, 2) * 0.5).sum(0)
+    return x, torch.zeros(e, h), gate_up, down, y
+
+
+# one token; planes in one and in two fragments of their own; one and two blocks of slots; passes
+@pytest.mark.parametrize("t,e", [(1, 4), (2, 4), (5, 4), (6, 4), (10, 4), (11, 4), (16, 40), (25, 4), (40, 40), (100, 32)])
+@pytest.mark.parametrize("four_bit", [False, True])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_inner_values_keep_their_24_bits(device, t, e, four_bit, dtype):
+    x, router, gate_up, down, want = exact_layer(t, four_bit, e)
+    print("exact layer", t, e, four_bit, dtype, flush=True)
+    args = [v.to(dtype).to(device) for v in (x, router, gate_up, down)]
+    for v, w in zip((x, gate_up, down), (args[0], args[2], args[3])):
+        assert torch.equal(w.cpu().float(), v)
+    if four_bit:
+        args[2:] = [quantize_mx4(v) for v in args[2:]]
+        for v, w in zip((gate_up, down), args[2:]):
+            assert torch.equal(w.dequantize().cpu(), v)
+    y, weights, experts = MoECUDA(k=2)(*args)
+    assert (weights == 0.5).all() and (experts.cpu() == torch.tensor([0, 1])).all()
+    assert want[0].abs().min() < 2.0 ** -7 < want[0].abs().max()      # far below the inner values' 32
+    assert torch.equal(y.cpu(), want.to(dtype))
