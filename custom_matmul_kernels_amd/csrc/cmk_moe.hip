@@ -399,20 +399,23 @@ __device__ __forceinline__ f32x4 mfma_f16(u32x4v a, u32x4v b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-// fp32 as the sum of three bf16, exactly.  An infinity or a NaN stays in the first alone.
+// fp32 as the sum of three bf16, exactly.  The first is cut, not rounded: a value that is
+// finite in fp32 stays so up to the end of the range.  An infinity or a NaN stays in the
+// first alone.
 __device__ __forceinline__ void split_f32(float v, u16& a, u16& b, u16& c) {
-  const __bf16 hi = (__bf16)v;
-  const float rest = __builtin_isfinite(v) ? v - (float)hi : 0.0f;
+  const bool finite = __builtin_isfinite(v);
+  const float hi = finite ? __uint_as_float(__float_as_uint(v) & 0xffff0000u) : v;
+  const float rest = finite ? v - hi : 0.0f;
   const __bf16 mid = (__bf16)rest;
-  a = __builtin_bit_cast(u16, hi);
+  a = __builtin_bit_cast(u16, (__bf16)hi);
   b = __builtin_bit_cast(u16, mid);
   c = __builtin_bit_cast(u16, (__bf16)(rest - (float)mid));
 }
 
 // Eight fp16 as the sum of two times eight bf16, exactly (11 bits = 8 + 3).  The
 // products with activations need it that may not fit fp16.  The second is 2^-9 of the
-// weight at most, and its product with the third plane of an activation (2^-17 of that)
-// below fp32's last bit: it is left out where the planes are products of their own.  An
+// weight at most, and its product with the third plane of an activation (2^-16 of that)
+// is below fp32's last bit: it is left out where the planes are products of their own.  An
 // infinite weight comes out as NaN.
 __device__ __forceinline__ void split_f16(u32x4v w, u32x4v& hi, u32x4v& lo) {
   const f16x8 f = __builtin_bit_cast(f16x8, w);

@@ -372,3 +372,21 @@ def test_inner_values_keep_their_24_bits(device, t, e, four_bit, dtype):
     assert (weights == 0.5).all() and (experts.cpu() == torch.tensor([0, 1])).all()
     assert want[0].abs().min() < 2.0 ** -7 < want[0].abs().max()      # far below the inner values' 32
     assert torch.equal(y.cpu(), want.to(dtype))
+
+
+@pytest.mark.parametrize("t,e", [(1, 4), (4, 4), (14, 4), (20, 4), (40, 40), (100, 32)])
+@pytest.mark.parametrize("four_bit", [False, True])
+def test_inner_values_at_the_end_of_the_range(device, t, e, four_bit):
+    """2^128 (1 - 2^-12) is finite, and the nearest bf16 is not: g = 2^64, up 2^64 - 2^52."""
+    h = i = 512
+    x, gate_up, down = torch.zeros(t, h), torch.zeros(e, 2 * i, h), torch.zeros(e, h, i)
+    x[:, 0], x[:, 64] = 2.0 ** 32, 2.0 ** 20
+    gate_up[:, :, 0] = 2.0 ** 32
+    gate_up[:, i:, 64] = -2.0 ** 32
+    down[:, torch.arange(h), torch.arange(h)] = 2.0 ** -100
+    args = [v.to(BF16).to(device) for v in (x, torch.zeros(e, h), gate_up, down)]
+    if four_bit:
+        args[2:] = [quantize_mx4(v) for v in args[2:]]
+        assert torch.equal(args[3].dequantize().cpu(), down)
+    y, _, _ = MoECUDA(k=2)(*args)
+    assert (y == 2.0 ** 28).all()        # 2^28 (1 - 2^-12), rounded
