@@ -390,3 +390,33 @@ def test_inner_values_at_the_end_of_the_range(device, t, e, four_bit):
         assert torch.equal(args[3].dequantize().cpu(), down)
     y, _, _ = MoECUDA(k=2)(*args)
     assert (y == 2.0 ** 28).all()        # 2^28 (1 - 2^-12), rounded
+
+
+def grouped(sizes, h, i, e, dtype, seed):
+    """A layer whose expert j is the choice of sizes[j] tokens, in a shuffled order."""
+    x, router, gate_up, down = make(sum(sizes), h, i, e, dtype, seed)
+    choice = torch.cat([torch.full((n,), j) for j, n in enumerate(sizes)])
+    choice = choice[torch.randperm(len(choice), generator=torch.Generator().manual_seed(seed))]
+    x[:, :e] = 0
+    x[torch.arange(len(choice)), choice] = 6
+    router[:, :e] = 8 * torch.eye(e)
+    return x, router, gate_up, down, choice
+
+
+# Slots of an expert decide how its rows are multiplied: planes packed in one fragment of
+# columns (up to 5) or two (up to 10), blocks of 16 and of 32, passes of 32; the extents
+# decide in how many pieces k goes through LDS, and by how many waves.
+@pytest.mark.parametrize("sizes,h,i,e", [
+    ((5, 9, 14, 27, 40), 1700, 1700, 5),     # few experts: waves share k in both products
+    ((5, 9, 14, 27, 40), 3700, 300, 5),
+    ((4, 10, 16, 32, 33), 300, 3700, 6),
+    ((6, 2), 4200, 1400, 9),                 # fewer slots than experts
+    ((5, 9, 14, 27, 40), 520, 1300, 33),     # more than 32 experts: rows of their own
+    ((4, 8, 16, 32, 49), 2300, 260, 33),
+])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("four_bit", [False, True])
+def test_experts_of_every_size(device, sizes, h, i, e, dtype, four_bit):
+    x, router, gate_up, down, choice = grouped(sizes, h, i, e, dtype, h + i)
+    got = check(MoECUDA(k=1), x, router, gate_up, down, device, four_bit)
+    assert torch.equal(got[2].cpu()[:, 0], choice)
