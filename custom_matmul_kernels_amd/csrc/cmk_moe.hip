@@ -8,6 +8,7 @@
 // For a few tokens the time is that of reading the chosen experts' weights once;
 // everything here is laid out around that stream.
 #include <algorithm>
+#include <type_traits>
 
 #include "cmk_mx4.hpp"
 
@@ -22,7 +23,7 @@ constexpr int kMoeWaves = 4;  // of the experts' kernels
 // act(gate) * up goes to the down product as the sum of three bf16, which holds all 24
 // bits of fp32 and its range.  Of the bf16 results of 64 tokens x 2048 x 1024 x 128
 // experts 0.03 % then differ from the formula's rounded ones; with two (16 bits) it was
-// 0.26 %, and 301 us instead of 307.
+// 0.26 %.
 constexpr int kInnerPlanes = 3;
 
 typedef double f64x4 __attribute__((ext_vector_type(4)));
@@ -65,7 +66,8 @@ struct MoeArgs {
   int act, renormalize;
   double* logits;
   int* chosen;     // [T*k]
-  u16 *xp, *hp;    // planes [planes][T][Hp], [kInnerPlanes][T*k][Ip]
+  u16* xp;         // planes [planes][T][Hp]
+  void* hp;        // fp32 [T*k][Ip], or planes [kInnerPlanes][T*k][Ip] (direct loads take them)
   float* yp;       // [T*k][H]
 };
 
@@ -412,6 +414,15 @@ __device__ __forceinline__ void split_f32(float v, u16& a, u16& b, u16& c) {
   c = __builtin_bit_cast(u16, (__bf16)(rest - (float)mid));
 }
 
+// The parts of eight values to LDS, `apart` bytes from each other.
+__device__ __forceinline__ void stage_parts(const Octet<float>& o, char* to, int apart) {
+  u16 part[kInnerPlanes][8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) split_f32(o.v[i], part[0][i], part[1][i], part[2][i]);
+#pragma unroll
+  for (int p = 0; p < kInnerPlanes; ++p) __builtin_memcpy(to + p * apart, part[p], 16);
+}
+
 // Eight fp16 as the sum of two times eight bf16, exactly (11 bits = 8 + 3).  The
 // products with activations need it that may not fit fp16.  The second is 2^-9 of the
 // weight at most, and its product with the third plane of an activation (2^-16 of that)
@@ -466,7 +477,8 @@ __device__ __forceinline__ float activate(float g, int act) {
 // the banks.  Where the rows do not fit whole, the pass goes through k in pieces.
 constexpr int kActBytes = 36 * 1024;       // gate and up
 // Down: four work-groups a compute unit where a wave takes rows of its own, one group of
-// them (64 tokens x 2048 x 1024 x 128 experts: 306 us, 309 with three); three elsewhere.
+// them (64 tokens x 2048 x 1024 x 128 experts, from planes: 306 us, 309 with three); three
+// elsewhere.
 constexpr int inner_bytes(int KS, int RG) { return (KS == 1 && RG == 1 ? 36 : 51) * 1024; }
 
 // The products of RG groups of 16 rows of one expert's matrix with the `count`
@@ -483,6 +495,10 @@ constexpr int inner_bytes(int KS, int RG) { return (KS == 1 && RG == 1 ? 36 : 51
 // caller adds them (add_planes).  A third (half) of the matrix instructions and LDS reads.
 // Whether that is done hangs on the expert's slots alone, not on a pass's, whose members
 // may differ from run to run.
+//
+// `source` gives rows of planes, or of fp32 that become planes on the way to LDS (two
+// thirds of the bytes: 64 tokens x 2048 x 1024 x 128 experts 307 us from planes, 297 from fp32; 16 x 4096
+// x 4096 x 8 experts in 4 bits 84 and 75).
 template <int WF, int PLANES, int M, int RG, int NB, int U, int KS, bool SPLIT, bool PACK, int BYTES, class Source>
 __device__ __forceinline__ void moe_products(f32x4 (&acc)[M][RG][NB], const void* base, const uint8_t* scales, long long rows,
                                              const long long (&row)[M][RG], long long ld, int K, int count, Source source,
@@ -517,10 +533,18 @@ __device__ __forceinline__ void moe_products(f32x4 (&acc)[M][RG][NB], const void
         if (first + share + u * KS < end) request(u, first + share + u * KS);
     if (first > 0) __syncthreads();
     const int units = (end - first) * 16;  // 16-byte units of a row
-    for (int v = threadIdx.x; v < PLANES * count * units; v += 64 * kMoeWaves) {
+    constexpr bool kFloats = std::is_same_v<decltype(source(0)), const float*>;
+    for (int v = threadIdx.x; v < (kFloats ? 1 : PLANES) * count * units; v += 64 * kMoeWaves) {
       const int line = v / units, at = v - line * units;
-      const int c = line % count, p = line / count;
-      *(u32x4v*)(lds + p * plane_bytes + c * pitch + at * 16) = *(const u32x4v*)(source(c) + p * plane + first * kSlab + at * 8);
+      if constexpr (kFloats) {
+        static_assert(PLANES == kInnerPlanes, "the parts of an fp32");
+        Octet<float> o;
+        __builtin_memcpy(o.v, source(line) + first * kSlab + at * 8, 32);
+        stage_parts(o, lds + line * pitch + at * 16, plane_bytes);
+      } else {
+        const int c = line % count, p = line / count;
+        *(u32x4v*)(lds + p * plane_bytes + c * pitch + at * 16) = *(const u32x4v*)(source(c) + p * plane + first * kSlab + at * 8);
+      }
     }
     __syncthreads();
     if (!idle)
@@ -664,26 +688,32 @@ __device__ __forceinline__ void moe_down_rows(const MoeArgs& a, int n0, long lon
   for (int g = 0; g < RG; ++g) row[0][g] = min(n0 + g * 16 + ((int)threadIdx.x & 15), a.H - 1);
 }
 
-// act(gate) * up of a wave's rows to the planes of the inner activations.
-template <int WF, int RG, int NB>
+// act(gate) * up of a wave's rows to the inner activations, as fp32 or as planes.
+template <int WF, bool PLANES, int RG, int NB>
 __device__ __forceinline__ void moe_store_inner(const MoeArgs& a, const f32x4 (&acc)[2][RG][NB], const int* list, int c0, int count, int i0) {
   const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
     const int c = c0 + b * 16 + r;
     if (c >= count) continue;
-    u16* h = a.hp + (long long)list[c] * a.Ip;
+    const long long row = (long long)list[c] * a.Ip;
 #pragma unroll
     for (int g = 0; g < RG; ++g) {
       const int i1 = i0 + g * 16 + q * 4;  // four consecutive inner features of one token
       if (i1 >= a.Ip) continue;
-      u16 part[kInnerPlanes][4];
+      const long long at = row + plane_position<WF == CMK_MX4>(i1);
+      float v[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        split_f32(i1 + i < a.I ? activate(acc[0][g][b][i], a.act) * acc[1][g][b][i] : 0.0f, part[0][i], part[1][i], part[2][i]);
-      u16* at = h + plane_position<WF == CMK_MX4>(i1);
+      for (int i = 0; i < 4; ++i) v[i] = i1 + i < a.I ? activate(acc[0][g][b][i], a.act) * acc[1][g][b][i] : 0.0f;
+      if constexpr (PLANES) {
+        u16 part[kInnerPlanes][4];
 #pragma unroll
-      for (int p = 0; p < kInnerPlanes; ++p) __builtin_memcpy(at + (long long)p * a.T * a.k * a.Ip, part[p], 8);
+        for (int i = 0; i < 4; ++i) split_f32(v[i], part[0][i], part[1][i], part[2][i]);
+#pragma unroll
+        for (int p = 0; p < kInnerPlanes; ++p) __builtin_memcpy((u16*)a.hp + at + (long long)p * a.T * a.k * a.Ip, part[p], 8);
+      } else {
+        __builtin_memcpy((float*)a.hp + at, v, 16);
+      }
     }
   }
 }
@@ -723,7 +753,7 @@ __device__ __forceinline__ void moe_gate_up_tokens(const MoeArgs& a, int expert,
   join_waves<KS, 2 * RG * NB, kActBytes>((f32x4(&)[2 * RG * NB])acc, (f32x4(*)[2 * RG * NB][64])lds, share);
   if (share == 0) {
     if constexpr (PACK) add_planes<PLANES>((f32x4(&)[2 * RG][NB])acc, count - c0);
-    moe_store_inner<WF, RG, NB>(a, acc, list, c0, count, i0);
+    moe_store_inner<WF, false, RG, NB>(a, acc, list, c0, count, i0);
   }
 }
 
@@ -773,9 +803,8 @@ __device__ __forceinline__ void moe_down_tokens(const MoeArgs& a, int expert, co
   long long row[1][RG];
   moe_down_rows<RG>(a, n0, row);
   f32x4 acc[1][RG][NB] = {};
-  auto source = [&](int c) { return a.hp + (long long)list[c0 + c] * a.Ip; };
-  moe_products<WF, kInnerPlanes, 1, RG, NB, U, KS, WF == CMK_F16, PACK, inner_bytes(KS, RG)>(acc, moe_down_base<WF>(a, expert), moe_down_scales<WF>(a, expert), a.H, row, a.ld_down, a.I, min(count - c0, NB * 16), source,
-                                                       (long long)a.T * a.k * a.Ip, share, n0 >= a.H, lds);
+  auto source = [&](int c) { return (const float*)a.hp + (long long)list[c0 + c] * a.Ip; };
+  moe_products<WF, kInnerPlanes, 1, RG, NB, U, KS, WF == CMK_F16, PACK, inner_bytes(KS, RG)>(acc, moe_down_base<WF>(a, expert), moe_down_scales<WF>(a, expert), a.H, row, a.ld_down, a.I, min(count - c0, NB * 16), source, 0, share, n0 >= a.H, lds);
   join_waves<KS, RG * NB, inner_bytes(KS, RG)>((f32x4(&)[RG * NB])acc, (f32x4(*)[RG * NB][64])lds, share);
   if (share == 0) {
     if constexpr (PACK) add_planes<kInnerPlanes>((f32x4(&)[RG][NB])acc, count - c0);
@@ -918,7 +947,7 @@ __device__ __forceinline__ void moe_gate_up_dense(const MoeArgs& a, int expert, 
   auto source = [&](int c) { return a.xp + (long long)(list[c0 + c] / a.k) * a.Hp; };
   moe_dense_products<WF, PLANES, 2, RG, NB, U, kGateUpStages, false>(acc, moe_gate_up_base<WF>(a, expert), moe_gate_up_scales<WF>(a, expert), 2 * a.I, row,
                                                       a.ld_gate_up, a.H, min(count - c0, NB * 16), source, (long long)a.T * a.Hp, lds);
-  moe_store_inner<WF, RG, NB>(a, acc, list, c0, count, i0);
+  moe_store_inner<WF, true, RG, NB>(a, acc, list, c0, count, i0);
 }
 
 template <int WF, int RG, int NB, int U>
@@ -928,7 +957,7 @@ __device__ __forceinline__ void moe_down_dense(const MoeArgs& a, int expert, con
   long long row[1][RG];
   f32x4 acc[1][RG][NB] = {};
   moe_down_rows<RG>(a, n0, row);
-  auto source = [&](int c) { return a.hp + (long long)list[c0 + c] * a.Ip; };
+  auto source = [&](int c) { return (const u16*)a.hp + (long long)list[c0 + c] * a.Ip; };
   moe_dense_products<WF, kInnerPlanes, 1, RG, NB, U, kDownStages, WF == CMK_F16>(acc, moe_down_base<WF>(a, expert), moe_down_scales<WF>(a, expert), a.H, row,
                                                          a.ld_down, a.I, min(count - c0, NB * 16), source, (long long)a.T * a.k * a.Ip, lds);
   moe_store_outer<RG, NB>(a, acc, list, c0, count, n0);
@@ -997,7 +1026,7 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(MoeArgs a) {
 // rows and all the chosen experts.  A unit is one slab of one of them; the W waves
 // take units in turn, a ring of U under way each, and their sums meet in LDS in the
 // order of the waves.  The activations are multiplied by the weights as they are
-// staged and split again.
+// staged and split.
 constexpr int kSingleUnits = 80;  // staged at a time: two work-groups a compute unit
 
 template <int WF, class T, int W, int U>
@@ -1010,7 +1039,6 @@ __global__ __launch_bounds__(64 * W) void moe_down_single_kernel(MoeArgs a) {
   const int n0 = blockIdx.x * 16;
   const int row = min(n0 + r, a.H - 1);
   const int slabs = a.Ip / kSlab, units = a.k * slabs;
-  const long long plane = (long long)a.k * a.Ip;
   f32x4 acc = {};
   unsigned worst = 0;
   for (int first = 0; first < units; first += kSingleUnits) {
@@ -1030,18 +1058,11 @@ __global__ __launch_bounds__(64 * W) void moe_down_single_kernel(MoeArgs a) {
       const int unit = v / (kSlab / 8), at = v % (kSlab / 8) * 8;
       const long long from = (long long)(first + unit) * kSlab + at;  // units are consecutive in memory
       const float weight = a.weights[(first + unit) / slabs];
-      u16 part[kInnerPlanes][8];
+      Octet<float> o;
+      __builtin_memcpy(o.v, (const float*)a.hp + from, 32);
 #pragma unroll
-      for (int p = 0; p < kInnerPlanes; ++p) __builtin_memcpy(part[p], a.hp + p * plane + from, 16);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        float f = 0;
-#pragma unroll
-        for (int p = 0; p < kInnerPlanes; ++p) f += __uint_as_float((unsigned)part[p][i] << 16);
-        split_f32(weight * f, part[0][i], part[1][i], part[2][i]);
-      }
-#pragma unroll
-      for (int p = 0; p < kInnerPlanes; ++p) __builtin_memcpy(lds + unit * kUnit + p * 2 * kSlab + at * 2, part[p], 16);
+      for (int i = 0; i < 8; ++i) o.v[i] *= weight;
+      stage_parts(o, lds + unit * kUnit + at * 2, 2 * kSlab);
     }
     __syncthreads();
     for (int s0 = first + wave; s0 < end; s0 += W * U) {
@@ -1134,7 +1155,7 @@ extern "C" int cmk_moe(const void* x, const void* router, const void* gate_up, c
   MoeArgs a{x, router, gate_up, down, gate_up_scales, down_scales, y, weights, experts,
             d->ld_x, d->ld_router, d->ld_gate_up, d->stride_gate_up, d->ld_down, d->stride_down,
             d->T, d->H, d->I, d->E, d->k, p.Hp, p.Ip, p.splits, d->activation, d->renormalize,
-            (double*)(ws + p.logits), (int*)(ws + p.chosen), (u16*)(ws + p.x), (u16*)(ws + p.h), (float*)(ws + p.y)};
+            (double*)(ws + p.logits), (int*)(ws + p.chosen), (u16*)(ws + p.x), ws + p.h, (float*)(ws + p.y)};
   hipStream_t st = (hipStream_t)stream;
   const bool r32 = d->router_dtype == CMK_F32, four = d->w_dtype == CMK_MX4;
   const bool small = d->T > 1 && small_router(d->E, p.Hp);
