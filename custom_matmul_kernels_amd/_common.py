@@ -6,6 +6,18 @@ import torch
 from . import _lib
 
 
+MAX_EXTENT = 2 ** 31 - 1
+
+
+def check_extents(*extents):
+    """The library's extents are C ints, and ctypes cuts a larger number to its low
+    32 bits without an error: an operand of 2^32 + 5 columns would be taken for one
+    of 5."""
+    for n in extents:
+        if n > MAX_EXTENT:
+            raise ValueError("extents are at most 2^31 - 1, got %s" % (tuple(extents),))
+
+
 def get_mode(A, B):
     """Layout letters of A[l,m,k] and B[l,k,n] as the reference infers them
     from strides (reference bmm.py:56-66): "n" when the last axis is
@@ -39,6 +51,7 @@ def check_operands(A, B):
     assert A.dtype == B.dtype
     if A.dtype != torch.float32:
         raise TypeError("only torch.float32 operands are supported, got %s" % A.dtype)
+    check_extents(*A.shape, B.shape[2])
     assert A.device.type == B.device.type == "cuda"
     assert A.device == B.device
 

@@ -9,7 +9,7 @@ import math
 
 import torch
 
-from . import _lib
+from . import _common, _lib
 
 
 def derive_masks(final_mask):
@@ -23,6 +23,7 @@ def derive_masks(final_mask):
         raise TypeError("the mask must be torch.bool or torch.uint8, got %s" % final_mask.dtype)
     if final_mask.dim() not in (2, 3):
         raise ValueError("the mask needs to be 2d or 3d")
+    _common.check_extents(*final_mask.shape)
     if final_mask.device.type != "cuda":
         raise ValueError("the mask must be a device tensor (got device %s)" % final_mask.device)
     lib = _lib.load()

@@ -70,6 +70,8 @@ class MoECUDA:
         assert router.shape == (e, h)
         assert two_i == 2 * i and i > 0 and h > 0
         assert 0 < self.k <= e
+        if e | two_i | h > _common.MAX_EXTENT:
+            _common.check_extents(e, two_i, h)
         _common.refuse_grad(x, router)
         gp, gs, ldg, sg = self._experts(gate_up, (e, two_i, h), dtype, "gate_up")
         dp, ds, ldd, sd = self._experts(down, (e, h, i), dtype, "down")

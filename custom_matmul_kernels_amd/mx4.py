@@ -29,6 +29,7 @@ class MX4Tensor:
         if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
             raise TypeError("codes and scales must be torch.uint8")
         assert k_axis in (-1, -2)
+        _common.check_extents(*codes.shape, k)
         assert codes.dim() == 4 and codes.shape[1] == slabs and codes.shape[3] == SLAB // 2
         assert tuple(scales.shape) == tuple(codes.shape[:3]) + (SLAB // BLOCK,)
         assert codes.device == scales.device
@@ -113,6 +114,7 @@ class MX4Tensor:
             codes, scales = codes[None], scales[None]
         blocks = -(-k // BLOCK)
         l, rows, _ = codes.shape
+        _common.check_extents(l, rows, k)
         assert tuple(codes.shape) == (l, rows, blocks * BLOCK // 2)
         assert tuple(scales.shape) == (l, rows, blocks)
         slabs = -(-k // SLAB)
@@ -147,10 +149,12 @@ def quantize_mx4(T, dim=-1):
         raise ValueError("the tensor needs to be 2d or 3d")
     k_axis = dim if dim < 0 else dim - n
     assert k_axis == -1 or k_axis == -2, "dim must be one of the two matrix axes"
-    assert device.type == "cuda"
-    _common.refuse_grad(T)
     l = 1 if n == 2 else shape[0]
     rows, k = shape[-3 - k_axis], shape[k_axis]
+    if l | rows | k > _common.MAX_EXTENT:
+        _common.check_extents(l, rows, k)
+    assert device.type == "cuda"
+    _common.refuse_grad(T)
     units = l * -(-k // SLAB) * rows
     storage = torch.empty(units * (SLAB // 2 + SLAB // BLOCK), dtype=torch.uint8, device=device)
     if units:
@@ -198,6 +202,8 @@ class MX4BMMCUDA:
         l = 1 if n == 2 else sa[0]
         assert sb[-2] == k
         assert n == 2 or sb[0] == l
+        if l | m | c | k > _common.MAX_EXTENT:
+            _common.check_extents(l, m, c, k)
         assert device.type == "cuda"
         assert device == B.device
         C = torch.empty((m, c) if n == 2 else (l, m, c), dtype=self.out_dtype, device=device)

@@ -95,3 +95,15 @@ def test_refusals_of_the_c_entry_point():
     need = lib.cmk_moe_workspace_bytes(desc())
     assert need > 0 and call(desc(), nbytes=need - 1) == _lib.ERR_WORKSPACE
     assert call(desc(T=0)) == 0                          # nothing to do
+
+
+def test_extents_beyond_a_c_int_are_refused():
+    """They would reach the library cut to 32 bits; meta tensors hold no elements."""
+    def layer(h, i, e):
+        def meta(*shape):
+            return torch.empty(*shape, dtype=torch.bfloat16, device="meta")
+        MoECUDA(k=1)(meta(3, h), meta(e, h), meta(e, 2 * i, h), meta(e, h, i))
+    for large in (2 ** 31, 2 ** 32 + 64):
+        for extents in ((large, 32, 4), (64, large, 4), (64, 32, large), (64, large // 2, 4)):
+            with pytest.raises(ValueError, match="2\\^31"):
+                layer(*extents)

@@ -194,3 +194,26 @@ def test_more_than_a_launch_holds_is_refused():
         assert lib.cmk_mx4_dequantize(ok, ok, ok, 0, large, 1, 1, rows_innermost, None) == _lib.ERR_UNSUPPORTED
     for m, n in [(1, 1), (64, 64)]:       # a work-group each
         assert lib.cmk_mx4_bmm(four, four, ok, 0, 1 << 24, m, n, 32, None, 0, None) == _lib.ERR_UNSUPPORTED
+
+
+@pytest.mark.parametrize("large", [2 ** 31, 2 ** 32, 2 ** 32 + 128])
+def test_extents_beyond_a_c_int_are_refused(large):
+    """They would reach the library cut to 32 bits; meta tensors hold no elements."""
+    def meta(*shape, dtype=torch.bfloat16):
+        return torch.empty(*shape, dtype=dtype, device="meta")
+    for shape in ((1, large), (large, 1), (large, 1, 1), (2, 3, large)):
+        for dim in (-1, -2):
+            with pytest.raises(ValueError, match="2\\^31"):
+                quantize_mx4(meta(*shape), dim=dim)
+    product = MX4BMMCUDA()
+    for a, b in (((1, large), (large, 1)), ((large, 4), (4, 1)), ((1, 4), (4, large)), ((large, 1, 1), (large, 1, 1))):
+        with pytest.raises(ValueError, match="2\\^31"):
+            product(meta(*a), meta(*b))
+    slabs = -(-large // 128)
+    u8 = dict(dtype=torch.uint8)
+    with pytest.raises(ValueError, match="2\\^31"):
+        MX4Tensor(meta(1, slabs, 1, 64, **u8), meta(1, slabs, 1, 4, **u8), large)
+    with pytest.raises(ValueError, match="2\\^31"):
+        MX4Tensor(meta(1, 1, large, 64, **u8), meta(1, 1, large, 4, **u8), 5)
+    with pytest.raises(ValueError, match="2\\^31"):
+        MX4Tensor.from_blocks(meta(1, -(-large // 32) * 16, **u8), meta(1, -(-large // 32), **u8), large)

@@ -180,3 +180,18 @@ def test_shared_unaligned_operand_is_copied_once():
     small = base[1:1 + 40 * 50].view(40, 50)[None].expand(4096, 40, 50)
     same, _, _, _ = _common._aligned(small, 0, 50, 0)
     assert same is small
+
+
+@pytest.mark.parametrize("large", [2 ** 31, 2 ** 32 + 5])
+def test_extents_beyond_a_c_int_are_refused(large):
+    """They would reach the library cut to 32 bits; meta tensors hold no elements."""
+    from custom_matmul_kernels_amd import MBMMCUDA, MinBMMCUDA, TopkBMMCUDA, derive_masks
+    def meta(*shape, dtype=torch.float32):
+        return torch.empty(*shape, dtype=dtype, device="meta")
+    for a, b in (((1, large), (large, 1)), ((large, 4), (4, 1)), ((1, 4), (4, large)), ((large, 1, 1), (large, 1, 1))):
+        for call in (BMMCUDA(), MinBMMCUDA(), TopkBMMCUDA(), lambda A, B: MBMMCUDA(share_mask=True)(A, B, None, None, None)):
+            with pytest.raises(ValueError, match="2\\^31"):
+                call(meta(*a), meta(*b))
+    for shape in ((large, 1), (1, large), (large, 1, 1)):
+        with pytest.raises(ValueError, match="2\\^31"):
+            derive_masks(meta(*shape, dtype=torch.bool))
