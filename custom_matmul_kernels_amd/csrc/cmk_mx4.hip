@@ -753,7 +753,9 @@ static void launch_rows(const Mx4RowsArgs& a, int L, hipStream_t st) {
 }
 
 static bool use_rows(int L, int M, int N, int K) {
-  if (M > kMx4Rows || L > 65535 || N >= 1 << 29) return false;  // (what one launch holds)
+  // What one launch holds: 65535 batches, and less than 2^32 threads along N (work-groups
+  // of 512 threads for 64 columns).
+  if (M > kMx4Rows || L > 65535 || ceil_div(N, 64) * 512LL > 0xffffffffLL) return false;
   // From 17 rows on the tiles win where there are enough of them (32 rows against
   // 16384 x 8192: 24 us by rows, 14 by tiles; 4096 x 4096: 5.4 and 7.6) or k is long
   // enough to be cut (1024 x 16384: 16 and 8).

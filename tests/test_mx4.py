@@ -217,3 +217,15 @@ def test_extents_beyond_a_c_int_are_refused(large):
         MX4Tensor(meta(1, 1, large, 64, **u8), meta(1, 1, large, 4, **u8), 5)
     with pytest.raises(ValueError, match="2\\^31"):
         MX4Tensor.from_blocks(meta(1, -(-large // 32) * 16, **u8), meta(1, -(-large // 32), **u8), large)
+
+
+def test_few_rows_take_tiles_where_a_launch_would_wrap_round():
+    """64 columns a work-group of 512 threads: 2^23 of them are 2^32 threads.  The kernel
+    for few rows quantises a float left operand by itself and needs no room for it."""
+    lib = _lib.load()
+    ok = ctypes.c_void_p(0x1000)          # never dereferenced
+    left, right = _lib.Mx4Operand(ok, None, _lib.F32, 0, 0, 128, 1), _lib.Mx4Operand(ok, ok, _lib.MX4)
+    for m in (1, 8):
+        assert lib.cmk_mx4_workspace_bytes(left, right, 1, m, (1 << 29) - 64, 128) == 0
+        assert lib.cmk_mx4_workspace_bytes(left, right, 1, m, (1 << 29) - 63, 128) > 0
+        assert lib.cmk_mx4_workspace_bytes(left, right, 1, m, 1 << 29, 128) > 0
