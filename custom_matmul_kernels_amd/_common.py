@@ -18,6 +18,12 @@ def check_extents(*extents):
             raise ValueError("extents are at most 2^31 - 1, got %s" % (tuple(extents),))
 
 
+def with_own_sign(T):
+    """T, or a copy of it where T is a lazily negated view (the imaginary part of a
+    conjugate): its memory, which the kernels read, has the other sign."""
+    return T.resolve_neg() if T.is_neg() else T
+
+
 def get_mode(A, B):
     """Layout letters of A[l,m,k] and B[l,k,n] as the reference infers them
     from strides (reference bmm.py:56-66): "n" when the last axis is
@@ -59,6 +65,7 @@ def check_operands(A, B):
 def _operand(T, want_inner, name):
     """Returns (tensor, trans, ld, batch_stride) for one [l, r, c] operand.
     A tensor whose strides fit neither layout is copied to row-major."""
+    T = with_own_sign(T)
     l, r, c = T.shape
     s0, s1, s2 = T.stride()
     # an axis of extent 1 can carry any stride; treat it as the natural one
@@ -115,8 +122,8 @@ def make_desc(A, B):
     A2, tA, lda, sA = _operand(A, k, "A")
     B2, tB, ldb, sB = _operand(B, n, "B")
     if sA < 0 or sB < 0:
-        A2, tA, lda, sA = A.contiguous(), 0, max(k, 1), m * k
-        B2, tB, ldb, sB = B.contiguous(), 0, max(n, 1), k * n
+        A2, tA, lda, sA = A2.contiguous(), 0, max(k, 1), m * k
+        B2, tB, ldb, sB = B2.contiguous(), 0, max(n, 1), k * n
     A2, tA, lda, sA = _aligned(A2, tA, lda, sA)
     B2, tB, ldb, sB = _aligned(B2, tB, ldb, sB)
     # the descriptor's trans flag for A is about [m,k] storage, for B about [k,n]

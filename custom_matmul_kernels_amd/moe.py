@@ -64,6 +64,11 @@ class MoECUDA:
             raise TypeError("router must be torch.float32 or of x's type, got %s" % router.dtype)
         if x.dim() != 2 or router.dim() != 2 or gate_up.dim() != 3 or down.dim() != 3:
             raise ValueError("x and router need to be 2d, gate_up and down 3d")
+        x, router = _common.with_own_sign(x), _common.with_own_sign(router)
+        if not isinstance(gate_up, MX4Tensor):
+            gate_up = _common.with_own_sign(gate_up)
+        if not isinstance(down, MX4Tensor):
+            down = _common.with_own_sign(down)
         t, h = x.shape
         e, two_i, _ = gate_up.shape
         i = two_i // 2

@@ -143,6 +143,7 @@ def quantize_mx4(T, dim=-1):
     scale, is one of the last two: -1 for the left operand of a product, -2 for
     the right one."""
     dtype = _common.float_type(T.dtype, "the tensor")
+    T = _common.with_own_sign(T)
     shape, stride, device = T.shape, T.stride(), T.device
     n = len(shape)
     if n not in (2, 3):
@@ -196,6 +197,10 @@ class MX4BMMCUDA:
         assert len(sb) == n
         if n not in (2, 3):
             raise ValueError("A and B need to be 2d or 3d")
+        if not isinstance(A, MX4Tensor):
+            A = _common.with_own_sign(A)
+        if not isinstance(B, MX4Tensor):
+            B = _common.with_own_sign(B)
         a, b = self._operand(A, -1, "A"), self._operand(B, -2, "B")
         m, k = sa[-2:]
         c = sb[-1]

@@ -90,7 +90,7 @@ class BitonicSort:
         if arr.dtype != torch.float32:
             raise TypeError("only torch.float32 is supported, got %s" % arr.dtype)
         assert arr.device.type == "cuda"
-        arr = arr.contiguous()
+        arr = _common.with_own_sign(arr.contiguous())
         values = torch.empty([k], device=arr.device, dtype=arr.dtype)
         indices = torch.empty([k], device=arr.device, dtype=torch.int64)
         ws, ws_bytes = _common.workspace(_lib.OP_TOPK_1D, 1, arr.numel(), 0, 0, 0, arr.device)

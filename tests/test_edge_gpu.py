@@ -417,3 +417,22 @@ def test_topk_config_5_every_row(device):
     rows = torch.arange(0, 1048576, 8209)
     at = O.gather_products(A[:, rows], B, 2, i[:, rows].cpu())
     O.check_values(v[:, rows].cpu(), at, 256, "value at index (float64)")
+
+
+def test_negated_views_are_read_with_their_sign(device):
+    """The imaginary part of a conjugate is a view whose memory has the other sign."""
+    from custom_matmul_kernels_amd import BMMCUDA, BitonicSort, MBMMCUDA, MinBMMCUDA, TopkBMMCUDA, derive_masks
+    z = torch.randn(2, 40, 30, dtype=torch.complex64, generator=torch.Generator().manual_seed(2)).to(device)
+    x = z.conj().imag
+    y = x.resolve_neg()
+    assert x.is_neg() and torch.equal(x, y)
+    masks = derive_masks(torch.ones(2, 40, 40, dtype=torch.bool, device=device))
+    for call in (BMMCUDA(), MinBMMCUDA(), MinBMMCUDA(distance="l2"), lambda a, b: TopkBMMCUDA()(a, b, k=3),
+                 lambda a, b: TopkBMMCUDA(distance="l1")(a, b, k=3), lambda a, b: MBMMCUDA()(a, b, *masks)):
+        want = call(y, y.transpose(1, 2))
+        for got in (call(x, y.transpose(1, 2)), call(y, x.transpose(1, 2)), call(x, x.transpose(1, 2))):
+            for a, b in zip(got, want):
+                assert torch.equal(a, b)
+    flat = torch._neg_view(torch.randn(700, generator=torch.Generator().manual_seed(3)).to(device))
+    for a, b in zip(BitonicSort()(flat, 5), BitonicSort()(flat.resolve_neg(), 5)):
+        assert torch.equal(a, b)

@@ -420,3 +420,15 @@ def test_experts_of_every_size(device, sizes, h, i, e, dtype, four_bit):
     x, router, gate_up, down, choice = grouped(sizes, h, i, e, dtype, h + i)
     got = check(MoECUDA(k=1), x, router, gate_up, down, device, four_bit)
     assert torch.equal(got[2].cpu()[:, 0], choice)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_negated_views_are_read_with_their_sign(device, dtype):
+    args = [v.to(device) for v in make(5, 96, 40, 6, dtype, 17)]
+    layer = MoECUDA(k=2)
+    want = layer(*args)
+    for n in range(4):
+        some = list(args)
+        some[n] = torch._neg_view(-args[n])
+        assert some[n].is_neg() and torch.equal(some[n], args[n])
+        assert all(torch.equal(a, b) for a, b in zip(layer(*some), want))

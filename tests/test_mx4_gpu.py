@@ -305,3 +305,23 @@ def test_as_many_matrices_as_a_launch_holds(device):
     assert torch.equal(c, want)
     with pytest.raises(RuntimeError):
         MX4BMMCUDA(torch.bfloat16)(x[:1].expand(l + 1, 1, 4), x[:1].expand(l + 1, 1, 4).transpose(1, 2))
+
+
+def test_negated_views_are_read_with_their_sign(device):
+    """The imaginary part of a conjugate is a view whose memory has the other sign."""
+    gen = torch.Generator().manual_seed(6)
+    z = torch.complex(torch.randn(2, 20, 300, generator=gen), torch.randn(2, 20, 300, generator=gen)).to(device)
+    for x in (z.conj().imag, torch._neg_view(z.real.contiguous().to(torch.bfloat16))):
+        y = x.resolve_neg()
+        assert x.is_neg() and not y.is_neg() and torch.equal(x, y)
+        for dim in (-1, -2):
+            a, b = quantize_mx4(x, dim=dim), quantize_mx4(y, dim=dim)
+            assert torch.equal(a.codes, b.codes) and torch.equal(a.scales, b.scales)
+        product, kept = MX4BMMCUDA(), quantize_mx4(y)
+        want = product(kept, kept.transpose())
+        for left, right in ((x, x.transpose(1, 2)), (x, kept.transpose()), (kept, x.transpose(1, 2))):
+            assert torch.equal(product(left, right), want)
+        # few rows, quantised by the product
+        assert torch.equal(product(x[:, :3], kept.transpose()), want[:, :3])
+        one = quantize_mx4(y[:, :1])
+        assert not torch.equal(product(one, kept.transpose()), product(quantize_mx4(-y[:, :1]), kept.transpose()))

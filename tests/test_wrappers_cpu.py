@@ -195,3 +195,15 @@ def test_extents_beyond_a_c_int_are_refused(large):
     for shape in ((large, 1), (1, large), (large, 1, 1)):
         with pytest.raises(ValueError, match="2\\^31"):
             derive_masks(meta(*shape, dtype=torch.bool))
+
+
+def test_negated_views_are_read_with_their_sign():
+    """The imaginary part of a conjugate is a view whose memory has the other sign."""
+    z = torch.randn(2, 6, 10, dtype=torch.complex64, generator=torch.Generator().manual_seed(1))
+    A, B = z.conj().imag, z.conj().imag.transpose(1, 2)
+    assert A.is_neg() and B.is_neg()
+    for left, right in ((A, B), (A[:1].expand(2, 6, 10), B), (A[:, :, :1], B[:, :1]), (A.contiguous(), B)):
+        A2, B2, d = _common.make_desc(left, right)
+        for want, got in ((left, A2), (right, B2)):
+            assert not got.is_neg() and torch.equal(got, want)
+        assert (d.L, d.M, d.K, d.N) == (2, 6, left.shape[2], 6)
