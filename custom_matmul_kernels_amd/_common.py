@@ -2,6 +2,7 @@
 strides, promotion of 2-D inputs to a batch of one, argument checks and the
 translation of a pair of tensors into a ``cmk_gemm_desc``."""
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -185,12 +186,15 @@ def float_type(dtype, what):
 
 
 def refuse_grad(*tensors):
-    """The operators for serving have no backward pass: an operand that asks for
-    a gradient is refused, not cut out of the graph in silence."""
+    """The operators for serving have no derivatives: an operand that asks for a
+    gradient, or carries a tangent of forward-mode differentiation (which
+    `requires_grad` does not tell), is refused, not cut out of the graph in silence."""
     for t in tensors:
         if t.requires_grad and torch.is_grad_enabled():
             raise RuntimeError("this operator has no backward pass; call it under torch.no_grad() or "
                                "with detached operands")
+        if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError("this operator has no forward-mode derivative; call it with the primal operands")
 
 
 def call(fn, device, *args):

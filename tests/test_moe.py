@@ -107,3 +107,14 @@ def test_extents_beyond_a_c_int_are_refused():
         for extents in ((large, 32, 4), (64, large, 4), (64, 32, large), (64, large // 2, 4)):
             with pytest.raises(ValueError, match="2\\^31"):
                 layer(*extents)
+
+
+def test_tangents_of_forward_mode_are_refused():
+    import torch.autograd.forward_ad as forward_ad
+    layer = MoECUDA(k=2)
+    for n in range(4):
+        args = list(operands())
+        with forward_ad.dual_level():
+            args[n] = forward_ad.make_dual(args[n], torch.ones_like(args[n]))
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                layer(*args)

@@ -229,3 +229,37 @@ def test_few_rows_take_tiles_where_a_launch_would_wrap_round():
         assert lib.cmk_mx4_workspace_bytes(left, right, 1, m, (1 << 29) - 64, 128) == 0
         assert lib.cmk_mx4_workspace_bytes(left, right, 1, m, (1 << 29) - 63, 128) > 0
         assert lib.cmk_mx4_workspace_bytes(left, right, 1, m, 1 << 29, 128) > 0
+
+
+def test_tangents_of_forward_mode_are_refused():
+    """A dual tensor does not require grad, and its tangent must not be dropped in silence."""
+    import torch.autograd.forward_ad as forward_ad
+    x, w = torch.randn(4, 40), torch.randn(40, 5)
+    product = MX4BMMCUDA()
+    with forward_ad.dual_level():
+        dx, dw = forward_ad.make_dual(x, torch.ones_like(x)), forward_ad.make_dual(w, torch.ones_like(w))
+        assert not dx.requires_grad
+        for args in ((dx, w), (x, dw)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                product(*args)
+        with pytest.raises(AssertionError):                            # not on a device: no tangent, no refusal
+            product(x, w)
+        with pytest.raises(AssertionError):
+            product(forward_ad.unpack_dual(dx).primal, w)
+    with pytest.raises(RuntimeError, match="forward-mode"):
+        torch.func.jvp(lambda v: product(v, w), (x,), (x,))
+
+
+def test_quantisation_refuses_what_has_a_derivative():
+    """(The check of the device comes first without a GPU.)"""
+    import torch.autograd.forward_ad as forward_ad
+    from custom_matmul_kernels_amd import _common
+    x = torch.randn(4, 40)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            _common.refuse_grad(dual)
+        _common.refuse_grad(x)
+    _common.refuse_grad(x)
+    with pytest.raises(RuntimeError, match="backward"):
+        _common.refuse_grad(x.requires_grad_())
