@@ -40,9 +40,9 @@ int check_desc(const cmk_gemm_desc* d) {
   return CMK_OK;
 }
 
-int check_grid(long long work_groups) {
-  if (work_groups + 8 > 0x7fffffffLL)
-    return fail(CMK_ERR_UNSUPPORTED, "problem needs %lld work-groups, more than one grid holds",
+int check_grid(long long work_groups, int threads) {
+  if (!fits_launch(work_groups, threads))
+    return fail(CMK_ERR_UNSUPPORTED, "problem needs %lld work-groups, more than a launch holds",
                 work_groups);
   return CMK_OK;
 }

@@ -291,16 +291,18 @@ __global__ __launch_bounds__(kThreads, 2) void bmm_kernel(BmmArgs a) {
 }
 
 template <bool MASKED, int B = 2>
-static hipError_t launch_bmm(const BmmArgs& a, int transA, int transB, hipStream_t st) {
-  const int total = a.L * ((a.tiles_m + a.run - 1) / a.run) * a.tiles_n;
-  const dim3 grid(((total + 7) / 8) * 8), block(kThreads);
+static int launch_bmm(const BmmArgs& a, int transA, int transB, hipStream_t st, const char* what) {
+  const long long total = (long long)a.L * ((a.tiles_m + a.run - 1) / a.run) * a.tiles_n;
+  const long long padded = (total + 7) / 8 * 8;
+  if (int e = check_grid(padded, kThreads)) return e;
+  const dim3 grid((unsigned)padded), block(kThreads);
   // A "n" is k-contiguous (KC), A "t" is m-contiguous (RC);
   // B "n" is n-contiguous (RC), B "t" is k-contiguous (KC).
   if (!transA && !transB) hipLaunchKernelGGL((bmm_kernel<KC, RC, MASKED, B>), grid, block, 0, st, a);
   else if (!transA && transB) hipLaunchKernelGGL((bmm_kernel<KC, KC, MASKED, B>), grid, block, 0, st, a);
   else if (transA && !transB) hipLaunchKernelGGL((bmm_kernel<RC, RC, MASKED, B>), grid, block, 0, st, a);
   else hipLaunchKernelGGL((bmm_kernel<RC, KC, MASKED, B>), grid, block, 0, st, a);
-  return hipGetLastError();
+  return hip_status(hipGetLastError(), what);
 }
 
 static BmmArgs make_args(const float* A, const float* B, float* C, const cmk_gemm_desc* d, int tile = 128) {
@@ -383,9 +385,8 @@ extern "C" int cmk_bmm_ws_f32(const float* A, const float* B, float* C, const cm
   a.ksplits = s;
   a.klen = klen;
   a.L = d->L * s;
-  if (int e = check_grid((long long)a.L * a.tiles_m * a.tiles_n)) return e;
   hipStream_t st = (hipStream_t)stream;
-  if (int e = hip_status(launch_bmm<false, 1>(a, d->transA, d->transB, st), "cmk_bmm_ws_f32 launch")) return e;
+  if (int e = launch_bmm<false, 1>(a, d->transA, d->transB, st, "cmk_bmm_ws_f32 launch")) return e;
   const long long mn = (long long)d->M * d->N, total = mn * d->L;
   const bool vec = (mn & 3) == 0 && ((reinterpret_cast<uintptr_t>(workspace) | reinterpret_cast<uintptr_t>(C)) & 15) == 0;
   const long long items = vec ? total / 4 : total;
@@ -403,20 +404,17 @@ extern "C" int cmk_bmm_f32(const float* A, const float* B, float* C, const cmk_g
   if (int e = check_desc(d)) return e;
   if (d->L == 0 || d->M == 0 || d->N == 0) return CMK_OK;
   if (!C || (d->K > 0 && (!A || !B))) return fail(CMK_ERR_INVALID_ARG, "cmk_bmm_f32: null pointer");
-  if (int e = check_grid((long long)d->L * ((d->M + 127) / 128) * ((d->N + 127) / 128))) return e;
   BmmArgs a = make_args(A, B, C, d);
   const long long tiles = (long long)d->L * a.tiles_m * a.tiles_n;
   if (tiles < 3 * compute_units()) {
     // too few 128x128 tiles for two even rounds of the chip (measured: up to ~600
     // tiles the smaller tile wins, at 1024 the larger): 64x64 tiles, four times as many
     a = make_args(A, B, C, d, 64);
-    return hip_status(launch_bmm<false, 1>(a, d->transA, d->transB, (hipStream_t)stream),
-                      "cmk_bmm_f32 launch");
+    return launch_bmm<false, 1>(a, d->transA, d->transB, (hipStream_t)stream, "cmk_bmm_f32 launch");
   }
   // longer runs amortise the pipeline fill; keep at least ~4 work-groups per CU
   a.run = tiles >= 8192 ? 4 : (tiles >= 4096 ? 2 : 1);
-  return hip_status(launch_bmm<false>(a, d->transA, d->transB, (hipStream_t)stream),
-                    "cmk_bmm_f32 launch");
+  return launch_bmm<false>(a, d->transA, d->transB, (hipStream_t)stream, "cmk_bmm_f32 launch");
 }
 
 extern "C" int cmk_mbmm_f32(const float* A, const float* B, float* C, const uint8_t* block_mask,
@@ -426,11 +424,10 @@ extern "C" int cmk_mbmm_f32(const float* A, const float* B, float* C, const uint
   if (d->L == 0 || d->M == 0 || d->N == 0) return CMK_OK;
   if (!C || (d->K > 0 && (!A || !B)) || !block_mask || !thread_mask || !element_mask)
     return fail(CMK_ERR_INVALID_ARG, "cmk_mbmm_f32: null pointer");
-  if (int e = check_grid((long long)d->L * ((d->M + 127) / 128) * ((d->N + 127) / 128))) return e;
   BmmArgs a = make_args(A, B, C, d);
   a.block_mask = block_mask;
   a.thread_mask = thread_mask;
   a.element_mask = element_mask;
   a.mask_batched = share_mask ? 0 : 1;
-  return hip_status(launch_bmm<true>(a, d->transA, d->transB, (hipStream_t)stream), "cmk_mbmm_f32 launch");
+  return launch_bmm<true>(a, d->transA, d->transB, (hipStream_t)stream, "cmk_mbmm_f32 launch");
 }

@@ -16,8 +16,12 @@ int hip_status(hipError_t e, const char* what);
 // Validates the fields every GEMM-family entry point shares.
 int check_desc(const cmk_gemm_desc* d);
 
-// A 1-D grid index must fit the hardware limit.
-int check_grid(long long work_groups);
+// A launch holds less than 2^32 threads along an axis; more of them wrap round without
+// an error, and work-groups are missing.
+static inline bool fits_launch(long long work_groups, int threads) { return work_groups <= 0xffffffffLL / threads; }
+
+// The same as a status.
+int check_grid(long long work_groups, int threads = 256);
 
 // 16-byte global loads need an aligned base and strides that keep it aligned.
 static inline int vec_ok(const void* p, long long ld, long long stride) {

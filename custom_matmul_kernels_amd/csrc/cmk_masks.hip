@@ -132,7 +132,7 @@ extern "C" int cmk_derive_masks_u8(const uint8_t* element_mask, uint8_t* block_m
   const int lpr = N > 512 ? 64 : (N > 256 ? 32 : 16);
   a.spans_n = ceil_div(N, lpr * 16);
   const long long groups = (long long)Lm * a.tiles_m * a.spans_n;
-  if (int e = check_grid(groups)) return e;
+  if (int e = check_grid(groups, kMaskThreads)) return e;
   const dim3 grid((unsigned)groups), block(kMaskThreads);
   hipStream_t st = (hipStream_t)stream;
   if (lpr == 64) hipLaunchKernelGGL(derive_masks_kernel<64>, grid, block, 0, st, a);

@@ -898,8 +898,8 @@ size_t min_l2_workspace_bytes(int L, int Xext, int Yext, int K) {
   if ((long long)L * Yext > 0x7fffffffLL) return 0;
   int ys, xt, sp, tps, yg;
   plan_min(L, Xext, Yext, K, &ys, &xt, &sp, &tps, &yg);
-  if ((long long)L * (xt + ys) > 0x7fffffffLL) return 0;
-  if ((long long)L * ceil_div(Xext, 64) * ceil_div(K, 64) > 0x7fffffffLL) return 0;
+  if (!fits_launch((long long)L * (xt + ys), 256)) return 0;
+  if (!fits_launch((long long)L * ceil_div(Xext, 64) * ceil_div(K, 64), 256)) return 0;
   return l2_layout(L, Xext, Yext, K, xt, sp).total;
 }
 
@@ -940,9 +940,10 @@ static int min_bmm_enqueue(const float* A, const float* B, float* values, long l
   a.K = d->K;
   plan_min(d->L, Xext, Yext, d->K, &a.ystrips, &a.xtiles, &a.splits, &a.tiles_per_split, &a.ygroup);
   const long long total = (long long)d->L * a.ystrips * a.splits;
-  if (int e = check_grid(total)) return e;
+  const long long padded = (total + 7) / 8 * 8;
+  if (int e = check_grid(padded, kThreads)) return e;
   a.total = (int)total;
-  const dim3 grid((unsigned)(((total + 7) / 8) * 8)), block(kThreads);
+  const dim3 grid((unsigned)padded), block(kThreads);
   hipStream_t st = (hipStream_t)stream;
   const long long rows = (long long)d->L * Yext;
   const dim3 fold_grid((unsigned)((rows + kFoldThreads - 1) / kFoldThreads)), fold_block(kFoldThreads);
@@ -994,7 +995,7 @@ static int min_bmm_enqueue(const float* A, const float* B, float* values, long l
     hipLaunchKernelGGL(min_l2_fold_kernel, dim3((unsigned)(d->L * ceil_div(Yext, kFoldThreads))), fold_block,
                        0, st, f);
     const long long tiled_grid = (long long)d->L * ceil_div(Xext, kTiledX);
-    if (d->K <= kTiledMaxK && tiled_grid <= 0x7fffffffLL) {
+    if (d->K <= kTiledMaxK && fits_launch(tiled_grid, 256)) {
       hipLaunchKernelGGL(min_l2_rows_tiled_kernel, dim3((unsigned)tiled_grid), dim3(256), 0, st, f);
     } else {
       const int row_parts = ceil_div(Xext, 256) < kRowMaxParts ? ceil_div(Xext, 256) : kRowMaxParts;

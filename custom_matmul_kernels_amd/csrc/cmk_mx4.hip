@@ -753,9 +753,9 @@ static void launch_rows(const Mx4RowsArgs& a, int L, hipStream_t st) {
 }
 
 static bool use_rows(int L, int M, int N, int K) {
-  // What one launch holds: 65535 batches, and less than 2^32 threads along N (work-groups
-  // of 512 threads for 64 columns).
-  if (M > kMx4Rows || L > 65535 || ceil_div(N, 64) * 512LL > 0xffffffffLL) return false;
+  // What one launch holds: 65535 batches, and along N work-groups of 512 threads for 64
+  // columns.
+  if (M > kMx4Rows || L > 65535 || !fits_launch(ceil_div(N, 64), 512)) return false;
   // From 17 rows on the tiles win where there are enough of them (32 rows against
   // 16384 x 8192: 24 us by rows, 14 by tiles; 4096 x 4096: 5.4 and 7.6) or k is long
   // enough to be cut (1024 x 16384: 16 and 8).
@@ -810,11 +810,10 @@ static int check_dtype(const char* who, int dtype) {
   return CMK_OK;
 }
 
-// A launch holds less than 2^32 threads; more of them wrap round without an error.
 constexpr int kThreads = 256;
 
 static int check_launch(const char* who, long long groups) {
-  if (groups > 0xffffffffLL / kThreads)
+  if (!fits_launch(groups, kThreads))
     return fail(CMK_ERR_UNSUPPORTED, "%s: needs %lld work-groups, more than a launch holds", who, groups);
   return CMK_OK;
 }

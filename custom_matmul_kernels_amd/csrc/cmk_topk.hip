@@ -185,7 +185,11 @@ extern "C" int cmk_topk_bmm_f32(const float* A, const float* B, float* values, l
     a.part = static_cast<entry_t*>(workspace);
   }
   const long long total = (long long)d->L * a.ystrips * a.splits;
-  if (int e = check_grid(total)) return e;
+  const long long rows = (long long)d->L * Yext;
+  if (total > 0x7fffffffLL - 8)
+    return fail(CMK_ERR_UNSUPPORTED, "cmk_topk_bmm_f32: problem needs %lld work items, at most 2^31 - 9 are supported", total);
+  if (a.splits > 1)
+    if (int e = check_grid((rows + 3) / 4, kThreads)) return e;
   // one sixteen-wave work-group per CU is resident at a time; a grid of two per CU evens out the tail
   const long long padded = ((total + 7) / 8) * 8;
   const long long machine = 2ll * compute_units();
@@ -198,8 +202,6 @@ extern "C" int cmk_topk_bmm_f32(const float* A, const float* B, float* values, l
   else launch_topk_dist(distance, xk, yk, multi, grid, block, st, a);
   if (int e = hip_status(hipGetLastError(), "cmk_topk_bmm_f32 launch")) return e;
   if (a.splits > 1) {
-    const long long rows = (long long)d->L * Yext;
-    if (int e = check_grid((rows + 3) / 4)) return e;
     hipLaunchKernelGGL(topk_merge_kernel, dim3((unsigned)((rows + 3) / 4)), dim3(kThreads), 0, st,
                        a.part, values, indices, rows, a.splits, k);
     if (int e = hip_status(hipGetLastError(), "cmk_topk_bmm_f32 merge launch")) return e;

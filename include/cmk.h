@@ -36,7 +36,9 @@ extern "C" {
 
 #define CMK_OK                 0
 #define CMK_ERR_INVALID_ARG   -1   /* bad shape / dim / k / null pointer          */
-#define CMK_ERR_UNSUPPORTED   -2   /* valid request that this build does not do   */
+#define CMK_ERR_UNSUPPORTED   -2   /* valid request that this build does not do;
+                                      2^24 work-groups of 256 threads and more,
+                                      which one launch does not hold, are one    */
 #define CMK_ERR_WORKSPACE     -3   /* workspace missing or too small              */
 
 /* operation ids for cmk_workspace_bytes() */

@@ -126,3 +126,22 @@ def test_check_maps_codes_to_exceptions(lib):
     with pytest.raises(_lib.CmkError):
         _lib.check(_lib.ERR_WORKSPACE)
     _lib.check(0)
+
+
+def test_more_than_a_launch_holds_is_refused():
+    """2^24 work-groups of 256 threads are 2^32 threads, which wrap round in a launch and
+    leave results unwritten."""
+    lib = _lib.load()
+    p = ctypes.c_void_p(0x1000)           # never dereferenced
+    l = 1 << 24
+    d = _lib.GemmDesc(l, 1, 1, 4, 0, 0, 4, 4, 4, 4)
+    assert lib.cmk_bmm_f32(p, p, p, d, None) == _lib.ERR_UNSUPPORTED
+    assert b"more than a launch holds" in lib.cmk_last_error()
+    assert lib.cmk_bmm_ws_f32(p, p, p, d, None, 0, None) == _lib.ERR_UNSUPPORTED
+    assert lib.cmk_mbmm_f32(p, p, p, p, p, p, 0, d, None) == _lib.ERR_UNSUPPORTED
+    for distance in (_lib.DIST_INNER, _lib.DIST_L2, _lib.DIST_L1):
+        for dim in (1, 2):
+            need = lib.cmk_workspace_bytes(_lib.OP_MIN_BMM_L2, l, 1, 1, 4, dim)
+            assert need == 0                                      # no screening of that many
+            assert lib.cmk_min_bmm_f32(p, p, p, p, d, dim, distance, p, 1 << 40, None) == _lib.ERR_UNSUPPORTED
+    assert lib.cmk_derive_masks_u8(p, p, p, l, 1, 1, None) == _lib.ERR_UNSUPPORTED
