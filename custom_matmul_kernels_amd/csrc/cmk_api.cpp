@@ -28,6 +28,8 @@ int check_desc(const cmk_gemm_desc* d) {
   if (d->L < 0 || d->M < 0 || d->N < 0 || d->K < 0)
     return fail(CMK_ERR_INVALID_ARG, "negative dimension (L=%d M=%d N=%d K=%d)", d->L, d->M, d->N,
                 d->K);
+  if (d->M > kMaxExtent || d->N > kMaxExtent || d->K > kMaxExtent)
+    return fail(CMK_ERR_UNSUPPORTED, "extents are at most %d (M=%d N=%d K=%d)", kMaxExtent, d->M, d->N, d->K);
   if ((d->transA != 0 && d->transA != 1) || (d->transB != 0 && d->transB != 1))
     return fail(CMK_ERR_INVALID_ARG, "transA/transB must be 0 or 1");
   const long long min_lda = d->transA ? d->M : d->K;
@@ -70,6 +72,7 @@ size_t topk1d_workspace_bytes(long long n);
 
 extern "C" size_t cmk_workspace_bytes(int op, int L, int M, int N, int K, int dim) {
   if (L < 0 || M < 0 || N < 0) return 0;
+  if (op != CMK_OP_TOPK_1D && (M > cmk::kMaxExtent || N > cmk::kMaxExtent || K > cmk::kMaxExtent)) return 0;
   switch (op) {
     case CMK_OP_BMM:
       return cmk::bmm_workspace_bytes(L, M, N, K);

@@ -28,7 +28,10 @@ static inline int vec_ok(const void* p, long long ld, long long stride) {
   return ((reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld & 3) == 0 && (stride & 3) == 0) ? 1 : 0;
 }
 
-static inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
+static inline int ceil_div(int a, int b) { return (int)(((long long)a + b - 1) / b); }
+
+// Extents are rounded up to whole tiles in ints.
+constexpr int kMaxExtent = 0x7fffffff - 1023;
 
 // Compute units of the current device (cached per device).
 int compute_units();

@@ -114,6 +114,8 @@ extern "C" int cmk_derive_masks_u8(const uint8_t* element_mask, uint8_t* block_m
                                    uint8_t* thread_mask, int Lm, int M, int N, void* stream) {
   if (Lm < 0 || M < 0 || N < 0)
     return fail(CMK_ERR_INVALID_ARG, "cmk_derive_masks_u8: negative extent (Lm=%d M=%d N=%d)", Lm, M, N);
+  if (M > kMaxExtent || N > kMaxExtent)
+    return fail(CMK_ERR_UNSUPPORTED, "extents are at most %d (M=%d N=%d)", kMaxExtent, M, N);
   if (Lm == 0 || M == 0 || N == 0) return CMK_OK;
   if (!element_mask || !block_mask || !thread_mask)
     return fail(CMK_ERR_INVALID_ARG, "cmk_derive_masks_u8: null pointer");

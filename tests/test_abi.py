@@ -145,3 +145,22 @@ def test_more_than_a_launch_holds_is_refused():
             assert need == 0                                      # no screening of that many
             assert lib.cmk_min_bmm_f32(p, p, p, p, d, dim, distance, p, 1 << 40, None) == _lib.ERR_UNSUPPORTED
     assert lib.cmk_derive_masks_u8(p, p, p, l, 1, 1, None) == _lib.ERR_UNSUPPORTED
+
+
+def test_extents_that_cannot_be_rounded_up_are_refused():
+    """Extents are rounded up to whole tiles in ints, on the host and in the kernels."""
+    lib = _lib.load()
+    p = ctypes.c_void_p(0x1000)           # never dereferenced
+    for large in ((1 << 31) - 1, (1 << 31) - 127):
+        for m, n, k in ((large, 1, 1), (1, large, 1), (1, 1, large)):
+            d = _lib.GemmDesc(1, m, n, k, 0, 0, k, n, 0, 0)
+            assert lib.cmk_bmm_f32(p, p, p, d, None) == _lib.ERR_UNSUPPORTED
+            assert b"extents are at most" in lib.cmk_last_error()
+            assert lib.cmk_bmm_ws_f32(p, p, p, d, p, 1 << 40, None) == _lib.ERR_UNSUPPORTED
+            assert lib.cmk_mbmm_f32(p, p, p, p, p, p, 0, d, None) == _lib.ERR_UNSUPPORTED
+            assert lib.cmk_min_bmm_f32(p, p, p, p, d, 2, 0, p, 1 << 40, None) == _lib.ERR_UNSUPPORTED
+            assert lib.cmk_topk_bmm_f32(p, p, p, p, d, 2, 5, 0, p, 1 << 40, None) == _lib.ERR_UNSUPPORTED
+            for op in range(4):
+                lib.cmk_workspace_bytes(op, 1, m, n, k, 1)         # any answer: the call is refused
+        assert lib.cmk_derive_masks_u8(p, p, p, 1, 1, large, None) == _lib.ERR_UNSUPPORTED
+        assert lib.cmk_derive_masks_u8(p, p, p, 1, large, 1, None) == _lib.ERR_UNSUPPORTED
