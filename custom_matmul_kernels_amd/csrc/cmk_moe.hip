@@ -1195,8 +1195,18 @@ extern "C" int cmk_moe(const void* x, const void* router, const void* gate_up, c
     hipLaunchKernelGGL(kernel, dim3(ceil_div(rows, 16 * rg * kMoeWaves / ks), units), dim3(64 * kMoeWaves), 0, st, a);
   };
   const bool many = units >= 32;
-  // six tokens an expert and enough rows for every compute unit
-  const bool dense = d->T * d->k >= 6 * d->E && (long long)d->E * std::min(d->H, d->I) >= 64LL * compute_units();
+  // Whether k is walked with the activations in a ring (no and yes, us; slots an expert in
+  // brackets).  4 bits: 64 experts x 2048 x 1024 (4) 68 and 74, (6) 72 and 75, (8) 76 and
+  // 76, (12) 90 and 85; 32 x 1024 x 1024 (6) 43 and 37; 8 x 4096 x 4096 (4) 75 and 80, (6)
+  // 82 and 81, (8) 88 and 81, (16) 121 and 91; 8 x 512 x 2048 (6) 30 and 33, (10) 34 and
+  // 33; 4 x 512 x 512 (16) 25 and 24.
+  // 16 bits read four times as much and lose more to the barrier of a slab, most where
+  // rows are few: 8 x 4096 x 4096 (8) 184 and 192, (12) 199 and 199, (16) 230 and 198; 64 x
+  // 2048 x 1024 (8) 172 and 189, (16) 202 and 199; 32 x 1024 x 1024 (8) 63 and 61, (12) 69
+  // and 64; but 32 x 512 x 512 (16) 43 and 44, 8 x 2048 x 2048 (16) 77 and 78, (32) 111 and
+  // 120, 4 x 1024 x 1024 (32) 46 and 62.
+  const bool dense = four ? d->T * d->k >= (many ? 6 : 8) * d->E
+                          : d->T * d->k >= 12 * d->E && (long long)d->E * std::min(d->H, d->I) >= 128LL * compute_units();
   auto dense_kernel = [&](auto kernel, int rows, int rg) {
     hipLaunchKernelGGL(kernel, dim3(ceil_div(rows, 16 * rg * kMoeWaves), units), dim3(64 * kMoeWaves), 0, st, a);
   };

@@ -326,7 +326,7 @@ def test_many_tokens_of_many_experts_in_four_bits(device, t, h, i, e, k, dtype):
     check(MoECUDA(k=k), *make(t, h, i, e, dtype, t + h + i), device, True)
 
 
-def exact_layer(t, four_bit, e=4, h=512, i=512):
+def exact_layer(t, e, h, i):
     """Operands (bf16) whose layer has an exact result, and that result in float64.
 
     g = 32 for every inner feature: 1 + exp(-32) is 1 in fp32, so silu(g) = 32 there.
@@ -354,13 +354,15 @@ def exact_layer(t, four_bit, e=4, h=512, i=512):
     return x, torch.zeros(e, h), gate_up, down, y
 
 
-# one token; planes in one and in two fragments of their own; one and two blocks of slots; passes
-@pytest.mark.parametrize("t,e", [(1, 4), (2, 4), (5, 4), (6, 4), (10, 4), (11, 4), (16, 40), (25, 4), (40, 40), (100, 32)])
+# one token; planes in one and in two fragments of their own; one and two blocks of slots;
+# passes; the ring of activations
+@pytest.mark.parametrize("t,e,size", [(1, 4, 512), (2, 4, 512), (5, 8, 512), (6, 4, 512), (10, 8, 512), (11, 8, 512), (16, 40, 512),
+                                      (25, 4, 512), (25, 16, 512), (40, 40, 512), (100, 32, 512), (200, 32, 1024), (240, 33, 1000)])
 @pytest.mark.parametrize("four_bit", [False, True])
 @pytest.mark.parametrize("dtype", [BF16, F16])
-def test_inner_values_keep_their_24_bits(device, t, e, four_bit, dtype):
-    x, router, gate_up, down, want = exact_layer(t, four_bit, e)
-    print("exact layer", t, e, four_bit, dtype, flush=True)
+def test_inner_values_keep_their_24_bits(device, t, e, size, four_bit, dtype):
+    x, router, gate_up, down, want = exact_layer(t, e, size, size)
+    print("exact layer", t, e, size, four_bit, dtype, flush=True)
     args = [v.to(dtype).to(device) for v in (x, router, gate_up, down)]
     for v, w in zip((x, gate_up, down), (args[0], args[2], args[3])):
         assert torch.equal(w.cpu().float(), v)
@@ -374,7 +376,7 @@ def test_inner_values_keep_their_24_bits(device, t, e, four_bit, dtype):
     assert torch.equal(y.cpu(), want.to(dtype))
 
 
-@pytest.mark.parametrize("t,e", [(1, 4), (4, 4), (14, 4), (20, 4), (40, 40), (100, 32)])
+@pytest.mark.parametrize("t,e", [(1, 4), (4, 8), (14, 8), (20, 4), (20, 16), (40, 40), (100, 32)])
 @pytest.mark.parametrize("four_bit", [False, True])
 def test_inner_values_at_the_end_of_the_range(device, t, e, four_bit):
     """2^128 (1 - 2^-12) is finite, and the nearest bf16 is not: g = 2^64, up 2^64 - 2^52."""
@@ -392,34 +394,63 @@ def test_inner_values_at_the_end_of_the_range(device, t, e, four_bit):
     assert (y == 2.0 ** 28).all()        # 2^28 (1 - 2^-12), rounded
 
 
-def grouped(sizes, h, i, e, dtype, seed):
-    """A layer whose expert j is the choice of sizes[j] tokens, in a shuffled order."""
-    x, router, gate_up, down = make(sum(sizes), h, i, e, dtype, seed)
-    choice = torch.cat([torch.full((n,), j) for j, n in enumerate(sizes)])
-    choice = choice[torch.randperm(len(choice), generator=torch.Generator().manual_seed(seed))]
-    x[:, :e] = 0
-    x[torch.arange(len(choice)), choice] = 6
-    router[:, :e] = 8 * torch.eye(e)
-    return x, router, gate_up, down, choice
+def check_grouped(sizes, h, i, e, dtype, four_bit, device):
+    """A layer of e experts whose expert j is the choice of sizes[j] tokens, in a shuffled
+    order; the other experts (zeros) are nobody's."""
+    print("grouped", sizes, h, i, e, dtype, four_bit, flush=True)
+    n, t = len(sizes), sum(sizes)
+    x, router, gate_up, down = make(t, h, i, n, dtype, h + i)
+    choice = torch.cat([torch.full((s,), j) for j, s in enumerate(sizes)])
+    choice = choice[torch.randperm(t, generator=torch.Generator().manual_seed(h))]
+    x[:, :n] = 0
+    x[torch.arange(t), choice] = 6
+    router[:, :n] = 8 * torch.eye(n)
+    def padded(v):
+        return torch.cat([v.to(device), torch.zeros((e - n,) + v.shape[1:], dtype=dtype, device=device)])
+    args = [x.to(device), padded(router), padded(gate_up), padded(down)]
+    if four_bit:
+        args[2:] = [quantize_mx4(v) for v in args[2:]]
+        gate_up, down = _mx4.rounded(gate_up), _mx4.rounded(down)
+    y, weights, experts = MoECUDA(k=1)(*args)
+    assert torch.equal(experts.cpu()[:, 0], choice) and (weights == 1).all()
+    want, dy, _, _, chosen = reference(x, router, gate_up, down, 1, "silu", True)
+    assert torch.equal(chosen[:, 0], choice)
+    fi = torch.finfo(dtype)
+    off = (y.cpu().double() - want).abs()
+    assert (off <= dy + (want.abs() + dy) * fi.eps / 2 + fi.smallest_normal * fi.eps).all()
 
 
 # Slots of an expert decide how its rows are multiplied: planes packed in one fragment of
 # columns (up to 5) or two (up to 10), blocks of 16 and of 32, passes of 32; the extents
 # decide in how many pieces k goes through LDS, and by how many waves.
 @pytest.mark.parametrize("sizes,h,i,e", [
-    ((5, 9, 14, 27, 40), 1700, 1700, 5),     # few experts: waves share k in both products
-    ((5, 9, 14, 27, 40), 3700, 300, 5),
-    ((4, 10, 16, 32, 33), 300, 3700, 6),
+    ((5, 9, 14, 27, 40), 1700, 1700, 16),    # few experts: waves share k in both products
+    ((5, 9, 14, 27, 40), 3700, 300, 16),
+    ((4, 10, 16, 32, 33), 300, 3700, 16),
     ((6, 2), 4200, 1400, 9),                 # fewer slots than experts
     ((5, 9, 14, 27, 40), 520, 1300, 33),     # more than 32 experts: rows of their own
     ((4, 8, 16, 32, 49), 2300, 260, 33),
+    ((5, 9, 14, 27, 40), 1100, 700, 5),      # the ring of activations in 4 bits
+    ((3, 17, 33, 64), 130, 1500, 4),
 ])
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("four_bit", [False, True])
 def test_experts_of_every_size(device, sizes, h, i, e, dtype, four_bit):
-    x, router, gate_up, down, choice = grouped(sizes, h, i, e, dtype, h + i)
-    got = check(MoECUDA(k=1), x, router, gate_up, down, device, four_bit)
-    assert torch.equal(got[2].cpu()[:, 0], choice)
+    check_grouped(sizes, h, i, e, dtype, four_bit, device)
+
+
+@pytest.mark.parametrize("t,h,i,e,k", [(200, 1024, 1100, 32, 2), (240, 821, 830, 40, 2)])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_many_tokens_of_many_large_experts(device, t, h, i, e, k, dtype):
+    """The ring of activations in 16 bits, one and two groups of rows a wave; four experts
+    are most tokens' choice, the others have a few slots."""
+    x, router, gate_up, down = make(t, h, i, e, dtype, t)
+    check(MoECUDA(k=k), x, router, gate_up, down, device, False)
+    x[:, 0] = 2
+    router[:4, 0] = 2
+    got = check(MoECUDA(k=k), x, router, gate_up, down, device, False)
+    count = got[2].flatten().bincount(minlength=e)
+    assert count.max() > 64 and 0 < count[4:].max() <= 16
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
