@@ -263,7 +263,9 @@ __global__ __launch_bounds__(256) void moe_select_kernel(MoeArgs a) {
 // Router and choice in one launch, for a router of few tiles: a work-group takes 16
 // tokens, a wave one of the units of 16 experts x one slab, then a token.  (7 tokens,
 // 10 experts, H = 1000, 8 units: 6.4 us, as two launches 4.2 + 3.6 and one more call on
-// the host; 32 units: 19 us, 5 + 4 apart.)
+// the host; a whole layer of 4 tokens and 64 inner features in two launches and in one: 8
+// units 19.9 and 19.9 us, 10 units 21.0 and 22.4, 12 units 21.6 and 23.0, 16 units 22.8 and
+// 25.6.)
 constexpr int kSmallUnits = 8, kSmallExperts = 128;
 
 static bool small_router(int E, int Hp) { return E <= kSmallExperts && (E + 15) / 16 * (Hp / kSlab) <= kSmallUnits; }
@@ -1194,6 +1196,11 @@ extern "C" int cmk_moe(const void* x, const void* router, const void* gate_up, c
   auto experts_kernel = [&](auto kernel, int rows, int rg, int ks) {
     hipLaunchKernelGGL(kernel, dim3(ceil_div(rows, 16 * rg * kMoeWaves / ks), units), dim3(64 * kMoeWaves), 0, st, a);
   };
+  // Whether waves take rows of their own, or share k (gate and up in 16 bits always do).
+  // Shared and own, us: 4 bits, 2048 x 1024, 16 units 30 and 36, 32 units 37 and 40 with
+  // one slot each, 51 and 48 with four, 64 units 53 and 51; 4096 x 1280, 16 units 57 and
+  // 59, 32 units 60 and 60, 86 and 77; 16 bits, 2048 x 1024, 16 units 47 and 47, 32 units
+  // 72 and 72, 64 units 113 and 111.
   const bool many = units >= 32;
   // Whether k is walked with the activations in a ring (no and yes, us; slots an expert in
   // brackets).  4 bits: 64 experts x 2048 x 1024 (4) 68 and 74, (6) 72 and 75, (8) 76 and
