@@ -105,7 +105,10 @@ struct DequantArgs {
 // before and what runs next keep their lines (dequantisation of 8192 x 8192 to bf16
 // 40 -> 34 us and the quantisation in front of it 38 -> 33; a product with 512 MB of
 // results 116 -> 119 us, the quantisation of the next call's operands 62 -> 24).  Only
-// where rows are whole cache lines: partial lines are merged by the L2 alone.
+// where rows are whole cache lines: partial lines are merged by the L2 alone.  (The
+// inverse down columns stores 1 KB of a row at a time in fp32 and gains at any width: 3 x
+// 4096 x 4095 there and back 111 -> 98 us; in 16 bits 8192 x 8192 92 -> 89, 8192 x 8190
+// would lose, 100 -> 106.)
 constexpr size_t kStreamBytes = 32u << 20;
 
 static int streams(const void* out, long long rows, long long row_bytes) {
@@ -880,7 +883,9 @@ extern "C" int cmk_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, v
   DequantArgs a{codes, scales, out, L, R, K, mx4_slabs(K), 0, 0};
   // four rows a lane where a wave's 256 rows are there
   const int v = rows_innermost && R >= 256 ? 4 : 1;
-  const bool past = rows_innermost ? (size_t)L * R * K * size >= kStreamBytes && v == 4 : streams(out, (long long)L * R, (long long)K * size);
+  const bool large = (size_t)L * R * K * size >= kStreamBytes;
+  const bool past = !rows_innermost ? streams(out, (long long)L * R, (long long)K * size)
+                                    : v == 4 && (size == 4 ? large : streams(out, (long long)L * K, (long long)R * size));
   a.row_groups = rows_innermost ? ((long long)R + 64 * v - 1) / (64 * v) : ((long long)R + 15) / 16;
   a.groups = a.row_groups * a.slabs * L;
   const long long grid = (a.groups + 3) / 4;
