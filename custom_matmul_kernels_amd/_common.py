@@ -58,7 +58,10 @@ def check_operands(A, B):
     assert A.dtype == B.dtype
     if A.dtype != torch.float32:
         raise TypeError("only torch.float32 operands are supported, got %s" % A.dtype)
-    check_extents(*A.shape, B.shape[2])
+    l, m, k = A.shape
+    n = B.shape[2]
+    if l | m | k | n > MAX_EXTENT:
+        check_extents(l, m, k, n)
     assert A.device.type == B.device.type == "cuda"
     assert A.device == B.device
 
@@ -66,7 +69,8 @@ def check_operands(A, B):
 def _operand(T, want_inner, name):
     """Returns (tensor, trans, ld, batch_stride) for one [l, r, c] operand.
     A tensor whose strides fit neither layout is copied to row-major."""
-    T = with_own_sign(T)
+    if T.is_neg():
+        T = with_own_sign(T)
     l, r, c = T.shape
     s0, s1, s2 = T.stride()
     # an axis of extent 1 can carry any stride; treat it as the natural one

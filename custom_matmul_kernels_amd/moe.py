@@ -2,6 +2,7 @@
 experts' products and their weighted sum.  No counterpart in the reference; the
 router is a top-k of a product and the experts are a routed batched product."""
 import torch
+from torch.autograd import forward_ad
 
 from . import _common, _lib
 from .mx4 import MX4Tensor
@@ -41,20 +42,24 @@ class MoECUDA:
 
     @staticmethod
     def _experts(W, shape, dtype, name):
-        """(pointer, scales' pointer, row stride, expert stride) of [e, r, c] weights."""
+        """[e, r, c] weights, to be kept until the launch, and their (pointer, scales'
+        pointer, row stride, expert stride)."""
         if isinstance(W, MX4Tensor):
             assert W.shape == shape
             assert W.k_axis == -1, "the blocks of %s must run along its last axis" % name
-            return W._pointers() + (0, 0)
+            return W, W._pointers() + (0, 0)
         if W.dtype != dtype:
             raise TypeError("%s must be an MX4Tensor or of x's type, got %s" % (name, W.dtype))
         assert W.shape == shape
-        _common.refuse_grad(W)
+        if W.requires_grad or forward_ad._current_level >= 0:
+            _common.refuse_grad(W)
+        if W.is_neg():
+            W = _common.with_own_sign(W)
         e, r, c = shape
         s0, s1, s2 = W.stride()
         if (s2 != 1 and c > 1) or (s1 < c and r > 1):
             raise ValueError("the last axis of %s must be contiguous" % name)
-        return W.data_ptr(), None, s1 if r > 1 else c, s0 if e > 1 else 0
+        return W, (W.data_ptr(), None, s1 if r > 1 else c, s0 if e > 1 else 0)
 
     def __call__(self, x, router, gate_up, down):
         dtype, device = x.dtype, x.device
@@ -64,11 +69,6 @@ class MoECUDA:
             raise TypeError("router must be torch.float32 or of x's type, got %s" % router.dtype)
         if x.dim() != 2 or router.dim() != 2 or gate_up.dim() != 3 or down.dim() != 3:
             raise ValueError("x and router need to be 2d, gate_up and down 3d")
-        x, router = _common.with_own_sign(x), _common.with_own_sign(router)
-        if not isinstance(gate_up, MX4Tensor):
-            gate_up = _common.with_own_sign(gate_up)
-        if not isinstance(down, MX4Tensor):
-            down = _common.with_own_sign(down)
         t, h = x.shape
         e, two_i, _ = gate_up.shape
         i = two_i // 2
@@ -77,12 +77,15 @@ class MoECUDA:
         assert 0 < self.k <= e
         if e | two_i | h > _common.MAX_EXTENT:
             _common.check_extents(e, two_i, h)
-        _common.refuse_grad(x, router)
-        gp, gs, ldg, sg = self._experts(gate_up, (e, two_i, h), dtype, "gate_up")
-        dp, ds, ldd, sd = self._experts(down, (e, h, i), dtype, "down")
+        if x.requires_grad or router.requires_grad or forward_ad._current_level >= 0:
+            _common.refuse_grad(x, router)
+        gate_up, (gp, gs, ldg, sg) = self._experts(gate_up, (e, two_i, h), dtype, "gate_up")
+        down, (dp, ds, ldd, sd) = self._experts(down, (e, h, i), dtype, "down")
         assert (gs is None) == (ds is None), "gate_up and down must be of one kind"
         assert device.type == "cuda"
         assert router.device == device and gate_up.device == device and down.device == device
+        if x.is_neg() or router.is_neg():
+            x, router = _common.with_own_sign(x), _common.with_own_sign(router)
         sx, sr = x.stride(), router.stride()
         if h > 1 and sx[1] != 1 or t > 1 and sx[0] < h:
             x = x.contiguous()

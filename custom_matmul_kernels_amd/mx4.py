@@ -2,6 +2,7 @@
 the batched product on the matrix pipe's scaled instructions.  No counterpart in
 the reference, whose products are fp32; the class stands beside BMMCUDA."""
 import torch
+from torch.autograd import forward_ad
 
 from . import _common, _lib
 
@@ -143,7 +144,8 @@ def quantize_mx4(T, dim=-1):
     scale, is one of the last two: -1 for the left operand of a product, -2 for
     the right one."""
     dtype = _common.float_type(T.dtype, "the tensor")
-    T = _common.with_own_sign(T)
+    if T.is_neg():
+        T = _common.with_own_sign(T)
     shape, stride, device = T.shape, T.stride(), T.device
     n = len(shape)
     if n not in (2, 3):
@@ -155,7 +157,8 @@ def quantize_mx4(T, dim=-1):
     if l | rows | k > _common.MAX_EXTENT:
         _common.check_extents(l, rows, k)
     assert device.type == "cuda"
-    _common.refuse_grad(T)
+    if T.requires_grad or forward_ad._current_level >= 0:
+        _common.refuse_grad(T)
     units = l * -(-k // SLAB) * rows
     storage = torch.empty(units * (SLAB // 2 + SLAB // BLOCK), dtype=torch.uint8, device=device)
     if units:
@@ -181,14 +184,18 @@ class MX4BMMCUDA:
 
     @staticmethod
     def _operand(T, k_axis, name):
-        """The library's description of an operand [l, rows, k] with k at `k_axis`."""
+        """The operand [l, rows, k] with k at `k_axis`, to be kept until the launch, and the
+        library's description of it."""
         if isinstance(T, MX4Tensor):
             assert T.k_axis == k_axis, "the blocks of %s must run along k" % name
-            return _lib.Mx4Operand(*T._pointers(), _lib.MX4)
+            return T, _lib.Mx4Operand(*T._pointers(), _lib.MX4)
         dtype = _common.float_type(T.dtype, name)
-        _common.refuse_grad(T)
+        if T.requires_grad or forward_ad._current_level >= 0:
+            _common.refuse_grad(T)
+        if T.is_neg():
+            T = _common.with_own_sign(T)
         stride = T.stride()
-        return _lib.Mx4Operand(T.data_ptr(), None, dtype, 0, stride[0] if len(stride) == 3 else 0,
+        return T, _lib.Mx4Operand(T.data_ptr(), None, dtype, 0, stride[0] if len(stride) == 3 else 0,
                                stride[-3 - k_axis], stride[k_axis])
 
     def __call__(self, A, B):
@@ -197,11 +204,8 @@ class MX4BMMCUDA:
         assert len(sb) == n
         if n not in (2, 3):
             raise ValueError("A and B need to be 2d or 3d")
-        if not isinstance(A, MX4Tensor):
-            A = _common.with_own_sign(A)
-        if not isinstance(B, MX4Tensor):
-            B = _common.with_own_sign(B)
-        a, b = self._operand(A, -1, "A"), self._operand(B, -2, "B")
+        A, a = self._operand(A, -1, "A")
+        B, b = self._operand(B, -2, "B")
         m, k = sa[-2:]
         c = sb[-1]
         l = 1 if n == 2 else sa[0]
