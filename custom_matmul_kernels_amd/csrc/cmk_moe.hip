@@ -833,7 +833,7 @@ __global__ __launch_bounds__(64 * kMoeWaves, 3) void moe_down_kernel(MoeArgs a) 
 
 // Where experts have many tokens each, the activations of a pass do not fit LDS and
 // staging them in pieces leaves the memory idle between them (8 experts of 4096 x
-// 4096, 64 tokens: 255 us in bf16, 151 in 4 bits).  These kernels walk k with a ring
+// 4096, 64 tokens: 230 us in bf16, 121 in 4 bits; as here 195 and 86).  These kernels walk k with a ring
 // of S slabs of activations in LDS, fetched by direct loads, and the weights in the
 // register ring as before; the four waves take rows of their own.  Within a row the 16
 // blocks of 16 bytes of a slab are stored at position block ^ (row & 15), so that the
@@ -848,7 +848,10 @@ __device__ __forceinline__ void moe_dense_products(f32x4 (&acc)[M][RG][NB], cons
   constexpr int kStage = NB * 16 * PLANES * 2 * kSlab;
   constexpr int kActs = NB * PLANES;                               // requests of a wave per slab of activations,
   constexpr int kWeights = M * RG * (WF == CMK_MX4 ? 2 : 4);       // and of weights
-  static_assert(U <= S - 1 && (S - 2) * kActs + U * kWeights < 64, "the count of requests under way");
+  // What has been requested behind a slab's activations when they are awaited: those of S
+  // - 2 more slabs, and weights in the S - 1 slabs of the loop since (at first, of U slabs).
+  constexpr int kBehind = (S - 2) * kActs + std::min(U, S - 1) * kWeights;
+  static_assert(kBehind < 64, "the count of requests under way");
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, q = lane >> 4;
   const int slabs = (K + kSlab - 1) / kSlab;
@@ -883,12 +886,11 @@ __device__ __forceinline__ void moe_dense_products(f32x4 (&acc)[M][RG][NB], cons
     for (int u = 0; u < U; ++u) {
       const int s = s0 + u;
       if (s >= slabs) break;
-      // Requests are awaited in the order of their issue.  Behind this slab's
-      // activations those of S - 2 more and weights of at least U slabs have been
-      // requested; near the end, where they have not (or the last, shorter slab of
-      // weights takes fewer instructions), everything is awaited.
+      // Requests are awaited in the order of their issue.  Near the end, where fewer are
+      // behind (or the last, shorter slab of weights takes fewer instructions), everything
+      // is awaited.
       asm volatile("" ::: "memory");
-      if (s + S - 1 < slabs) wait_loads<(S - 2) * kActs + U * kWeights>();
+      if (s + std::max(U, S - 1) < slabs) wait_loads<kBehind>();
       else wait_loads<0>();
       wait_lds();
       meet();
@@ -1218,8 +1220,9 @@ extern "C" int cmk_moe(const void* x, const void* router, const void* gate_up, c
     hipLaunchKernelGGL(kernel, dim3(ceil_div(rows, 16 * rg * kMoeWaves), units), dim3(64 * kMoeWaves), 0, st, a);
   };
   // The down products take as few groups of 16 rows a wave as let all work-groups run at
-  // once, two a compute unit.  One, two and four groups: 4 bits, 8 experts x 4096 x 4096,
-  // 64 tokens 91, 95, 126 us; 8 x 5000 x 5000, 48 tokens 149, 125, 152; 16 x 6144 x 2048,
+  // once, two a compute unit, and then ask for weights as far ahead as registers hold (4
+  // bits, one group: four slabs 86 us, two 91).  One, two and four groups of two, two and
+  // one slabs: 4 bits, 8 experts x 4096 x 4096, 64 tokens 91, 95, 126 us; 8 x 5000 x 5000, 48 tokens 149, 125, 152; 16 x 6144 x 2048,
   // 128 tokens 130, 120, 116; 64 x 2048 x 1024, 256 tokens 158, 142, 139.  One and two,
   // 16 bits: 8 x 4096 x 4096, 64 tokens 197 and 199; 64 x 2048 x 1024, 256 tokens 306 and 296.
   auto all_at_once = [&](int rg) { return d->E * ceil_div(d->H, 16 * rg * kMoeWaves) <= 2 * compute_units(); };
@@ -1227,17 +1230,17 @@ extern "C" int cmk_moe(const void* x, const void* router, const void* gate_up, c
     if (d->w_dtype == CMK_MX4) {
       if (p.x_planes == 1) dense_kernel(moe_gate_up_dense_kernel<CMK_MX4, 1, 1, 3>, p.Ip, 1);
       else dense_kernel(moe_gate_up_dense_kernel<CMK_MX4, 2, 1, 3>, p.Ip, 1);
-      if (all_at_once(1)) dense_kernel(moe_down_dense_kernel<CMK_MX4, 1, 2>, d->H, 1);
-      else if (all_at_once(2)) dense_kernel(moe_down_dense_kernel<CMK_MX4, 2, 2>, d->H, 2);
+      if (all_at_once(1)) dense_kernel(moe_down_dense_kernel<CMK_MX4, 1, 4>, d->H, 1);
+      else if (all_at_once(2)) dense_kernel(moe_down_dense_kernel<CMK_MX4, 2, 4>, d->H, 2);
       else dense_kernel(moe_down_dense_kernel<CMK_MX4, 4, 1>, d->H, 4);
     } else if (d->w_dtype == CMK_BF16) {
       dense_kernel(moe_gate_up_dense_kernel<CMK_BF16, 1, 1, 2>, p.Ip, 1);
-      if (all_at_once(1)) dense_kernel(moe_down_dense_kernel<CMK_BF16, 1, 2>, d->H, 1);
-      else dense_kernel(moe_down_dense_kernel<CMK_BF16, 2, 2>, d->H, 2);
+      if (all_at_once(1)) dense_kernel(moe_down_dense_kernel<CMK_BF16, 1, 3>, d->H, 1);
+      else dense_kernel(moe_down_dense_kernel<CMK_BF16, 2, 1>, d->H, 2);
     } else {
       dense_kernel(moe_gate_up_dense_kernel<CMK_F16, 1, 1, 2>, p.Ip, 1);
-      if (all_at_once(1)) dense_kernel(moe_down_dense_kernel<CMK_F16, 1, 2>, d->H, 1);
-      else dense_kernel(moe_down_dense_kernel<CMK_F16, 2, 2>, d->H, 2);
+      if (all_at_once(1)) dense_kernel(moe_down_dense_kernel<CMK_F16, 1, 3>, d->H, 1);
+      else dense_kernel(moe_down_dense_kernel<CMK_F16, 2, 1>, d->H, 2);
     }
   } else if (d->w_dtype == CMK_MX4) {
     if (p.x_planes == 1) {
