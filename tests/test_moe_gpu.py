@@ -5,7 +5,8 @@ by at most n * 2^-23 * sum |.| (any order, rounding or truncating adders), the
 activation by a few steps, the kept inner values by 2^-16 (two bf16; in front of
 fp16 weights, which are split too, the smallest of the four partial products is
 left out: 2^-16 more), y by half a step of its type.  The bound is carried through the
-formula in 64 bits, element by element."""
+formula in 64 bits, element by element.  (It is the bound of inner values of 16 bits; they
+have 24, which layers with an exact result check to the bit.)"""
 import math
 
 import pytest
