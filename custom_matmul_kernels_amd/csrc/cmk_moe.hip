@@ -403,9 +403,9 @@ __device__ __forceinline__ f32x4 mfma_f16(u32x4v a, u32x4v b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-// fp32 as the sum of three bf16, exactly.  The first is cut, not rounded: a value that is
-// finite in fp32 stays so up to the end of the range.  An infinity or a NaN stays in the
-// first alone.
+// fp32 as the sum of three bf16, exactly (but for bits below 2^-133).  The first is cut,
+// not rounded: a value that is finite in fp32 stays so up to the end of the range.  An
+// infinity or a NaN stays in the first alone.
 __device__ __forceinline__ void split_f32(float v, u16& a, u16& b, u16& c) {
   const bool finite = __builtin_isfinite(v);
   const float hi = finite ? __uint_as_float(__float_as_uint(v) & 0xffff0000u) : v;
@@ -499,8 +499,8 @@ constexpr int inner_bytes(int KS, int RG) { return (KS == 1 && RG == 1 ? 36 : 51
 // may differ from run to run.
 //
 // `source` gives rows of planes, or of fp32 that become planes on the way to LDS (two
-// thirds of the bytes: 64 tokens x 2048 x 1024 x 128 experts 307 us from planes, 297 from fp32; 16 x 4096
-// x 4096 x 8 experts in 4 bits 84 and 75).
+// thirds of the bytes: 64 tokens x 2048 x 1024 x 128 experts 307 us from planes, 297 from
+// fp32; 16 x 4096 x 4096 x 8 experts in 4 bits 84 and 75).
 template <int WF, int PLANES, int M, int RG, int NB, int U, int KS, bool SPLIT, bool PACK, int BYTES, class Source>
 __device__ __forceinline__ void moe_products(f32x4 (&acc)[M][RG][NB], const void* base, const uint8_t* scales, long long rows,
                                              const long long (&row)[M][RG], long long ld, int K, int count, Source source,
@@ -806,7 +806,9 @@ __device__ __forceinline__ void moe_down_tokens(const MoeArgs& a, int expert, co
   moe_down_rows<RG>(a, n0, row);
   f32x4 acc[1][RG][NB] = {};
   auto source = [&](int c) { return (const float*)a.hp + (long long)list[c0 + c] * a.Ip; };
-  moe_products<WF, kInnerPlanes, 1, RG, NB, U, KS, WF == CMK_F16, PACK, inner_bytes(KS, RG)>(acc, moe_down_base<WF>(a, expert), moe_down_scales<WF>(a, expert), a.H, row, a.ld_down, a.I, min(count - c0, NB * 16), source, 0, share, n0 >= a.H, lds);
+  moe_products<WF, kInnerPlanes, 1, RG, NB, U, KS, WF == CMK_F16, PACK, inner_bytes(KS, RG)>(
+      acc, moe_down_base<WF>(a, expert), moe_down_scales<WF>(a, expert), a.H, row, a.ld_down, a.I, min(count - c0, NB * 16), source, 0,
+      share, n0 >= a.H, lds);
   join_waves<KS, RG * NB, inner_bytes(KS, RG)>((f32x4(&)[RG * NB])acc, (f32x4(*)[RG * NB][64])lds, share);
   if (share == 0) {
     if constexpr (PACK) add_planes<kInnerPlanes>((f32x4(&)[RG][NB])acc, count - c0);
@@ -833,11 +835,11 @@ __global__ __launch_bounds__(64 * kMoeWaves, 3) void moe_down_kernel(MoeArgs a) 
 
 // Where experts have many tokens each, the activations of a pass do not fit LDS and
 // staging them in pieces leaves the memory idle between them (8 experts of 4096 x
-// 4096, 64 tokens: 230 us in bf16, 121 in 4 bits; as here 195 and 86).  These kernels walk k with a ring
-// of S slabs of activations in LDS, fetched by direct loads, and the weights in the
-// register ring as before; the four waves take rows of their own.  Within a row the 16
-// blocks of 16 bytes of a slab are stored at position block ^ (row & 15), so that the
-// 16 rows of a fragment spread over the banks.
+// 4096, 64 tokens: 230 us in bf16, 121 in 4 bits; as here 195 and 86).  These kernels
+// walk k with a ring of S slabs of activations in LDS, fetched by direct loads, and the
+// weights in the register ring as before; the four waves take rows of their own.  Within a
+// row the 16 blocks of 16 bytes of a slab are stored at position block ^ (row & 15), so
+// that the 16 rows of a fragment spread over the banks.
 constexpr int kGateUpStages = 4, kDownStages = 3;
 constexpr int kDenseBlocks = 2;  // blocks of 16 slots of a pass (four would leave a compute unit one work-group)
 
