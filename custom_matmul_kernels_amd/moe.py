@@ -29,7 +29,8 @@ class MoECUDA:
     Made for a few tokens, where reading the chosen experts' weights is all there
     is; more than 256 run in portions of 256.  A y_j whose sum an infinite weight of
     `down` or an infinite inner product enters may be NaN instead of an infinity.
-    There is no backward pass."""
+    There is no backward pass and no forward-mode derivative: operands that ask for
+    one are refused."""
 
     def __init__(self, k=2, activation="silu", renormalize=True):
         if activation not in ACTIVATIONS:

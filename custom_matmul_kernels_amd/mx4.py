@@ -175,7 +175,8 @@ class MX4BMMCUDA:
 
     An operand is an MX4Tensor whose blocks run along k (A: ``dim=-1``, B:
     ``dim=-2``) or a float tensor, which is quantised in the call.  Sums are held
-    in fp32 and rounded once.  There is no backward pass."""
+    in fp32 and rounded once.  There is no backward pass and no forward-mode
+    derivative: operands that ask for one are refused."""
 
     def __init__(self, out_dtype=torch.float32):
         self._out = _common.float_type(out_dtype, "out_dtype")

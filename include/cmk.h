@@ -63,7 +63,8 @@ extern "C" {
 #define CMK_DIST_L2    1   /* c += (a-b)^2    ("squared_l2") */
 #define CMK_DIST_L1    2   /* c += |a-b|      ("l1")         */
 
-/* Operand description shared by all GEMM-family entry points. */
+/* Operand description shared by all GEMM-family entry points.  M, N and K are at
+ * most 2^31 - 1024: they are rounded up to whole tiles in ints. */
 typedef struct cmk_gemm_desc {
   int L, M, N, K;            /* batch, rows of C, cols of C, contraction length */
   int transA, transB;        /* 0 = "n", 1 = "t" (see above)                    */
